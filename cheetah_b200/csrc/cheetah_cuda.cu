@@ -38,6 +38,7 @@
 #include "gemv_qmma.cuh"
 #include "gemv_mma.cuh"
 #include "gemm_tcgen05.cuh"
+#include "launch.cuh"
 #include "prefill_attention.cuh"
 #include "prefill_attention_tc.cuh"
 #include "store.h"
@@ -68,28 +69,6 @@ int env_int(const char *name, int fallback) {
     if (v == nullptr || v[0] == '\0') return fallback;
     const int x = std::atoi(v);
     return x > 0 ? x : fallback;
-}
-
-int sm_count(int device) {
-    int count = 0;
-    cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
-    return count > 0 ? count : 148;
-}
-
-template <typename Kernel, typename... Args>
-cudaError_t launch_ex(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                      bool pdl, Args... args) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = grid;
-    config.blockDim = block;
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
-    config.attrs = attr;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 int pick_ksplit(int cols) {
@@ -311,21 +290,6 @@ int attention_splits(int batch, int kv_heads, int max_len, int sms) {
     const int target = std::max(1, (2 * sms) / std::max(1, batch * kv_heads));
     const int by_len = std::max(1, (max_len + kWarp - 1) / kWarp);
     return std::max(1, std::min(std::min(target, by_len), kMaxSplits));
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no -lcuda).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult status;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &status) == cudaSuccess &&
-            status == cudaDriverEntryPointSuccess) {
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-        }
-    });
-    return fn;
 }
 
 // 2D map over a bf16 KV pool viewed as [rows][head_dim]: 64-column boxes of

@@ -45,34 +45,6 @@ inline size_t prefill_attention_tc_smem() {
     return (size_t)kTcQBytes + (size_t)kTcStages * 2 * kTcKvBytes + kTcPBytes + 1024;
 }
 
-// MN-major operand with 128-byte swizzle (rows of 128 B along N, 8-row atoms
-// along K, SBO = 1024 B between K atoms); one 64-element atom along N.
-__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr) {
-    uint64_t desc = 0;
-    desc |= (uint64_t)((addr >> 4) & 0x3FFF);
-    desc |= (uint64_t)1 << 16;
-    desc |= (uint64_t)(1024 >> 4) << 32;
-    desc |= (uint64_t)1 << 46;
-    desc |= (uint64_t)2 << 61;
-    return desc;
-}
-
-__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, float *v) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
 // Pool rows of key tile `tile`'s two 64-key spans for KV head `kvh` (a span
 // never crosses a page: page_tokens is a multiple of 64). A span past the
 // chunk's last position `pos_last` holds only masked keys: it re-reads span 0
