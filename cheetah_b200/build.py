@@ -23,7 +23,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libcheetah_cuda.so"
 
-SOURCES = ["cheetah_cuda.cu", "store.cpp"]
+SOURCES = ["cheetah_cuda.cu", "verify_ops.cu", "store.cpp"]
 HEADERS = ["common.cuh", "gemv.cuh", "attention.cuh", "kernels_misc.cuh", "store.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -50,7 +50,7 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: Path | No
     if not force and not defines and out is None and not _stale():
         return LIB
     sources = [str(CSRC / s) for s in SOURCES]
-    cmd = [nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared",
+    cmd = [nvcc(), *ARCH_FLAGS, "--threads", "0", "-O3", "-lineinfo", "-std=c++17", "-shared",
            "-Xcompiler", "-fPIC,-ffp-contract=off,-fvisibility=hidden",
            "-I", str(INCLUDE), "-I", str(CSRC),
            "--expt-relaxed-constexpr",

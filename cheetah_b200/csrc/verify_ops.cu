@@ -1,0 +1,226 @@
+// The op entries of a step that verifies drafted tokens (include/cheetah_cuda.h):
+// page slots, q/k norm with rotation and cache append, tree attention, token
+// log probabilities. Each checks its arguments, launches on the caller's
+// stream and keeps nothing.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+#include <string>
+
+#include "cheetah_cuda.h"
+#include "common.cuh"
+#include "launch.cuh"
+#include "page_slots.cuh"
+#include "qk_norm_rope.cuh"
+#include "token_logprobs.cuh"
+#include "tree_attention.cuh"
+
+using cheetah::launch_ex;
+
+namespace {
+
+bool aligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// A pool's slots are numbered in 32 bits.
+bool pool_in_range(uint32_t num_pages, uint32_t page_tokens) {
+    return num_pages > 0 && page_tokens > 0 && (uint64_t)num_pages * page_tokens <= 0x7FFFFFFFull;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cheetah_cuda_op_page_slots(const CheetahCudaPageSlots *a, void *stream) {
+    CH_REQUIRE(a != nullptr && a->cached && a->new_tokens && a->free_count && a->page_table && a->row_starts &&
+                   a->seq_lens && a->positions && a->seq_ids && a->slots && a->counts,
+               "cheetah_cuda_op_page_slots: null argument");
+    CH_REQUIRE(a->free_pages != nullptr || a->free_capacity == 0, "cheetah_cuda_op_page_slots: null free list");
+    CH_REQUIRE(a->batch > 0 && a->batch <= (uint32_t)cheetah::kSlotMaxBatch,
+               "cheetah_cuda_op_page_slots: batch must be 1.." + std::to_string(cheetah::kSlotMaxBatch));
+    CH_REQUIRE(a->max_tokens > 0 && a->max_tokens <= 0x7FFFFFFFu && a->free_capacity <= 0x7FFFFFFFu,
+               "cheetah_cuda_op_page_slots: max_tokens must be positive, and lengths below 2^31");
+    CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens) && pool_in_range(a->max_pages_per_seq, a->page_tokens),
+               "cheetah_cuda_op_page_slots: a pool and a table row hold 1 .. 2^31-1 tokens");
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    cheetah::PageSlotParams p = {};
+    p.cached = a->cached;
+    p.new_tokens = a->new_tokens;
+    p.free_pages = a->free_pages;
+    p.free_count = a->free_count;
+    p.free_capacity = (int)a->free_capacity;
+    p.batch = (int)a->batch;
+    p.page_table = a->page_table;
+    p.max_pages = (int)a->max_pages_per_seq;
+    p.num_pages = (int)a->num_pages;
+    p.page_tokens = (int)a->page_tokens;
+    p.max_tokens = (int)a->max_tokens;
+    p.row_starts = a->row_starts;
+    p.seq_lens = a->seq_lens;
+    p.positions = a->positions;
+    p.seq_ids = a->seq_ids;
+    p.slots = a->slots;
+    p.counts = a->counts;
+    const size_t smem = (size_t)a->batch * 3 * sizeof(int32_t);
+    if (smem > 48 * 1024)
+        CH_CUDA_TRY(cudaFuncSetAttribute(cheetah::page_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int blocks = std::max(1, std::min(cheetah::sm_count(device),
+                                            (p.max_tokens + cheetah::kSlotThreads - 1) / cheetah::kSlotThreads));
+    CH_CUDA_TRY(launch_ex(cheetah::page_slots_kernel, dim3(blocks), dim3(cheetah::kSlotThreads), smem,
+                          static_cast<cudaStream_t>(stream), true, p));
+    return 0;
+}
+
+int cheetah_cuda_op_qk_norm_rope(const CheetahCudaQkNormRope *a, void *stream) {
+    CH_REQUIRE(a != nullptr && a->qkv && a->rope_cos && a->rope_sin && a->positions && a->slots && a->q_out &&
+                   a->k_pool && a->v_pool,
+               "cheetah_cuda_op_qk_norm_rope: null argument");
+    CH_REQUIRE((a->dtype == CHEETAH_CUDA_KV_BF16 || a->dtype == CHEETAH_CUDA_KV_F32) &&
+                   (a->kv_dtype == CHEETAH_CUDA_KV_BF16 || a->kv_dtype == CHEETAH_CUDA_KV_F32),
+               "cheetah_cuda_op_qk_norm_rope: unknown dtype");
+    CH_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "cheetah_cuda_op_qk_norm_rope: head_dim must be 64 or 128");
+    CH_REQUIRE(a->rotary_dim > 0 && a->rotary_dim % 16 == 0 && a->rotary_dim <= a->head_dim,
+               "cheetah_cuda_op_qk_norm_rope: rotary_dim must be a multiple of 16 up to head_dim");
+    CH_REQUIRE(a->tokens > 0 && a->tokens <= 0x7FFFFFFFu && a->max_positions > 0 && a->max_positions <= 0x7FFFFFFFu,
+               "cheetah_cuda_op_qk_norm_rope: empty shape");
+    CH_REQUIRE(a->q_heads > 0 && a->kv_heads > 0 && a->q_heads <= 1024 && a->kv_heads <= 1024,
+               "cheetah_cuda_op_qk_norm_rope: head counts must be 1..1024");
+    CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens),
+               "cheetah_cuda_op_qk_norm_rope: a pool holds 1 .. 2^31-1 tokens");
+    const bool bf16 = a->dtype == CHEETAH_CUDA_KV_BF16;
+    const size_t heads = (size_t)a->q_heads + 2 * (size_t)a->kv_heads;
+    CH_REQUIRE(a->qkv_stride >= heads * a->head_dim && a->qkv_stride % (bf16 ? 8 : 4) == 0 &&
+                   a->qkv_stride < ((size_t)1 << 40),
+               "cheetah_cuda_op_qk_norm_rope: qkv rows must not overlap and must be 16-byte aligned");
+    CH_REQUIRE(aligned(a->qkv, 16) && aligned(a->q_out, 16) && aligned(a->k_pool, 16) && aligned(a->v_pool, 16) &&
+                   aligned(a->rope_cos, 16) && aligned(a->rope_sin, 16) && aligned(a->q_norm, 16) && aligned(a->k_norm, 16),
+               "cheetah_cuda_op_qk_norm_rope: buffers must be 16-byte aligned");
+    cheetah::QkNormRopeParams p = {};
+    p.qkv = a->qkv;
+    p.qkv_stride = (long long)a->qkv_stride;
+    p.q_norm = a->q_norm;
+    p.k_norm = a->k_norm;
+    p.eps = a->eps;
+    p.rope_cos = a->rope_cos;
+    p.rope_sin = a->rope_sin;
+    p.max_positions = (int)a->max_positions;
+    p.rotary_dim = (int)a->rotary_dim;
+    p.positions = a->positions;
+    p.slots = a->slots;
+    p.tokens = (int)a->tokens;
+    p.q_heads = (int)a->q_heads;
+    p.kv_heads = (int)a->kv_heads;
+    p.head_dim = (int)a->head_dim;
+    p.q_out = a->q_out;
+    p.k_pool = a->k_pool;
+    p.v_pool = a->v_pool;
+    p.num_pages = (int)a->num_pages;
+    p.page_tokens = (int)a->page_tokens;
+    const bool kv_bf16 = a->kv_dtype == CHEETAH_CUDA_KV_BF16;
+    const uint64_t blocks = ((uint64_t)a->tokens * heads + 3) / 4;
+    CH_REQUIRE(blocks <= 0x7FFFFFFFull, "cheetah_cuda_op_qk_norm_rope: too many rows");
+    auto kernel = bf16 ? (kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<uint16_t, uint16_t>
+                                  : cheetah::qk_norm_rope_rows_kernel<uint16_t, float>)
+                       : (kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<float, uint16_t>
+                                  : cheetah::qk_norm_rope_rows_kernel<float, float>);
+    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)blocks), dim3(128), 0, static_cast<cudaStream_t>(stream), true, p));
+    return 0;
+}
+
+static int check_tree_attention(const CheetahCudaTreeAttention *a) {
+    CH_REQUIRE(a != nullptr, "cheetah_cuda_op_tree_attention: null argument");
+    CH_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "cheetah_cuda_op_tree_attention: head_dim must be 64 or 128");
+    CH_REQUIRE(a->kv_heads > 0 && a->q_heads > 0 && a->q_heads % a->kv_heads == 0 && a->q_heads / a->kv_heads <= 32 &&
+                   a->q_heads <= 1024,
+               "cheetah_cuda_op_tree_attention: q_heads must be a multiple of kv_heads (group <= 32)");
+    CH_REQUIRE(a->batch > 0 && a->batch <= 4096, "cheetah_cuda_op_tree_attention: batch must be 1..4096");
+    CH_REQUIRE(a->rows > 0 && a->rows <= (1u << 24), "cheetah_cuda_op_tree_attention: rows must be 1..2^24");
+    CH_REQUIRE(a->page_tokens > 0 && a->page_tokens % 16 == 0,
+               "cheetah_cuda_op_tree_attention: page_tokens must be a multiple of 16");
+    CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens) && pool_in_range(a->max_pages_per_seq, a->page_tokens) &&
+                   (uint64_t)a->num_pages * a->kv_heads * a->page_tokens <= 0x7FFFFFFFull,
+               "cheetah_cuda_op_tree_attention: a pool holds 1 .. 2^31-1 rows of one head, a table row as many tokens");
+    CH_REQUIRE(a->mask_words > 0 && a->mask_words <= 16, "cheetah_cuda_op_tree_attention: mask_words must be 1..16");
+    CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu, "cheetah_cuda_op_tree_attention: sliding_window is too large");
+    return 0;
+}
+
+int cheetah_cuda_op_tree_attention_workspace(const CheetahCudaTreeAttention *a, size_t *bytes) {
+    CH_REQUIRE(bytes != nullptr, "cheetah_cuda_op_tree_attention_workspace: null argument");
+    if (check_tree_attention(a) != 0) return -1;
+    *bytes = 0;
+    return 0;
+}
+
+int cheetah_cuda_op_tree_attention(const CheetahCudaTreeAttention *a, void *stream) {
+    if (check_tree_attention(a) != 0) return -1;
+    CH_REQUIRE(a->q && a->k_pool && a->v_pool && a->page_table && a->seq_lens && a->row_starts && a->tree_mask && a->out,
+               "cheetah_cuda_op_tree_attention: null argument");
+    CH_REQUIRE(a->sliding_window == 0 || a->positions != nullptr,
+               "cheetah_cuda_op_tree_attention: a sliding window needs the rows' positions");
+    CH_REQUIRE(a->q_stride >= (size_t)a->q_heads * a->head_dim && a->q_stride % 8 == 0 && a->q_stride < ((size_t)1 << 32),
+               "cheetah_cuda_op_tree_attention: q rows must not overlap and must be 16-byte aligned");
+    CH_REQUIRE(aligned(a->q, 16) && aligned(a->k_pool, 16) && aligned(a->v_pool, 16) && aligned(a->out, 16) &&
+                   aligned(a->tree_mask, 8),
+               "cheetah_cuda_op_tree_attention: q, out and the pools must be 16-byte aligned, the mask 8-byte");
+    cheetah::TreeAttnParams p = {};
+    p.q = static_cast<const uint16_t *>(a->q);
+    p.q_stride = (long long)a->q_stride;
+    p.rows = (int)a->rows;
+    p.k_pool = static_cast<const uint16_t *>(a->k_pool);
+    p.v_pool = static_cast<const uint16_t *>(a->v_pool);
+    p.page_table = a->page_table;
+    p.max_pages = (int)a->max_pages_per_seq;
+    p.num_pages = (int)a->num_pages;
+    p.page_tokens = (int)a->page_tokens;
+    p.seq_lens = a->seq_lens;
+    p.row_starts = a->row_starts;
+    p.batch = (int)a->batch;
+    p.tree_mask = reinterpret_cast<const unsigned long long *>(a->tree_mask);
+    p.mask_words = (int)a->mask_words;
+    p.positions = a->positions;
+    p.window = (int)a->sliding_window;
+    p.q_heads = (int)a->q_heads;
+    p.kv_heads = (int)a->kv_heads;
+    p.scale = 1.0f / sqrtf((float)a->head_dim);
+    p.out = static_cast<uint16_t *>(a->out);
+    auto kernel = a->head_dim == 64 ? cheetah::tree_attention_rows_kernel<64> : cheetah::tree_attention_rows_kernel<128>;
+    CH_CUDA_TRY(launch_ex(kernel, dim3(a->rows, a->q_heads), dim3(cheetah::kTreeKeys), 0,
+                          static_cast<cudaStream_t>(stream), true, p));
+    return 0;
+}
+
+int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogprobs *a, void *stream) {
+    CH_REQUIRE(a != nullptr && a->logits && a->tokens && a->logprob, "cheetah_cuda_op_token_logprobs: null argument");
+    CH_REQUIRE(a->dtype == CHEETAH_CUDA_KV_BF16 || a->dtype == CHEETAH_CUDA_KV_F32,
+               "cheetah_cuda_op_token_logprobs: unknown dtype");
+    CH_REQUIRE(a->rows > 0 && a->rows <= 0x7FFFFFFFu && a->vocab > 0 && a->vocab <= 0x7FFFFFFFu,
+               "cheetah_cuda_op_token_logprobs: empty shape");
+    CH_REQUIRE(a->top <= (uint32_t)cheetah::kLpMaxTop && a->top <= a->vocab,
+               "cheetah_cuda_op_token_logprobs: top must be at most 32 and at most vocab");
+    CH_REQUIRE(a->top == 0 || (a->top_ids && a->top_logprobs),
+               "cheetah_cuda_op_token_logprobs: top needs top_ids and top_logprobs");
+    CH_REQUIRE((a->row_stride >= a->vocab || a->rows == 1) && a->row_stride < ((size_t)1 << 40),
+               "cheetah_cuda_op_token_logprobs: rows must not overlap");
+    const bool bf16 = a->dtype == CHEETAH_CUDA_KV_BF16;
+    CH_REQUIRE(aligned(a->logits, bf16 ? 2 : 4), "cheetah_cuda_op_token_logprobs: logits must be aligned to their type");
+    cheetah::LogprobParams p = {};
+    p.logits = a->logits;
+    p.row_stride = (long long)a->row_stride;
+    p.rows = (int)a->rows;
+    p.vocab = (int)a->vocab;
+    p.tokens = a->tokens;
+    p.top = (int)a->top;
+    p.logprob = a->logprob;
+    p.rank = a->rank;
+    p.entropy = a->entropy;
+    p.top_ids = a->top_ids;
+    p.top_logprobs = a->top_logprobs;
+    auto kernel = bf16 ? cheetah::token_logprobs_kernel<uint16_t> : cheetah::token_logprobs_kernel<float>;
+    CH_CUDA_TRY(launch_ex(kernel, dim3(a->rows), dim3(cheetah::kLpThreads), 0, static_cast<cudaStream_t>(stream), true, p));
+    return 0;
+}
+
+}  // extern "C"

@@ -332,6 +332,156 @@ CHEETAH_CUDA_API int cheetah_cuda_op_prefill_attention(const CheetahCudaPrefillA
 CHEETAH_CUDA_API int cheetah_cuda_op_decode_attention_noalloc(const CheetahCudaDecodeAttention *args,
                                                               void *stream);
 
+/* ---- One step that verifies drafted tokens ----
+ *
+ * The four entries below are the device side of a step in which every
+ * sequence of a batch appends several tokens at once (a drafted tree, a
+ * prompt chunk, a single decoded token), in the order they run:
+ * cheetah_cuda_op_page_slots gives each new token its cell of the paged pool,
+ * cheetah_cuda_op_qk_norm_rope fills the cells, cheetah_cuda_op_tree_attention
+ * attends over them and cheetah_cuda_op_token_logprobs scores the step's
+ * tokens. The tokens of a step are rows, sequence after sequence: those of
+ * sequence b are rows row_starts[b] .. row_starts[b+1]-1. All four are
+ * asynchronous on `stream` (a stream of the current device), allocate
+ * nothing, keep nothing between calls and may be captured into a graph. No
+ * counterpart in the reference (it decodes one token of one sequence). */
+
+/* Block tables and slot maps from request lengths. Sequence b appends
+ * new_tokens[b] positions to its cached[b]; the pages it lacks come from
+ * free_pages in sequence order, entries [0, need_0) to sequence 0 and so on.
+ * A slot is page * page_tokens + the position within the page.
+ *
+ * A sequence is refused where a length is negative or its positions pass the
+ * table's width (it then counts as no rows), where its rows pass max_tokens, or
+ * where its pages pass the end of the free list (every later sequence that
+ * needs a page is then refused too). A refused sequence takes no page, its
+ * table row stays, seq_lens is 0 and its rows hold position and slot -1. Rows
+ * behind the last sequence, up to max_tokens, hold -1 throughout, so a step
+ * captured at a fixed row count skips them. A page id outside the pool gives
+ * slot -1. Calling again with the same arguments gives the same result. */
+typedef struct CheetahCudaPageSlots {
+    const int32_t *cached;      /* [batch] positions already in the cache */
+    const int32_t *new_tokens;  /* [batch] positions to append */
+    const int32_t *free_pages;  /* [free_capacity] page ids to hand out, in order */
+    const int32_t *free_count;  /* [1] how many of them are valid (clamped to free_capacity) */
+    uint32_t free_capacity;
+    uint32_t batch;             /* 1..16384 */
+    int32_t *page_table;        /* [batch][max_pages_per_seq], updated in place */
+    uint32_t max_pages_per_seq;
+    uint32_t num_pages;         /* pages in the pool */
+    uint32_t page_tokens;
+    uint32_t max_tokens;        /* length of the per-row outputs, at least 1 */
+    int32_t *row_starts;        /* [batch+1] first row of each sequence (at most max_tokens) */
+    int32_t *seq_lens;          /* [batch] cached + new positions */
+    int32_t *positions;         /* [max_tokens] absolute position of each row */
+    int32_t *seq_ids;           /* [max_tokens] sequence of each row */
+    int32_t *slots;             /* [max_tokens] pool slot of each row */
+    int32_t *counts;            /* [3] rows asked for, pages taken, sequences refused */
+} CheetahCudaPageSlots;
+CHEETAH_CUDA_API int cheetah_cuda_op_page_slots(const CheetahCudaPageSlots *args, void *stream);
+
+/* Per-head RMSNorm of q and k (`ops.rs:1130-1152`, the qwen3 family), the
+ * rotate-half rotation (`ops.rs:693-740`) at a position given for each row,
+ * and the append of K and V at a slot given for each row (the nodes of a
+ * drafted tree share positions but not slots). Rows whose position is outside
+ * the rotary table are skipped (q_out and the pool keep what they held); rows
+ * whose slot is outside the pool get their q but append nothing. The slots of
+ * one call must be distinct. f32 arithmetic, one rounding to each output. */
+typedef struct CheetahCudaQkNormRope {
+    const void *qkv;           /* [tokens][q_heads + 2*kv_heads][head_dim]: q, k, v heads of a row */
+    size_t qkv_stride;         /* elements between rows */
+    int32_t dtype;             /* of qkv and q_out: CHEETAH_CUDA_KV_BF16 or _F32 */
+    int32_t kv_dtype;          /* of the pools: CHEETAH_CUDA_KV_* */
+    const float *q_norm;       /* [head_dim] or NULL: q is not normalised */
+    const float *k_norm;       /* [head_dim] or NULL */
+    float eps;
+    const float *rope_cos;     /* [max_positions][rotary_dim/2] */
+    const float *rope_sin;
+    uint32_t max_positions;
+    uint32_t rotary_dim;       /* a multiple of 16, at most head_dim; later dimensions pass through */
+    const int32_t *positions;  /* [tokens] */
+    const int32_t *slots;      /* [tokens] */
+    uint32_t tokens;
+    uint32_t q_heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;         /* 64 or 128 */
+    void *q_out;               /* [tokens][q_heads][head_dim] */
+    void *k_pool;              /* [num_pages][kv_heads][page_tokens][head_dim] */
+    void *v_pool;
+    uint32_t num_pages;
+    uint32_t page_tokens;
+} CheetahCudaQkNormRope;
+CHEETAH_CUDA_API int cheetah_cuda_op_qk_norm_rope(const CheetahCudaQkNormRope *args, void *stream);
+
+/* Attention of a batch's drafted nodes over their sequences' paged caches.
+ * Sequence b has n = row_starts[b+1] - row_starts[b] rows and seq_lens[b]
+ * cached positions, the last n of which are its rows' own K/V in row order.
+ * Row i of b sees every earlier position (the context, seq_lens[b] - n keys)
+ * and those nodes j of b whose bit is set in its mask row: bit j % 64 of
+ * tree_mask[row][j / 64] (its ancestors and itself, for a tree). With a
+ * window, a key is seen only if its position is above positions[row] -
+ * sliding_window, where a context key's position is its index and node j's is
+ * positions[its row]. A row that sees nothing gives zeros, whatever it reads;
+ * cells a row does not see never reach it, non-finite ones included. Rows
+ * from row_starts[batch] on stay as they were; a sequence with seq_lens[b] <
+ * n gives zeros, and keys on a page outside the pool count as unseen. q and
+ * the softmax weights are bf16 in the products, sums and statistics are f32.
+ *
+ * `workspace` holds partial results between the two launches of a call:
+ * cheetah_cuda_op_tree_attention_workspace says how many bytes (256-byte
+ * aligned; the contents need no initialisation and are garbage afterwards).
+ * Calls that may overlap on the GPU, graphs included, each need their own. */
+typedef struct CheetahCudaTreeAttention {
+    const void *q;             /* bf16 [rows][q_heads][head_dim], RoPE applied */
+    size_t q_stride;           /* elements between rows, a multiple of 8 */
+    uint32_t rows;             /* rows of q and out: at least row_starts[batch] */
+    const void *k_pool;        /* bf16 [num_pages][kv_heads][page_tokens][head_dim] */
+    const void *v_pool;        /* same layout */
+    const int32_t *page_table; /* [batch][max_pages_per_seq] */
+    uint32_t max_pages_per_seq;
+    uint32_t num_pages;
+    uint32_t page_tokens;      /* a multiple of 16 */
+    const int32_t *seq_lens;   /* [batch] */
+    const int32_t *row_starts; /* [batch+1], ascending from 0 */
+    uint32_t batch;            /* 1..4096 */
+    const uint64_t *tree_mask; /* [rows][mask_words] */
+    uint32_t mask_words;       /* 1..16; nodes from 64*mask_words on are unseen by other rows and themselves */
+    const int32_t *positions;  /* [rows]; may be NULL without a window */
+    uint32_t sliding_window;   /* 0 = full */
+    uint32_t q_heads;
+    uint32_t kv_heads;         /* q_heads / kv_heads: 1..32 */
+    uint32_t head_dim;         /* 64 or 128 */
+    void *out;                 /* bf16 [rows][q_heads][head_dim] */
+    void *workspace;
+    size_t workspace_bytes;
+} CheetahCudaTreeAttention;
+CHEETAH_CUDA_API int cheetah_cuda_op_tree_attention_workspace(const CheetahCudaTreeAttention *args, size_t *bytes);
+CHEETAH_CUDA_API int cheetah_cuda_op_tree_attention(const CheetahCudaTreeAttention *args, void *stream);
+
+/* For each row of logits: the natural log probability of a given token, its
+ * rank (1 + the number of larger logits), the entropy of the row's softmax
+ * and the `top` likeliest tokens with their log probabilities (by value
+ * descending, equal values by ascending id) — what an answer's `logprobs`
+ * lists, without copying the vocabulary to the host. A logit of -inf has
+ * probability 0. A token outside the vocabulary gives NaN and rank 0. A row
+ * that holds a NaN or +inf, or nothing above -inf, has no distribution: its
+ * floats are NaN, its rank 0 and its top ids -1. */
+typedef struct CheetahCudaTokenLogprobs {
+    const void *logits;        /* [rows][vocab] */
+    size_t row_stride;         /* elements between rows */
+    int32_t dtype;             /* CHEETAH_CUDA_KV_F32 or _BF16 */
+    uint32_t rows;
+    uint32_t vocab;
+    const int32_t *tokens;     /* [rows] */
+    uint32_t top;              /* 0..32, at most vocab */
+    float *logprob;            /* [rows] */
+    int32_t *rank;             /* [rows] or NULL */
+    float *entropy;            /* [rows] or NULL */
+    int32_t *top_ids;          /* [rows][top], may be NULL when top is 0 */
+    float *top_logprobs;       /* [rows][top] */
+} CheetahCudaTokenLogprobs;
+CHEETAH_CUDA_API int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogprobs *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,592 @@
+"""The drafted-token operators on the GPU against 64-bit references
+(`tests/verify_ref.py`), at the sizes, masks and values where they can go
+wrong, and a run of all four as a verification step uses them."""
+
+import math
+
+import numpy as np
+import pytest
+
+from tests import verify_ref as V
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from cheetah_b200 import runtime
+    runtime.lib()
+
+
+def i32(values):
+    return torch.tensor(np.asarray(values), dtype=torch.int32, device="cuda")
+
+
+# ---- page_slots ---------------------------------------------------------------
+
+def _slots_case(cached, new, width, page_tokens, seed=0, free=None, free_count=None, max_tokens=None, num_pages=None, stale=False):
+    rng = np.random.default_rng(seed)
+    num_pages = num_pages or 4 * len(cached) * width + 8
+    ids = rng.permutation(num_pages)
+    table = ids[:len(cached) * width].reshape(len(cached), width).copy()
+    if stale:
+        table[:, ::2] = num_pages + 7  # ids outside the pool
+    have = [-(-max(c, 0) // page_tokens) for c in cached]
+    need = sum(max(0, -(-(max(c, 0) + max(n, 0)) // page_tokens) - h) for c, n, h in zip(cached, new, have))
+    free = list(ids[len(cached) * width:][:need + 2]) if free is None else free
+    free_count = len(free) if free_count is None else free_count
+    max_tokens = max_tokens or max(1, sum(max(n, 0) for n in new)) + 5
+    return dict(cached=list(cached), new=list(new), free=[int(f) for f in free], free_count=free_count, table=table,
+                num_pages=num_pages, page_tokens=page_tokens, max_tokens=max_tokens)
+
+
+def _check_slots(case):
+    from cheetah_b200 import runtime as R
+    table = i32(case["table"])
+    args = (i32(case["cached"]), i32(case["new"]), i32(case["free"]), i32([case["free_count"]]), table,
+            case["num_pages"], case["page_tokens"], case["max_tokens"])
+    want = V.page_slots(**case)
+    for _ in range(2):  # the same call again gives the same result
+        got = R.page_slots(*args)
+        for name in ("row_starts", "seq_lens", "positions", "seq_ids", "slots", "counts"):
+            np.testing.assert_array_equal(getattr(got, name).cpu().numpy(), np.array(want[name]), err_msg=name)
+        np.testing.assert_array_equal(table.cpu().numpy(), want["table"])
+    return want
+
+
+@pytest.mark.parametrize("batch,page_tokens,most", [(1, 16, 1), (1, 64, 5000), (3, 1, 9), (31, 64, 17), (64, 48, 200),
+                                                    (511, 16, 3), (513, 16, 40), (2049, 128, 5), (16384, 16, 2)])
+def test_page_slots_random(batch, page_tokens, most):
+    rng = np.random.default_rng(batch + most)
+    cached, new = rng.integers(0, 300, batch), rng.integers(0, most + 1, batch)
+    _check_slots(_slots_case(cached.tolist(), new.tolist(), -(-(300 + most) // page_tokens), page_tokens, seed=batch))
+
+
+@pytest.mark.parametrize("name,cached,new,more", [
+    ("nothing new", [0, 16, 17], [0, 0, 0], {}),
+    ("empty cache", [0, 0], [1, 33], {}),
+    ("page borders", [15, 16, 17, 31], [1, 1, 1, 2], {}),
+    ("negative lengths", [-1, 5, 5], [3, -2, 4], {}),
+    ("past the table", [60, 3, 64, 64], [5, 4, 0, 1], {}),
+    ("lengths near 2^31", [2 ** 31 - 1, 1, 2 ** 31 - 1], [2 ** 31 - 1, 2, 0], dict(max_tokens=20)),
+    ("free list too short", [0, 10, 0, 16], [20, 3, 17, 9], dict(free=[3, 1, 2])),
+    ("free list empty", [0, 10], [1, 3], dict(free=[], free_count=0)),
+    ("free count above the list", [0, 0], [16, 17], dict(free=[3, 1], free_count=9)),
+    ("free count below the list", [0, 0], [16, 17], dict(free=[3, 1, 5], free_count=1)),
+    ("negative free count", [0, 0], [16, 0], dict(free=[3, 1, 5], free_count=-4)),
+    ("rows past max_tokens", [0, 5, 0], [10, 10, 10], dict(max_tokens=15)),
+    ("page ids outside the pool", [5, 40], [20, 30], dict(stale=True, num_pages=64)),
+    ("free ids outside the pool", [0, 0], [16, 16], dict(free=[-1, 1 << 30])),
+])
+def test_page_slots_edges(name, cached, new, more):
+    _check_slots(_slots_case(cached, new, 4, 16, **more))
+
+
+# ---- qk_norm_rope -------------------------------------------------------------
+
+@pytest.mark.parametrize("q_heads,kv_heads,D,rotary", [(14, 2, 64, 64), (28, 4, 128, 128), (4, 4, 64, 32), (3, 1, 128, 16),
+                                                       (8, 4, 128, 96)])
+@pytest.mark.parametrize("dtype,kv_dtype", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("tokens,norm", [(1, True), (7, False), (131, True)])
+def test_qk_norm_rope(q_heads, kv_heads, D, rotary, dtype, kv_dtype, tokens, norm):
+    from cheetah_b200 import runtime as R
+    types = {"bf16": torch.bfloat16, "f32": torch.float32}
+    g = torch.Generator().manual_seed(tokens + D + rotary)
+    heads, pt, pages, max_pos = q_heads + 2 * kv_heads, 16, 12, 50
+    wide = torch.randn(tokens, heads * D + 16, generator=g).to(types[dtype])  # rows lie apart
+    x = wide[:, :heads * D]
+    slots = torch.randperm(pages * pt, generator=g)[:tokens].to(torch.int32)
+    positions = torch.randint(0, max_pos, (tokens,), generator=g).to(torch.int32)
+    if tokens > 3:
+        slots[1], slots[2], positions[3], positions[4] = -1, pages * pt, -1, max_pos
+    angle = torch.rand(max_pos, rotary // 2, generator=g) * 6.0
+    cos, sin = angle.cos(), angle.sin()
+    w = [1.0 + 0.3 * torch.randn(D, generator=g) if norm else None for _ in range(2)]
+    pools = [torch.randn(pages, kv_heads, pt, D, generator=g).to(types[kv_dtype]) for _ in range(2)]
+    k_pool, v_pool = pools[0].cuda(), pools[1].cuda()
+    q_out = torch.full((tokens, q_heads, D), 7.0, dtype=types[dtype], device="cuda")
+    got = R.qk_norm_rope(wide.cuda()[:, :heads * D], q_heads, kv_heads, positions.cuda(), slots.cuda(), cos.cuda(), sin.cuda(),
+                         k_pool, v_pool, q_norm=w[0].cuda() if norm else None, k_norm=w[1].cuda() if norm else None,
+                         eps=1e-5, q_out=q_out)
+    assert got is q_out
+    # Sum of squares: D roundings, halved by the square root; then a handful.
+    f32 = (D / 2 + 10) * 2.0 ** -24
+    step = {"bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+    want_k, want_v = pools[0].double(), pools[1].clone()
+    tol_k = torch.zeros_like(want_k)
+    q, k_got = got.cpu().double(), k_pool.cpu().double()
+    for t in range(tokens):
+        p, s = int(positions[t]), int(slots[t])
+        if not 0 <= p < max_pos:
+            assert bool((q[t] == 7.0).all())
+            continue
+        row = x[t].reshape(heads, D)
+        for h in range(q_heads):
+            z, mag = V.norm_rope_head(row[h], w[0], 1e-5, cos[p], sin[p])
+            assert bool(((q[t, h] - z).abs() <= mag * f32 + z.abs() * step[dtype] + 1e-30).all()), (t, h)
+        if not 0 <= s < pages * pt:
+            continue
+        for h in range(kv_heads):
+            z, mag = V.norm_rope_head(row[q_heads + h], w[1], 1e-5, cos[p], sin[p])
+            want_k[s // pt, h, s % pt] = z
+            tol_k[s // pt, h, s % pt] = mag * f32 + z.abs() * step[kv_dtype] + 1e-30
+            want_v[s // pt, h, s % pt] = row[q_heads + kv_heads + h].to(types[kv_dtype])
+    assert bool(((k_got - want_k).abs() <= tol_k).all())  # cells not named: unchanged
+    assert torch.equal(v_pool.cpu(), want_v)
+
+
+def test_qk_norm_rope_large_values_and_zero_rows():
+    """A zero row stays zero, values near the type's limits keep their scale,
+    a non-finite value stays in its own head."""
+    from cheetah_b200 import runtime as R
+    D, pt = 64, 16
+    x = torch.zeros(4, 3, D)
+    x[1] = 1e18  # squares reach 1e36
+    x[2] = 1e-18
+    x[3, 0, 5] = math.inf
+    x[3, 1:] = 1.0
+    one = torch.ones(2, D // 2)
+    k, v = torch.zeros(2, 1, pt, D, device="cuda"), torch.zeros(2, 1, pt, D, device="cuda")
+    w = torch.ones(D, device="cuda")
+    q = R.qk_norm_rope(x.cuda(), 1, 1, i32([0, 0, 0, 0]), i32([0, 1, 2, 3]), one.cuda(), torch.zeros(2, D // 2, device="cuda"),
+                       k, v, q_norm=w, k_norm=w, eps=1e-6).cpu()
+    assert bool((q[0] == 0).all()) and torch.allclose(q[1], torch.ones(1, D), rtol=1e-5)
+    assert torch.allclose(q[2].double(), torch.full((1, D), 1e-15, dtype=torch.float64), rtol=1e-4)
+    assert torch.isnan(q[3, 0, 5]) and torch.allclose(k[0, 0, 3].cpu(), torch.ones(D), rtol=1e-5)
+    assert bool((v[0, 0, 3] == 1).all())
+
+
+# ---- tree_attention -----------------------------------------------------------
+
+class Tree:
+    """A batch of random trees over a shuffled paged pool, and its reference."""
+
+    def __init__(self, ctx, nodes, q_heads, kv_heads, D, page_tokens=64, window=0, seed=0, words=None, masks=None,
+                 scale=1.0, extra_rows=0, fill=float("nan"), width=None):
+        rng = np.random.default_rng(seed)
+        g = torch.Generator().manual_seed(seed)
+        self.window, self.kv_heads, self.group = window, kv_heads, q_heads // kv_heads
+        self.ctx, self.nodes = ctx, nodes
+        lens = [c + n for c, n in zip(ctx, nodes)]
+        per = [-(-n // page_tokens) for n in lens]
+        pages = sum(per) + 2
+        order = rng.permutation(pages)
+        self.table = np.full((len(ctx), width or max(max(per), 1)), -1, np.int32)
+        # Cells that hold no position are NaN (a fresh pool holds anything).
+        kp = torch.full((pages, kv_heads, page_tokens, D), fill)
+        vp = torch.full_like(kp, fill)
+        self.k, self.v = [], []
+        cursor = 0
+        for b, n in enumerate(lens):
+            k = torch.randn(n, kv_heads, D, generator=g).bfloat16()
+            v = torch.randn(n, kv_heads, D, generator=g).bfloat16()
+            for p in range(per[b]):
+                page = int(order[cursor])
+                cursor += 1
+                if p < self.table.shape[1]:
+                    self.table[b, p] = page
+                lo, hi = p * page_tokens, min(n, (p + 1) * page_tokens)
+                kp[page, :, :hi - lo] = k[lo:hi].transpose(0, 1).float()
+                vp[page, :, :hi - lo] = v[lo:hi].transpose(0, 1).float()
+            self.k.append(k.double())
+            self.v.append(v.double())
+        self.starts = np.concatenate([[0], np.cumsum(nodes)])
+        total = int(self.starts[-1])
+        self.rows = max(1, total + extra_rows)
+        words = words or max(1, -(-max(nodes + [1]) // 64))
+        self.seen, depth = [], []
+        for b, n in enumerate(nodes):
+            bits, d = V.tree_bits(V.random_tree(rng, n))
+            if masks is not None:
+                bits = masks(rng, n)
+            self.seen.append(bits)
+            depth.append(d + ctx[b])
+        self.positions = np.concatenate(depth + [np.full(self.rows - total, -1)]).astype(np.int64)
+        mask = np.zeros((self.rows, words), np.int64)
+        for b, bits in enumerate(self.seen):
+            if nodes[b]:
+                mask[self.starts[b]:self.starts[b + 1]] = V.pack_bits(bits, words)
+        self.words, self.mask = words, mask
+        self.q = (torch.randn(self.rows, q_heads, D, generator=g) * scale).bfloat16()
+        self.dev = dict(q=self.q.cuda(), k_pool=kp.bfloat16().cuda(), v_pool=vp.bfloat16().cuda(), page_table=i32(self.table),
+                        seq_lens=i32(lens), row_starts=i32(self.starts), tree_mask=torch.from_numpy(mask).cuda(),
+                        positions=i32(self.positions), sliding_window=window)
+
+    def run(self, **more):
+        from cheetah_b200 import runtime as R
+        return R.tree_attention(**{**self.dev, **more})
+
+    def visible(self, b, i):
+        n, c = self.nodes[b], self.ctx[b]
+        seen = np.ones(c + n, bool)
+        bits = np.zeros(n, bool)
+        w = min(n, 64 * self.words)
+        bits[:w] = self.seen[b][i][:w]
+        seen[c:] = bits
+        if self.window:
+            where = np.arange(c + n)
+            where[c:] = self.positions[self.starts[b]:self.starts[b + 1]]
+            seen &= where > self.positions[self.starts[b] + i] - self.window
+        return torch.from_numpy(seen)
+
+    def check(self, out, rows=None):
+        out = out.cpu().double()
+        rng = np.random.default_rng(1)
+        for b, n in enumerate(self.nodes):
+            picked = range(n) if n <= 6 else sorted(set([0, 1, n - 1, n // 2]) | set(rng.integers(0, n, 3).tolist()))
+            for i in picked:
+                seen = self.visible(b, i)
+                r = int(self.starts[b]) + i
+                for h in range(self.q.shape[1]):
+                    kvh = h // self.group
+                    want, tol = V.tree_row(self.q[r, h].double(), self.k[b][:, kvh], self.v[b][:, kvh], seen)
+                    err = (out[r, h] - want).abs()
+                    assert bool((err <= tol).all()), f"sequence {b} node {i} head {h}: {float((err - tol).max())} over"
+
+
+HEADS = [(14, 2, 64), (28, 4, 128), (4, 4, 64), (16, 1, 128), (8, 4, 128), (6, 2, 64)]
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,D", HEADS)
+@pytest.mark.parametrize("ctx,nodes", [
+    ([0], [1]), ([0], [8]), ([1], [1]), ([63], [1]), ([64], [3]), ([127], [2]), ([128], [5]), ([300], [17]),
+    ([120, 0, 700], [9, 1, 0]), ([1000, 3, 65], [1, 64, 20]), ([2500], [70]),
+])
+def test_tree_attention(q_heads, kv_heads, D, ctx, nodes):
+    case = Tree(ctx, nodes, q_heads, kv_heads, D, seed=sum(ctx) + sum(nodes))
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("page_tokens", [16, 32, 48, 128, 192])
+def test_tree_attention_page_sizes(page_tokens):
+    case = Tree([333, 90, 0], [13, 40, 130], 14, 2, 64, page_tokens=page_tokens, seed=page_tokens)
+    case.check(case.run())
+    case = Tree([333, 16], [13, 5], 8, 4, 128, page_tokens=page_tokens, seed=page_tokens)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("window", [1, 5, 48, 130, 5000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tree_attention_window(window, D):
+    case = Tree([400, 1, 129], [20, 70, 3], 8, 2, D, window=window, seed=window)
+    case.check(case.run())
+
+
+def test_tree_attention_long_and_wide():
+    case = Tree([9000, 20, 4097], [33, 300, 150], 14, 2, 64, seed=3)
+    case.check(case.run())
+    case = Tree([5000, 1], [130, 257], 28, 4, 128, seed=4)
+    case.check(case.run())
+
+
+def test_tree_attention_many_sequences():
+    rng = np.random.default_rng(8)
+    case = Tree(rng.integers(0, 200, 300).tolist(), rng.integers(0, 4, 300).tolist(), 14, 2, 64, seed=8)
+    case.check(case.run())
+
+
+def test_tree_attention_rows_that_see_nothing():
+    """Empty mask rows over an empty context give zeros; beside them rows that
+    see one node, and NaN in every cell that holds no position."""
+    def masks(rng, n):
+        bits = np.zeros((n, n), bool)
+        bits[1::2, 0] = True
+        return bits
+    case = Tree([0, 0], [7, 90], 14, 2, 64, masks=masks, seed=5)
+    out = case.run()
+    assert bool((out[0] == 0).all()) and bool((out[2] == 0).all())
+    case.check(out)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tree_attention_non_finite_cells_reach_only_the_rows_that_see_them(value, D):
+    """A node's K and V are non-finite: rows that do not see it are as without
+    it; and with a window, so is a context key that has left it."""
+    case = Tree([140, 50], [12, 9], 8, 2, D, seed=21)
+    for b, j in ((0, 3), (1, 2)):
+        pos = case.ctx[b] + j
+        page, cell = int(case.table[b, pos // 64]), pos % 64
+        case.dev["k_pool"][page, :, cell] = value
+        case.dev["v_pool"][page, :, cell] = value
+    out = case.run()
+    for b, j in ((0, 3), (1, 2)):
+        for i in range(case.nodes[b]):
+            row = out[int(case.starts[b]) + i]
+            if case.seen[b][i][j]:
+                assert not bool(torch.isfinite(row).all())
+            else:
+                assert bool(torch.isfinite(row).all())
+    clean = Tree([140, 50], [12, 9], 8, 2, D, seed=21).run()
+    for b, j in ((0, 3), (1, 2)):
+        for i in range(case.nodes[b]):
+            if not case.seen[b][i][j]:
+                assert torch.equal(out[int(case.starts[b]) + i], clean[int(case.starts[b]) + i])
+    case = Tree([140], [12], 8, 2, D, window=30, seed=22)
+    want = case.run()
+    first = int(case.positions[:12].max()) - 30  # the deepest node no longer sees it
+    page, cell = int(case.table[0, first // 64]), first % 64
+    case.dev["v_pool"][page, :, cell] = value
+    out = case.run()
+    for i in range(12):
+        if not bool(case.visible(0, i)[first]):
+            assert torch.equal(out[i], want[i])
+
+
+def test_tree_attention_large_scores():
+    """Scores of a few hundred: one weight is 1 and the others underflow."""
+    case = Tree([300, 40], [10, 70], 14, 2, 64, seed=9, scale=40.0)
+    case.check(case.run())
+
+
+def test_tree_attention_bad_lengths_pages_and_padding():
+    """Sequences without room for their rows give zeros, keys on a page outside
+    the pool are unseen, rows behind the last sequence stay."""
+    case = Tree([200, 30, 100], [6, 5, 4], 14, 2, 64, seed=11, extra_rows=9)
+    case.dev["seq_lens"][1] = 3
+    out = torch.full_like(case.dev["q"], 5.0)
+    got = case.run(out=out)
+    assert got is out
+    assert bool((out[6:11] == 0).all()) and bool((out[15:] == 5.0).all())
+    case.nodes, starts = [6, 0, 4], case.starts
+    case.check(out)
+    case.dev["page_table"][0, 1] = 10 ** 6
+    case.dev["page_table"][0, 2] = -3
+    out = case.run()
+    seen = case.visible(0, 2)
+    seen[64:192] = False
+    for h in range(14):
+        want, tol = V.tree_row(case.q[2, h].double(), case.k[0][:, h // 7], case.v[0][:, h // 7], seen)
+        assert bool(((out[2, h].cpu().double() - want).abs() <= tol).all())
+    assert list(starts) == [0, 6, 11, 15]
+
+
+def test_tree_attention_mask_words_cut_later_nodes():
+    case = Tree([50], [100], 4, 4, 64, words=1, seed=12)
+    case.check(case.run())
+
+
+def test_tree_attention_strided_q_and_table_wider_than_needed():
+    case = Tree([500, 77], [20, 30], 14, 2, 64, seed=13, width=40)
+    wide = torch.zeros(case.rows, 18, 64, dtype=torch.bfloat16, device="cuda")
+    wide[:, :14] = case.dev["q"]
+    case.check(case.run(q=wide[:, :14]))
+
+
+def test_tree_attention_repeats_bit_for_bit():
+    case = Tree([3000, 17, 900], [30, 64, 5], 28, 4, 128, seed=14)
+    a = case.run()
+    for _ in range(3):
+        assert torch.equal(a, case.run())
+
+
+def test_tree_attention_single_nodes_match_decode_attention():
+    """One node that sees itself is the decode attention of its position."""
+    from cheetah_b200 import runtime as R
+    case = Tree([700, 63, 2000], [1, 1, 1], 14, 2, 64, seed=15, fill=0.0)
+    d = case.dev
+    want = R.decode_attention(d["q"].float(), d["k_pool"], d["v_pool"], d["page_table"], d["seq_lens"], 2001)
+    assert (case.run().float() - want).abs().max().item() < 1e-2  # the decode kernel's own contract
+
+
+def test_tree_attention_on_other_streams_and_in_graphs():
+    """Calls that overlap: two streams, and two captured graphs replayed on
+    two streams, each with its own workspace."""
+    cases = [Tree([4000, 100], [20, 64], 14, 2, 64, seed=s) for s in (31, 32)]
+    want = [c.run() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [c.run(stream=s) for _ in range(8) for c, s in zip(cases, streams)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2])
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(c.run())
+        graphs.append(g)
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
+# ---- token_logprobs -----------------------------------------------------------
+
+def _check_logprobs(x, tokens, top, dtype):
+    from cheetah_b200 import runtime as R
+    x = x.to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+    got = R.token_logprobs(x if x.is_cuda else x.cuda(), i32(tokens), top=top)
+    rows = x.cpu()
+    for r, token in enumerate(tokens):
+        ref = V.logprobs_row(rows[r], token, top)
+        lp, h, rank = float(got.logprob[r]), float(got.entropy[r]), int(got.rank[r])
+        ids, lps = got.top_ids[r].tolist(), got.top_logprobs[r].cpu().double()
+        if ref["bad"]:
+            assert math.isnan(lp) and math.isnan(h) and rank == 0 and ids == [-1] * top and bool(torch.isnan(lps).all())
+            continue
+        assert ids == ref["top_ids"], f"row {r}"
+        for a, b in zip(lps.tolist(), ref["top_logprobs"].tolist()):
+            assert a == b or abs(a - b) <= V.tol_logprob(ref, b), f"row {r}: {a} vs {b}"
+        assert abs(h - ref["entropy"]) <= ref["tol_entropy"], f"row {r}: entropy {h} vs {ref['entropy']}"
+        if not ref["known"]:
+            assert math.isnan(lp) and rank == 0
+            continue
+        assert rank == ref["rank"]
+        assert lp == ref["logprob"] or abs(lp - ref["logprob"]) <= V.tol_logprob(ref, ref["logprob"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 2, 0), (3, 7, 7), (5, 33, 32), (2, 1000, 5), (4, 4096, 20), (7, 32001, 32),
+                                            (1, 151936, 20), (3, 152064, 5), (40, 20011, 1), (300, 5003, 3)])
+def test_token_logprobs(dtype, rows, vocab, top):
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = torch.randn(rows, vocab, generator=g) * 3.0
+    tokens = torch.randint(0, vocab, (rows,), generator=g).tolist()
+    _check_logprobs(x, tokens, top, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [100, 5000, 40000])
+def test_token_logprobs_orders_that_fill_every_buffer(dtype, vocab):
+    """Ascending, descending, all equal, two values, signed zeros: the
+    alternatives stay exact whatever order the values come in."""
+    up = torch.linspace(-5, 5, vocab)
+    equal = torch.full((vocab,), 0.25)
+    two = torch.where(torch.arange(vocab) % 3 == 1, 2.0, -1.0)
+    zeros = torch.where(torch.arange(vocab) % 2 == 1, 0.0, -0.0)
+    late = torch.cat([torch.full((vocab - 40,), -3.0), torch.linspace(0, 1, 40)])
+    x = torch.stack([up, up.flip(0), equal, two, zeros, late])
+    _check_logprobs(x, [vocab - 1, 0, vocab // 2, 1, 5, vocab - 2], 32, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_token_logprobs_masked_and_broken_rows(dtype):
+    """-inf logits have probability 0; NaN, +inf and all -inf rows are refused
+    row by row; tokens outside the vocabulary give NaN."""
+    vocab = 3001
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(10, vocab, generator=g)
+    x[0, ::2] = -math.inf
+    x[1, 3:] = -math.inf                     # fewer than `top` above -inf
+    x[2, :] = -math.inf
+    x[3, 17] = math.nan
+    x[4, vocab - 1] = math.inf
+    x[5, :] = torch.finfo(torch.bfloat16).min  # the type's lowest value throughout
+    x[6, 1:] = torch.finfo(torch.bfloat16).min
+    x[7] *= 1e30
+    _check_logprobs(x, [0, 5, 1, 2, 3, 4, 0, 7, -1, vocab], 8, dtype)
+
+
+def test_token_logprobs_strided_unaligned_rows():
+    g = torch.Generator().manual_seed(4)
+    for dtype in ("f32", "bf16"):
+        base = torch.randn(9, 5011, generator=g).to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype]).cuda()
+        _check_logprobs(base[:, 3:4998], list(range(9)), 5, dtype)
+        _check_logprobs(base[::2, 1:], list(range(5)), 5, dtype)
+
+
+def test_token_logprobs_captured():
+    from cheetah_b200 import runtime as R
+    x = torch.randn(6, 30000, device="cuda")
+    t = i32(range(6))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = R.token_logprobs(x, t, top=4)
+    x.copy_(torch.randn(6, 30000, device="cuda") * 2)
+    g.replay()
+    want = R.token_logprobs(x, t, top=4)
+    for a, b in zip(out, want):
+        assert torch.equal(a, b)
+
+
+# ---- the four together ----------------------------------------------------------
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("q_heads,kv_heads,D", [(14, 2, 64), (8, 4, 128)])
+def test_verification_step(q_heads, kv_heads, D, captured):
+    """Slots, append, attention and log probabilities of one step over caches
+    that an earlier step of the same operators filled; rows padded to a fixed
+    count, one sequence without new rows and one that finds no pages."""
+    from cheetah_b200 import runtime as R
+    g = torch.Generator().manual_seed(D)
+    rng = np.random.default_rng(D)
+    pt, width, rows, vocab, B = 16, 24, 64, 1003, 4
+    ctx, nodes = [130, 77, 33, 20], [12, 0, 21, 60]
+    heads = q_heads + 2 * kv_heads
+    num_pages = 1 + sum(-(-c // pt) for c in ctx) + 3
+    free = i32(rng.permutation(num_pages)[:num_pages - 1])
+    table = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    k_pool = torch.full((num_pages, kv_heads, pt, D), math.nan, dtype=torch.bfloat16, device="cuda")
+    v_pool = k_pool.clone()
+    angle = torch.rand(400, D // 2, generator=g) * 6.0
+    cos, sin = angle.cos().cuda(), angle.sin().cuda()
+    w = [(1.0 + 0.2 * torch.randn(D, generator=g)).cuda() for _ in range(2)]
+
+    def step(cached, new, free, count, x, mask, head, tokens, positions=None):
+        s = R.page_slots(cached, new, free, count, table, num_pages, pt, x.shape[0])
+        pos = s.positions if positions is None else torch.where(s.positions >= 0, positions, -1)
+        q = R.qk_norm_rope(x, q_heads, kv_heads, pos, s.slots, cos, sin, k_pool, v_pool, q_norm=w[0], k_norm=w[1])
+        o = R.tree_attention(q, k_pool, v_pool, table, s.seq_lens, s.row_starts, mask, positions=pos,
+                             out=torch.zeros_like(q))
+        return s, q, o, R.token_logprobs(o.float().reshape(x.shape[0], -1) @ head, tokens, top=3)
+
+    # The prompts, as chains.
+    total = sum(ctx)
+    prompt = torch.randn(total, heads, D, generator=g).bfloat16()
+    chain = np.concatenate([np.tril(np.ones((c, 192), bool)) for c in ctx])
+    chain = V.pack_bits(chain, 3)
+    head = torch.randn(q_heads * D, vocab, generator=g).cuda()
+    first = step(i32([0] * B), i32(ctx), free, i32([free.numel()]), prompt.cuda(), torch.from_numpy(chain).cuda(), head,
+                 i32(rng.integers(0, vocab, total)))
+    used = int(first[0].counts[1])
+    assert first[0].counts.tolist() == [total, sum(-(-c // pt) for c in ctx), 0]
+    # The drafted trees; the last sequence needs more pages than are left.
+    x = torch.randn(rows + 40, heads, D, generator=g).bfloat16()
+    trees = [V.tree_bits(V.random_tree(rng, n)) for n in nodes]
+    mask = np.zeros((rows + 40, 1), np.int64)
+    mask[:sum(nodes)] = np.concatenate([V.pack_bits(t[0], 1) for t in trees if len(t[0])])
+    depth = np.full(rows + 40, -1)
+    depth[:sum(nodes)] = np.concatenate([t[1] + c for t, c in zip(trees, ctx)])
+    tokens = rng.integers(0, vocab, rows + 40)
+    args = (i32(ctx), i32(nodes), free[used:].contiguous(), i32([free.numel() - used]), x.cuda(), torch.from_numpy(mask).cuda(),
+            head, i32(tokens), i32(depth))
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s, q, o, lp = step(*args)
+        graph.replay()
+    else:
+        s, q, o, lp = step(*args)
+    torch.cuda.synchronize()
+    assert s.counts.tolist()[2] == 1 and s.seq_lens.tolist() == [142, 77, 54, 0]
+    at = np.concatenate([[0], np.cumsum(nodes)])
+    # K/V in the pool are what the rows give (checked above); attention over them.
+    kc, vc, tab = k_pool.cpu().double(), v_pool.cpu().double(), table.cpu().numpy()
+    ocpu = o.cpu().double()
+    for b in (0, 2):
+        pages = tab[b, :-(-(ctx[b] + nodes[b]) // pt)].astype(np.int64)
+        n = ctx[b] + nodes[b]
+        kd = kc[pages].transpose(1, 2).reshape(-1, kv_heads, D)[:n]
+        vd = vc[pages].transpose(1, 2).reshape(-1, kv_heads, D)[:n]
+        assert bool(torch.isfinite(kd).all())
+        for i in (0, nodes[b] // 2, nodes[b] - 1):
+            seen = torch.from_numpy(np.concatenate([np.ones(ctx[b], bool), trees[b][0][i]]))
+            for h in range(q_heads):
+                kvh = h * kv_heads // q_heads
+                want, tol = V.tree_row(q[at[b] + i, h].cpu().double(), kd[:, kvh], vd[:, kvh], seen)
+                assert bool(((ocpu[at[b] + i, h] - want).abs() <= tol).all())
+    assert bool((ocpu[at[3]:] == 0).all())  # refused, and the padding as it was
+    logits = o.float().reshape(rows + 40, -1) @ head
+    again = R.token_logprobs(logits, i32(tokens), top=3)
+    assert torch.equal(again.top_ids[:at[3]], lp.top_ids[:at[3]])
+    for r in (0, 5, int(at[2]) + 3):
+        ref = V.logprobs_row(logits[r].cpu(), int(tokens[r]), 3)
+        assert abs(float(lp.logprob[r]) - ref["logprob"]) <= V.tol_logprob(ref, ref["logprob"])
