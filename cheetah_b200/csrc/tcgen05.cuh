@@ -32,6 +32,17 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t a, uint64_t 
         : "memory");
 }
 
+// A from TMEM (row = lane, two bf16 of consecutive k per column), B from shared memory.
+__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -82,11 +93,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
 }
 
 // MN-major operand with 128-byte swizzle (rows of 128 B along N, 8-row atoms
-// along K, SBO = 1024 B between K atoms); one 64-element atom along N.
-__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr) {
+// along K, SBO = 1024 B between K atoms); one 64-element atom along N, or
+// several that lie `atom_stride` bytes apart.
+__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr, uint32_t atom_stride = 16) {
     uint64_t desc = 0;
     desc |= (uint64_t)((addr >> 4) & 0x3FFF);
-    desc |= (uint64_t)1 << 16;
+    desc |= (uint64_t)(atom_stride >> 4) << 16;
     desc |= (uint64_t)(1024 >> 4) << 32;
     desc |= (uint64_t)1 << 46;
     desc |= (uint64_t)2 << 61;
@@ -108,6 +120,19 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, float *v) {
 }
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 32 columns of packed 32-bit words, without the wait.
+__device__ __forceinline__ void tmem_st32_nowait(uint32_t taddr, const uint32_t *w) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]),
+        "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15]), "r"(w[16]), "r"(w[17]), "r"(w[18]),
+        "r"(w[19]), "r"(w[20]), "r"(w[21]), "r"(w[22]), "r"(w[23]), "r"(w[24]), "r"(w[25]), "r"(w[26]), "r"(w[27]),
+        "r"(w[28]), "r"(w[29]), "r"(w[30]), "r"(w[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }

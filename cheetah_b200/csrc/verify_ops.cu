@@ -28,6 +28,64 @@ bool pool_in_range(uint32_t num_pages, uint32_t page_tokens) {
     return num_pages > 0 && page_tokens > 0 && (uint64_t)num_pages * page_tokens <= 0x7FFFFFFFull;
 }
 
+// 2D map over a bf16 pool viewed as [rows][head_dim]: 64-column boxes of
+// `box_rows` rows of one page, 128-byte swizzle.
+int make_pool_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t head_dim, uint32_t box_rows) {
+    auto encode = cheetah::tensor_map_encoder();
+    CH_REQUIRE(encode != nullptr, "CUDA backend: cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[2] = {head_dim, rows};
+    cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
+    cuuint32_t box[2] = {64u, box_rows};
+    cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CH_REQUIRE(r == CUDA_SUCCESS, "CUDA backend: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return 0;
+}
+
+// 3D map over q [rows][q_heads][head_dim]: boxes of 64 columns, the heads of
+// one KV group and the nodes of a Q tile. Rows past the end read as zero.
+int make_q_map(CUtensorMap *map, const CheetahCudaTreeAttention &a, uint32_t group, uint32_t tile_nodes) {
+    auto encode = cheetah::tensor_map_encoder();
+    CH_REQUIRE(encode != nullptr, "CUDA backend: cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[3] = {a.head_dim, a.q_heads, a.rows};
+    cuuint64_t strides[2] = {(cuuint64_t)a.head_dim * 2, (cuuint64_t)a.q_stride * 2};
+    cuuint32_t box[3] = {64u, group, tile_nodes};
+    cuuint32_t estr[3] = {1u, 1u, 1u};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(a.q), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CH_REQUIRE(r == CUDA_SUCCESS, "CUDA backend: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return 0;
+}
+
+// Workspace of a tree attention call on a GPU of `ctas` SMs.
+struct TreeWorkspace {
+    size_t splits, ml, o, bytes;
+};
+TreeWorkspace tree_workspace(int ctas, uint32_t head_dim) {
+    auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+    TreeWorkspace w;
+    w.splits = 0;
+    w.ml = up(ctas * sizeof(cheetah::TreeSplit));
+    w.o = w.ml + up((size_t)ctas * 512 * sizeof(float2));
+    w.bytes = w.o + (size_t)ctas * 512 * head_dim * sizeof(float);
+    return w;
+}
+
+template <int HD>
+int launch_tree_attention(const CUtensorMap &q_map, const CUtensorMap &k_map, const CUtensorMap &v_map,
+                          const cheetah::TreeAttnParams &p, int ctas, cudaStream_t stream) {
+    constexpr size_t smem = cheetah::tree_attention_smem<HD>();
+    CH_CUDA_TRY(cudaFuncSetAttribute(cheetah::tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CH_CUDA_TRY(launch_ex(cheetah::tree_attention_kernel<HD>, dim3(ctas), dim3(cheetah::kTreeThreads), smem, stream, true,
+                          q_map, k_map, v_map, p));
+    CH_CUDA_TRY(launch_ex(cheetah::tree_merge_kernel<HD>, dim3(ctas, cheetah::kTreeMergeSplit), dim3(cheetah::kTreeMergeThreads),
+                          0, stream, true, p));
+    return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -150,46 +208,68 @@ static int check_tree_attention(const CheetahCudaTreeAttention *a) {
 int cheetah_cuda_op_tree_attention_workspace(const CheetahCudaTreeAttention *a, size_t *bytes) {
     CH_REQUIRE(bytes != nullptr, "cheetah_cuda_op_tree_attention_workspace: null argument");
     if (check_tree_attention(a) != 0) return -1;
-    *bytes = 0;
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    *bytes = tree_workspace(cheetah::sm_count(device), a->head_dim).bytes;
     return 0;
 }
 
 int cheetah_cuda_op_tree_attention(const CheetahCudaTreeAttention *a, void *stream) {
     if (check_tree_attention(a) != 0) return -1;
-    CH_REQUIRE(a->q && a->k_pool && a->v_pool && a->page_table && a->seq_lens && a->row_starts && a->tree_mask && a->out,
+    CH_REQUIRE(a->q && a->k_pool && a->v_pool && a->page_table && a->seq_lens && a->row_starts && a->tree_mask && a->out &&
+                   a->workspace,
                "cheetah_cuda_op_tree_attention: null argument");
     CH_REQUIRE(a->sliding_window == 0 || a->positions != nullptr,
                "cheetah_cuda_op_tree_attention: a sliding window needs the rows' positions");
     CH_REQUIRE(a->q_stride >= (size_t)a->q_heads * a->head_dim && a->q_stride % 8 == 0 && a->q_stride < ((size_t)1 << 32),
                "cheetah_cuda_op_tree_attention: q rows must not overlap and must be 16-byte aligned");
     CH_REQUIRE(aligned(a->q, 16) && aligned(a->k_pool, 16) && aligned(a->v_pool, 16) && aligned(a->out, 16) &&
-                   aligned(a->tree_mask, 8),
-               "cheetah_cuda_op_tree_attention: q, out and the pools must be 16-byte aligned, the mask 8-byte");
+                   aligned(a->tree_mask, 8) && aligned(a->workspace, 256),
+               "cheetah_cuda_op_tree_attention: q, out and the pools must be 16-byte aligned, the mask 8-byte, the "
+               "workspace 256-byte");
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    const int ctas = cheetah::sm_count(device);
+    const TreeWorkspace w = tree_workspace(ctas, a->head_dim);
+    CH_REQUIRE(a->workspace_bytes >= w.bytes,
+               "cheetah_cuda_op_tree_attention: the workspace holds " + std::to_string(a->workspace_bytes) + " of " +
+                   std::to_string(w.bytes) + " bytes");
+    const uint32_t group = a->q_heads / a->kv_heads;
     cheetah::TreeAttnParams p = {};
-    p.q = static_cast<const uint16_t *>(a->q);
-    p.q_stride = (long long)a->q_stride;
-    p.rows = (int)a->rows;
-    p.k_pool = static_cast<const uint16_t *>(a->k_pool);
-    p.v_pool = static_cast<const uint16_t *>(a->v_pool);
     p.page_table = a->page_table;
     p.max_pages = (int)a->max_pages_per_seq;
     p.num_pages = (int)a->num_pages;
     p.page_tokens = (int)a->page_tokens;
+    p.box_keys = a->page_tokens % 64 == 0 ? 64 : (a->page_tokens % 32 == 0 ? 32 : 16);
     p.seq_lens = a->seq_lens;
     p.row_starts = a->row_starts;
     p.batch = (int)a->batch;
-    p.tree_mask = reinterpret_cast<const unsigned long long *>(a->tree_mask);
-    p.mask_words = (int)a->mask_words;
+    p.rows = (int)a->rows;
+    p.tree_mask = reinterpret_cast<const uint32_t *>(a->tree_mask);
+    p.mask_words32 = 2 * (int)a->mask_words;
     p.positions = a->positions;
     p.window = (int)a->sliding_window;
     p.q_heads = (int)a->q_heads;
     p.kv_heads = (int)a->kv_heads;
-    p.scale = 1.0f / sqrtf((float)a->head_dim);
+    p.group = (int)group;
+    p.tile_nodes = cheetah::kTreeRows / (int)group;
+    p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
+    p.v_pool = static_cast<const uint16_t *>(a->v_pool);
     p.out = static_cast<uint16_t *>(a->out);
-    auto kernel = a->head_dim == 64 ? cheetah::tree_attention_rows_kernel<64> : cheetah::tree_attention_rows_kernel<128>;
-    CH_CUDA_TRY(launch_ex(kernel, dim3(a->rows, a->q_heads), dim3(cheetah::kTreeKeys), 0,
-                          static_cast<cudaStream_t>(stream), true, p));
-    return 0;
+    uint8_t *ws = static_cast<uint8_t *>(a->workspace);
+    p.splits = reinterpret_cast<cheetah::TreeSplit *>(ws + w.splits);
+    p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
+    p.part_o = reinterpret_cast<float *>(ws + w.o);
+    CUtensorMap q_map, k_map, v_map;
+    const uint64_t rows = (uint64_t)a->num_pages * a->kv_heads * a->page_tokens;
+    if (make_q_map(&q_map, *a, group, (uint32_t)p.tile_nodes) != 0 ||
+        make_pool_map(&k_map, a->k_pool, rows, a->head_dim, (uint32_t)p.box_keys) != 0 ||
+        make_pool_map(&v_map, a->v_pool, rows, a->head_dim, (uint32_t)p.box_keys) != 0) {
+        return -1;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a->head_dim == 64 ? launch_tree_attention<64>(q_map, k_map, v_map, p, ctas, st)
+                             : launch_tree_attention<128>(q_map, k_map, v_map, p, ctas, st);
 }
 
 int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogprobs *a, void *stream) {

@@ -421,7 +421,8 @@ CHEETAH_CUDA_API int cheetah_cuda_op_qk_norm_rope(const CheetahCudaQkNormRope *a
  * tree_mask[row][j / 64] (its ancestors and itself, for a tree). With a
  * window, a key is seen only if its position is above positions[row] -
  * sliding_window, where a context key's position is its index and node j's is
- * positions[its row]. A row that sees nothing gives zeros, whatever it reads;
+ * positions[its row]; positions below the context's end count as its end. A
+ * row that sees nothing gives zeros, whatever it reads;
  * cells a row does not see never reach it, non-finite ones included. Rows
  * from row_starts[batch] on stay as they were; a sequence with seq_lens[b] <
  * n gives zeros, and keys on a page outside the pool count as unseen. q and
