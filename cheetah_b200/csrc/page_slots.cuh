@@ -51,6 +51,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long *warp_sum
     return warp > 0 ? v + before : v;
 }
 
+// VEC 4 needs 16-byte aligned per-row outputs.
+template <int VEC>
 __global__ void __launch_bounds__(kSlotThreads) page_slots_kernel(const PageSlotParams p) {
     // Per sequence: end of its rows, free-list index minus its first new
     // page's table column, and that column (-1: refused).
@@ -63,8 +65,7 @@ __global__ void __launch_bounds__(kSlotThreads) page_slots_kernel(const PageSlot
     pdl_launch_dependents();
     const int free_count = min(max(p.free_count[0], 0), p.free_capacity);
 
-    long long rows_before = 0, pages_before = 0, pages_taken = 0;
-    long long refused = 0;
+    long long rows_before = 0, pages_before = 0, tally = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kSlotThreads) {
         const int b = b0 + threadIdx.x;
         const bool real = b < p.batch;
@@ -81,10 +82,10 @@ __global__ void __launch_bounds__(kSlotThreads) page_slots_kernel(const PageSlot
         const long long page_end = pages_before + block_scan(need, warp_sums, total);
         pages_before += total;
         const bool got = ok && (need == 0 || page_end <= free_count);
-        block_scan(got ? need : 0, warp_sums, total);
-        pages_taken += total;
-        block_scan(real && !got ? 1 : 0, warp_sums, total);
-        refused += total;
+        if (blockIdx.x == 0) {  // pages taken (< 2^31) and sequences refused (< 2^15) in one sum
+            block_scan(((got ? need : 0) << 16) + (real && !got ? 1 : 0), warp_sums, total);
+            tally += total;
+        }
         if (real) {
             row_end[b] = (int)min(end, (long long)p.max_tokens);
             free_base[b] = got ? (int)(page_end - need - have) : 0;
@@ -98,37 +99,61 @@ __global__ void __launch_bounds__(kSlotThreads) page_slots_kernel(const PageSlot
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         p.row_starts[0] = 0;
         p.counts[0] = (int)min(rows_before, 0x7FFFFFFFll);
-        p.counts[1] = (int)pages_taken;
-        p.counts[2] = (int)refused;
+        p.counts[1] = (int)(tally >> 16);
+        p.counts[2] = (int)(tally & 0xFFFF);
     }
     __syncthreads();
 
-    // Rows: sequence by binary search of the row ends, page from the free list
-    // or from the part of the table that this launch leaves alone.
-    const int live_rows = p.batch > 0 ? row_end[p.batch - 1] : 0;
-    for (long long t = (long long)blockIdx.x * kSlotThreads + threadIdx.x; t < p.max_tokens;
-         t += (long long)gridDim.x * kSlotThreads) {
-        int pos = -1, seq = -1, slot = -1;
-        if (t < live_rows) {
-            int lo = 0, hi = p.batch - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (row_end[mid] > t) hi = mid;
-                else lo = mid + 1;
-            }
-            seq = lo;
-            const int fresh = first_new[lo];
-            if (fresh >= 0) {
-                pos = p.cached[lo] + (int)(t - (lo > 0 ? row_end[lo - 1] : 0));
-                const int col = pos / P;
-                const int page = col >= fresh ? p.free_pages[free_base[lo] + col]
-                                              : p.page_table[(long long)lo * p.max_pages + col];
-                if (page >= 0 && page < p.num_pages) slot = page * P + pos % P;
+    // Rows, VEC at a time: the first one's sequence by binary search of the row
+    // ends, the others' by stepping on; pages from the free list or from the
+    // part of the table that this launch leaves alone.
+    const int live_rows = row_end[p.batch - 1];
+    for (long long t0 = ((long long)blockIdx.x * kSlotThreads + threadIdx.x) * VEC; t0 < p.max_tokens;
+         t0 += (long long)gridDim.x * kSlotThreads * VEC) {
+        int pos[VEC], seq[VEC], slot[VEC];
+        int b = 0;
+        if (t0 < live_rows) {
+            int hi = p.batch - 1;
+            while (b < hi) {
+                const int mid = (b + hi) >> 1;
+                if (row_end[mid] > t0) hi = mid;
+                else b = mid + 1;
             }
         }
-        p.positions[t] = pos;
-        p.seq_ids[t] = seq;
-        p.slots[t] = slot;
+        int col_have = -1, page = -1;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const long long t = t0 + i;
+            pos[i] = seq[i] = slot[i] = -1;
+            if (t >= live_rows) continue;
+            while (row_end[b] <= t) {
+                ++b;
+                col_have = -1;
+            }
+            seq[i] = b;
+            const int fresh = first_new[b];
+            if (fresh < 0) continue;
+            pos[i] = p.cached[b] + (int)(t - (b > 0 ? row_end[b - 1] : 0));
+            const int col = pos[i] / P;
+            if (col != col_have) {
+                col_have = col;
+                page = col >= fresh ? p.free_pages[free_base[b] + col] : p.page_table[(long long)b * p.max_pages + col];
+            }
+            if (page >= 0 && page < p.num_pages) slot[i] = page * P + pos[i] - col * P;
+        }
+        if constexpr (VEC == 4) {
+            if (t0 + VEC <= p.max_tokens) {
+                *reinterpret_cast<int4 *>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+                *reinterpret_cast<int4 *>(p.seq_ids + t0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+                *reinterpret_cast<int4 *>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+                continue;
+            }
+        }
+        for (int i = 0; i < VEC && t0 + i < p.max_tokens; ++i) {
+            p.positions[t0 + i] = pos[i];
+            p.seq_ids[t0 + i] = seq[i];
+            p.slots[t0 + i] = slot[i];
+        }
     }
     // Table entries of the new pages, a warp per sequence.
     const int lane = threadIdx.x % kWarp;

@@ -4,12 +4,21 @@
 //   y = x * (1/sqrt(mean(x^2) + eps) * w)        (heads with a norm weight)
 //   (a, b) -> (a cos - b sin, b cos + a sin)      (pairs i, i + rotary/2)
 //
-// One warp per (row, head); f32 arithmetic, one rounding to the output type.
+// Bound by memory: every element is read and written once. A lane holds the
+// 16-byte chunk of a head's first half and the chunk of its second half that
+// it is rotated with, so the rotation needs no exchange and the norm only a
+// sum over the head's HD/2/VEC lanes; a warp takes several heads at a time and
+// walks over the heads of one row, whose cos/sin chunk and q weights it keeps
+// in registers. kQkUnroll heads' loads are issued before the first is used.
+// f32 arithmetic, one rounding to the output type.
 #pragma once
 
 #include "common.cuh"
 
 namespace cheetah {
+
+constexpr int kQkWarps = 4;
+constexpr int kQkUnroll = 3;
 
 struct QkNormRopeParams {
     const void *qkv;
@@ -19,69 +28,160 @@ struct QkNormRopeParams {
     const float *rope_cos, *rope_sin;
     int max_positions, rotary_dim;
     const int32_t *positions, *slots;
-    int tokens, q_heads, kv_heads, head_dim;
+    int tokens, q_heads, kv_heads;
     void *q_out, *k_pool, *v_pool;
     int num_pages, page_tokens;
+    int steps;      // head groups a warp takes
+    int row_units;  // warps per row
 };
 
-template <typename T>
-__device__ __forceinline__ float load_f32(const void *base, long long i) {
-    if constexpr (sizeof(T) == 2) return bf16_to_f32(static_cast<const uint16_t *>(base)[i]);
-    else return static_cast<const float *>(base)[i];
-}
-template <typename T>
-__device__ __forceinline__ void store_f32(void *base, long long i, float v) {
-    if constexpr (sizeof(T) == 2) static_cast<uint16_t *>(base)[i] = f32_to_bf16_rne(v);
-    else static_cast<float *>(base)[i] = v;
+template <int N>
+__device__ __forceinline__ void load_floats(const float *src, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const float4 f = __ldg(reinterpret_cast<const float4 *>(src) + i);
+        v[4 * i] = f.x;
+        v[4 * i + 1] = f.y;
+        v[4 * i + 2] = f.z;
+        v[4 * i + 3] = f.w;
+    }
 }
 
-template <typename TIN, typename TKV>
-__global__ void __launch_bounds__(128) qk_norm_rope_rows_kernel(const QkNormRopeParams p) {
-    const int heads = p.q_heads + 2 * p.kv_heads;
+// VEC elements of a 16-byte chunk as f32.
+template <typename T, int VEC>
+__device__ __forceinline__ void widen_chunk(const uint4 &raw, float (&v)[VEC]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            v[2 * i] = bf16_lo(w[i]);
+            v[2 * i + 1] = bf16_hi(w[i]);
+        } else {
+            v[i] = __uint_as_float(w[i]);
+        }
+    }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_chunk(void *base, long long at, const float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t w[VEC / 2];
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+        uint16_t *dst = static_cast<uint16_t *>(base) + at;
+        if constexpr (VEC == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    } else {
+        float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(base) + at);
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+}
+
+template <typename TIN, typename TKV, int HD>
+__global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(const QkNormRopeParams p) {
+    constexpr int VEC = 16 / sizeof(TIN);
+    constexpr int kLanes = HD / 2 / VEC;        // lanes of a head
+    constexpr int kHeads = kWarp / kLanes;      // heads a warp takes at a time
     const int lane = threadIdx.x % kWarp;
-    const long long item = (long long)blockIdx.x * 4 + threadIdx.x / kWarp;
+    const int c = lane % kLanes, sub = lane / kLanes;
+    const long long unit = (long long)blockIdx.x * kQkWarps + threadIdx.x / kWarp;
+    const int t = (int)(unit / p.row_units);
+    const int step0 = (int)(unit % p.row_units) * p.steps;
+    const int heads = p.q_heads + 2 * p.kv_heads;
+    const int half = p.rotary_dim / 2;
+    // This lane's two chunks of a head: rotated against each other, or the
+    // halves of the part that passes through.
+    const bool turned = c * VEC < half;
+    const int rest = c * VEC - half;
+    const int da = turned ? c * VEC : 2 * half + rest;
+    const int db = turned ? half + c * VEC : 2 * half + (HD - 2 * half) / 2 + rest;
     pdl_wait();
     pdl_launch_dependents();
-    if (item >= (long long)p.tokens * heads) return;
-    const int t = (int)(item / heads), head = (int)(item % heads);
+    if (t >= p.tokens) return;
+    float wa[VEC], wb[VEC];
+    if (p.q_norm) {
+        load_floats(p.q_norm + da, wa);
+        load_floats(p.q_norm + db, wb);
+    }
     const int pos = p.positions[t];
     if (pos < 0 || pos >= p.max_positions) return;
-    const int hd = p.head_dim, half = p.rotary_dim / 2;
-    const bool is_q = head < p.q_heads;
-    const bool is_k = !is_q && head < p.q_heads + p.kv_heads;
-    const float *w = is_q ? p.q_norm : (is_k ? p.k_norm : nullptr);
-    const long long src = t * p.qkv_stride + (long long)head * hd;
-    float inv = 1.0f;
-    if (w) {
-        float ss = 0.0f;
-        for (int d = lane; d < hd; d += kWarp) {
-            const float x = load_f32<TIN>(p.qkv, src + d);
-            ss = fmaf(x, x, ss);
-        }
-        inv = 1.0f / sqrtf(warp_sum(ss) / (float)hd + p.eps);
+    const int slot = p.slots[t];
+    const int page = slot / p.page_tokens;
+    const bool cell_ok = slot >= 0 && page < p.num_pages;
+    float cs[VEC], sn[VEC];
+    if (turned) {
+        load_floats(p.rope_cos + (long long)pos * half + da, cs);
+        load_floats(p.rope_sin + (long long)pos * half + da, sn);
     }
-    long long dst;
-    if (is_q) {
-        dst = ((long long)t * p.q_heads + head) * hd;
-    } else {
-        const int slot = p.slots[t];
-        if (slot < 0 || slot / p.page_tokens >= p.num_pages) return;
-        const int kvh = is_k ? head - p.q_heads : head - p.q_heads - p.kv_heads;
-        dst = (((long long)(slot / p.page_tokens) * p.kv_heads + kvh) * p.page_tokens + slot % p.page_tokens) * hd;
-    }
-    for (int d = lane; d < hd; d += kWarp) {
-        float x = load_f32<TIN>(p.qkv, src + d);
-        if (w) x *= inv * w[d];
-        if ((is_q || is_k) && d < 2 * half) {
-            const int i = d < half ? d : d - half;
-            const int other = d < half ? d + half : d - half;
-            float y = load_f32<TIN>(p.qkv, src + other);
-            if (w) y *= inv * w[other];
-            const float c = p.rope_cos[(long long)pos * half + i], s = p.rope_sin[(long long)pos * half + i];
-            x = d < half ? x * c - y * s : x * c + y * s;
+    const TIN *row = static_cast<const TIN *>(p.qkv) + t * p.qkv_stride;
+    const int steps = (heads + kHeads - 1) / kHeads;
+    const int step1 = min(steps, step0 + p.steps);
+    for (int s0 = step0; s0 < step1; s0 += kQkUnroll) {
+        uint4 raw[kQkUnroll][2];
+#pragma unroll
+        for (int u = 0; u < kQkUnroll; ++u) {
+            const int head = (s0 + u) * kHeads + sub;
+            raw[u][0] = raw[u][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (s0 + u < step1 && head < heads) {
+                raw[u][0] = __ldcs(reinterpret_cast<const uint4 *>(row + (long long)head * HD + da));
+                raw[u][1] = __ldcs(reinterpret_cast<const uint4 *>(row + (long long)head * HD + db));
+            }
         }
-        if (is_q) store_f32<TIN>(p.q_out, dst + d, x);
-        else store_f32<TKV>(is_k ? p.k_pool : p.v_pool, dst + d, x);
+#pragma unroll
+        for (int u = 0; u < kQkUnroll; ++u) {
+            if (s0 + u >= step1) break;
+            const int head = (s0 + u) * kHeads + sub;
+            const bool is_q = head < p.q_heads;
+            const bool is_k = !is_q && head < p.q_heads + p.kv_heads;
+            float a[VEC], b[VEC];
+            widen_chunk<TIN>(raw[u][0], a);
+            widen_chunk<TIN>(raw[u][1], b);
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+            if (head >= heads) continue;
+            if (is_q ? p.q_norm != nullptr : is_k && p.k_norm != nullptr) {
+                const float inv = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
+                if (is_q) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        a[i] *= inv * wa[i];
+                        b[i] *= inv * wb[i];
+                    }
+                } else {
+                    float ka[VEC], kb[VEC];
+                    load_floats(p.k_norm + da, ka);
+                    load_floats(p.k_norm + db, kb);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        a[i] *= inv * ka[i];
+                        b[i] *= inv * kb[i];
+                    }
+                }
+            }
+            if ((is_q || is_k) && turned) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float x = a[i];
+                    a[i] = x * cs[i] - b[i] * sn[i];
+                    b[i] = b[i] * cs[i] + x * sn[i];
+                }
+            }
+            if (is_q) {
+                const long long at = ((long long)t * p.q_heads + head) * HD;
+                store_chunk<TIN>(p.q_out, at + da, a);
+                store_chunk<TIN>(p.q_out, at + db, b);
+            } else if (cell_ok) {
+                const int kvh = is_k ? head - p.q_heads : head - p.q_heads - p.kv_heads;
+                const long long at = (((long long)page * p.kv_heads + kvh) * p.page_tokens + (slot - page * p.page_tokens)) * HD;
+                void *pool = is_k ? p.k_pool : p.v_pool;
+                store_chunk<TKV>(pool, at + da, a);
+                store_chunk<TKV>(pool, at + db, b);
+            }
+        }
     }
 }
 

@@ -1,19 +1,40 @@
 // Log probability of a given token, its rank, the entropy and the likeliest
-// tokens of each row of logits.
+// tokens of each row of logits, in one pass over the row.
 //
 //   S = sum exp(x - m),  lse = m + log S,  log p_t = x_t - lse
 //   H = log S + sum (m - x) exp(x - m) / S   (both terms >= 0: no cancellation)
 //
-// One CTA per row: a pass for the maximum, a pass for the sums, a pass per
-// alternative.
+// with a running maximum per thread: moving m to m' multiplies S by f =
+// exp(m - m') and G = sum (x - m) exp(x - m) becomes f (G + (m - m') S).
+//
+// Bound by memory where rows are many, by latency where they are few: a row
+// is split over a cluster of 1..16 CTAs that join their results in the first
+// one's shared memory, so a call is one launch and needs no workspace.
+//
+// Alternatives. Each (warp, j) pair owns a contiguous run of 512-byte lines
+// of the CTA's part and one iteration reads the next line of every run, so
+// the first iteration samples the whole part. The `top`-th best of the
+// threads' first maxima is a lower bound of the part's `top`-th best value;
+// elements at or above it (about top * part / sample of them) go to a buffer,
+// from which each warp sorts its share in registers and the warps' lists are
+// merged pairwise. Where they do not fit (an adversarial order), the exact
+// `top`-th key is found by a radix selection over the part instead, in 8 more
+// passes.
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "common.cuh"
 
 namespace cheetah {
 
 constexpr int kLpThreads = 512;
+constexpr int kLpWarps = kLpThreads / kWarp;
 constexpr int kLpMaxTop = 32;
+constexpr int kLpMaxCluster = 16;
+constexpr int kLpLoads = 4;        // 16-byte loads in flight per thread
+constexpr int kLpBuffer = 1024;    // candidates of a CTA
+constexpr float kLpFloor = -1.0e4f;  // exp of it is 0; keeps (x - m) * 0 finite
 
 struct LogprobParams {
     const void *logits;
@@ -28,91 +49,351 @@ struct LogprobParams {
     float *top_logprobs;
 };
 
-template <typename T>
-__device__ __forceinline__ float logit_at(const void *row, int i) {
-    if constexpr (sizeof(T) == 2) return bf16_to_f32(static_cast<const uint16_t *>(row)[i]);
-    else return static_cast<const float *>(row)[i];
-}
+using TopKey = unsigned long long;
 
 // Order of the alternatives: larger value first, then the lower id, as one
 // integer key (larger is better; 0 is none).
-__device__ __forceinline__ unsigned long long top_key(float value, int id) {
+__device__ __forceinline__ TopKey top_key(float value, int id) {
     if (value == 0.0f) value = 0.0f;  // -0 and +0 are equal logits
-    return ((unsigned long long)total_order_key(value) << 32) | (uint32_t)~id;
+    return ((TopKey)total_order_key(value) << 32) | (uint32_t)~id;
 }
-__device__ __forceinline__ float top_key_value(unsigned long long key) {
+__device__ __forceinline__ float top_key_value(TopKey key) {
     const uint32_t k = (uint32_t)(key >> 32);
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
-template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, V *scratch, F f) {
-    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    __syncthreads();
-    if (lane == 0) scratch[warp] = v;
-    __syncthreads();
-    V r = scratch[0];
-    for (int w = 1; w < kLpThreads / kWarp; ++w) r = f(r, scratch[w]);
+// max(a, b), NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const LogprobParams p) {
-    __shared__ float f_scratch[kLpThreads / kWarp];
-    __shared__ int i_scratch[kLpThreads / kWarp];
-    __shared__ unsigned long long k_scratch[kLpThreads / kWarp];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int r = blockIdx.x;
-    const void *row = static_cast<const T *>(p.logits) + r * p.row_stride;
-    float m = -INFINITY;
-    int bad = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
-        const float x = logit_at<T>(row, i);
-        bad |= !(x < INFINITY);
-        m = fmaxf(m, x);
+// Running sums of a row part about the maximum m. A NaN or +inf logit makes s
+// NaN; a part without a logit above -inf has s = 0.
+struct RowSums {
+    float m, s, gap;
+
+    __device__ __forceinline__ void init() {
+        m = -3.402823466e38f;
+        s = gap = 0.0f;
     }
-    m = block_reduce(m, f_scratch, [](float a, float b) { return fmaxf(a, b); });
-    bad = block_reduce(bad, i_scratch, [](int a, int b) { return a | b; });
-    bad |= m == -INFINITY;
-    const int token = p.tokens[r];
-    const bool known = token >= 0 && token < p.vocab;
-    const float chosen = known && !bad ? logit_at<T>(row, token) : __int_as_float(0x7FC00000);
-    float s = 0.0f, gap = 0.0f;
-    int above = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
-        const float x = logit_at<T>(row, i);
-        const float e = expf(x - m);
+    __device__ __forceinline__ void raise(float to) {
+        const float d = max_nan(m - to, kLpFloor);
+        const float f = fast_exp2(d * 1.4426950408889634f);
+        gap = f * fmaf(d, s, gap);
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ void add(float x) {
+        const float d = max_nan(x - m, kLpFloor);
+        const float e = fast_exp2(d * 1.4426950408889634f);
         s += e;
-        gap += e > 0.0f ? (m - x) * e : 0.0f;
-        above += x > chosen;
+        gap = fmaf(d, e, gap);
     }
-    s = block_reduce(s, f_scratch, [](float a, float b) { return a + b; });
-    gap = block_reduce(gap, f_scratch, [](float a, float b) { return a + b; });
-    above = block_reduce(above, i_scratch, [](int a, int b) { return a + b; });
-    const float nan = __int_as_float(0x7FC00000);
-    const float log_s = logf(s);
-    if (threadIdx.x == 0) {
-        p.logprob[r] = bad || !known ? nan : (chosen - m) - log_s;
-        if (p.rank) p.rank[r] = bad || !known ? 0 : 1 + above;
-        if (p.entropy) p.entropy[r] = bad ? nan : log_s + gap / s;
+    __device__ __forceinline__ void join(const RowSums &o) {
+        RowSums other = o;
+        const float to = fmaxf(m, o.m);
+        raise(to);
+        other.raise(to);
+        s += other.s;
+        gap += other.gap;
     }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-        unsigned long long best = 0ull;
-        if (!bad) {
-            for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
-                const unsigned long long key = top_key(logit_at<T>(row, i), i);
-                if (key < last && key > best) best = key;
+};
+
+template <typename T>
+struct LogitVec {
+    static constexpr int N = 16 / sizeof(T);
+    static __device__ __forceinline__ void widen(const uint4 &raw, float *v) {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                v[2 * i] = bf16_lo(w[i]);
+                v[2 * i + 1] = bf16_hi(w[i]);
+            } else {
+                v[i] = __uint_as_float(w[i]);
             }
         }
-        best = block_reduce(best, k_scratch, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-        last = best;
-        if (threadIdx.x == 0) {
-            p.top_ids[(long long)r * p.top + k] = bad ? -1 : (int)~(uint32_t)best;
-            p.top_logprobs[(long long)r * p.top + k] = bad ? nan : (top_key_value(best) - m) - log_s;
+    }
+    static __device__ __forceinline__ float one(const T *row, long long i) {
+        if constexpr (sizeof(T) == 2) return bf16_to_f32(reinterpret_cast<const uint16_t *>(row)[i]);
+        else return row[i];
+    }
+};
+
+struct LogprobShared {
+    TopKey buffer[kLpBuffer];
+    TopKey lists[kLpWarps][kWarp];            // sorted lists on their way to one
+    TopKey joined[kLpMaxCluster][kWarp];      // first CTA: every part's best
+    float4 part[kLpMaxCluster];               // first CTA: m, s, gap, rank count bits
+    float4 warp_part[kLpWarps];
+    TopKey prefix;
+    int histogram[256];
+    int count, need;
+};
+static_assert(kLpMaxTop <= kWarp && kLpMaxCluster <= kLpWarps, "a list is one key per lane, merged by a warp each");
+
+// Bitonic steps over the warp's lanes; the best key ends in lane 0.
+__device__ __forceinline__ TopKey lane_exchange(TopKey k, int stride, bool best_low) {
+    const TopKey other = __shfl_xor_sync(0xFFFFFFFFu, k, stride);
+    const bool low = (threadIdx.x & stride) == 0;
+    return (low == best_low) == (k > other) ? k : other;
+}
+__device__ __forceinline__ TopKey warp_sort(TopKey k) {
+#pragma unroll
+    for (int size = 2; size <= kWarp; size <<= 1) {
+#pragma unroll
+        for (int stride = size / 2; stride > 0; stride >>= 1) k = lane_exchange(k, stride, (threadIdx.x & size & (kWarp - 1)) == 0);
+    }
+    return k;
+}
+// The best 32 of two sorted lists, sorted.
+__device__ __forceinline__ TopKey warp_merge(TopKey a, TopKey b) {
+    const TopKey back = __shfl_sync(0xFFFFFFFFu, b, (kWarp - 1) - (threadIdx.x & (kWarp - 1)));
+    TopKey k = a > back ? a : back;
+#pragma unroll
+    for (int stride = kWarp / 2; stride > 0; stride >>= 1) k = lane_exchange(k, stride, true);
+    return k;
+}
+// Merges lists[0..n) (n a power of two) into lists[0]. Every thread of the
+// block calls it, the lists' writers before a barrier of this function's.
+__device__ __forceinline__ void merge_lists(TopKey (*lists)[kWarp], int n) {
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    __syncthreads();
+    for (int half = n / 2; half > 0; half >>= 1) {
+        if (warp < half) lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + half][lane]);
+        __syncthreads();
+    }
+}
+// The best 32 of keys[0..n), sorted, to lists[0].
+__device__ __forceinline__ void pick_best(const TopKey *keys, int n, TopKey (*lists)[kWarp]) {
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    TopKey mine = 0ull;
+    for (int i = warp * kWarp; i < n; i += kLpThreads) {
+        const TopKey k = warp_sort(i + lane < n ? keys[i + lane] : 0ull);
+        mine = i < kLpThreads ? k : warp_merge(mine, k);
+    }
+    lists[warp][lane] = mine;
+    merge_lists(lists, kLpWarps);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogprobParams p) {
+    namespace cg = cooperative_groups;
+    using V = LogitVec<T>;
+    constexpr int N = V::N;
+    __shared__ LogprobShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int r = blockIdx.x / parts;
+    const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+    if (tid == 0) sh.count = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    const T *row = static_cast<const T *>(p.logits) + r * p.row_stride;
+    // Elements before the first 16-byte boundary, whole vectors, the rest.
+    const int head = min(p.vocab, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
+    const int vecs = (p.vocab - head) / N;
+    const int tail0 = head + vecs * N;
+    const uint4 *vec = reinterpret_cast<const uint4 *>(row + head);
+    const int v0 = (int)((long long)vecs * rank / parts), v1 = (int)((long long)vecs * (rank + 1) / parts);
+    const int lines = (v1 - v0 + kWarp - 1) / kWarp;
+    const int run = (lines + kLpWarps * kLpLoads - 1) / (kLpWarps * kLpLoads);
+    // Vector of load j in iteration it (>= v1: none).
+    auto vector_at = [&](int it, int j) -> int { return v0 + ((warp * kLpLoads + j) * run + it) * kWarp + lane; };
+    // The odd elements at the row's ends: one each for a few threads of the first CTA.
+    int odd = -1;
+    if (rank == 0) {
+        if (tid < head) odd = tid;
+        else if (tid - head < p.vocab - tail0) odd = tail0 + tid - head;
+    }
+
+    const int token = p.tokens[r];
+    const bool known = token >= 0 && token < p.vocab;
+    const float chosen = known ? V::one(row, token) : INFINITY;
+
+    RowSums sums;
+    sums.init();
+    int above = 0;
+    float tau = INFINITY;
+    TopKey tau_key = ~0ull;
+    auto push = [&](float x, int id) {
+        const TopKey key = top_key(x, id);
+        if (key < tau_key) return;
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kLpBuffer) sh.buffer[at] = key;
+    };
+    auto consume = [&](const uint4 (&raw)[kLpLoads], int it) {
+#pragma unroll
+        for (int j = 0; j < kLpLoads; ++j) {
+            const int v = vector_at(it, j);
+            if (v >= v1) break;
+            float x[N];
+            V::widen(raw[j], x);
+            float mx = x[0];
+#pragma unroll
+            for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+            if (mx > sums.m) sums.raise(mx);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sums.add(x[i]);
+                above += x[i] > chosen;
+            }
+            if (mx >= tau) {
+                for (int i = 0; i < N; ++i) {
+                    if (x[i] >= tau) push(x[i], head + v * N + i);
+                }
+            }
+        }
+    };
+    auto load = [&](uint4 (&raw)[kLpLoads], int it) {
+#pragma unroll
+        for (int j = 0; j < kLpLoads; ++j) {
+            const int v = vector_at(it, j);
+            if (it < run && v < v1) raw[j] = __ldcs(vec + v);
+        }
+    };
+    uint4 raw[kLpLoads];
+    load(raw, 0);
+    if (p.top > 0) {
+        TopKey mine = odd >= 0 ? top_key(V::one(row, odd), odd) : 0ull;
+#pragma unroll
+        for (int j = 0; j < kLpLoads; ++j) {
+            const int v = vector_at(0, j);
+            if (run == 0 || v >= v1) break;
+            float x[N];
+            V::widen(raw[j], x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const TopKey key = x[i] == x[i] ? top_key(x[i], head + v * N + i) : 0ull;
+                mine = key > mine ? key : mine;
+            }
+        }
+        sh.lists[warp][lane] = warp_sort(mine);
+        merge_lists(sh.lists, kLpWarps);
+        tau_key = sh.lists[0][p.top - 1];
+        tau = tau_key ? top_key_value(tau_key) : -INFINITY;
+    }
+    for (int it = 0; it < run; ++it) {
+        uint4 next[kLpLoads];
+        load(next, it + 1);
+        consume(raw, it);
+#pragma unroll
+        for (int j = 0; j < kLpLoads; ++j) raw[j] = next[j];
+    }
+    if (odd >= 0) {
+        const float x = V::one(row, odd);
+        if (x > sums.m) sums.raise(x);
+        sums.add(x);
+        above += x > chosen;
+        if (p.top > 0 && x >= tau) push(x, odd);
+    }
+
+    // This part's sums, and its best keys.
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        RowSums other;
+        other.m = __shfl_xor_sync(0xFFFFFFFFu, sums.m, o);
+        other.s = __shfl_xor_sync(0xFFFFFFFFu, sums.s, o);
+        other.gap = __shfl_xor_sync(0xFFFFFFFFu, sums.gap, o);
+        sums.join(other);
+        above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
+    }
+    if (lane == 0) sh.warp_part[warp] = make_float4(sums.m, sums.s, sums.gap, __int_as_float(above));
+    __syncthreads();
+    if (p.top > 0) {
+        if (sh.count <= kLpBuffer) {
+            pick_best(sh.buffer, sh.count, sh.lists);
+        } else {
+            // The top-th key of this part, 8 bits at a time from the highest.
+            auto for_each = [&](auto f) {
+                for (int v = v0 + tid; v < v1; v += kLpThreads) {
+                    float x[N];
+                    V::widen(vec[v], x);
+                    for (int i = 0; i < N; ++i) {
+                        if (x[i] == x[i]) f(top_key(x[i], head + v * N + i));
+                    }
+                }
+                if (odd >= 0) f(top_key(V::one(row, odd), odd));
+            };
+            if (tid == 0) {
+                sh.prefix = 0ull;
+                sh.need = p.top;
+            }
+            for (int shift = 56; shift >= 0; shift -= 8) {
+                if (tid < 256) sh.histogram[tid] = 0;
+                __syncthreads();
+                const TopKey prefix = sh.prefix;
+                for_each([&](TopKey k) {
+                    if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&sh.histogram[(k >> shift) & 255], 1);
+                });
+                __syncthreads();
+                if (tid == 0) {
+                    int need = sh.need, digit = 255;
+                    while (digit > 0 && sh.histogram[digit] < need) need -= sh.histogram[digit--];
+                    sh.need = need;
+                    sh.prefix = prefix | ((TopKey)digit << shift);
+                    sh.count = 0;
+                }
+                __syncthreads();
+            }
+            const TopKey last = sh.prefix;
+            for_each([&](TopKey k) {
+                if (k >= last) sh.buffer[atomicAdd(&sh.count, 1)] = k;
+            });
+            __syncthreads();
+            pick_best(sh.buffer, min(sh.count, kLpBuffer), sh.lists);
+        }
+    }
+
+    // Join the parts in the first CTA.
+    LogprobShared *first = cluster.map_shared_rank(&sh, 0);
+    if (tid == 0) {
+        RowSums all;
+        all.init();
+        int count = 0;
+        for (int w = 0; w < kLpWarps; ++w) {
+            const float4 q = sh.warp_part[w];
+            RowSums other;
+            other.m = q.x;
+            other.s = q.y;
+            other.gap = q.z;
+            all.join(other);
+            count += __float_as_int(q.w);
+        }
+        first->part[rank] = make_float4(all.m, all.s, all.gap, __int_as_float(count));
+    }
+    if (p.top > 0 && tid < kWarp) first->joined[rank][tid] = sh.lists[0][tid];
+    cluster.sync();
+    if (rank != 0) return;
+    RowSums all;
+    all.init();
+    int count = 0;
+    for (int w = 0; w < parts; ++w) {
+        const float4 q = sh.part[w];
+        RowSums other;
+        other.m = q.x;
+        other.s = q.y;
+        other.gap = q.z;
+        all.join(other);
+        count += __float_as_int(q.w);
+    }
+    const bool bad = !(all.s > 0.0f);
+    const float nan = __int_as_float(0x7FC00000);
+    const float log_s = logf(all.s);
+    if (tid == 0) {
+        p.logprob[r] = bad || !known ? nan : (chosen - all.m) - log_s;
+        if (p.rank) p.rank[r] = bad || !known ? 0 : 1 + count;
+        if (p.entropy) p.entropy[r] = bad ? nan : log_s - all.gap / all.s;
+    }
+    if (p.top > 0) {
+        merge_lists(sh.joined, parts);
+        if (tid < p.top) {
+            const TopKey key = sh.joined[0][tid];
+            const long long at = (long long)r * p.top + tid;
+            p.top_ids[at] = bad ? -1 : (int)~(uint32_t)key;
+            p.top_logprobs[at] = bad ? nan : (top_key_value(key) - all.m) - log_s;
         }
     }
 }

@@ -60,6 +60,53 @@ int make_q_map(CUtensorMap *map, const CheetahCudaTreeAttention &a, uint32_t gro
     return 0;
 }
 
+// Warps of a q/k norm call: a warp walks over a whole row where rows fill the
+// GPU (its cos/sin and weights are then read once), over one group of heads
+// where they do not.
+template <typename TIN, int HD>
+int launch_qk(cheetah::QkNormRopeParams p, bool kv_bf16, cudaStream_t stream) {
+    constexpr int kHeads = cheetah::kWarp / (HD / 2 / (16 / (int)sizeof(TIN)));
+    const int steps = (p.q_heads + 2 * p.kv_heads + kHeads - 1) / kHeads;
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    const long long fill = (long long)cheetah::sm_count(device) * 16;
+    p.steps = p.tokens >= fill ? steps : 1;
+    p.row_units = (steps + p.steps - 1) / p.steps;
+    const uint64_t blocks = ((uint64_t)p.tokens * p.row_units + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
+    CH_REQUIRE(blocks <= 0x7FFFFFFFull, "cheetah_cuda_op_qk_norm_rope: too many rows");
+    auto kernel = kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<TIN, uint16_t, HD> : cheetah::qk_norm_rope_rows_kernel<TIN, float, HD>;
+    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)blocks), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream, true, p));
+    return 0;
+}
+
+// A cluster of CTAs per row: as many as keep every SM busy while each has at
+// least one full sample (kLpThreads threads x kLpLoads vectors) to read.
+int launch_logprobs(const cheetah::LogprobParams &p, bool bf16, cudaStream_t stream) {
+    auto kernel = bf16 ? cheetah::token_logprobs_kernel<uint16_t> : cheetah::token_logprobs_kernel<float>;
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    const long long sms = cheetah::sm_count(device);
+    const int sample = cheetah::kLpThreads * cheetah::kLpLoads * (bf16 ? 8 : 4);
+    int parts = 1;
+    while (parts < cheetah::kLpMaxCluster && (long long)p.rows * parts * 2 <= sms && p.vocab / (parts * 2) >= sample / 2) parts *= 2;
+    CH_REQUIRE((uint64_t)p.rows * parts <= 0x7FFFFFFFull, "cheetah_cuda_op_token_logprobs: too many rows");
+    if (parts > 8) CH_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(p.rows * parts));
+    config.blockDim = dim3(cheetah::kLpThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 2;
+    CH_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+    return 0;
+}
+
 // Workspace of a tree attention call on a GPU of `ctas` SMs.
 struct TreeWorkspace {
     size_t splits, ml, o, bytes;
@@ -122,12 +169,13 @@ int cheetah_cuda_op_page_slots(const CheetahCudaPageSlots *a, void *stream) {
     p.slots = a->slots;
     p.counts = a->counts;
     const size_t smem = (size_t)a->batch * 3 * sizeof(int32_t);
+    const int vec = aligned(a->positions, 16) && aligned(a->seq_ids, 16) && aligned(a->slots, 16) ? 4 : 1;
+    auto kernel = vec == 4 ? cheetah::page_slots_kernel<4> : cheetah::page_slots_kernel<1>;
     if (smem > 48 * 1024)
-        CH_CUDA_TRY(cudaFuncSetAttribute(cheetah::page_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int blocks = std::max(1, std::min(cheetah::sm_count(device),
-                                            (p.max_tokens + cheetah::kSlotThreads - 1) / cheetah::kSlotThreads));
-    CH_CUDA_TRY(launch_ex(cheetah::page_slots_kernel, dim3(blocks), dim3(cheetah::kSlotThreads), smem,
-                          static_cast<cudaStream_t>(stream), true, p));
+        CH_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int per_block = cheetah::kSlotThreads * vec;
+    const int blocks = (int)std::min<long long>(2 * cheetah::sm_count(device), ((long long)p.max_tokens + per_block - 1) / per_block);
+    CH_CUDA_TRY(launch_ex(kernel, dim3(blocks), dim3(cheetah::kSlotThreads), smem, static_cast<cudaStream_t>(stream), true, p));
     return 0;
 }
 
@@ -170,21 +218,15 @@ int cheetah_cuda_op_qk_norm_rope(const CheetahCudaQkNormRope *a, void *stream) {
     p.tokens = (int)a->tokens;
     p.q_heads = (int)a->q_heads;
     p.kv_heads = (int)a->kv_heads;
-    p.head_dim = (int)a->head_dim;
     p.q_out = a->q_out;
     p.k_pool = a->k_pool;
     p.v_pool = a->v_pool;
     p.num_pages = (int)a->num_pages;
     p.page_tokens = (int)a->page_tokens;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool kv_bf16 = a->kv_dtype == CHEETAH_CUDA_KV_BF16;
-    const uint64_t blocks = ((uint64_t)a->tokens * heads + 3) / 4;
-    CH_REQUIRE(blocks <= 0x7FFFFFFFull, "cheetah_cuda_op_qk_norm_rope: too many rows");
-    auto kernel = bf16 ? (kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<uint16_t, uint16_t>
-                                  : cheetah::qk_norm_rope_rows_kernel<uint16_t, float>)
-                       : (kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<float, uint16_t>
-                                  : cheetah::qk_norm_rope_rows_kernel<float, float>);
-    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)blocks), dim3(128), 0, static_cast<cudaStream_t>(stream), true, p));
-    return 0;
+    if (a->head_dim == 64) return bf16 ? launch_qk<uint16_t, 64>(p, kv_bf16, st) : launch_qk<float, 64>(p, kv_bf16, st);
+    return bf16 ? launch_qk<uint16_t, 128>(p, kv_bf16, st) : launch_qk<float, 128>(p, kv_bf16, st);
 }
 
 static int check_tree_attention(const CheetahCudaTreeAttention *a) {
@@ -298,9 +340,7 @@ int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogprobs *a, void *stre
     p.entropy = a->entropy;
     p.top_ids = a->top_ids;
     p.top_logprobs = a->top_logprobs;
-    auto kernel = bf16 ? cheetah::token_logprobs_kernel<uint16_t> : cheetah::token_logprobs_kernel<float>;
-    CH_CUDA_TRY(launch_ex(kernel, dim3(a->rows), dim3(cheetah::kLpThreads), 0, static_cast<cudaStream_t>(stream), true, p));
-    return 0;
+    return launch_logprobs(p, bf16, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
