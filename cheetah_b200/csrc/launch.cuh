@@ -5,6 +5,9 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
+#include <stdint.h>
+
+#include <atomic>
 #include <mutex>
 
 namespace cheetah {
@@ -13,6 +16,17 @@ inline int sm_count(int device) {
     int count = 0;
     cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
     return count > 0 ? count : 148;
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory; asked of the driver
+// once per kernel and device (`done` is the kernel's own, a bit per device).
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t bytes, int device, std::atomic<uint64_t> &done) {
+    const uint64_t bit = device >= 0 && device < 64 ? uint64_t(1) << device : 0;
+    if (bit != 0 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return err;
 }
 
 template <typename Kernel, typename... Args>

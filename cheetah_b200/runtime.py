@@ -529,31 +529,35 @@ def prefill_attention(q, k_pool, v_pool, page_table, offset: int, sliding_window
 #
 # The calls take torch CUDA tensors of one device and run on its current
 # stream, or on `stream`; what they allocate belongs to that stream, as if the
-# call stood inside `torch.cuda.stream(stream)`.
+# call stood inside `torch.cuda.stream(stream)`. A step runs them once per
+# layer or token, so they keep the host's part short.
 
-def _require(ok: bool, message: str) -> None:
-    if not ok:
-        raise CheetahCudaError(message)
-
-
-def _on_stream(fn, device, stream, *args, **kwargs):
-    """fn(stream pointer, ...) with `device` current and, given one, inside `stream`."""
+def _context(device: int, stream):
+    """The context in which `device` is current and, given one, `stream`."""
     import torch
-    if stream is not None:
-        _require(stream.device == device, "the stream belongs to another device than the tensors")
-        with torch.cuda.stream(stream):
-            return fn(stream.cuda_stream, *args, **kwargs)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return fn(torch.cuda.current_stream().cuda_stream, *args, **kwargs)
-    return fn(torch.cuda.current_stream().cuda_stream, *args, **kwargs)
+    if stream is None:
+        return torch.cuda.device(device)
+    if not (stream.device.index == device):
+        raise CheetahCudaError("the stream belongs to another device than the tensors")
+    return torch.cuda.stream(stream)
 
 
-def _check_tensors(op: str, device, dtype, **tensors) -> None:
+def _elsewhere(device: int, stream) -> bool:
+    """Whether the call has to enter a context first."""
+    import torch
+    return stream is not None or device != torch._C._cuda_getDevice()
+
+
+def _raw_stream(device: int) -> int:
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _check_tensors(op: str, device: int, dtype, names: str, *tensors) -> None:
     """Every given tensor: contiguous, of this dtype, on this device."""
-    for name, t in tensors.items():
-        if t is not None and (t.dtype is not dtype or t.device != device or not t.is_contiguous()):
-            raise CheetahCudaError(f"{op}: {name} must be a contiguous {dtype} tensor on {device}")
+    for i, t in enumerate(tensors):
+        if t is not None and (t.dtype is not dtype or t.get_device() != device or not t.is_contiguous()):
+            raise CheetahCudaError(f"{op}: {names.split()[i]} must be a contiguous {dtype} tensor on cuda:{device}")
 
 
 class PageSlots(NamedTuple):
@@ -573,35 +577,40 @@ def page_slots(cached, new_tokens, free_pages, free_count, page_table, num_pages
     int32 [B, max_pages] is extended in place. Sequences that do not fit are
     refused, not raised: see counts."""
     import torch
-    device = page_table.device
-    _require(page_table.is_cuda and page_table.dim() == 2, "page_slots: page_table must be a CUDA tensor [batch, max_pages]")
-    _check_tensors("page_slots", device, torch.int32, cached=cached, new_tokens=new_tokens, free_pages=free_pages,
-                   free_count=free_count, page_table=page_table)
+    device = page_table.get_device()
+    if not (device >= 0 and page_table.dim() == 2):
+        raise CheetahCudaError("page_slots: page_table must be a CUDA tensor [batch, max_pages]")
+    if _elsewhere(device, stream):
+        with _context(device, stream):
+            return page_slots(cached, new_tokens, free_pages, free_count, page_table, num_pages, page_tokens, max_tokens)
+    _check_tensors("page_slots", device, torch.int32, "cached new_tokens free_pages free_count page_table",
+                   cached, new_tokens, free_pages, free_count, page_table)
     B, width = page_table.shape
-    _require(cached.numel() == B and new_tokens.numel() == B and free_count.numel() == 1,
-             "page_slots: cached and new_tokens must hold one length per table row, free_count one number")
-    _require(0 < max_tokens < 2 ** 31 and 0 < num_pages < 2 ** 31 and 0 < page_tokens < 2 ** 31,
-             "page_slots: max_tokens, num_pages and page_tokens must be positive and below 2^31")
-
-    def call(stream_ptr):
-        starts, lens, positions, ids, slots, counts = torch.empty(
-            2 * B + 4 + 3 * max_tokens, dtype=torch.int32, device=device).split(
-                (B + 1, B, max_tokens, max_tokens, max_tokens, 3))
-        args = PageSlotsArgs(cached.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-                             free_pages.numel(), B, page_table.data_ptr(), width, num_pages, page_tokens, max_tokens,
-                             starts.data_ptr(), lens.data_ptr(), positions.data_ptr(), ids.data_ptr(),
-                             slots.data_ptr(), counts.data_ptr())
-        _check(lib().cheetah_cuda_op_page_slots(C.byref(args), stream_ptr))
-        return PageSlots(starts, lens, positions, ids, slots, counts)
-
-    return _on_stream(call, device, stream)
+    if not (cached.numel() == B and new_tokens.numel() == B and free_count.numel() == 1):
+        raise CheetahCudaError("page_slots: cached and new_tokens must hold one length per table row, free_count one number")
+    if not (0 < max_tokens < 2 ** 31 and 0 < num_pages < 2 ** 31 and 0 < page_tokens < 2 ** 31):
+        raise CheetahCudaError("page_slots: max_tokens, num_pages and page_tokens must be positive and below 2^31")
+    # One buffer; the per-row outputs begin at 16-byte boundaries.
+    pad = -max_tokens % 4
+    buffer = torch.empty(3 * (max_tokens + pad) + 2 * B + 4, dtype=torch.int32, device=page_table.device)
+    if pad:
+        positions, _, ids, _, slots, _, starts, lens, counts = buffer.split_with_sizes(
+            (max_tokens, pad, max_tokens, pad, max_tokens, pad, B + 1, B, 3))
+    else:
+        positions, ids, slots, starts, lens, counts = buffer.split_with_sizes(
+            (max_tokens, max_tokens, max_tokens, B + 1, B, 3))
+    args = PageSlotsArgs(cached.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+                         free_pages.numel(), B, page_table.data_ptr(), width, num_pages, page_tokens, max_tokens,
+                         starts.data_ptr(), lens.data_ptr(), positions.data_ptr(), ids.data_ptr(),
+                         slots.data_ptr(), counts.data_ptr())
+    _check(lib().cheetah_cuda_op_page_slots(C.byref(args), _raw_stream(device)))
+    return PageSlots(starts, lens, positions, ids, slots, counts)
 
 
 def _pool_dtype(op: str, k_pool, v_pool) -> int:
     import torch
-    _require(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype
-             and k_pool.dtype in (torch.bfloat16, torch.float32),
-             f"{op}: the pools must be bf16 or f32 [pages, kv_heads, page_tokens, head_dim] of one shape")
+    if not (k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and k_pool.dtype in (torch.bfloat16, torch.float32)):
+        raise CheetahCudaError(f"{op}: the pools must be bf16 or f32 [pages, kv_heads, page_tokens, head_dim] of one shape")
     return KV_F32 if k_pool.dtype == torch.float32 else KV_BF16
 
 
@@ -613,38 +622,42 @@ def qk_norm_rope(qkv, q_heads: int, kv_heads: int, positions, slots, rope_cos, r
     int32 [T], -1 skips; rope_cos, rope_sin f32 [max_positions, rotary_dim/2];
     the pools bf16 or f32, written in place. Returns q_out [T, q_heads, D]."""
     import torch
-    device = qkv.device
+    device = qkv.get_device()
+    if not (device >= 0 and qkv.dtype in (torch.bfloat16, torch.float32)):
+        raise CheetahCudaError("qk_norm_rope: qkv must be a bf16 or f32 CUDA tensor")
+    if _elsewhere(device, stream):
+        with _context(device, stream):
+            return qk_norm_rope(qkv, q_heads, kv_heads, positions, slots, rope_cos, rope_sin, k_pool, v_pool, q_norm,
+                                k_norm, eps, q_out)
     kv_dtype = _pool_dtype("qk_norm_rope", k_pool, v_pool)
     pages, kvh, pt, D = k_pool.shape
-    heads = q_heads + 2 * kv_heads
-    _require(qkv.is_cuda and qkv.dtype in (torch.bfloat16, torch.float32), "qk_norm_rope: qkv must be a bf16 or f32 CUDA tensor")
-    T = qkv.shape[0]
-    inner = qkv.stride(1) == D and qkv.stride(2) == 1 if qkv.dim() == 3 else qkv.dim() == 2 and qkv.stride(1) == 1
-    _require(T > 0 and kvh == kv_heads and qkv.numel() == T * heads * D and inner,
-             "qk_norm_rope: qkv must be [tokens, q_heads + 2 kv_heads, head_dim] with contiguous rows")
-    _check_tensors("qk_norm_rope", device, torch.int32, positions=positions, slots=slots)
-    _check_tensors("qk_norm_rope", device, torch.float32, rope_cos=rope_cos, rope_sin=rope_sin, q_norm=q_norm, k_norm=k_norm)
-    _check_tensors("qk_norm_rope", device, k_pool.dtype, k_pool=k_pool, v_pool=v_pool)
-    _check_tensors("qk_norm_rope", device, qkv.dtype, q_out=q_out)
-    _require(positions.numel() == T and slots.numel() == T, "qk_norm_rope: positions and slots must hold one entry per row")
-    _require(rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape,
-             "qk_norm_rope: rope_cos and rope_sin must be [max_positions, rotary_dim/2]")
-    _require(all(w is None or w.numel() == D for w in (q_norm, k_norm)), "qk_norm_rope: a norm weight must be [head_dim]")
-    _require(q_out is None or q_out.numel() == T * q_heads * D, "qk_norm_rope: q_out must be [tokens, q_heads, head_dim]")
-
-    def call(stream_ptr):
-        q = torch.empty(T, q_heads, D, dtype=qkv.dtype, device=device) if q_out is None else q_out
-        args = QkNormRopeArgs(qkv.data_ptr(), qkv.stride(0) if T > 1 else heads * D,
-                              KV_F32 if qkv.dtype == torch.float32 else KV_BF16, kv_dtype,
-                              q_norm.data_ptr() if q_norm is not None else None,
-                              k_norm.data_ptr() if k_norm is not None else None, eps, rope_cos.data_ptr(),
-                              rope_sin.data_ptr(), rope_cos.shape[0], 2 * rope_cos.shape[1], positions.data_ptr(),
-                              slots.data_ptr(), T, q_heads, kv_heads, D, q.data_ptr(), k_pool.data_ptr(),
-                              v_pool.data_ptr(), pages, pt)
-        _check(lib().cheetah_cuda_op_qk_norm_rope(C.byref(args), stream_ptr))
-        return q
-
-    return _on_stream(call, device, stream)
+    T, dims = qkv.shape[0], qkv.dim()
+    width = (q_heads + 2 * kv_heads) * D
+    inner = (qkv.stride(1) == D and qkv.stride(2) == 1) if dims == 3 else dims == 2 and qkv.stride(1) == 1
+    if not (T > 0 and kvh == kv_heads and q_heads > 0 and qkv.numel() == T * width and inner and (dims == 2 or qkv.shape[2] == D)):
+        raise CheetahCudaError("qk_norm_rope: qkv must be [tokens, q_heads + 2 kv_heads, head_dim] with contiguous rows")
+    _check_tensors("qk_norm_rope", device, torch.int32, "positions slots", positions, slots)
+    _check_tensors("qk_norm_rope", device, torch.float32, "rope_cos rope_sin q_norm k_norm", rope_cos, rope_sin, q_norm, k_norm)
+    _check_tensors("qk_norm_rope", device, k_pool.dtype, "k_pool v_pool", k_pool, v_pool)
+    _check_tensors("qk_norm_rope", device, qkv.dtype, "q_out", q_out)
+    if not (positions.numel() == T and slots.numel() == T):
+        raise CheetahCudaError("qk_norm_rope: positions and slots must hold one entry per row")
+    if not (rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape):
+        raise CheetahCudaError("qk_norm_rope: rope_cos and rope_sin must be [max_positions, rotary_dim/2]")
+    if not ((q_norm is None or q_norm.numel() == D) and (k_norm is None or k_norm.numel() == D)):
+        raise CheetahCudaError("qk_norm_rope: a norm weight must be [head_dim]")
+    if not (q_out is None or q_out.numel() == T * q_heads * D):
+        raise CheetahCudaError("qk_norm_rope: q_out must be [tokens, q_heads, head_dim]")
+    q = qkv.new_empty((T, q_heads, D)) if q_out is None else q_out
+    args = QkNormRopeArgs(qkv.data_ptr(), qkv.stride(0) if T > 1 else width,
+                          KV_F32 if qkv.dtype == torch.float32 else KV_BF16, kv_dtype,
+                          q_norm.data_ptr() if q_norm is not None else None,
+                          k_norm.data_ptr() if k_norm is not None else None, eps, rope_cos.data_ptr(),
+                          rope_sin.data_ptr(), rope_cos.shape[0], 2 * rope_cos.shape[1], positions.data_ptr(),
+                          slots.data_ptr(), T, q_heads, kv_heads, D, q.data_ptr(), k_pool.data_ptr(),
+                          v_pool.data_ptr(), pages, pt)
+    _check(lib().cheetah_cuda_op_qk_norm_rope(C.byref(args), _raw_stream(device)))
+    return q
 
 
 def tree_attention(q, k_pool, v_pool, page_table, seq_lens, row_starts, tree_mask, positions=None,
@@ -655,47 +668,68 @@ def tree_attention(q, k_pool, v_pool, page_table, seq_lens, row_starts, tree_mas
     max_pages]; seq_lens int32 [B]; row_starts int32 [B + 1]; tree_mask int64
     [rows, words], bit j % 64 of word j / 64 for node j; positions int32 [rows]
     (needed with a window). Rows behind the last sequence stay as `out` holds
-    them. workspace: a uint8 tensor of tree_attention_workspace bytes that no
+    them. workspace: a uint8 tensor of `tree_attention_workspace` bytes that no
     overlapping call uses; None takes one from torch's allocator."""
     import torch
-    device = q.device
-    _require(q.is_cuda and q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[0] > 0
-             and q.stride(1) == q.shape[2] and q.stride(2) == 1,
-             "tree_attention: q must be a bf16 CUDA tensor [rows, q_heads, head_dim] with contiguous rows")
+    device = q.get_device()
+    if not (device >= 0 and q.dim() == 3 and q.dtype == torch.bfloat16):
+        raise CheetahCudaError("tree_attention: q must be a bf16 CUDA tensor [rows, q_heads, head_dim]")
+    if _elsewhere(device, stream):
+        with _context(device, stream):
+            return tree_attention(q, k_pool, v_pool, page_table, seq_lens, row_starts, tree_mask, positions,
+                                  sliding_window, out, workspace)
     rows, qh, D = q.shape
-    _require(_pool_dtype("tree_attention", k_pool, v_pool) == KV_BF16 and k_pool.shape[3] == D,
-             "tree_attention: the pools must be bf16 and of q's head_dim")
+    if not (rows > 0 and q.stride(1) == D and q.stride(2) == 1):
+        raise CheetahCudaError("tree_attention: q must have contiguous rows")
+    if not (_pool_dtype("tree_attention", k_pool, v_pool) == KV_BF16 and k_pool.shape[3] == D):
+        raise CheetahCudaError("tree_attention: the pools must be bf16 and of q's head_dim")
     pages, kvh, pt, _ = k_pool.shape
-    _check_tensors("tree_attention", device, torch.bfloat16, k_pool=k_pool, v_pool=v_pool, out=out)
-    _check_tensors("tree_attention", device, torch.int32, page_table=page_table, seq_lens=seq_lens,
-                   row_starts=row_starts, positions=positions)
-    _check_tensors("tree_attention", device, torch.int64, tree_mask=tree_mask)
-    _check_tensors("tree_attention", device, torch.uint8, workspace=workspace)
+    _check_tensors("tree_attention", device, torch.bfloat16, "k_pool v_pool out", k_pool, v_pool, out)
+    _check_tensors("tree_attention", device, torch.int32, "page_table seq_lens row_starts positions",
+                   page_table, seq_lens, row_starts, positions)
+    _check_tensors("tree_attention", device, torch.int64, "tree_mask", tree_mask)
+    _check_tensors("tree_attention", device, torch.uint8, "workspace", workspace)
     B = seq_lens.numel()
-    _require(page_table.dim() == 2 and page_table.shape[0] == B and row_starts.numel() == B + 1,
-             "tree_attention: page_table must be [batch, max_pages] and row_starts [batch + 1]")
-    _require(tree_mask.dim() == 2 and tree_mask.shape[0] == rows, "tree_attention: tree_mask must be [rows, words]")
-    _require(positions is None or positions.numel() == rows, "tree_attention: positions must hold one entry per row")
-    _require(out is None or out.shape == q.shape, "tree_attention: out must have q's shape")
-    _require(0 <= sliding_window < 2 ** 31, "tree_attention: sliding_window must be 0 .. 2^31-1")
+    if not (page_table.dim() == 2 and page_table.shape[0] == B and row_starts.numel() == B + 1):
+        raise CheetahCudaError("tree_attention: page_table must be [batch, max_pages] and row_starts [batch + 1]")
+    if not (tree_mask.dim() == 2 and tree_mask.shape[0] == rows):
+        raise CheetahCudaError("tree_attention: tree_mask must be [rows, words]")
+    if not (positions is None or positions.numel() == rows):
+        raise CheetahCudaError("tree_attention: positions must hold one entry per row")
+    if not (out is None or out.shape == q.shape):
+        raise CheetahCudaError("tree_attention: out must have q's shape")
+    if not (0 <= sliding_window < 2 ** 31):
+        raise CheetahCudaError("tree_attention: sliding_window must be 0 .. 2^31-1")
+    if workspace is None:
+        workspace = torch.empty(tree_attention_workspace(D, device), dtype=torch.uint8, device=q.device)
+    o = q.new_empty((rows, qh, D)) if out is None else out
+    args = TreeAttentionArgs(q.data_ptr(), q.stride(0) if rows > 1 else qh * D, rows, k_pool.data_ptr(),
+                             v_pool.data_ptr(), page_table.data_ptr(), page_table.shape[1], pages, pt,
+                             seq_lens.data_ptr(), row_starts.data_ptr(), B, tree_mask.data_ptr(),
+                             tree_mask.shape[1], positions.data_ptr() if positions is not None else None,
+                             sliding_window, qh, kvh, D, o.data_ptr(), workspace.data_ptr(), workspace.numel())
+    _check(lib().cheetah_cuda_op_tree_attention(C.byref(args), _raw_stream(device)))
+    return o
 
-    def call(stream_ptr):
-        o = torch.empty(rows, qh, D, dtype=torch.bfloat16, device=device) if out is None else out
-        args = TreeAttentionArgs(q.data_ptr(), q.stride(0) if rows > 1 else qh * D, rows, k_pool.data_ptr(),
-                                 v_pool.data_ptr(), page_table.data_ptr(), page_table.shape[1], pages, pt,
-                                 seq_lens.data_ptr(), row_starts.data_ptr(), B, tree_mask.data_ptr(),
-                                 tree_mask.shape[1], positions.data_ptr() if positions is not None else None,
-                                 sliding_window, qh, kvh, D, o.data_ptr(), None, 0)
-        ws = workspace
-        if ws is None:
-            n = C.c_size_t(0)
+
+_tree_workspace_bytes: dict = {}  # (device, head_dim) -> bytes, a property of the GPU
+
+
+def tree_attention_workspace(head_dim: int, device: Optional[int] = None) -> int:
+    """Bytes of a `tree_attention` workspace on `device` (default: the current one)."""
+    import torch
+    if device is None:
+        device = torch.cuda.current_device()
+    bytes_ = _tree_workspace_bytes.get((device, head_dim))
+    if bytes_ is None:
+        # Every field but head_dim is the least that passes the checks.
+        args = TreeAttentionArgs(rows=1, max_pages_per_seq=1, num_pages=1, page_tokens=16, batch=1, mask_words=1,
+                                 q_heads=1, kv_heads=1, head_dim=head_dim)
+        n = C.c_size_t(0)
+        with torch.cuda.device(device):
             _check(lib().cheetah_cuda_op_tree_attention_workspace(C.byref(args), C.byref(n)))
-            ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-        _check(lib().cheetah_cuda_op_tree_attention(C.byref(args), stream_ptr))
-        return o
-
-    return _on_stream(call, device, stream)
+        bytes_ = _tree_workspace_bytes[(device, head_dim)] = n.value
+    return bytes_
 
 
 class TokenLogprobs(NamedTuple):
@@ -711,25 +745,27 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     vocab] (f32 or bf16, rows may be strided), the row's entropy and its `top`
     likeliest tokens (`cheetah_cuda_op_token_logprobs`)."""
     import torch
-    device = logits.device
-    _require(logits.is_cuda and logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32)
-             and logits.numel() > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-             "token_logprobs: logits must be a bf16 or f32 CUDA tensor [rows, vocab] with contiguous rows")
+    device = logits.get_device()
+    if not (device >= 0 and logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32)):
+        raise CheetahCudaError("token_logprobs: logits must be a bf16 or f32 CUDA tensor [rows, vocab]")
+    if _elsewhere(device, stream):
+        with _context(device, stream):
+            return token_logprobs(logits, tokens, top)
     rows, vocab = logits.shape
-    _check_tensors("token_logprobs", device, torch.int32, tokens=tokens)
-    _require(tokens.numel() == rows, "token_logprobs: tokens must hold one id per row")
-    _require(0 <= top <= min(32, vocab), "token_logprobs: top must be at most 32 and at most vocab")
-
-    def call(stream_ptr):
-        floats = torch.empty(rows * (2 + top), dtype=torch.float32, device=device)
-        ints = torch.empty(rows * (1 + top), dtype=torch.int32, device=device)
-        logprob, entropy, rest = floats[:rows], floats[rows:2 * rows], floats[2 * rows:].view(rows, top)
-        rank, ids = ints[:rows], ints[rows:].view(rows, top)
-        args = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
-                                 KV_F32 if logits.dtype == torch.float32 else KV_BF16, rows, vocab,
-                                 tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(), entropy.data_ptr(),
-                                 ids.data_ptr() if top else None, rest.data_ptr() if top else None)
-        _check(lib().cheetah_cuda_op_token_logprobs(C.byref(args), stream_ptr))
-        return TokenLogprobs(logprob, entropy, rank, ids, rest)
-
-    return _on_stream(call, device, stream)
+    if not (rows > 0 and vocab > 0 and (logits.stride(1) == 1 or vocab == 1)):
+        raise CheetahCudaError("token_logprobs: logits must have contiguous rows")
+    _check_tensors("token_logprobs", device, torch.int32, "tokens", tokens)
+    if not (tokens.dim() == 1 and tokens.numel() == rows):
+        raise CheetahCudaError("token_logprobs: tokens must be [rows]")
+    if not (0 <= top <= min(32, vocab)):
+        raise CheetahCudaError("token_logprobs: top must be at most 32 and at most vocab")
+    rank = torch.empty_like(tokens)
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    ids, best = tokens.new_empty((rows, top)), logprob.new_empty((rows, top))
+    args = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+                             KV_F32 if logits.dtype == torch.float32 else KV_BF16, rows, vocab,
+                             tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(), entropy.data_ptr(),
+                             ids.data_ptr() if top else None, best.data_ptr() if top else None)
+    _check(lib().cheetah_cuda_op_token_logprobs(C.byref(args), _raw_stream(device)))
+    return TokenLogprobs(logprob, entropy, rank, ids, best)
