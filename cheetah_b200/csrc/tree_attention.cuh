@@ -18,20 +18,23 @@
 // the GPU alike. An item cut by a share's end leaves partial (o, m, l) in the
 // workspace and tree_merge_kernel joins them, always in the same order.
 //
-// A CTA (12 warps; the last two idle):
-//   warp 0     TMA producer: Q boxes [64 dims, group heads, nodes], K and V
-//              tiles in boxes of up to 64 keys of one page, through a ring of
-//              single K or V tiles in the order the MMAs use them;
+// A CTA (three warpgroups):
+//   warps 0, 2 TMA producers of Q and K, and of V: boxes [64 dims, group
+//              heads, nodes] of Q, boxes of up to 64 keys of one page, through
+//              a ring of single K or V tiles in the order the MMAs use them;
 //   warp 1     owns TMEM; lane 0 issues S = Q K^T (128 x 128) and O += P V for
 //              jobs i = 0, 1, 2, ... of the groups i % 2: S(0), S(1), then
 //              PV(i), S(i+2), so one group's products run during the other's
 //              softmax;
-//   warps 2-9  two softmax groups, one thread per row: read the S row from
+//   warp 3     scheduler: cuts the CTA's share into segments (a run of key
+//              tiles of one item) and publishes them ahead in a queue;
+//   warps 4-11 two softmax groups, one thread per row: read the S row from
 //              TMEM, mask, exponentials, P as bf16 back into S's columns (the
-//              A operand of PV is read from TMEM). The running maximum moves
-//              only when it grows by more than 2^8 (P and l use the same one,
-//              so the quotient is the same), and O is rescaled in TMEM only
-//              then.
+//              A operand of PV is read from TMEM) in two halves, so that the
+//              first half's products run during the second's exponentials.
+//              The running maximum moves only when it grows by more than 2^8
+//              (P and l use the same one, so the quotient is the same), and O
+//              is rescaled in TMEM only then.
 // P is rounded to bf16 because the tensor cores multiply bf16; sums,
 // statistics and O stay f32.
 //
@@ -55,12 +58,18 @@ namespace cheetah {
 
 constexpr int kTreeKeys = 128;      // keys per tile
 constexpr int kTreeRows = 128;      // rows of a Q tile
-constexpr int kTreeThreads = 320;
+constexpr int kTreeThreads = 384;   // warpgroups: loads and MMAs, softmax A, softmax B
 constexpr int kTreeMinShare = 2;    // key tiles a CTA takes at least (one per softmax group)
 constexpr float kTreeRescaleLog2 = 8.0f;
 constexpr uint32_t kTreeOCol = 256; // S_A | S_B | O_A | O_B
 constexpr int kTreeMergeThreads = 256;
-constexpr int kTreeMergeSplit = 8;
+constexpr int kTreeMergeCtas = 4;     // per SM
+constexpr int kTreeMergeWarps = kTreeMergeThreads / kWarp;
+constexpr int kTreeMaxCtas = 256;     // CTAs of the attention launch that a merge can list
+// Registers per thread after the split of the launch's 168: 128 x 64 + 256 x
+// 216 is below 384 x 168.
+constexpr int kTreeLeanRegs = 64, kTreeSoftmaxRegs = 216;
+static_assert(128 * kTreeLeanRegs + 256 * kTreeSoftmaxRegs <= kTreeThreads * 168, "register split");
 
 template <int HD>
 struct TreeCfg {
@@ -73,10 +82,10 @@ struct TreeCfg {
 
 // What a split item needs to be joined, written by the CTA that begins it.
 struct TreeSplit {
-    int row0, nodes, kvh, two_tiles;
+    int row0, nodes, kvh;
     int first_slot;  // of the beginning; the other parts are slot 0 of the next CTAs
     int parts;       // 0: nothing to join
-    int pad[2];
+    int pad[3];
 };
 
 struct TreeAttnParams {
@@ -93,7 +102,7 @@ struct TreeAttnParams {
     const uint16_t *v_pool;
     uint16_t *out;
     TreeSplit *splits;  // [CTAs]
-    float *part_o;      // [CTAs][2][256][HD], unnormalised
+    float4 *part_o;     // [CTAs][2][HD/4][256] unnormalised: lanes (rows) write and read side by side
     float2 *part_ml;    // [CTAs][2][256]
 };
 
@@ -103,15 +112,16 @@ struct TreeSegment {
     int ctx, len;          // context keys; cached positions within the table
     int b, kvh;
     int node0, nodes;      // the item's nodes within the sequence
-    int t0, t1, first_tile, last_tile;
-    int jobs;              // MMA jobs of this segment (0: rows to be zeroed)
-    bool two_tiles;
+    int t0, t1;
+    int jobs;              // MMA jobs (0: rows to be zeroed; -1: no more segments)
+    int two_tiles;
     int low;               // first key any row may see
+    int slot;              // workspace slot of a part; -1: the segment is its whole item
 };
 
 // Rows, context and tile range of sequence b.
 struct TreeSeq {
-    int row0, n, ctx, len, tile_lo, tiles, row_items;
+    int row0, n, ctx, len, low, tile_lo, tiles, row_items;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnParams &p, int b) {
     TreeSeq s;
@@ -120,92 +130,51 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnParams &p, int b) {
     s.n = max(min(r1, p.rows) - s.row0, 0);
     s.ctx = len - s.n;
     s.len = (int)min((long long)len, (long long)p.max_pages * p.page_tokens);
-    const int low = p.window > 0 ? max(0, s.ctx - p.window + 1) : 0;
-    s.tile_lo = low / kTreeKeys;
+    s.low = p.window > 0 ? max(0, s.ctx - p.window + 1) : 0;
+    s.tile_lo = s.low / kTreeKeys;
     // Without room for its rows a sequence is one unit that writes zeros.
     s.tiles = s.ctx < 0 ? 1 : max(1, (s.len + kTreeKeys - 1) / kTreeKeys - s.tile_lo);
     s.row_items = (s.n + 2 * p.tile_nodes - 1) / (2 * p.tile_nodes);
     return s;
 }
-__device__ __forceinline__ long long tree_units(const TreeAttnParams &p, const TreeSeq &s) {
-    return (long long)s.row_items * p.kv_heads * s.tiles;
+__device__ __forceinline__ int tree_units(const TreeAttnParams &p, int b) {
+    const TreeSeq s = tree_seq(p, b);
+    return s.row_items * p.kv_heads * s.tiles;
 }
-
-// Walks the segments of one CTA's share of the unit axis.
-struct TreeWalk {
-    int b;
-    long long off;   // units into sequence b
-    long long left;  // units left in the share
-    TreeSeq s;
-    bool fresh;
-
-    __device__ __forceinline__ void start(int b0, long long off0, long long count) {
-        b = b0;
-        off = off0;
-        left = count;
-        fresh = true;
-    }
-    __device__ __forceinline__ bool next(const TreeAttnParams &p, TreeSegment &g) {
-        if (left <= 0) return false;
-        while (true) {
-            if (b >= p.batch) return false;
-            if (fresh) {
-                s = tree_seq(p, b);
-                fresh = false;
-            }
-            if (off < tree_units(p, s)) break;
-            off = 0;
-            ++b;
-            fresh = true;
-        }
-        const int item = (int)(off / s.tiles), at = (int)(off % s.tiles);
-        const int take = (int)min(left, (long long)(s.tiles - at));
-        off += take;
-        left -= take;
-        const int rt = item % s.row_items;
-        g.row0 = s.row0;
-        g.n = s.n;
-        g.ctx = s.ctx;
-        g.len = s.len;
-        g.b = b;
-        g.kvh = item / s.row_items;
-        g.node0 = rt * 2 * p.tile_nodes;
-        g.nodes = min(s.n - g.node0, 2 * p.tile_nodes);
-        g.two_tiles = g.nodes > p.tile_nodes;
-        g.first_tile = s.tile_lo;
-        g.last_tile = s.tile_lo + s.tiles;
-        g.t0 = s.tile_lo + at;
-        g.t1 = g.t0 + take;
-        g.jobs = s.ctx < 0 ? 0 : (g.two_tiles ? 2 * take : take);
-        g.low = p.window > 0 ? max(0, s.ctx - p.window + 1) : 0;
-        return true;
-    }
-};
 
 // The ring position of tile i's K and V within a segment of T tiles, in the
 // order of first use: K0 V0 K1 V1 .. where both groups use each tile, and
 // K0 K1 V0 K2 V1 K3 .. where they alternate.
-__device__ __forceinline__ int tree_pos_k(bool two, int i, int T) {
-    return two ? 2 * i : (i < 2 ? i : 2 * i - 1);
-}
+__device__ __forceinline__ int tree_pos_k(bool two, int i) { return two ? 2 * i : (i < 2 ? i : 2 * i - 1); }
 __device__ __forceinline__ int tree_pos_v(bool two, int i, int T) {
     return two ? 2 * i + 1 : (T == 1 ? 1 : 2 + i + min(i, T - 2));
 }
 
+constexpr int kTreeQueue = 4;              // segments the scheduler may be ahead
+constexpr int kTreeQueueReaders = 3 + 8;   // two producers, the MMA thread, the softmax warps
 struct TreeShared {
     uint64_t full[12], empty[12];
-    uint64_t q_full, q_empty, s_full[2], p_full[2], seg_done, exchange, drain;
-    long long warp_sums[10];
-    long long total, start_off, share;
+    uint64_t seg_full[kTreeQueue], seg_empty[kTreeQueue];
+    uint64_t q_full, q_empty, s_full[2], p_full[2][2], seg_done, exchange, drain;
+    TreeSegment queue[kTreeQueue];
+    int warp_units[kTreeThreads / kWarp];
     uint32_t tmem;
-    int start_b, abort_flag, non_finite;
-    uint32_t valid[12];  // per ring buffer: which 16-key parts hold loaded positions
+    int start_b, start_off, abort_flag, non_finite;
+    uint32_t valid[12];  // per ring buffer: which 16-key parts of V hold loaded positions
     float2 ml[2][kTreeRows];
 };
 
 template <int HD>
 constexpr size_t tree_attention_smem() { return (size_t)TreeCfg<HD>::kTiles + 3072; }
-static_assert(sizeof(TreeShared) <= 3072 - 512, "fits behind the tiles");
+static_assert(sizeof(TreeShared) <= 3072, "fits behind the tiles");
+
+// The role's next segment, once the scheduler has published it; false at the
+// end of the share or when a wait gave up (then *ok is false).
+__device__ __forceinline__ bool tree_next(TreeShared &sh, int seg, bool &ok) {
+    ok = __all_sync(__activemask(), mbar_wait(smem_u32(&sh.seg_full[seg % kTreeQueue]), (seg / kTreeQueue) & 1));
+    return ok && sh.queue[seg % kTreeQueue].jobs >= 0;
+}
+__device__ __forceinline__ void tree_release(TreeShared &sh, int seg) { mbar_arrive(smem_u32(&sh.seg_empty[seg % kTreeQueue])); }
 
 // Bits js .. js+31 of a row's mask (js may be negative or past the end).
 __device__ __forceinline__ uint32_t tree_mask_bits(const uint32_t *mask, int words, int js) {
@@ -242,9 +211,42 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeAttnParams &p, const 
 
 __device__ __forceinline__ bool bf16_non_finite(uint32_t half) { return (half & 0x7F80u) == 0x7F80u; }
 
+// One V row of a masked tile in shared memory: zero where it holds no
+// position, finite elsewhere (its non-finite values are noted for patch_row).
+template <int HD>
+__device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, bool holds) {
+#pragma unroll 1
+    for (int c = 0; c < HD / 8; ++c) {
+        uint4 *cell = reinterpret_cast<uint4 *>(v_row + (c >> 3) * TreeCfg<HD>::kHalfBytes + (c & 7) * 16);
+        if (!holds) {
+            *cell = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
+        uint32_t w[4] = {cell->x, cell->y, cell->z, cell->w};
+        bool bad = false;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (bf16_non_finite(w[x])) {
+                w[x] &= 0xFFFF0000u;
+                bad = true;
+            }
+            if (bf16_non_finite(w[x] >> 16)) {
+                w[x] &= 0x0000FFFFu;
+                bad = true;
+            }
+        }
+        if (bad) {
+            *reinterpret_cast<volatile int *>(&sh.non_finite) = 1;
+            __threadfence_block();  // flag before the zeros that hide it from the other group
+            *cell = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 // Adds the non-finite values of the V rows that `row` sees in [t0, t1) to the
-// result this thread has just stored (columns d0 .. d0+cols). Their products
-// were left out of the MMAs.
+// result this thread's warp has just stored (columns d0 .. d0+cols). Their
+// products were left out of the MMAs.
 template <int HD>
 __device__ __noinline__ void patch_row(const TreeAttnParams &p, const TreeSegment &g, int row, int d0, int cols,
                                        uint16_t *out, float *part) {
@@ -257,10 +259,38 @@ __device__ __noinline__ void patch_row(const TreeAttnParams &p, const TreeSegmen
             const uint16_t *v = p.v_pool + (((long long)page * p.kv_heads + g.kvh) * p.page_tokens + pos % p.page_tokens) * HD;
             for (int d = d0; d < d0 + cols; ++d) {
                 if (!bf16_non_finite(v[d])) continue;
-                if (part) part[d] += bf16_to_f32(v[d]);
+                if (part) part[(d / 4) * 1024 + d % 4] += bf16_to_f32(v[d]);
                 else out[d] = f32_to_bf16_rne(bf16_to_f32(out[d]) + bf16_to_f32(v[d]));
             }
         }
+    }
+}
+
+// Stores 64 bytes of each lane's row (four 16-byte cells), with the four cells
+// of a row written by neighbouring lanes: lane l's v[j] becomes lane j's v[l]
+// among each four lanes, so a store covers 8 rows instead of 32.
+__device__ __forceinline__ void store_rows4(uint16_t *dst, uint32_t (&v)[4][4], uint32_t live_mask) {
+    const int lane = threadIdx.x % kWarp;
+#pragma unroll
+    for (int s = 1; s < 4; s <<= 1) {
+        const bool high = lane & s;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j & s) continue;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, high ? v[j][x] : v[j | s][x], s);
+                if (high) v[j][x] = got;
+                else v[j | s][x] = got;
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int from = (lane & ~3) + j;
+        uint16_t *row = reinterpret_cast<uint16_t *>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), from));
+        if (live_mask >> from & 1)
+            *reinterpret_cast<uint4 *>(row + (lane & 3) * 8) = make_uint4(v[j][0], v[j][1], v[j][2], v[j][3]);
     }
 }
 
@@ -271,12 +301,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     using C = TreeCfg<HD>;
     constexpr uint32_t kIdescS = umma_idesc_bf16(kTreeRows, kTreeKeys);
     constexpr uint32_t kIdescPV = umma_idesc_bf16(kTreeRows, HD) | (1u << 16);  // V MN-major
+    // The kernel's only shared memory, so it begins at a 1024-byte boundary
+    // (the swizzled tiles' alignment).
     extern __shared__ __align__(1024) uint8_t tree_smem[];
-    // The kernel has no other shared memory, so the dynamic part begins at a
-    // 1024-byte boundary; 512 bytes of slack are left all the same.
-    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
-    uint8_t *q_s = base, *ring = base + 2 * C::kTile;
-    TreeShared &sh = *reinterpret_cast<TreeShared *>(base + C::kTiles);
+    uint8_t *q_s = tree_smem, *ring = tree_smem + 2 * C::kTile;
+    TreeShared &sh = *reinterpret_cast<TreeShared *>(tree_smem + C::kTiles);
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
 
     if (threadIdx.x == 0) {
@@ -284,11 +313,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             mbar_init(smem_u32(&sh.full[i]), 1);
             mbar_init(smem_u32(&sh.empty[i]), 1);
         }
+        for (int i = 0; i < kTreeQueue; ++i) {
+            mbar_init(smem_u32(&sh.seg_full[i]), 1);
+            mbar_init(smem_u32(&sh.seg_empty[i]), kTreeQueueReaders);
+        }
         mbar_init(smem_u32(&sh.q_full), 1);
         mbar_init(smem_u32(&sh.q_empty), 1);
         for (int g = 0; g < 2; ++g) {
             mbar_init(smem_u32(&sh.s_full[g]), 1);
-            mbar_init(smem_u32(&sh.p_full[g]), 4);
+            mbar_init(smem_u32(&sh.p_full[g][0]), 4);
+            mbar_init(smem_u32(&sh.p_full[g][1]), 4);
         }
         mbar_init(smem_u32(&sh.seg_done), 1);
         mbar_init(smem_u32(&sh.exchange), 8);
@@ -296,6 +330,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         sh.abort_flag = 0;
         sh.non_finite = 0;
         sh.start_b = p.batch;
+        sh.start_off = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -306,299 +341,350 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     pdl_wait();
     pdl_launch_dependents();
 
-    // Total units, then the sequence in which this CTA's share begins.
-    long long mine = 0;
-    for (int b = threadIdx.x; b < p.batch; b += kTreeThreads) mine += tree_units(p, tree_seq(p, b));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
-    if (lane == 0) sh.warp_sums[warp] = mine;
+    // Total units, then the sequence in which this CTA's share begins (the
+    // host has checked that the units of any lengths fit 31 bits).
+    constexpr int kWarps = kTreeThreads / kWarp;
+    const int mine = (int)threadIdx.x < p.batch ? tree_units(p, threadIdx.x) : 0;
+    int sum = mine;
+    for (int b = threadIdx.x + kTreeThreads; b < p.batch; b += kTreeThreads) sum += tree_units(p, b);
+    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+    if (lane == 0) sh.warp_units[warp] = sum;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    long long total = 0;
-    for (int w = 0; w < kTreeThreads / kWarp; ++w) total += sh.warp_sums[w];
-    const long long share = max((long long)kTreeMinShare, (total + gridDim.x - 1) / gridDim.x);
-    const long long u0 = blockIdx.x * share;
-    long long before = 0;
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += sh.warp_units[w];
+    const int share = max(kTreeMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+    const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
+    int before = 0;
     for (int b0 = 0; b0 < p.batch && u0 < total; b0 += kTreeThreads) {
         const int b = b0 + threadIdx.x;
-        const long long units = b < p.batch ? tree_units(p, tree_seq(p, b)) : 0;
-        long long v = units;
+        const int units = b0 == 0 ? mine : (b < p.batch ? tree_units(p, b) : 0);
+        int end = units;
 #pragma unroll
         for (int o = 1; o < kWarp; o <<= 1) {
-            const long long up = __shfl_up_sync(0xFFFFFFFFu, v, o);
-            if (lane >= o) v += up;
+            const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
+            if (lane >= o) end += up;
         }
-        __syncthreads();
-        if (lane == kWarp - 1) sh.warp_sums[warp] = v;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) v += sh.warp_sums[w];
-        v += before;
-        if (v - units <= u0 && u0 < v) {
+        if (p.batch > kTreeThreads) {
+            __syncthreads();
+            if (lane == kWarp - 1) sh.warp_units[warp] = end;
+            __syncthreads();
+        }
+        int chunk = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const int x = sh.warp_units[w];
+            if (w < warp) end += x;
+            chunk += x;
+        }
+        end += before;
+        before += chunk;
+        if (end - units <= u0 && u0 < end) {
             sh.start_b = b;
-            sh.start_off = u0 - (v - units);
+            sh.start_off = u0 - (end - units);
         }
-        for (int w = 0; w < kTreeThreads / kWarp; ++w) before += sh.warp_sums[w];
     }
     __syncthreads();
-    TreeWalk walk;
-    walk.start(sh.start_b, sh.start_off, u0 < total ? min(share, total - u0) : 0);
-    TreeSegment g;
 
-    int ring_at = 0;       // ring positions of the segments before
-    int issued = 0;        // producer: positions requested
+    int ring_at = 0;   // ring positions of the segments before
+    int issued = 0;    // producers: tiles requested are at positions below this
     int q_issued = 0;
-    if (warp == 0) {
-        const int boxes = kTreeKeys / p.box_keys;
-        const int parts = p.box_keys / 16;  // 16-key parts of a box
-        int segs = 0;
-        bool ok = true;
-        while (ok && walk.next(p, g)) {
-            if (g.jobs == 0) continue;
-            const int T = g.t1 - g.t0;
-            const int32_t *table = p.page_table + (long long)g.b * p.max_pages;
-            // Page ids of 32 consecutive boxes, one per lane, for K and for V.
-            int base_k = -1, base_v = -1, page_k = -1, page_v = -1;
-            auto page_of = [&](int box, int &first, int &page) -> int {
-                if (first < 0 || box < first || box >= first + kWarp) {
-                    first = box;
-                    const long long pos = (long long)(box + lane) * p.box_keys;
-                    page = -1;
-                    if (pos < g.len && pos + p.box_keys > g.low) {
-                        const int id = table[(int)pos / p.page_tokens];
-                        if (id >= 0 && id < p.num_pages) page = id;
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTreeLeanRegs));
+    if (warp == 3) {
+        // Scheduler: walks over the share's items and publishes its segments.
+        if (lane == 0) {
+            int b = sh.start_b, left = min(share, total - u0), unit = u0, seg = 0;
+            int at = sh.start_off, kvh = 0, rt = 0;
+            TreeSplit split = {};
+            bool ok = true;
+            while (true) {
+                TreeSegment g = {};
+                g.jobs = -1;
+                ok = mbar_wait(smem_u32(&sh.seg_empty[seg % kTreeQueue]), ((seg / kTreeQueue) & 1) ^ 1);
+                if (!ok) break;
+                if (left > 0 && b < p.batch) {
+                    TreeSeq s = tree_seq(p, b);
+                    while (s.row_items == 0 || kvh >= p.kv_heads) {  // no (more) items in b
+                        if (++b >= p.batch) break;
+                        at = kvh = rt = 0;
+                        s = tree_seq(p, b);
                     }
-                }
-                return first;
-            };
-            for (int pos = 0; ok && pos < 2 * T; ++pos) {
-                if (pos == min(2, 2 * T - 1)) {
-                    // Q, once the previous segment's S products are done.
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.q_empty), (segs & 1) ^ 1));
-                    if (!ok) break;
-                    if (lane == 0) {
-                        const int tiles = g.two_tiles ? 2 : 1;
-                        mbar_expect_tx(smem_u32(&sh.q_full), (uint32_t)(tiles * C::kHalves * p.group * p.tile_nodes * 128));
-                        for (int t = 0; t < tiles; ++t) {
-                            for (int h = 0; h < C::kHalves; ++h) {
-                                tma_load_3d(smem_u32(q_s + t * C::kTile + h * C::kHalfBytes), &q_map, h * 64, g.kvh * p.group,
-                                            g.row0 + g.node0 + t * p.tile_nodes, smem_u32(&sh.q_full));
+                    if (b < p.batch) {
+                        if (at >= s.tiles) {  // the share's beginning: items to skip
+                            const int item = at / s.tiles;
+                            at -= item * s.tiles;
+                            kvh = item / s.row_items;
+                            rt = item - kvh * s.row_items;
+                        }
+                        const int take = min(left, s.tiles - at);
+                        const bool whole = take == s.tiles;
+                        g.row0 = s.row0;
+                        g.n = s.n;
+                        g.ctx = s.ctx;
+                        g.len = s.len;
+                        g.b = b;
+                        g.kvh = kvh;
+                        g.node0 = rt * 2 * p.tile_nodes;
+                        g.nodes = min(s.n - g.node0, 2 * p.tile_nodes);
+                        g.two_tiles = g.nodes > p.tile_nodes;
+                        g.t0 = s.tile_lo + at;
+                        g.t1 = g.t0 + take;
+                        g.jobs = s.ctx < 0 ? 0 : (g.two_tiles ? 2 * take : take);
+                        g.low = s.low;
+                        g.slot = whole ? -1 : (seg == 0 ? 0 : 1);
+                        if (at == 0 && !whole) {
+                            split.row0 = s.row0 + g.node0;
+                            split.nodes = g.nodes;
+                            split.kvh = kvh;
+                            split.first_slot = g.slot;
+                            split.parts = (unit + s.tiles - 1) / share - (int)blockIdx.x + 1;
+                        }
+                        unit += take;
+                        left -= take;
+                        at += take;
+                        if (at == s.tiles) {
+                            at = 0;
+                            if (++rt == s.row_items) {
+                                rt = 0;
+                                ++kvh;
                             }
                         }
                     }
-                    ++q_issued;
-                    ++segs;
                 }
-                bool is_v;
-                int i;
-                if (g.two_tiles) {
-                    i = pos >> 1;
-                    is_v = pos & 1;
-                } else if (T == 1 || pos < 2) {
-                    i = T == 1 ? 0 : pos;
-                    is_v = T == 1 && pos == 1;
-                } else {
-                    const int x = pos - 2, mixed = 2 * (T - 2);
-                    is_v = x >= mixed || (x & 1) == 0;
-                    i = x >= mixed ? T - 2 + (x - mixed) : (is_v ? x >> 1 : 2 + (x >> 1));
-                }
-                const int at = ring_at + pos;
-                const int buf = at % C::kBufs;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.empty[buf]), ((at / C::kBufs) & 1) ^ 1));
-                if (!ok) break;
-                const int box0 = (g.t0 + i) * boxes;
-                // A tile's boxes never straddle the 32 ids (32 is a multiple of 2, 4 and 8).
-                const int first = is_v ? page_of(box0, base_v, page_v) : page_of(box0, base_k, page_k);
-                const int box = lane % boxes, half = lane / boxes;
-                const int page = __shfl_sync(0xFFFFFFFFu, is_v ? page_v : page_k, box0 + box - first);
-                const uint32_t good = __ballot_sync(0xFFFFFFFFu, page >= 0) & low_bits(boxes);
-                const uint32_t bar = smem_u32(&sh.full[buf]);
-                if (lane == 0) {
-                    uint32_t valid = 0;
-                    for (int x = 0; x < boxes; ++x) {
-                        if (good >> x & 1) valid |= low_bits(parts) << (x * parts);
-                    }
-                    sh.valid[buf] = valid;
-                    mbar_expect_tx(bar, (uint32_t)(__popc(good) * p.box_keys * HD * 2));
-                }
-                __syncwarp();
-                if (half < C::kHalves && page >= 0) {
-                    const int key = (box0 + box) * p.box_keys;
-                    const int row = (int)(((long long)page * p.kv_heads + g.kvh) * p.page_tokens + key % p.page_tokens);
-                    tma_load_2d(smem_u32(ring + buf * C::kTile + half * C::kHalfBytes + box * p.box_keys * 128),
-                                is_v ? &v_map : &k_map, half * 64, row, bar);
-                }
-                issued = at + 1;
+                sh.queue[seg % kTreeQueue] = g;
+                mbar_arrive(smem_u32(&sh.seg_full[seg % kTreeQueue]));
+                ++seg;
+                if (g.jobs < 0) break;
             }
-            ring_at += 2 * T;
+            p.splits[blockIdx.x] = split;
+            if (!ok) sh.abort_flag = 1;
+        }
+    } else if (warp == 0 || warp == 2) {
+        // Producers: warp 0 loads Q and K tiles, warp 2 V tiles.
+        const bool is_v = warp == 2;
+        const CUtensorMap *map = is_v ? &v_map : &k_map;
+        const int boxes = kTreeKeys / p.box_keys;
+        bool ok = true;
+        for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
+            const TreeSegment &g = sh.queue[seg % kTreeQueue];
+            const int T = g.t1 - g.t0;
+            const bool two = g.two_tiles;
+            const int len = g.len, low = g.low, kvh = g.kvh, t0 = g.t0;
+            const int32_t *table = p.page_table + (long long)g.b * p.max_pages;
+            if (g.jobs > 0) {
+                // Pool rows of 32 consecutive boxes, one per lane (-1: not
+                // loaded); a tile's boxes never straddle them (32 is a
+                // multiple of 2, 4 and 8).
+                int first = -kWarp, my_row = -1;
+                uint32_t loaded = 0;
+                for (int i = 0; i < T; ++i) {
+                    const int at = ring_at + (is_v ? tree_pos_v(two, i, T) : tree_pos_k(two, i));
+                    const int buf = at % C::kBufs;
+                    const int box0 = (t0 + i) * boxes;
+                    if (box0 >= first + kWarp) {
+                        first = box0;
+                        const long long pos = (long long)(box0 + lane) * p.box_keys;
+                        my_row = -1;
+                        if (pos < len && pos + p.box_keys > low) {
+                            const int col = (int)pos / p.page_tokens;
+                            const int page = table[col];
+                            if (page >= 0 && page < p.num_pages)
+                                my_row = (page * p.kv_heads + kvh) * p.page_tokens + ((int)pos - col * p.page_tokens);
+                        }
+                        loaded = __ballot_sync(0xFFFFFFFFu, my_row >= 0);
+                    }
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.empty[buf]), ((at / C::kBufs) & 1) ^ 1));
+                    if (!ok) break;
+                    const uint32_t good = (loaded >> (box0 - first)) & low_bits(boxes);
+                    const uint32_t bar = smem_u32(&sh.full[buf]);
+                    const uint32_t dst = smem_u32(ring + buf * C::kTile);
+                    if (lane == 0) {
+                        if (is_v) {
+                            uint32_t valid = 0;
+                            for (int x = 0; x < boxes; ++x) {
+                                if (good >> x & 1) valid |= low_bits(8 / boxes) << (x * (8 / boxes));
+                            }
+                            sh.valid[buf] = valid;
+                        }
+                        mbar_expect_tx(bar, (uint32_t)(__popc(good) * p.box_keys * HD * 2));
+                    }
+                    for (int x = 0; x < boxes; ++x) {
+                        const int row = __shfl_sync(0xFFFFFFFFu, my_row, box0 - first + x);
+                        if (lane == 0 && row >= 0) {
+#pragma unroll
+                            for (int h = 0; h < C::kHalves; ++h)
+                                tma_load_2d(dst + h * C::kHalfBytes + x * p.box_keys * 128, map, h * 64, row, bar);
+                        }
+                    }
+                    issued = at + 1;
+                    if (!is_v && i == min(1, T - 1)) {
+                        // Q, once the previous segment's S products are done.
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.q_empty), (q_issued & 1) ^ 1));
+                        if (!ok) break;
+                        if (lane == 0) {
+                            const int tiles = two ? 2 : 1;
+                            mbar_expect_tx(smem_u32(&sh.q_full), (uint32_t)(tiles * C::kHalves * p.group * p.tile_nodes * 128));
+                            for (int t = 0; t < tiles; ++t) {
+                                for (int h = 0; h < C::kHalves; ++h) {
+                                    tma_load_3d(smem_u32(q_s + t * C::kTile + h * C::kHalfBytes), &q_map, h * 64, kvh * p.group,
+                                                g.row0 + g.node0 + t * p.tile_nodes, smem_u32(&sh.q_full));
+                                }
+                            }
+                        }
+                        ++q_issued;
+                    }
+                }
+                ring_at += 2 * T;
+            }
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) tree_release(sh, seg);
         }
         if (!ok) sh.abort_flag = 1;
     } else if (warp == 1) {
         if (lane == 0) {
-            int segs = 0;
-            int seen[2] = {0, 0};  // P tiles consumed per group
+            int q_seen = 0;
+            uint32_t p_phase[2] = {0, 0};
+            // The next ring position; buffers are first used in ring order.
+            int next_buf = 0;
+            uint32_t next_phase = 0;
+            int k_buf = 0, v_buf = 0;
+            const uint64_t q_desc = umma_smem_desc(smem_u32(q_s));
+            const uint64_t k_desc = umma_smem_desc(smem_u32(ring));
+            const uint64_t v_desc = umma_smem_desc_mn(smem_u32(ring), HD > 64 ? C::kHalfBytes : 16);
             bool ok = true;
-            while (ok && walk.next(p, g)) {
-                if (g.jobs == 0) continue;
-                const int T = g.t1 - g.t0;
+            auto take = [&](int &buf) -> bool {
+                buf = next_buf;
+                const bool landed = mbar_wait(smem_u32(&sh.full[buf]), next_phase);
+                if (++next_buf == C::kBufs) {
+                    next_buf = 0;
+                    next_phase ^= 1;
+                }
+                return landed;
+            };
+            for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
+                const bool two = sh.queue[seg % kTreeQueue].two_tiles;
+                const int jobs = sh.queue[seg % kTreeQueue].jobs;
                 auto issue_s = [&](int i) -> bool {
-                    const int grp = i & 1, tile = g.two_tiles ? i >> 1 : i;
-                    const int at = ring_at + tree_pos_k(g.two_tiles, tile, T), buf = at % C::kBufs;
-                    if (!mbar_wait(smem_u32(&sh.full[buf]), (at / C::kBufs) & 1)) return false;
+                    const int grp = i & 1;
+                    if ((!two || grp == 0) && !take(k_buf)) return false;
                     tc_fence_after();
-                    const uint32_t k_addr = smem_u32(ring + buf * C::kTile);
-                    const uint32_t q_addr = smem_u32(q_s + (g.two_tiles ? grp * C::kTile : 0));
+                    const uint64_t qd = q_desc + (two ? grp * (C::kTile >> 4) : 0);
+                    const uint64_t kd = k_desc + (uint32_t)(k_buf * (C::kTile >> 4));
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
-                        const uint32_t off = (uint32_t)((k >> 2) * C::kHalfBytes + (k & 3) * 32);
-                        umma_bf16(tmem + grp * kTreeKeys, umma_smem_desc(q_addr + off), umma_smem_desc(k_addr + off), kIdescS,
-                                  k > 0 ? 1u : 0u);
+                        const uint32_t off = (uint32_t)((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
+                        umma_bf16(tmem + grp * kTreeKeys, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
                     }
                     umma_commit(smem_u32(&sh.s_full[grp]));
-                    if (!g.two_tiles || grp == 1) umma_commit(smem_u32(&sh.empty[buf]));
-                    if (i == g.jobs - 1) umma_commit(smem_u32(&sh.q_empty));
+                    if (!two || grp == 1) umma_commit(smem_u32(&sh.empty[k_buf]));
+                    if (i == jobs - 1) umma_commit(smem_u32(&sh.q_empty));
                     return true;
                 };
                 auto issue_pv = [&](int i) -> bool {
-                    const int grp = i & 1, tile = g.two_tiles ? i >> 1 : i;
-                    const int at = ring_at + tree_pos_v(g.two_tiles, tile, T), buf = at % C::kBufs;
-                    if (!mbar_wait(smem_u32(&sh.p_full[grp]), seen[grp] & 1)) return false;
-                    ++seen[grp];
-                    if (!mbar_wait(smem_u32(&sh.full[buf]), (at / C::kBufs) & 1)) return false;
-                    tc_fence_after();
-                    const uint32_t v_addr = smem_u32(ring + buf * C::kTile);
+                    const int grp = i & 1;
+                    if ((!two || grp == 0) && !take(v_buf)) return false;
+                    const uint64_t vd = v_desc + (uint32_t)(v_buf * (C::kTile >> 4));
 #pragma unroll
-                    for (int k = 0; k < kTreeKeys / 16; ++k) {
-                        umma_bf16_ta(tmem + kTreeOCol + grp * HD, tmem + grp * kTreeKeys + k * 8,
-                                     umma_smem_desc_mn(v_addr + k * 2048, HD > 64 ? C::kHalfBytes : 16), kIdescPV,
-                                     (i > 1 || k > 0) ? 1u : 0u);
+                    for (int h = 0; h < 2; ++h) {
+                        if (!mbar_wait(smem_u32(&sh.p_full[grp][h]), p_phase[grp])) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 4 * h; k < 4 * h + 4; ++k) {
+                            umma_bf16_ta(tmem + kTreeOCol + grp * HD, tmem + grp * kTreeKeys + k * 8, vd + (k * 2048 >> 4),
+                                         kIdescPV, (i > 1 || k > 0) ? 1u : 0u);
+                        }
                     }
-                    if (!g.two_tiles || grp == 1) umma_commit(smem_u32(&sh.empty[buf]));
-                    if (i == g.jobs - 1) umma_commit(smem_u32(&sh.seg_done));
+                    p_phase[grp] ^= 1;
+                    if (!two || grp == 1) umma_commit(smem_u32(&sh.empty[v_buf]));
+                    if (i == jobs - 1) umma_commit(smem_u32(&sh.seg_done));
                     return true;
                 };
-                ok = mbar_wait(smem_u32(&sh.q_full), segs & 1);
-                ++segs;
-                if (ok) ok = issue_s(0) && (g.jobs < 2 || issue_s(1));
-                for (int i = 0; ok && i < g.jobs; ++i) ok = issue_pv(i) && (i + 2 >= g.jobs || issue_s(i + 2));
-                ring_at += 2 * T;
+                if (jobs > 0) {
+                    ok = mbar_wait(smem_u32(&sh.q_full), q_seen & 1);
+                    ++q_seen;
+                    if (ok) ok = issue_s(0) && (jobs < 2 || issue_s(1));
+                    for (int i = 0; ok && i < jobs; ++i) ok = issue_pv(i) && (i + 2 >= jobs || issue_s(i + 2));
+                    if (!ok) break;
+                }
+                tree_release(sh, seg);
             }
             if (!ok) sh.abort_flag = 1;
         }
     } else {
-        const int grp = (warp - 2) / 4, quad = warp % 4;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTreeSoftmaxRegs));
+        const int grp = (warp - 4) / 4, quad = warp % 4;
         const int r = quad * 32 + lane;
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + lane_off + grp * kTreeKeys;
         const uint32_t o_addr = tmem + lane_off + kTreeOCol + grp * HD;
         const int node_of_r = r / p.group, head_of_r = r % p.group;
-        int done_s = 0, done_seg = 0, done_x = 0;
-        bool ok = true, cut = false;
-        int cut_first_slot = 0, cut_parts = 0;
-        TreeSegment cut_seg;
-        long long at_unit = u0;
-        bool first_seg = true;
-        while (ok && walk.next(p, g)) {
-            const int T = g.t1 - g.t0;
-            const int tile_grp = g.two_tiles ? grp : 0;
-            const int node = g.node0 + tile_grp * p.tile_nodes + node_of_r;
+        uint32_t s_phase = 0, done_phase = 0, x_phase = 0;
+        bool ok = true;
+        for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
+            const TreeSegment &g = sh.queue[seg % kTreeQueue];
+            const int jobs = g.jobs, T = g.t1 - g.t0;
+            const bool two = g.two_tiles;
+            const int node = g.node0 + (two ? grp * p.tile_nodes : 0) + node_of_r;
             const bool live = node_of_r < p.tile_nodes && node < g.node0 + g.nodes;
             const int row = g.row0 + node;
-            const int head = g.kvh * p.group + head_of_r;
-            uint16_t *out_row = p.out + ((long long)row * p.q_heads + head) * HD;
-            const bool whole = g.t0 == g.first_tile && g.t1 == g.last_tile;
-            const int slot = first_seg ? 0 : 1;
-            if (g.t0 == g.first_tile && !whole) {
-                cut = true;
-                cut_first_slot = slot;
-                cut_seg = g;
-                cut_parts = (int)((at_unit + (g.last_tile - g.first_tile) - 1) / share - blockIdx.x) + 1;
-            }
-            at_unit += T;
-            first_seg = false;
-            if (g.jobs == 0) {
-                if (live && (g.two_tiles || grp == 0)) {
+            uint16_t *out_row = p.out + ((long long)row * p.q_heads + g.kvh * p.group + head_of_r) * HD;
+            if (jobs == 0) {
+                if (live && (two || grp == 0)) {
 #pragma unroll
                     for (int i = 0; i < HD / 8; ++i) reinterpret_cast<uint4 *>(out_row)[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
+                __syncwarp();
+                if (lane == 0) tree_release(sh, seg);
                 continue;
             }
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
+            const int ctx = g.ctx;
             float m_run = -INFINITY, l_run = 0.0f;
-            for (int i = grp; i < g.jobs; i += 2) {
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.s_full[grp]), done_s & 1))) {
+            for (int i = grp; i < jobs; i += 2) {
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.s_full[grp]), s_phase))) {
                     ok = false;
                     break;
                 }
-                ++done_s;
-                const int tile = g.two_tiles ? i >> 1 : i;
-                const int at = ring_at + tree_pos_v(g.two_tiles, tile, T), buf = at % C::kBufs;
+                s_phase ^= 1;
+                tc_fence_after();
+                float sc[kTreeKeys];
+                if (warp_live) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, sc + c * 32);
+                }
+                const int tile = two ? i >> 1 : i;
+                const int at = ring_at + tree_pos_v(two, tile, T), buf = at % C::kBufs;
                 // V of this tile stays until this group's P is consumed, so
                 // its phase cannot have moved on.
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.full[buf]), (at / C::kBufs) & 1))) {
+                    tmem_wait_ld();
                     ok = false;
                     break;
                 }
-                tc_fence_after();
                 const int p0 = (g.t0 + tile) * kTreeKeys;
                 const uint32_t valid = sh.valid[buf];
-                const bool masked = p.window > 0 || p0 + kTreeKeys > g.ctx || valid != 0xFFu;
-                uint32_t vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                const bool masked = p.window > 0 || p0 + kTreeKeys > ctx || valid != 0xFFu;
+                tmem_wait_ld();
                 if (masked) {
-                    // V row r: zero where no position is, finite elsewhere.
-                    uint8_t *v_row = ring + buf * C::kTile + r * 128;
-                    const bool holds = p0 + r < g.len && (valid >> (r >> 4) & 1);
-#pragma unroll 1
-                    for (int c = 0; c < HD / 8; ++c) {
-                        uint4 *cell = reinterpret_cast<uint4 *>(v_row + (c >> 3) * C::kHalfBytes + (c & 7) * 16);
-                        if (!holds) {
-                            *cell = make_uint4(0u, 0u, 0u, 0u);
-                            continue;
-                        }
-                        uint32_t w[4] = {cell->x, cell->y, cell->z, cell->w};
-                        bool bad = false;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if (bf16_non_finite(w[x])) {
-                                w[x] &= 0xFFFF0000u;
-                                bad = true;
-                            }
-                            if (bf16_non_finite(w[x] >> 16)) {
-                                w[x] &= 0x0000FFFFu;
-                                bad = true;
-                            }
-                        }
-                        if (bad) {
-                            *reinterpret_cast<volatile int *>(&sh.non_finite) = 1;
-                            __threadfence_block();  // flag before the zeros that hide it from the other group
-                            *cell = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1));
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const uint32_t part = (valid >> (2 * c) & 1 ? 0x0000FFFFu : 0u) | (valid >> (2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
-                        vis[c] = live ? tree_visible(p, g, row, p0 + 32 * c) & part : 0u;
+                        const uint32_t vis = live ? tree_visible(p, g, row, p0 + 32 * c) & part : 0u;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) sc[32 * c + k] = (vis >> k & 1) ? sc[32 * c + k] : -INFINITY;
                     }
                 }
                 if (warp_live) {
                     float mx[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
+                    for (int k = 0; k < 8; ++k) mx[k] = sc[k];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float sc[64];
-                        tmem_ld32_nowait(s_addr + h * 64, sc);
-                        tmem_ld32_nowait(s_addr + h * 64 + 32, sc + 32);
-                        tmem_wait_ld();
-                        if (masked) {
-#pragma unroll
-                            for (int k = 0; k < 64; ++k) sc[k] = (vis[2 * h + (k >> 5)] >> (k & 31) & 1) ? sc[k] : -INFINITY;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 64; ++k) mx[k & 7] = fmaxf(mx[k & 7], sc[k]);
-                    }
+                    for (int k = 8; k < kTreeKeys; ++k) mx[k & 7] = fmaxf(mx[k & 7], sc[k]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], mx[k + 4]);
                     const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
@@ -608,88 +694,84 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
                     if (i > 1 && __any_sync(0xFFFFFFFFu, alpha < 1.0f)) {
 #pragma unroll 1
-                        for (int c = 0; c < HD / 32; ++c) {
-                            float ov[32];
-                            tmem_ld32(o_addr + c * 32, ov);
+                        for (int c = 0; c < HD / 16; ++c) {
+                            float ov[16];
+                            tmem_ld16(o_addr + c * 16, ov);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) ov[k] *= alpha;
-                            tmem_st32(o_addr + c * 32, ov);
+                            for (int k = 0; k < 16; ++k) ov[k] *= alpha;
+                            tmem_st16(o_addr + c * 16, ov);
                         }
                     }
-                    float sums[8];
+                    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) sums[k] = 0.0f;
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float sc[64];
-                        tmem_ld32_nowait(s_addr + h * 64, sc);
-                        tmem_ld32_nowait(s_addr + h * 64 + 32, sc + 32);
-                        tmem_wait_ld();
-                        if (masked) {
-#pragma unroll
-                            for (int k = 0; k < 64; ++k) sc[k] = (vis[2 * h + (k >> 5)] >> (k & 31) & 1) ? sc[k] : -INFINITY;
-                        }
-                        uint32_t w[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const float e0 = fast_exp2(fmaf(sc[2 * k], p.scale_log2, neg_m));
-                            const float e1 = fast_exp2(fmaf(sc[2 * k + 1], p.scale_log2, neg_m));
-                            sums[k & 7] += e0 + e1;
+                        for (int k = 0; k < 16; ++k) {
+                            const float e0 = fast_exp2(fmaf(sc[32 * c + 2 * k], p.scale_log2, neg_m));
+                            const float e1 = fast_exp2(fmaf(sc[32 * c + 2 * k + 1], p.scale_log2, neg_m));
+                            sums[k & 3] += e0 + e1;
                             w[k] = pack_bf16(e0, e1);
                         }
-                        // P columns 32h..32h+31: S columns already read.
-                        tmem_st32_nowait(s_addr + h * 32, w);
+                        tmem_st16_nowait(s_addr + c * 16, w);
+                        if (c & 1) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[grp][c >> 1]));
+                        }
                     }
-                    tmem_wait_st();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sums[k] += sums[k + 4];
                     l_run = l_run * alpha + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
                     m_run = m_new;
+                } else {
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&sh.p_full[grp][0]));
+                        mbar_arrive(smem_u32(&sh.p_full[grp][1]));
+                    }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[grp]));
             }
             ring_at += 2 * T;
             if (!ok) break;
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.seg_done), done_seg & 1))) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.seg_done), done_phase))) {
                 ok = false;
                 break;
             }
-            ++done_seg;
+            done_phase ^= 1;
             tc_fence_after();
             // Weights of this row's accumulators: its own, and the other
             // group's where both hold the same row.
             float w_own = 1.0f, w_other = 0.0f, l = l_run, m = m_run;
-            int d0 = 0, cols = HD;
-            if (!g.two_tiles) {
+            if (!two) {
                 sh.ml[grp][r] = make_float2(m_run, l_run);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.exchange));
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.exchange), done_x & 1))) {
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.exchange), x_phase))) {
                     ok = false;
                     break;
                 }
-                ++done_x;
+                x_phase ^= 1;
                 const float2 other = sh.ml[grp ^ 1][r];
                 m = fmaxf(m_run, other.x);
                 w_own = m_run == -INFINITY ? 0.0f : exp2f(m_run - m);
                 w_other = other.x == -INFINITY ? 0.0f : exp2f(other.x - m);
                 l = l_run * w_own + other.y * w_other;
-                // Group A finishes the first half of the columns, B the second.
-                d0 = grp * (HD / 2);
-                cols = HD / 2;
             }
-            const bool joined = !g.two_tiles && g.jobs > 1;
-            const uint32_t own = o_addr, other_addr = tmem + lane_off + kTreeOCol + (grp ^ 1) * HD;
-            // Where one tile was all, only group A has accumulated.
-            const uint32_t only = tmem + lane_off + kTreeOCol;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const long long part_row = (long long)(2 * blockIdx.x + slot) * 256 + tile_grp * kTreeRows + r;
-            float *part = p.part_o + part_row * HD;
             if (warp_live) {
+                const bool joined = !two && jobs > 1;
+                // Where there was one job, only group A has accumulated.
+                const uint32_t own = two || joined ? o_addr : tmem + lane_off + kTreeOCol;
+                const uint32_t other_addr = tmem + lane_off + kTreeOCol + (grp ^ 1) * HD;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int slot = g.slot;
+                const long long part_row = (long long)(2 * blockIdx.x + max(slot, 0)) * 256 + (two ? grp * kTreeRows : 0) + r;
+                float4 *part = p.part_o + (part_row / 256) * (HD / 4) * 256 + part_row % 256;
+                const uint32_t live_mask = __ballot_sync(0xFFFFFFFFu, live);
+                // Two Q tiles: every column of the own row. One: group A
+                // finishes the first half of the columns, B the second.
+                const int d0 = two ? 0 : grp * (HD / 2), d1 = two ? HD : d0 + HD / 2;
 #pragma unroll 1
-                for (int c = d0; c < d0 + cols; c += 32) {
+                for (int c = d0; c < d1; c += 32) {
                     float ov[32];
                     if (joined) {
                         float ox[32];
@@ -699,26 +781,30 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
                         for (int k = 0; k < 32; ++k) ov[k] = ov[k] * w_own + ox[k] * w_other;
                     } else {
-                        tmem_ld32(g.two_tiles ? own + c : only + c, ov);
+                        tmem_ld32(own + c, ov);
                     }
-                    if (!live) continue;
-                    if (whole) {
+                    if (slot >= 0) {
+                        if (live) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            reinterpret_cast<uint4 *>(out_row + c)[k] =
-                                make_uint4(pack_bf16(ov[8 * k] * inv, ov[8 * k + 1] * inv), pack_bf16(ov[8 * k + 2] * inv, ov[8 * k + 3] * inv),
-                                           pack_bf16(ov[8 * k + 4] * inv, ov[8 * k + 5] * inv), pack_bf16(ov[8 * k + 6] * inv, ov[8 * k + 7] * inv));
+                            for (int k = 0; k < 8; ++k)
+                                part[(c / 4 + k) * 256] = make_float4(ov[4 * k], ov[4 * k + 1], ov[4 * k + 2], ov[4 * k + 3]);
                         }
                     } else {
+                        // 64 bytes of a row: 4 lanes write them together.
+                        uint32_t v[4][4];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            reinterpret_cast<float4 *>(part + c)[k] = make_float4(ov[4 * k], ov[4 * k + 1], ov[4 * k + 2], ov[4 * k + 3]);
+                        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) v[k][x] = pack_bf16(ov[8 * k + 2 * x] * inv, ov[8 * k + 2 * x + 1] * inv);
+                        }
+                        store_rows4(out_row + c, v, live_mask);
                     }
                 }
+                __syncwarp();  // patch_row reads what the warp has stored
                 if (live) {
-                    if (!whole && (g.two_tiles || grp == 0)) p.part_ml[part_row] = make_float2(m, l);
+                    if (slot >= 0 && (two || grp == 0)) p.part_ml[part_row] = make_float2(m, l);
                     if (*reinterpret_cast<volatile int *>(&sh.non_finite))
-                        patch_row<HD>(p, g, row, d0, cols, out_row, whole ? nullptr : part);
+                        patch_row<HD>(p, g, row, d0, d1 - d0, out_row, slot >= 0 ? reinterpret_cast<float *>(part) : nullptr);
                 }
             }
             tc_fence_before();
@@ -726,32 +812,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             // neither group may fall a segment behind the other's barriers.
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.exchange));
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.exchange), done_x & 1))) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.exchange), x_phase))) {
                 ok = false;
                 break;
             }
-            ++done_x;
+            x_phase ^= 1;
+            if (lane == 0) tree_release(sh, seg);
         }
         if (!ok) sh.abort_flag = 1;
-        if (threadIdx.x == 2 * kWarp) {
-            TreeSplit s = {};
-            if (cut) {
-                s.row0 = cut_seg.row0 + cut_seg.node0;
-                s.nodes = cut_seg.nodes;
-                s.kvh = cut_seg.kvh;
-                s.two_tiles = cut_seg.two_tiles;
-                s.first_slot = cut_first_slot;
-                s.parts = cut_parts;
-            }
-            p.splits[blockIdx.x] = s;
-        }
     }
     tc_fence_before();
     __syncthreads();
     if (sh.abort_flag) {
         // A wait gave up: let this CTA's copies and MMAs still in flight land
         // before its shared memory and TMEM are released (bounded waits).
-        if (warp == 0 && lane == 0) {
+        if ((warp == 0 || warp == 2) && lane == 0) {
             if (q_issued > 0) mbar_wait(smem_u32(&sh.q_full), (q_issued - 1) & 1);
             for (int at = max(0, issued - C::kBufs); at < issued; ++at)
                 mbar_wait(smem_u32(&sh.full[at % C::kBufs]), (at / C::kBufs) & 1);
@@ -769,32 +844,67 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 }
 
 // Joins the parts of the items that shares cut: o = sum_k 2^(m_k - m) o_k /
-// sum_k 2^(m_k - m) l_k, parts in key order. CTA (x, y): the item that CTA x
-// began, every kTreeMergeSplit-th block of its rows; HD/4 lanes per row.
+// sum_k 2^(m_k - m) l_k, parts in a fixed order. The CTAs list the split items
+// and share their blocks of 32 rows x 32 columns: a lane per row, a warp per
+// four columns (as the parts lie in the workspace), then the block is written
+// from shared memory row by row.
 template <int HD>
-__global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const TreeAttnParams p) {
-    constexpr int kLanes = HD / 4;
-    constexpr int kRowsPerCta = kTreeMergeThreads / kLanes;
+__global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const TreeAttnParams p, int ctas) {
+    static_assert(kTreeMaxCtas == kTreeMergeThreads, "a thread per listed CTA");
+    static_assert(kTreeMergeWarps == 8, "a warp per four of 32 columns");
+    constexpr int kColBlocks = HD / 32;
+    __shared__ TreeSplit split_s[kTreeMaxCtas];
+    __shared__ int unit_end[kTreeMaxCtas];
+    __shared__ int warp_units[kTreeMergeWarps];
+    __shared__ uint2 block_s[kWarp][kTreeMergeWarps + 1];
+    const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
     pdl_wait();
     pdl_launch_dependents();
-    const TreeSplit s = p.splits[blockIdx.x];
-    if (s.parts < 2) return;
-    const int lane = threadIdx.x % kLanes;
-    const int first = 2 * blockIdx.x + s.first_slot;
-    for (int i = blockIdx.y * kRowsPerCta + threadIdx.x / kLanes; i < s.nodes * p.group; i += kTreeMergeSplit * kRowsPerCta) {
-        const int node = i / p.group, head = i % p.group;
+    int units = 0;
+    if (tid < ctas) {
+        const TreeSplit s = p.splits[tid];
+        split_s[tid] = s;
+        units = s.parts > 1 ? (s.nodes * p.group + kWarp - 1) / kWarp * kColBlocks : 0;
+    }
+#pragma unroll
+    for (int o = 1; o < kWarp; o <<= 1) {
+        const int up = __shfl_up_sync(0xFFFFFFFFu, units, o);
+        if (lane >= o) units += up;
+    }
+    if (lane == kWarp - 1) warp_units[warp] = units;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) units += warp_units[w];
+    unit_end[tid] = units;
+    __syncthreads();
+    const int total = unit_end[kTreeMergeThreads - 1];
+    for (int u = blockIdx.x; u < total; u += gridDim.x) {
+        int c = 0, hi = kTreeMergeThreads - 1;
+        while (c < hi) {
+            const int mid = (c + hi) >> 1;
+            if (unit_end[mid] > u) hi = mid;
+            else c = mid + 1;
+        }
+        const TreeSplit s = split_s[c];
+        const int at = u - (c > 0 ? unit_end[c - 1] : 0);
+        const int col = at % kColBlocks;
+        const int i0 = at / kColBlocks * kWarp;
+        const int rows = s.nodes * p.group;
+        const int i = min(i0 + lane, rows - 1);
+        const int node = i / p.group;
         const int tile = node / p.tile_nodes;
-        const int r = tile * kTreeRows + (node - tile * p.tile_nodes) * p.group + head;
-        auto part_at = [&](int k) -> long long { return (long long)(k == 0 ? first : 2 * (blockIdx.x + k)) * 256 + r; };
+        const int r = tile * kTreeRows + i - tile * p.tile_nodes * p.group;
+        auto slot_of = [&](int k) -> int { return k == 0 ? 2 * c + s.first_slot : 2 * (c + k); };
         float m = -INFINITY;
-        for (int k = 0; k < s.parts; ++k) m = fmaxf(m, p.part_ml[part_at(k)].x);
+#pragma unroll 8
+        for (int k = 0; k < s.parts; ++k) m = fmaxf(m, p.part_ml[slot_of(k) * 256 + r].x);
         float l = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+        const float4 *part = p.part_o + (long long)(col * 8 + warp) * 256 + r;
+#pragma unroll 8
         for (int k = 0; k < s.parts; ++k) {
-            const long long at = part_at(k);
-            const float2 ml = p.part_ml[at];
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at * HD + lane * 4);
+            const int slot = slot_of(k);
+            const float2 ml = p.part_ml[slot * 256 + r];
+            const float4 v = part[(long long)slot * (HD / 4) * 256];
             const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
             l = fmaf(ml.y, w, l);
             o.x = fmaf(v.x, w, o.x);
@@ -803,8 +913,15 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const Tre
             o.w = fmaf(v.w, w, o.w);
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *reinterpret_cast<uint2 *>(p.out + ((long long)(s.row0 + node) * p.q_heads + s.kvh * p.group + head) * HD + lane * 4) =
-            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        block_s[lane][warp] = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        __syncthreads();
+        const int j = i0 + tid / kTreeMergeWarps;  // 8 threads write 64 bytes of a row
+        if (j < rows) {
+            const int n = j / p.group, h = j - n * p.group;
+            *reinterpret_cast<uint2 *>(p.out + ((long long)(s.row0 + n) * p.q_heads + s.kvh * p.group + h) * HD + col * 32 +
+                                       (tid % kTreeMergeWarps) * 4) = block_s[tid / kTreeMergeWarps][tid % kTreeMergeWarps];
+        }
+        __syncthreads();
     }
 }
 

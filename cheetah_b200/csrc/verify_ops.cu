@@ -108,7 +108,9 @@ int launch_logprobs(const cheetah::LogprobParams &p, bool bf16, cudaStream_t str
     return 0;
 }
 
-// Workspace of a tree attention call on a GPU of `ctas` SMs.
+int tree_ctas(int device) { return std::min(cheetah::sm_count(device), cheetah::kTreeMaxCtas); }
+
+// Workspace of a tree attention call of `ctas` CTAs.
 struct TreeWorkspace {
     size_t splits, ml, o, bytes;
 };
@@ -130,8 +132,8 @@ int launch_tree_attention(const CUtensorMap &q_map, const CUtensorMap &k_map, co
     CH_CUDA_TRY(cheetah::allow_smem(cheetah::tree_attention_kernel<HD>, smem, device, done));
     CH_CUDA_TRY(launch_ex(cheetah::tree_attention_kernel<HD>, dim3(ctas), dim3(cheetah::kTreeThreads), smem, stream, true,
                           q_map, k_map, v_map, p));
-    CH_CUDA_TRY(launch_ex(cheetah::tree_merge_kernel<HD>, dim3(ctas, cheetah::kTreeMergeSplit), dim3(cheetah::kTreeMergeThreads),
-                          0, stream, true, p));
+    CH_CUDA_TRY(launch_ex(cheetah::tree_merge_kernel<HD>, dim3(ctas * cheetah::kTreeMergeCtas), dim3(cheetah::kTreeMergeThreads),
+                          0, stream, true, p, ctas));
     return 0;
 }
 
@@ -249,6 +251,11 @@ static int check_tree_attention(const CheetahCudaTreeAttention *a) {
                "cheetah_cuda_op_tree_attention: a pool holds 1 .. 2^31-1 rows of one head, a table row as many tokens");
     CH_REQUIRE(a->mask_words > 0 && a->mask_words <= 16, "cheetah_cuda_op_tree_attention: mask_words must be 1..16");
     CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu, "cheetah_cuda_op_tree_attention: sliding_window is too large");
+    // The kernel counts (item, key tile) units in 31 bits.
+    const uint64_t tile_rows = 2 * (cheetah::kTreeRows / (a->q_heads / a->kv_heads));
+    const uint64_t items = ((uint64_t)a->rows / tile_rows + a->batch + 1) * a->kv_heads;
+    const uint64_t tiles = (uint64_t)a->max_pages_per_seq * a->page_tokens / cheetah::kTreeKeys + 1;
+    CH_REQUIRE(items * tiles <= 0x7FFFFFFFull, "cheetah_cuda_op_tree_attention: too many rows and cached positions");
     return 0;
 }
 
@@ -257,7 +264,7 @@ int cheetah_cuda_op_tree_attention_workspace(const CheetahCudaTreeAttention *a, 
     if (check_tree_attention(a) != 0) return -1;
     int device = 0;
     CH_CUDA_TRY(cudaGetDevice(&device));
-    *bytes = tree_workspace(cheetah::sm_count(device), a->head_dim).bytes;
+    *bytes = tree_workspace(tree_ctas(device), a->head_dim).bytes;
     return 0;
 }
 
@@ -276,7 +283,7 @@ int cheetah_cuda_op_tree_attention(const CheetahCudaTreeAttention *a, void *stre
                "workspace 256-byte");
     int device = 0;
     CH_CUDA_TRY(cudaGetDevice(&device));
-    const int ctas = cheetah::sm_count(device);
+    const int ctas = tree_ctas(device);
     const TreeWorkspace w = tree_workspace(ctas, a->head_dim);
     CH_REQUIRE(a->workspace_bytes >= w.bytes,
                "cheetah_cuda_op_tree_attention: the workspace holds " + std::to_string(a->workspace_bytes) + " of " +
@@ -306,7 +313,7 @@ int cheetah_cuda_op_tree_attention(const CheetahCudaTreeAttention *a, void *stre
     uint8_t *ws = static_cast<uint8_t *>(a->workspace);
     p.splits = reinterpret_cast<cheetah::TreeSplit *>(ws + w.splits);
     p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
-    p.part_o = reinterpret_cast<float *>(ws + w.o);
+    p.part_o = reinterpret_cast<float4 *>(ws + w.o);
     CUtensorMap q_map, k_map, v_map;
     const uint64_t rows = (uint64_t)a->num_pages * a->kv_heads * a->page_tokens;
     if (make_q_map(&q_map, *a, group, (uint32_t)p.tile_nodes) != 0 ||
