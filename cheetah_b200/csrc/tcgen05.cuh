@@ -32,6 +32,19 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t a, uint64_t 
         : "memory");
 }
 
+// One lane of a converged warp. MMAs issued under this predicate keep their
+// descriptors in uniform registers; under `lane == 0` each costs about 50
+// cycles of issue instead of 15.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 // A from TMEM (row = lane, two bf16 of consecutive k per column), B from shared memory.
 __device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc,
                                              uint32_t accumulate) {

@@ -22,7 +22,7 @@
 //   warps 0, 2 TMA producers of Q and K, and of V: boxes [64 dims, group
 //              heads, nodes] of Q, boxes of up to 64 keys of one page, through
 //              a ring of single K or V tiles in the order the MMAs use them;
-//   warp 1     owns TMEM; lane 0 issues S = Q K^T (128 x 128) and O += P V for
+//   warp 1     owns TMEM; one lane issues S = Q K^T (128 x 128) and O += P V for
 //              jobs i = 0, 1, 2, ... of the groups i % 2: S(0), S(1), then
 //              PV(i), S(i+2), so one group's products run during the other's
 //              softmax;
@@ -545,35 +545,37 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         }
         if (!ok) sh.abort_flag = 1;
     } else if (warp == 1) {
-        if (lane == 0) {
-            int q_seen = 0;
-            uint32_t p_phase[2] = {0, 0};
-            // The next ring position; buffers are first used in ring order.
-            int next_buf = 0;
-            uint32_t next_phase = 0;
-            int k_buf = 0, v_buf = 0;
-            const uint64_t q_desc = umma_smem_desc(smem_u32(q_s));
-            const uint64_t k_desc = umma_smem_desc(smem_u32(ring));
-            const uint64_t v_desc = umma_smem_desc_mn(smem_u32(ring), HD > 64 ? C::kHalfBytes : 16);
-            bool ok = true;
-            auto take = [&](int &buf) -> bool {
-                buf = next_buf;
-                const bool landed = mbar_wait(smem_u32(&sh.full[buf]), next_phase);
-                if (++next_buf == C::kBufs) {
-                    next_buf = 0;
-                    next_phase ^= 1;
-                }
-                return landed;
-            };
-            for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
-                const bool two = sh.queue[seg % kTreeQueue].two_tiles;
-                const int jobs = sh.queue[seg % kTreeQueue].jobs;
-                auto issue_s = [&](int i) -> bool {
-                    const int grp = i & 1;
-                    if ((!two || grp == 0) && !take(k_buf)) return false;
-                    tc_fence_after();
-                    const uint64_t qd = q_desc + (two ? grp * (C::kTile >> 4) : 0);
-                    const uint64_t kd = k_desc + (uint32_t)(k_buf * (C::kTile >> 4));
+        // The whole warp walks, one elected lane issues.
+        const bool leader = elect_one();
+        uint32_t q_phase = 0, p_phase[2] = {0, 0};
+        // The next ring position; buffers are first used in ring order.
+        int next_buf = 0;
+        uint32_t next_phase = 0;
+        int k_buf = 0, v_buf = 0;
+        const uint64_t q_desc = umma_smem_desc(smem_u32(q_s));
+        const uint64_t k_desc = umma_smem_desc(smem_u32(ring));
+        const uint64_t v_desc = umma_smem_desc_mn(smem_u32(ring), HD > 64 ? C::kHalfBytes : 16);
+        bool ok = true;
+        auto wait = [&](uint64_t &bar, uint32_t phase) -> bool { return __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&bar), phase)); };
+        auto take = [&](int &buf) -> bool {
+            buf = next_buf;
+            const bool landed = wait(sh.full[buf], next_phase);
+            if (++next_buf == C::kBufs) {
+                next_buf = 0;
+                next_phase ^= 1;
+            }
+            return landed;
+        };
+        for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
+            const bool two = sh.queue[seg % kTreeQueue].two_tiles;
+            const int jobs = sh.queue[seg % kTreeQueue].jobs;
+            auto issue_s = [&](int i) -> bool {
+                const int grp = i & 1;
+                if ((!two || grp == 0) && !take(k_buf)) return false;
+                tc_fence_after();
+                const uint64_t qd = q_desc + (two ? grp * (C::kTile >> 4) : 0);
+                const uint64_t kd = k_desc + (uint32_t)(k_buf * (C::kTile >> 4));
+                if (leader) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
                         const uint32_t off = (uint32_t)((k >> 2) * C::kHalfBytes + (k & 3) * 32) >> 4;
@@ -582,38 +584,46 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     umma_commit(smem_u32(&sh.s_full[grp]));
                     if (!two || grp == 1) umma_commit(smem_u32(&sh.empty[k_buf]));
                     if (i == jobs - 1) umma_commit(smem_u32(&sh.q_empty));
-                    return true;
-                };
-                auto issue_pv = [&](int i) -> bool {
-                    const int grp = i & 1;
-                    if ((!two || grp == 0) && !take(v_buf)) return false;
-                    const uint64_t vd = v_desc + (uint32_t)(v_buf * (C::kTile >> 4));
+                }
+                __syncwarp();
+                return true;
+            };
+            auto issue_pv = [&](int i) -> bool {
+                const int grp = i & 1;
+                if ((!two || grp == 0) && !take(v_buf)) return false;
+                const uint64_t vd = v_desc + (uint32_t)(v_buf * (C::kTile >> 4));
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (!mbar_wait(smem_u32(&sh.p_full[grp][h]), p_phase[grp])) return false;
-                        tc_fence_after();
+                for (int h = 0; h < 2; ++h) {
+                    if (!wait(sh.p_full[grp][h], p_phase[grp])) return false;
+                    tc_fence_after();
+                    if (leader) {
 #pragma unroll
                         for (int k = 4 * h; k < 4 * h + 4; ++k) {
                             umma_bf16_ta(tmem + kTreeOCol + grp * HD, tmem + grp * kTreeKeys + k * 8, vd + (k * 2048 >> 4),
                                          kIdescPV, (i > 1 || k > 0) ? 1u : 0u);
                         }
                     }
-                    p_phase[grp] ^= 1;
+                    __syncwarp();
+                }
+                p_phase[grp] ^= 1;
+                if (leader) {
                     if (!two || grp == 1) umma_commit(smem_u32(&sh.empty[v_buf]));
                     if (i == jobs - 1) umma_commit(smem_u32(&sh.seg_done));
-                    return true;
-                };
-                if (jobs > 0) {
-                    ok = mbar_wait(smem_u32(&sh.q_full), q_seen & 1);
-                    ++q_seen;
-                    if (ok) ok = issue_s(0) && (jobs < 2 || issue_s(1));
-                    for (int i = 0; ok && i < jobs; ++i) ok = issue_pv(i) && (i + 2 >= jobs || issue_s(i + 2));
-                    if (!ok) break;
                 }
-                tree_release(sh, seg);
+                __syncwarp();
+                return true;
+            };
+            if (jobs > 0) {
+                ok = wait(sh.q_full, q_phase);
+                q_phase ^= 1;
+                if (ok) ok = issue_s(0) && (jobs < 2 || issue_s(1));
+                for (int i = 0; ok && i < jobs; ++i) ok = issue_pv(i) && (i + 2 >= jobs || issue_s(i + 2));
+                if (!ok) break;
             }
-            if (!ok) sh.abort_flag = 1;
+            if (lane == 0) tree_release(sh, seg);
+            __syncwarp();
         }
+        if (!ok) sh.abort_flag = 1;
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTreeSoftmaxRegs));
         const int grp = (warp - 4) / 4, quad = warp % 4;
