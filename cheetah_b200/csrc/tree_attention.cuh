@@ -22,19 +22,22 @@
 //   warps 0, 2 TMA producers of Q and K, and of V: boxes [64 dims, group
 //              heads, nodes] of Q, boxes of up to 64 keys of one page, through
 //              a ring of single K or V tiles in the order the MMAs use them;
-//   warp 1     owns TMEM; one lane issues S = Q K^T (128 x 128) and O += P V for
-//              jobs i = 0, 1, 2, ... of the groups i % 2: S(0), S(1), then
-//              PV(i), S(i+2), so one group's products run during the other's
-//              softmax;
+//   warp 1     owns TMEM; one lane issues S = Q K^T (128 x 128) and O += P V
+//              for jobs i = 0, 1, 2, ... of the groups i % 2, so one group's
+//              products run during the other's softmax;
 //   warp 3     scheduler: cuts the CTA's share into segments (a run of key
 //              tiles of one item) and publishes them ahead in a queue;
 //   warps 4-11 two softmax groups, one thread per row: read the S row from
-//              TMEM, mask, exponentials, P as bf16 back into S's columns (the
-//              A operand of PV is read from TMEM) in two halves, so that the
-//              first half's products run during the second's exponentials.
-//              The running maximum moves only when it grows by more than 2^8
-//              (P and l use the same one, so the quotient is the same), and O
-//              is rescaled in TMEM only then.
+//              TMEM 64 keys at a time, mask, exponentials, P as bf16 into
+//              TMEM (the A operand of PV is read from there). The reference m
+//              is a whole number of log2 units that moves only when a score
+//              lies 2^24 above it (P, l and O share it, so the quotient is the
+//              same), so a tile usually takes one pass over S: exponentials
+//              about the old m and the maximum beside them. O, l and P are
+//              rescaled, by a power of two, only when m moves.
+// With head_dim 64 TMEM has columns of its own for P, so S(i + 2) is computed
+// while the softmax of S(i) still runs; with head_dim 128 P takes S's columns
+// and S(i + 2) follows PV(i).
 // P is rounded to bf16 because the tensor cores multiply bf16; sums,
 // statistics and O stay f32.
 //
@@ -60,8 +63,7 @@ constexpr int kTreeKeys = 128;      // keys per tile
 constexpr int kTreeRows = 128;      // rows of a Q tile
 constexpr int kTreeThreads = 384;   // warpgroups: loads and MMAs, softmax A, softmax B
 constexpr int kTreeMinShare = 2;    // key tiles a CTA takes at least (one per softmax group)
-constexpr float kTreeRescaleLog2 = 8.0f;
-constexpr uint32_t kTreeOCol = 256; // S_A | S_B | O_A | O_B
+constexpr float kTreeHeadroomLog2 = 24.0f;
 constexpr int kTreeMergeThreads = 256;
 constexpr int kTreeMergeCtas = 4;     // per SM
 constexpr int kTreeMergeWarps = kTreeMergeThreads / kWarp;
@@ -78,6 +80,13 @@ struct TreeCfg {
     static constexpr int kTile = kTreeKeys * HD * 2;     // one K, V or Q tile
     static constexpr int kBufs = HD == 64 ? 12 : 5;      // ring
     static constexpr int kTiles = 2 * kTile + kBufs * kTile;
+    // TMEM columns: S_A | S_B | O_A | O_B and, where they fit, P_A | P_B;
+    // else P takes the columns of the S it came from.
+    static constexpr bool kOwnP = HD == 64;
+    static constexpr uint32_t kOCol = 2 * kTreeKeys;
+    static constexpr uint32_t kPCol = kOwnP ? kOCol + 2 * HD : 0;
+    static constexpr uint32_t kPStep = kOwnP ? kTreeKeys / 2 : kTreeKeys;  // columns from P_A to P_B
+    static_assert((kOwnP ? kPCol + kTreeKeys : kOCol + 2 * HD) <= 512, "TMEM columns");
 };
 
 // What a split item needs to be joined, written by the CTA that begins it.
@@ -143,11 +152,18 @@ __device__ __forceinline__ int tree_units(const TreeAttnParams &p, int b) {
 }
 
 // The ring position of tile i's K and V within a segment of T tiles, in the
-// order of first use: K0 V0 K1 V1 .. where both groups use each tile, and
-// K0 K1 V0 K2 V1 K3 .. where they alternate.
-__device__ __forceinline__ int tree_pos_k(bool two, int i) { return two ? 2 * i : (i < 2 ? i : 2 * i - 1); }
+// order of first use. Both groups on each tile: K0 V0 K1 V1 .., or K0 K1 V0
+// K2 V1 .. with S a job ahead; alternating groups: K0 K1 V0 K2 V1 K3 .., or
+// K0 K1 K2 V0 K3 V1 ...
+template <bool kAhead>
+__device__ __forceinline__ int tree_pos_k(bool two, int i) {
+    if (kAhead) return two ? max(2 * i - 1, 0) : (i < 2 ? i : 2 * i - 2);
+    return two ? 2 * i : (i < 2 ? i : 2 * i - 1);
+}
+template <bool kAhead>
 __device__ __forceinline__ int tree_pos_v(bool two, int i, int T) {
-    return two ? 2 * i + 1 : (T == 1 ? 1 : 2 + i + min(i, T - 2));
+    if (kAhead) return two ? min(2 * i + 2, 2 * T - 1) : min(2 * i + 3, T + i);
+    return two ? 2 * i + 1 : min(2 * i + 2, T + i);
 }
 
 constexpr int kTreeQueue = 4;              // segments the scheduler may be ahead
@@ -155,7 +171,7 @@ constexpr int kTreeQueueReaders = 3 + 8;   // two producers, the MMA thread, the
 struct TreeShared {
     uint64_t full[12], empty[12];
     uint64_t seg_full[kTreeQueue], seg_empty[kTreeQueue];
-    uint64_t q_full, q_empty, s_full[2], p_full[2][2], seg_done, exchange, drain;
+    uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2], seg_done, exchange, drain;
     TreeSegment queue[kTreeQueue];
     int warp_units[kTreeThreads / kWarp];
     uint32_t tmem;
@@ -266,6 +282,37 @@ __device__ __noinline__ void patch_row(const TreeAttnParams &p, const TreeSegmen
     }
 }
 
+// Two f32 per instruction (sm_100's packed forms).
+__device__ __forceinline__ unsigned long long pair_f32(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair_f32(unsigned long long v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Products of two bf16 pairs (exact for powers of two within range).
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Stores 64 bytes of each lane's row (four 16-byte cells), with the four cells
 // of a row written by neighbouring lanes: lane l's v[j] becomes lane j's v[l]
 // among each four lanes, so a store covers 8 rows instead of 32.
@@ -321,8 +368,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         mbar_init(smem_u32(&sh.q_empty), 1);
         for (int g = 0; g < 2; ++g) {
             mbar_init(smem_u32(&sh.s_full[g]), 1);
-            mbar_init(smem_u32(&sh.p_full[g][0]), 4);
-            mbar_init(smem_u32(&sh.p_full[g][1]), 4);
+            mbar_init(smem_u32(&sh.s_free[g]), 4);
+            mbar_init(smem_u32(&sh.p_full[g]), 4);
+            mbar_init(smem_u32(&sh.pv_done[g]), 1);
         }
         mbar_init(smem_u32(&sh.seg_done), 1);
         mbar_init(smem_u32(&sh.exchange), 8);
@@ -481,7 +529,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 int first = -kWarp, my_row = -1;
                 uint32_t loaded = 0;
                 for (int i = 0; i < T; ++i) {
-                    const int at = ring_at + (is_v ? tree_pos_v(two, i, T) : tree_pos_k(two, i));
+                    const int at = ring_at + (is_v ? tree_pos_v<C::kOwnP>(two, i, T) : tree_pos_k<C::kOwnP>(two, i));
                     const int buf = at % C::kBufs;
                     const int box0 = (t0 + i) * boxes;
                     if (box0 >= first + kWarp) {
@@ -547,7 +595,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     } else if (warp == 1) {
         // The whole warp walks, one elected lane issues.
         const bool leader = elect_one();
-        uint32_t q_phase = 0, p_phase[2] = {0, 0};
+        uint32_t q_phase = 0, p_phase[2] = {0, 0}, free_phase[2] = {0, 0};
         // The next ring position; buffers are first used in ring order.
         int next_buf = 0;
         uint32_t next_phase = 0;
@@ -592,32 +640,38 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 const int grp = i & 1;
                 if ((!two || grp == 0) && !take(v_buf)) return false;
                 const uint64_t vd = v_desc + (uint32_t)(v_buf * (C::kTile >> 4));
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (!wait(sh.p_full[grp][h], p_phase[grp])) return false;
-                    tc_fence_after();
-                    if (leader) {
-#pragma unroll
-                        for (int k = 4 * h; k < 4 * h + 4; ++k) {
-                            umma_bf16_ta(tmem + kTreeOCol + grp * HD, tmem + grp * kTreeKeys + k * 8, vd + (k * 2048 >> 4),
-                                         kIdescPV, (i > 1 || k > 0) ? 1u : 0u);
-                        }
-                    }
-                    __syncwarp();
-                }
+                if (!wait(sh.p_full[grp], p_phase[grp])) return false;
                 p_phase[grp] ^= 1;
+                tc_fence_after();
                 if (leader) {
+#pragma unroll
+                    for (int k = 0; k < kTreeKeys / 16; ++k) {
+                        umma_bf16_ta(tmem + C::kOCol + grp * HD, tmem + C::kPCol + grp * C::kPStep + k * 8, vd + (k * 2048 >> 4),
+                                     kIdescPV, (i > 1 || k > 0) ? 1u : 0u);
+                    }
+                    if (C::kOwnP) umma_commit(smem_u32(&sh.pv_done[grp]));
                     if (!two || grp == 1) umma_commit(smem_u32(&sh.empty[v_buf]));
                     if (i == jobs - 1) umma_commit(smem_u32(&sh.seg_done));
                 }
                 __syncwarp();
                 return true;
             };
+            // S(i + 2) goes into S(i)'s columns: once the softmax has read
+            // them, or, where P lies there, behind PV(i).
+            auto free_s = [&](int i) -> bool { return wait(sh.s_free[i & 1], free_phase[i & 1]); };
             if (jobs > 0) {
                 ok = wait(sh.q_full, q_phase);
                 q_phase ^= 1;
                 if (ok) ok = issue_s(0) && (jobs < 2 || issue_s(1));
-                for (int i = 0; ok && i < jobs; ++i) ok = issue_pv(i) && (i + 2 >= jobs || issue_s(i + 2));
+                for (int i = 0; ok && i < jobs; ++i) {
+                    if (C::kOwnP) {
+                        if (i + 2 < jobs) ok = free_s(i) && issue_s(i + 2);
+                        free_phase[i & 1] ^= 1;
+                        ok = ok && issue_pv(i);
+                    } else {
+                        ok = issue_pv(i) && (i + 2 >= jobs || issue_s(i + 2));
+                    }
+                }
                 if (!ok) break;
             }
             if (lane == 0) tree_release(sh, seg);
@@ -630,9 +684,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         const int r = quad * 32 + lane;
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + lane_off + grp * kTreeKeys;
-        const uint32_t o_addr = tmem + lane_off + kTreeOCol + grp * HD;
+        const uint32_t o_addr = tmem + lane_off + C::kOCol + grp * HD;
+        const uint32_t p_addr = tmem + lane_off + C::kPCol + grp * C::kPStep;
         const int node_of_r = r / p.group, head_of_r = r % p.group;
-        uint32_t s_phase = 0, done_phase = 0, x_phase = 0;
+        uint32_t s_phase = 0, pv_phase = 0, done_phase = 0, x_phase = 0;
         bool ok = true;
         for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
             const TreeSegment &g = sh.queue[seg % kTreeQueue];
@@ -661,85 +716,111 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 }
                 s_phase ^= 1;
                 tc_fence_after();
-                float sc[kTreeKeys];
-                if (warp_live) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32_nowait(s_addr + c * 32, sc + c * 32);
-                }
                 const int tile = two ? i >> 1 : i;
-                const int at = ring_at + tree_pos_v(two, tile, T), buf = at % C::kBufs;
+                const int at = ring_at + tree_pos_v<C::kOwnP>(two, tile, T), buf = at % C::kBufs;
                 // V of this tile stays until this group's P is consumed, so
                 // its phase cannot have moved on.
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.full[buf]), (at / C::kBufs) & 1))) {
-                    tmem_wait_ld();
-                    ok = false;
-                    break;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.full[buf]), (at / C::kBufs) & 1));
+                // P's columns and O are this thread's once PV(i - 2) is done
+                // (where P lies in S's columns, S(i) has come after it).
+                if (C::kOwnP) {
+                    if (ok && i > 1) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.pv_done[grp]), pv_phase ^ 1));
+                    pv_phase ^= 1;
                 }
+                if (!ok) break;
+                tc_fence_after();
                 const int p0 = (g.t0 + tile) * kTreeKeys;
                 const uint32_t valid = sh.valid[buf];
                 const bool masked = p.window > 0 || p0 + kTreeKeys > ctx || valid != 0xFFu;
-                tmem_wait_ld();
-                if (masked) {
+                if (masked)
                     tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1));
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t part = (valid >> (2 * c) & 1 ? 0x0000FFFFu : 0u) | (valid >> (2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
-                        const uint32_t vis = live ? tree_visible(p, g, row, p0 + 32 * c) & part : 0u;
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) sc[32 * c + k] = (vis >> k & 1) ? sc[32 * c + k] : -INFINITY;
-                    }
-                }
                 if (warp_live) {
-                    float mx[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) mx[k] = sc[k];
-#pragma unroll
-                    for (int k = 8; k < kTreeKeys; ++k) mx[k & 7] = fmaxf(mx[k & 7], sc[k]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], mx[k + 4]);
-                    const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                    const float m_cand = fmaxf(m_run, tmax);
-                    const float m_new = m_cand > m_run + kTreeRescaleLog2 ? m_cand : m_run;
-                    const float alpha = m_new == -INFINITY ? 1.0f : exp2f(m_run - m_new);
-                    const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;
-                    if (i > 1 && __any_sync(0xFFFFFFFFu, alpha < 1.0f)) {
+                    const unsigned long long scale2 = pair_f32(p.scale_log2, p.scale_log2);
 #pragma unroll 1
-                        for (int c = 0; c < HD / 16; ++c) {
-                            float ov[16];
-                            tmem_ld16(o_addr + c * 16, ov);
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) ov[k] *= alpha;
-                            tmem_st16(o_addr + c * 16, ov);
-                        }
-                    }
-                    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float e0 = fast_exp2(fmaf(sc[32 * c + 2 * k], p.scale_log2, neg_m));
-                            const float e1 = fast_exp2(fmaf(sc[32 * c + 2 * k + 1], p.scale_log2, neg_m));
-                            sums[k & 3] += e0 + e1;
-                            w[k] = pack_bf16(e0, e1);
-                        }
-                        tmem_st16_nowait(s_addr + c * 16, w);
-                        if (c & 1) {
-                            tmem_wait_st();
+                    for (int h = 0; h < 2; ++h) {
+                        float sc[64];
+                        tmem_ld32_nowait(s_addr + h * 64, sc);
+                        tmem_ld32_nowait(s_addr + h * 64 + 32, sc + 32);
+                        tmem_wait_ld();
+                        if (C::kOwnP && h == 1) {
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[grp][c >> 1]));
+                            if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[grp]));
                         }
+                        if (masked) {
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const uint32_t part = (valid >> (4 * h + 2 * c) & 1 ? 0x0000FFFFu : 0u) |
+                                                      (valid >> (4 * h + 2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
+                                const uint32_t vis = live ? tree_visible(p, g, row, p0 + 64 * h + 32 * c) & part : 0u;
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) sc[32 * c + k] = (vis >> k & 1) ? sc[32 * c + k] : -INFINITY;
+                            }
+                        }
+                        // Exponentials about the present m, and the largest
+                        // score beside them; only if it lies too far above m,
+                        // m moves and they are done again.
+                        uint32_t w[32];
+                        float s0, s1;
+                        while (true) {
+                            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+                            const unsigned long long neg_m2 = pair_f32(neg_m, neg_m);
+                            unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};
+                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                mx[k & 3] = max3(mx[k & 3], sc[2 * k], sc[2 * k + 1]);
+                                float e0, e1;
+                                unpair_f32(fma_pair(pair_f32(sc[2 * k], sc[2 * k + 1]), scale2, neg_m2), e0, e1);
+                                e0 = fast_exp2(e0);
+                                e1 = fast_exp2(e1);
+                                sums[k & 3] = add_pair(sums[k & 3], pair_f32(e0, e1));
+                                w[k] = pack_bf16(e0, e1);
+                            }
+                            unpair_f32(add_pair(add_pair(sums[0], sums[1]), add_pair(sums[2], sums[3])), s0, s1);
+                            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                            const bool far = top > m_run + kTreeHeadroomLog2;
+                            if (!__any_sync(0xFFFFFFFFu, far)) break;
+                            // m is a whole number, so every rescaling is exact.
+                            const float m_new = far ? ceilf(top) : m_run;
+                            const float f = m_new == m_run ? 1.0f : exp2f(m_run - m_new);
+                            m_run = m_new;
+                            l_run *= f;
+                            if (h == 1) {
+                                const uint32_t f2 = pack_bf16(f, f);
+                                tmem_wait_st();
+#pragma unroll 1
+                                for (int c = 0; c < 2; ++c) {
+                                    float pv[16];
+                                    tmem_ld16(p_addr + c * 16, pv);
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) pv[k] = __uint_as_float(mul_bf16x2(__float_as_uint(pv[k]), f2));
+                                    tmem_st16(p_addr + c * 16, pv);
+                                }
+                            }
+                            if (i > 1) {
+#pragma unroll 1
+                                for (int c = 0; c < HD / 16; ++c) {
+                                    float ov[16];
+                                    tmem_ld16(o_addr + c * 16, ov);
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) ov[k] *= f;
+                                    tmem_st16(o_addr + c * 16, ov);
+                                }
+                            }
+                        }
+                        l_run += s0 + s1;
+                        // In S's columns, P's 32 are among the 64 just read.
+                        tmem_st16_nowait(p_addr + h * 32, w);
+                        tmem_st16_nowait(p_addr + h * 32 + 16, w + 16);
                     }
-                    l_run = l_run * alpha + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
-                    m_run = m_new;
-                } else {
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&sh.p_full[grp][0]));
-                        mbar_arrive(smem_u32(&sh.p_full[grp][1]));
-                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                } else if (C::kOwnP && lane == 0) {
+                    mbar_arrive(smem_u32(&sh.s_free[grp]));
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[grp]));
             }
             ring_at += 2 * T;
             if (!ok) break;
@@ -770,8 +851,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             if (warp_live) {
                 const bool joined = !two && jobs > 1;
                 // Where there was one job, only group A has accumulated.
-                const uint32_t own = two || joined ? o_addr : tmem + lane_off + kTreeOCol;
-                const uint32_t other_addr = tmem + lane_off + kTreeOCol + (grp ^ 1) * HD;
+                const uint32_t own = two || joined ? o_addr : tmem + lane_off + C::kOCol;
+                const uint32_t other_addr = tmem + lane_off + C::kOCol + (grp ^ 1) * HD;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const int slot = g.slot;
                 const long long part_row = (long long)(2 * blockIdx.x + max(slot, 0)) * 256 + (two ? grp * kTreeRows : 0) + r;
@@ -854,19 +935,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 }
 
 // Joins the parts of the items that shares cut: o = sum_k 2^(m_k - m) o_k /
-// sum_k 2^(m_k - m) l_k, parts in a fixed order. The CTAs list the split items
-// and share their blocks of 32 rows x 32 columns: a lane per row, a warp per
-// four columns (as the parts lie in the workspace), then the block is written
-// from shared memory row by row.
+// sum_k 2^(m_k - m) l_k, in a fixed order. The CTAs list the split items and
+// share their row blocks. A lane has a row and, where an item has many parts,
+// every fourth of them (then a block is 8 rows instead of 32); a warp has
+// every eighth column group of four, as the parts lie in the workspace. The
+// block is written from shared memory row by row.
 template <int HD>
 __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const TreeAttnParams p, int ctas) {
     static_assert(kTreeMaxCtas == kTreeMergeThreads, "a thread per listed CTA");
-    static_assert(kTreeMergeWarps == 8, "a warp per four of 32 columns");
-    constexpr int kColBlocks = HD / 32;
+    constexpr int kCols = HD / 4 / kTreeMergeWarps;  // column groups of a warp
+    constexpr int kFew = 4;
     __shared__ TreeSplit split_s[kTreeMaxCtas];
     __shared__ int unit_end[kTreeMaxCtas];
     __shared__ int warp_units[kTreeMergeWarps];
-    __shared__ uint2 block_s[kWarp][kTreeMergeWarps + 1];
+    __shared__ uint2 block_s[kWarp][HD / 4 + 1];
     const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
     pdl_wait();
     pdl_launch_dependents();
@@ -874,7 +956,8 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const Tre
     if (tid < ctas) {
         const TreeSplit s = p.splits[tid];
         split_s[tid] = s;
-        units = s.parts > 1 ? (s.nodes * p.group + kWarp - 1) / kWarp * kColBlocks : 0;
+        const int block = s.parts > kFew ? kWarp / 4 : kWarp;
+        units = s.parts > 1 ? (s.nodes * p.group + block - 1) / block : 0;
     }
 #pragma unroll
     for (int o = 1; o < kWarp; o <<= 1) {
@@ -895,41 +978,68 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const Tre
             else c = mid + 1;
         }
         const TreeSplit s = split_s[c];
-        const int at = u - (c > 0 ? unit_end[c - 1] : 0);
-        const int col = at % kColBlocks;
-        const int i0 = at / kColBlocks * kWarp;
+        const bool few = s.parts <= kFew;
+        const int block = few ? kWarp : kWarp / 4, step = few ? 1 : 4;
+        const int i0 = (u - (c > 0 ? unit_end[c - 1] : 0)) * block;
         const int rows = s.nodes * p.group;
-        const int i = min(i0 + lane, rows - 1);
-        const int node = i / p.group;
-        const int tile = node / p.tile_nodes;
+        const int i = min(i0 + lane % block, rows - 1);
+        const int tile = i / (p.tile_nodes * p.group);
         const int r = tile * kTreeRows + i - tile * p.tile_nodes * p.group;
         auto slot_of = [&](int k) -> int { return k == 0 ? 2 * c + s.first_slot : 2 * (c + k); };
         float m = -INFINITY;
-#pragma unroll 8
-        for (int k = 0; k < s.parts; ++k) m = fmaxf(m, p.part_ml[slot_of(k) * 256 + r].x);
+#pragma unroll 4
+        for (int k = lane / block; k < s.parts; k += step) m = fmaxf(m, p.part_ml[slot_of(k) * 256 + r].x);
+        if (!few) {
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
+        }
         float l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float4 *part = p.part_o + (long long)(col * 8 + warp) * 256 + r;
-#pragma unroll 8
-        for (int k = 0; k < s.parts; ++k) {
+        float4 o[kCols];
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int k = lane / block; k < s.parts; k += step) {
             const int slot = slot_of(k);
             const float2 ml = p.part_ml[slot * 256 + r];
-            const float4 v = part[(long long)slot * (HD / 4) * 256];
             const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
             l = fmaf(ml.y, w, l);
-            o.x = fmaf(v.x, w, o.x);
-            o.y = fmaf(v.y, w, o.y);
-            o.z = fmaf(v.z, w, o.z);
-            o.w = fmaf(v.w, w, o.w);
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                const float4 v = p.part_o[((long long)slot * (HD / 4) + j * kTreeMergeWarps + warp) * 256 + r];
+                o[j].x = fmaf(v.x, w, o[j].x);
+                o[j].y = fmaf(v.y, w, o[j].y);
+                o[j].z = fmaf(v.z, w, o[j].z);
+                o[j].w = fmaf(v.w, w, o[j].w);
+            }
+        }
+        if (!few) {
+#pragma unroll
+            for (int x = 8; x < kWarp; x <<= 1) {
+                l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    o[j].x += __shfl_xor_sync(0xFFFFFFFFu, o[j].x, x);
+                    o[j].y += __shfl_xor_sync(0xFFFFFFFFu, o[j].y, x);
+                    o[j].z += __shfl_xor_sync(0xFFFFFFFFu, o[j].z, x);
+                    o[j].w += __shfl_xor_sync(0xFFFFFFFFu, o[j].w, x);
+                }
+            }
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        block_s[lane][warp] = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        if (lane < block) {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                block_s[lane][j * kTreeMergeWarps + warp] =
+                    make_uint2(pack_bf16(o[j].x * inv, o[j].y * inv), pack_bf16(o[j].z * inv, o[j].w * inv));
+            }
+        }
         __syncthreads();
-        const int j = i0 + tid / kTreeMergeWarps;  // 8 threads write 64 bytes of a row
-        if (j < rows) {
+        for (int x = tid; x < block * (HD / 4); x += kTreeMergeThreads) {
+            const int j = i0 + x / (HD / 4);
+            if (j >= rows) break;
             const int n = j / p.group, h = j - n * p.group;
-            *reinterpret_cast<uint2 *>(p.out + ((long long)(s.row0 + n) * p.q_heads + s.kvh * p.group + h) * HD + col * 32 +
-                                       (tid % kTreeMergeWarps) * 4) = block_s[tid / kTreeMergeWarps][tid % kTreeMergeWarps];
+            *reinterpret_cast<uint2 *>(p.out + ((long long)(s.row0 + n) * p.q_heads + s.kvh * p.group + h) * HD + x % (HD / 4) * 4) =
+                block_s[x / (HD / 4)][x % (HD / 4)];
         }
         __syncthreads();
     }
