@@ -62,7 +62,6 @@ namespace cheetah {
 constexpr int kTreeKeys = 128;      // keys per tile
 constexpr int kTreeRows = 128;      // rows of a Q tile
 constexpr int kTreeThreads = 384;   // warpgroups: loads and MMAs, softmax A, softmax B
-constexpr int kTreeMinShare = 2;    // key tiles a CTA takes at least (one per softmax group)
 constexpr float kTreeHeadroomLog2 = 24.0f;
 constexpr int kTreeMergeThreads = 256;
 constexpr int kTreeMergeCtas = 4;     // per SM
@@ -80,6 +79,12 @@ struct TreeCfg {
     static constexpr int kTile = kTreeKeys * HD * 2;     // one K, V or Q tile
     static constexpr int kBufs = HD == 64 ? 12 : 5;      // ring
     static constexpr int kTiles = 2 * kTile + kBufs * kTile;
+    // Cost units of the shares: a key tile of an item with one Q tile (bound
+    // by its loads) and with two (by the products and exponentials), and an
+    // item's beginning and end. Measured in halves of a one-tile key tile.
+    static constexpr int kOne = 2, kTwo = HD == 64 ? 4 : 3, kItem = HD == 64 ? 8 : 6;
+    static constexpr int kMinShare = 4;
+    static_assert(kMinShare >= kTwo, "every share holds a tile");
     // TMEM columns: S_A | S_B | O_A | O_B and, where they fit, P_A | P_B;
     // else P takes the columns of the S it came from.
     static constexpr bool kOwnP = HD == 64;
@@ -130,7 +135,9 @@ struct TreeSegment {
 
 // Rows, context and tile range of sequence b.
 struct TreeSeq {
-    int row0, n, ctx, len, low, tile_lo, tiles, row_items;
+    int row0, n, ctx, len, low, tile_lo, tiles;
+    int pairs;  // items of two Q tiles
+    int items;  // pairs, and one of a single Q tile where nodes are left for it
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnParams &p, int b) {
     TreeSeq s;
@@ -141,14 +148,25 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnParams &p, int b) {
     s.len = (int)min((long long)len, (long long)p.max_pages * p.page_tokens);
     s.low = p.window > 0 ? max(0, s.ctx - p.window + 1) : 0;
     s.tile_lo = s.low / kTreeKeys;
-    // Without room for its rows a sequence is one unit that writes zeros.
+    // Without room for its rows a sequence's items are one tile that writes zeros.
     s.tiles = s.ctx < 0 ? 1 : max(1, (s.len + kTreeKeys - 1) / kTreeKeys - s.tile_lo);
-    s.row_items = (s.n + 2 * p.tile_nodes - 1) / (2 * p.tile_nodes);
+    const int rest = s.n % (2 * p.tile_nodes);
+    s.pairs = s.n / (2 * p.tile_nodes) + (rest > p.tile_nodes);
+    s.items = s.pairs + (rest > 0 && rest <= p.tile_nodes);
     return s;
 }
+template <int HD>
+__device__ __forceinline__ int tree_item_units(const TreeSeq &s, bool two) {
+    return TreeCfg<HD>::kItem + s.tiles * (two ? TreeCfg<HD>::kTwo : TreeCfg<HD>::kOne);
+}
+// Units of one KV head of a sequence.
+template <int HD>
+__device__ __forceinline__ int tree_head_units(const TreeSeq &s) {
+    return s.pairs * tree_item_units<HD>(s, true) + (s.items - s.pairs) * tree_item_units<HD>(s, false);
+}
+template <int HD>
 __device__ __forceinline__ int tree_units(const TreeAttnParams &p, int b) {
-    const TreeSeq s = tree_seq(p, b);
-    return s.row_items * p.kv_heads * s.tiles;
+    return tree_head_units<HD>(tree_seq(p, b)) * p.kv_heads;
 }
 
 // The ring position of tile i's K and V within a segment of T tiles, in the
@@ -233,7 +251,8 @@ template <int HD>
 __device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, bool holds) {
 #pragma unroll 1
     for (int c = 0; c < HD / 8; ++c) {
-        uint4 *cell = reinterpret_cast<uint4 *>(v_row + (c >> 3) * TreeCfg<HD>::kHalfBytes + (c & 7) * 16);
+        // Each lane begins at another cell: the rows lie 128 bytes apart.
+        uint4 *cell = reinterpret_cast<uint4 *>(v_row + (c >> 3) * TreeCfg<HD>::kHalfBytes + ((c + threadIdx.x) & 7) * 16);
         if (!holds) {
             *cell = make_uint4(0u, 0u, 0u, 0u);
             continue;
@@ -392,9 +411,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     // Total units, then the sequence in which this CTA's share begins (the
     // host has checked that the units of any lengths fit 31 bits).
     constexpr int kWarps = kTreeThreads / kWarp;
-    const int mine = (int)threadIdx.x < p.batch ? tree_units(p, threadIdx.x) : 0;
+    const int mine = (int)threadIdx.x < p.batch ? tree_units<HD>(p, threadIdx.x) : 0;
     int sum = mine;
-    for (int b = threadIdx.x + kTreeThreads; b < p.batch; b += kTreeThreads) sum += tree_units(p, b);
+    for (int b = threadIdx.x + kTreeThreads; b < p.batch; b += kTreeThreads) sum += tree_units<HD>(p, b);
     sum = __reduce_add_sync(0xFFFFFFFFu, sum);
     if (lane == 0) sh.warp_units[warp] = sum;
     tc_fence_before();
@@ -404,12 +423,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     int total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) total += sh.warp_units[w];
-    const int share = max(kTreeMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+    const int share = max(C::kMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
     const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
     int before = 0;
     for (int b0 = 0; b0 < p.batch && u0 < total; b0 += kTreeThreads) {
         const int b = b0 + threadIdx.x;
-        const int units = b0 == 0 ? mine : (b < p.batch ? tree_units(p, b) : 0);
+        const int units = b0 == 0 ? mine : (b < p.batch ? tree_units<HD>(p, b) : 0);
         int end = units;
 #pragma unroll
         for (int o = 1; o < kWarp; o <<= 1) {
@@ -445,30 +464,29 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         // Scheduler: walks over the share's items and publishes its segments.
         if (lane == 0) {
             int b = sh.start_b, left = min(share, total - u0), unit = u0, seg = 0;
-            int at = sh.start_off, kvh = 0, rt = 0;
+            TreeSeq s = {};
+            int kvh = 0, rt = 0, at = sh.start_off;  // unit within the item
+            if (left > 0) {
+                s = tree_seq(p, b);
+                const int head = tree_head_units<HD>(s), pair = tree_item_units<HD>(s, true);
+                kvh = at / head;
+                at -= kvh * head;
+                rt = min(at / pair, s.pairs);
+                at -= rt * pair;
+            }
             TreeSplit split = {};
             bool ok = true;
             while (true) {
                 TreeSegment g = {};
                 g.jobs = -1;
-                ok = mbar_wait(smem_u32(&sh.seg_empty[seg % kTreeQueue]), ((seg / kTreeQueue) & 1) ^ 1);
-                if (!ok) break;
-                if (left > 0 && b < p.batch) {
-                    TreeSeq s = tree_seq(p, b);
-                    while (s.row_items == 0 || kvh >= p.kv_heads) {  // no (more) items in b
-                        if (++b >= p.batch) break;
-                        at = kvh = rt = 0;
-                        s = tree_seq(p, b);
-                    }
-                    if (b < p.batch) {
-                        if (at >= s.tiles) {  // the share's beginning: items to skip
-                            const int item = at / s.tiles;
-                            at -= item * s.tiles;
-                            kvh = item / s.row_items;
-                            rt = item - kvh * s.row_items;
-                        }
-                        const int take = min(left, s.tiles - at);
-                        const bool whole = take == s.tiles;
+                while (left > 0) {
+                    const bool two = rt < s.pairs;
+                    const int units = tree_item_units<HD>(s, two), cost = two ? C::kTwo : C::kOne;
+                    const int take = min(left, units - at);
+                    // Tiles of this piece; an item's first kItem units hold none.
+                    const int t0 = max(at - C::kItem, 0) / cost, t1 = max(at + take - C::kItem, 0) / cost;
+                    if (t1 > t0) {
+                        const bool whole = t1 - t0 == s.tiles;
                         g.row0 = s.row0;
                         g.n = s.n;
                         g.ctx = s.ctx;
@@ -477,31 +495,42 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                         g.kvh = kvh;
                         g.node0 = rt * 2 * p.tile_nodes;
                         g.nodes = min(s.n - g.node0, 2 * p.tile_nodes);
-                        g.two_tiles = g.nodes > p.tile_nodes;
-                        g.t0 = s.tile_lo + at;
-                        g.t1 = g.t0 + take;
-                        g.jobs = s.ctx < 0 ? 0 : (g.two_tiles ? 2 * take : take);
+                        g.two_tiles = two;
+                        g.t0 = s.tile_lo + t0;
+                        g.t1 = s.tile_lo + t1;
+                        g.jobs = s.ctx < 0 ? 0 : (two ? 2 : 1) * (t1 - t0);
                         g.low = s.low;
                         g.slot = whole ? -1 : (seg == 0 ? 0 : 1);
-                        if (at == 0 && !whole) {
+                        if (t0 == 0 && !whole) {
                             split.row0 = s.row0 + g.node0;
                             split.nodes = g.nodes;
                             split.kvh = kvh;
                             split.first_slot = g.slot;
-                            split.parts = (unit + s.tiles - 1) / share - (int)blockIdx.x + 1;
-                        }
-                        unit += take;
-                        left -= take;
-                        at += take;
-                        if (at == s.tiles) {
-                            at = 0;
-                            if (++rt == s.row_items) {
-                                rt = 0;
-                                ++kvh;
-                            }
+                            split.parts = (unit - at + units - 1) / share - (int)blockIdx.x + 1;
                         }
                     }
+                    unit += take;
+                    left -= take;
+                    at += take;
+                    if (at == units) {
+                        at = 0;
+                        if (++rt == s.items) {
+                            rt = 0;
+                            ++kvh;
+                        }
+                        while (left > 0 && kvh >= (s.items > 0 ? p.kv_heads : 0)) {  // the next sequence with rows
+                            if (++b >= p.batch) {
+                                left = 0;
+                                break;
+                            }
+                            s = tree_seq(p, b);
+                            kvh = 0;
+                        }
+                    }
+                    if (t1 > t0) break;
                 }
+                ok = mbar_wait(smem_u32(&sh.seg_empty[seg % kTreeQueue]), ((seg / kTreeQueue) & 1) ^ 1);
+                if (!ok) break;
                 sh.queue[seg % kTreeQueue] = g;
                 mbar_arrive(smem_u32(&sh.seg_full[seg % kTreeQueue]));
                 ++seg;
@@ -710,13 +739,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             const int ctx = g.ctx;
             float m_run = -INFINITY, l_run = 0.0f;
             for (int i = grp; i < jobs; i += 2) {
+                const int tile = two ? i >> 1 : i;
+                const int p0 = (g.t0 + tile) * kTreeKeys;
+                // What the row sees of a tile that holds nodes or a window's
+                // edge, while S is on its way.
+                const bool partial = p.window > 0 || p0 + kTreeKeys > ctx;
+                uint32_t vis[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                if (partial) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) vis[c] = live ? tree_visible(p, g, row, p0 + 32 * c) : 0u;
+                }
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.s_full[grp]), s_phase))) {
                     ok = false;
                     break;
                 }
                 s_phase ^= 1;
                 tc_fence_after();
-                const int tile = two ? i >> 1 : i;
                 const int at = ring_at + tree_pos_v<C::kOwnP>(two, tile, T), buf = at % C::kBufs;
                 // V of this tile stays until this group's P is consumed, so
                 // its phase cannot have moved on.
@@ -729,9 +767,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 }
                 if (!ok) break;
                 tc_fence_after();
-                const int p0 = (g.t0 + tile) * kTreeKeys;
                 const uint32_t valid = sh.valid[buf];
-                const bool masked = p.window > 0 || p0 + kTreeKeys > ctx || valid != 0xFFu;
+                const bool masked = partial || valid != 0xFFu;
                 if (masked)
                     tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1));
                 if (warp_live) {
@@ -752,9 +789,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                             for (int c = 0; c < 2; ++c) {
                                 const uint32_t part = (valid >> (4 * h + 2 * c) & 1 ? 0x0000FFFFu : 0u) |
                                                       (valid >> (4 * h + 2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
-                                const uint32_t vis = live ? tree_visible(p, g, row, p0 + 64 * h + 32 * c) & part : 0u;
+                                const uint32_t seen = (h == 0 ? vis[c] : vis[2 + c]) & part;
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) sc[32 * c + k] = (vis >> k & 1) ? sc[32 * c + k] : -INFINITY;
+                                for (int k = 0; k < 32; ++k) sc[32 * c + k] = (seen >> k & 1) ? sc[32 * c + k] : -INFINITY;
                             }
                         }
                         // Exponentials about the present m, and the largest

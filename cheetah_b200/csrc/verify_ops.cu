@@ -133,7 +133,7 @@ int launch_tree_attention(const CUtensorMap &q_map, const CUtensorMap &k_map, co
     CH_CUDA_TRY(launch_ex(cheetah::tree_attention_kernel<HD>, dim3(ctas), dim3(cheetah::kTreeThreads), smem, stream, true,
                           q_map, k_map, v_map, p));
     CH_CUDA_TRY(launch_ex(cheetah::tree_merge_kernel<HD>, dim3(ctas * cheetah::kTreeMergeCtas), dim3(cheetah::kTreeMergeThreads),
-                          0, stream, true, p, ctas));
+                          0, stream, false, p, ctas));
     return 0;
 }
 
@@ -251,11 +251,12 @@ static int check_tree_attention(const CheetahCudaTreeAttention *a) {
                "cheetah_cuda_op_tree_attention: a pool holds 1 .. 2^31-1 rows of one head, a table row as many tokens");
     CH_REQUIRE(a->mask_words > 0 && a->mask_words <= 16, "cheetah_cuda_op_tree_attention: mask_words must be 1..16");
     CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu, "cheetah_cuda_op_tree_attention: sliding_window is too large");
-    // The kernel counts (item, key tile) units in 31 bits.
+    // The kernel counts its cost units (at most 4 per key tile of an item, and
+    // 8 per item) in 31 bits.
     const uint64_t tile_rows = 2 * (cheetah::kTreeRows / (a->q_heads / a->kv_heads));
     const uint64_t items = ((uint64_t)a->rows / tile_rows + a->batch + 1) * a->kv_heads;
     const uint64_t tiles = (uint64_t)a->max_pages_per_seq * a->page_tokens / cheetah::kTreeKeys + 1;
-    CH_REQUIRE(items * tiles <= 0x7FFFFFFFull, "cheetah_cuda_op_tree_attention: too many rows and cached positions");
+    CH_REQUIRE(items * (4 * tiles + 8) <= 0x7FFFFFFFull, "cheetah_cuda_op_tree_attention: too many rows and cached positions");
     return 0;
 }
 
