@@ -191,9 +191,8 @@ struct TreeShared {
     uint64_t seg_full[kTreeQueue], seg_empty[kTreeQueue];
     uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2], seg_done, exchange, drain;
     TreeSegment queue[kTreeQueue];
-    int warp_units[kTreeThreads / kWarp];
     uint32_t tmem;
-    int start_b, start_off, abort_flag, non_finite;
+    int abort_flag, non_finite;
     uint32_t valid[12];  // per ring buffer: which 16-key parts of V hold loaded positions
     float2 ml[2][kTreeRows];
 };
@@ -396,8 +395,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         mbar_init(smem_u32(&sh.drain), 1);
         sh.abort_flag = 0;
         sh.non_finite = 0;
-        sh.start_b = p.batch;
-        sh.start_off = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -405,67 +402,54 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                      "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    pdl_wait();
-    pdl_launch_dependents();
-
-    // Total units, then the sequence in which this CTA's share begins (the
-    // host has checked that the units of any lengths fit 31 bits).
-    constexpr int kWarps = kTreeThreads / kWarp;
-    const int mine = (int)threadIdx.x < p.batch ? tree_units<HD>(p, threadIdx.x) : 0;
-    int sum = mine;
-    for (int b = threadIdx.x + kTreeThreads; b < p.batch; b += kTreeThreads) sum += tree_units<HD>(p, b);
-    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-    if (lane == 0) sh.warp_units[warp] = sum;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += sh.warp_units[w];
-    const int share = max(C::kMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
-    const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
-    int before = 0;
-    for (int b0 = 0; b0 < p.batch && u0 < total; b0 += kTreeThreads) {
-        const int b = b0 + threadIdx.x;
-        const int units = b0 == 0 ? mine : (b < p.batch ? tree_units<HD>(p, b) : 0);
-        int end = units;
-#pragma unroll
-        for (int o = 1; o < kWarp; o <<= 1) {
-            const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
-            if (lane >= o) end += up;
-        }
-        if (p.batch > kTreeThreads) {
-            __syncthreads();
-            if (lane == kWarp - 1) sh.warp_units[warp] = end;
-            __syncthreads();
-        }
-        int chunk = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const int x = sh.warp_units[w];
-            if (w < warp) end += x;
-            chunk += x;
-        }
-        end += before;
-        before += chunk;
-        if (end - units <= u0 && u0 < end) {
-            sh.start_b = b;
-            sh.start_off = u0 - (end - units);
-        }
-    }
-    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
 
     int ring_at = 0;   // ring positions of the segments before
     int issued = 0;    // producers: tiles requested are at positions below this
     int q_issued = 0;
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTreeLeanRegs));
     if (warp == 3) {
-        // Scheduler: walks over the share's items and publishes its segments.
+        // Scheduler. Total units, and the sequence in which this CTA's share
+        // begins (the host has checked that the units of any lengths fit 31
+        // bits); a lane per sequence, other warps wait for the first segment.
+        int total = 0, mine = 0;
+        for (int b = lane; b < p.batch; b += kWarp) {
+            const int units = tree_units<HD>(p, b);
+            if (b == lane) mine = units;
+            total += units;
+        }
+        total = __reduce_add_sync(0xFFFFFFFFu, total);
+        const int share = max(C::kMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+        const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
+        int start = -1, before = 0;
+        int at = 0;  // unit within the sequence, then within the item
+        for (int b0 = 0; b0 < p.batch && start < 0 && u0 < total; b0 += kWarp) {
+            const int b = b0 + lane;
+            const int units = b0 == 0 ? mine : (b < p.batch ? tree_units<HD>(p, b) : 0);
+            int end = units;
+#pragma unroll
+            for (int o = 1; o < kWarp; o <<= 1) {
+                const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
+                if (lane >= o) end += up;
+            }
+            end += before;
+            const uint32_t here = __ballot_sync(0xFFFFFFFFu, end - units <= u0 && u0 < end);
+            if (here) {
+                start = b0 + __ffs(here) - 1;
+                at = u0 - __shfl_sync(0xFFFFFFFFu, end - units, __ffs(here) - 1);
+            }
+            before = __shfl_sync(0xFFFFFFFFu, end, kWarp - 1);
+        }
+        // It walks over the share's items and publishes its segments.
         if (lane == 0) {
-            int b = sh.start_b, left = min(share, total - u0), unit = u0, seg = 0;
+            int b = start, left = min(share, total - u0), unit = u0, seg = 0;
             TreeSeq s = {};
-            int kvh = 0, rt = 0, at = sh.start_off;  // unit within the item
+            int kvh = 0, rt = 0;
             if (left > 0) {
                 s = tree_seq(p, b);
                 const int head = tree_head_units<HD>(s), pair = tree_item_units<HD>(s, true);
@@ -545,6 +529,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         const CUtensorMap *map = is_v ? &v_map : &k_map;
         const int boxes = kTreeKeys / p.box_keys;
         bool ok = true;
+        // Q, once the previous segment's S products are done (in the first
+        // segment before the keys, later behind the first of them).
+        auto load_q = [&](const TreeSegment &g) -> bool {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.q_empty), (q_issued & 1) ^ 1))) return false;
+            if (lane == 0) {
+                const int tiles = g.two_tiles ? 2 : 1;
+                mbar_expect_tx(smem_u32(&sh.q_full), (uint32_t)(tiles * C::kHalves * p.group * p.tile_nodes * 128));
+                for (int t = 0; t < tiles; ++t) {
+                    for (int h = 0; h < C::kHalves; ++h) {
+                        tma_load_3d(smem_u32(q_s + t * C::kTile + h * C::kHalfBytes), &q_map, h * 64, g.kvh * p.group,
+                                    g.row0 + g.node0 + t * p.tile_nodes, smem_u32(&sh.q_full));
+                    }
+                }
+            }
+            ++q_issued;
+            return true;
+        };
         for (int seg = 0; tree_next(sh, seg, ok); ++seg) {
             const TreeSegment &g = sh.queue[seg % kTreeQueue];
             const int T = g.t1 - g.t0;
@@ -557,6 +558,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 // multiple of 2, 4 and 8).
                 int first = -kWarp, my_row = -1;
                 uint32_t loaded = 0;
+                if (!is_v && seg == 0) load_q(g);
                 for (int i = 0; i < T; ++i) {
                     const int at = ring_at + (is_v ? tree_pos_v<C::kOwnP>(two, i, T) : tree_pos_k<C::kOwnP>(two, i));
                     const int buf = at % C::kBufs;
@@ -597,21 +599,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                         }
                     }
                     issued = at + 1;
-                    if (!is_v && i == min(1, T - 1)) {
-                        // Q, once the previous segment's S products are done.
-                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.q_empty), (q_issued & 1) ^ 1));
-                        if (!ok) break;
-                        if (lane == 0) {
-                            const int tiles = two ? 2 : 1;
-                            mbar_expect_tx(smem_u32(&sh.q_full), (uint32_t)(tiles * C::kHalves * p.group * p.tile_nodes * 128));
-                            for (int t = 0; t < tiles; ++t) {
-                                for (int h = 0; h < C::kHalves; ++h) {
-                                    tma_load_3d(smem_u32(q_s + t * C::kTile + h * C::kHalfBytes), &q_map, h * 64, kvh * p.group,
-                                                g.row0 + g.node0 + t * p.tile_nodes, smem_u32(&sh.q_full));
-                                }
-                            }
-                        }
-                        ++q_issued;
+                    if (!is_v && seg > 0 && i == min(1, T - 1) && !load_q(g)) {
+                        ok = false;
+                        break;
                     }
                 }
                 ring_at += 2 * T;
@@ -799,6 +789,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                         // m moves and they are done again.
                         uint32_t w[32];
                         float s0, s1;
+                        if (i == grp && h == 0) {
+                            // The first keys set m.
+                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) mx[k & 3] = max3(mx[k & 3], sc[2 * k], sc[2 * k + 1]);
+                            m_run = ceilf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+                        }
                         while (true) {
                             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
                             const unsigned long long neg_m2 = pair_f32(neg_m, neg_m);
