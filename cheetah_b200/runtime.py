@@ -530,34 +530,52 @@ def prefill_attention(q, k_pool, v_pool, page_table, offset: int, sliding_window
 # The calls take torch CUDA tensors of one device and run on its current
 # stream, or on `stream`; what they allocate belongs to that stream, as if the
 # call stood inside `torch.cuda.stream(stream)`. A step runs them once per
-# layer or token, so they keep the host's part short.
+# layer or token, so the host's part of a call is kept short: torch's and the
+# library's names are looked up once (`_bind`), checks stand inline.
+
+_bound = None
+
+
+class _Bound:
+    """What the calls need of torch and of the library, looked up once."""
+
+    def __init__(self):
+        import torch
+        self.current_device = torch._C._cuda_getDevice
+        self.raw_stream = torch._C._cuda_getCurrentRawStream
+        self.empty, self.empty_like = torch.empty, torch.empty_like
+        self.i32, self.i64, self.u8 = torch.int32, torch.int64, torch.uint8
+        self.bf16, self.f32 = torch.bfloat16, torch.float32
+        handle = lib()
+        for name in ("page_slots", "qk_norm_rope", "tree_attention", "token_logprobs"):
+            setattr(self, name, getattr(handle, "cheetah_cuda_op_" + name))
+
+
+def _bind() -> _Bound:
+    global _bound
+    _bound = _Bound()
+    return _bound
+
 
 def _context(device: int, stream):
     """The context in which `device` is current and, given one, `stream`."""
     import torch
     if stream is None:
         return torch.cuda.device(device)
-    if not (stream.device.index == device):
+    if stream.device.index != device:
         raise CheetahCudaError("the stream belongs to another device than the tensors")
     return torch.cuda.stream(stream)
 
 
-def _elsewhere(device: int, stream) -> bool:
-    """Whether the call has to enter a context first."""
-    import torch
-    return stream is not None or device != torch._C._cuda_getDevice()
+def _fits(t, dtype, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.is_contiguous()
 
 
-def _raw_stream(device: int) -> int:
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-def _check_tensors(op: str, device: int, dtype, names: str, *tensors) -> None:
-    """Every given tensor: contiguous, of this dtype, on this device."""
-    for i, t in enumerate(tensors):
-        if t is not None and (t.dtype is not dtype or t.get_device() != device or not t.is_contiguous()):
-            raise CheetahCudaError(f"{op}: {names.split()[i]} must be a contiguous {dtype} tensor on cuda:{device}")
+def _refuse(op: str, device: int, **wanted) -> None:
+    """Raises for the first of name=(tensor, dtype) that `_fits` refuses."""
+    for name, (t, dtype) in wanted.items():
+        if t is not None and not _fits(t, dtype, device):
+            raise CheetahCudaError(f"{op}: {name} must be a contiguous {dtype} tensor on cuda:{device}")
 
 
 class PageSlots(NamedTuple):
@@ -576,42 +594,40 @@ def page_slots(cached, new_tokens, free_pages, free_count, page_table, num_pages
     int32 [F], of which the first free_count (int32 [1]) are free; page_table
     int32 [B, max_pages] is extended in place. Sequences that do not fit are
     refused, not raised: see counts."""
-    import torch
+    o = _bound or _bind()
     device = page_table.get_device()
-    if not (device >= 0 and page_table.dim() == 2):
+    if device < 0 or page_table.dim() != 2:
         raise CheetahCudaError("page_slots: page_table must be a CUDA tensor [batch, max_pages]")
-    if _elsewhere(device, stream):
+    if stream is not None or device != o.current_device():
         with _context(device, stream):
             return page_slots(cached, new_tokens, free_pages, free_count, page_table, num_pages, page_tokens, max_tokens)
-    _check_tensors("page_slots", device, torch.int32, "cached new_tokens free_pages free_count page_table",
-                   cached, new_tokens, free_pages, free_count, page_table)
+    i32 = o.i32
+    if not (_fits(cached, i32, device) and _fits(new_tokens, i32, device) and _fits(free_pages, i32, device)
+            and _fits(free_count, i32, device) and _fits(page_table, i32, device)):
+        _refuse("page_slots", device, cached=(cached, i32), new_tokens=(new_tokens, i32), free_pages=(free_pages, i32),
+                free_count=(free_count, i32), page_table=(page_table, i32))
     B, width = page_table.shape
-    if not (cached.numel() == B and new_tokens.numel() == B and free_count.numel() == 1):
+    if cached.numel() != B or new_tokens.numel() != B or free_count.numel() != 1:
         raise CheetahCudaError("page_slots: cached and new_tokens must hold one length per table row, free_count one number")
     if not (0 < max_tokens < 2 ** 31 and 0 < num_pages < 2 ** 31 and 0 < page_tokens < 2 ** 31):
         raise CheetahCudaError("page_slots: max_tokens, num_pages and page_tokens must be positive and below 2^31")
     # One buffer; the per-row outputs begin at 16-byte boundaries.
     pad = -max_tokens % 4
-    buffer = torch.empty(3 * (max_tokens + pad) + 2 * B + 4, dtype=torch.int32, device=page_table.device)
+    row = max_tokens + pad
+    buffer = o.empty(3 * row + 2 * B + 4, dtype=i32, device=page_table.device)
     if pad:
         positions, _, ids, _, slots, _, starts, lens, counts = buffer.split_with_sizes(
             (max_tokens, pad, max_tokens, pad, max_tokens, pad, B + 1, B, 3))
     else:
-        positions, ids, slots, starts, lens, counts = buffer.split_with_sizes(
-            (max_tokens, max_tokens, max_tokens, B + 1, B, 3))
+        positions, ids, slots, starts, lens, counts = buffer.split_with_sizes((row, row, row, B + 1, B, 3))
+    at = buffer.data_ptr()
     args = PageSlotsArgs(cached.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
                          free_pages.numel(), B, page_table.data_ptr(), width, num_pages, page_tokens, max_tokens,
-                         starts.data_ptr(), lens.data_ptr(), positions.data_ptr(), ids.data_ptr(),
-                         slots.data_ptr(), counts.data_ptr())
-    _check(lib().cheetah_cuda_op_page_slots(C.byref(args), _raw_stream(device)))
+                         at + 12 * row, at + 12 * row + 4 * (B + 1), at, at + 4 * row, at + 8 * row,
+                         at + 12 * row + 8 * B + 4)
+    if o.page_slots(args, o.raw_stream(device)):
+        _check(-1)
     return PageSlots(starts, lens, positions, ids, slots, counts)
-
-
-def _pool_dtype(op: str, k_pool, v_pool) -> int:
-    import torch
-    if not (k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and k_pool.dtype in (torch.bfloat16, torch.float32)):
-        raise CheetahCudaError(f"{op}: the pools must be bf16 or f32 [pages, kv_heads, page_tokens, head_dim] of one shape")
-    return KV_F32 if k_pool.dtype == torch.float32 else KV_BF16
 
 
 def qk_norm_rope(qkv, q_heads: int, kv_heads: int, positions, slots, rope_cos, rope_sin, k_pool, v_pool,
@@ -621,43 +637,52 @@ def qk_norm_rope(qkv, q_heads: int, kv_heads: int, positions, slots, rope_cos, r
     (or the same flattened) bf16 or f32, rows may be strided; positions, slots
     int32 [T], -1 skips; rope_cos, rope_sin f32 [max_positions, rotary_dim/2];
     the pools bf16 or f32, written in place. Returns q_out [T, q_heads, D]."""
-    import torch
+    o = _bound or _bind()
     device = qkv.get_device()
-    if not (device >= 0 and qkv.dtype in (torch.bfloat16, torch.float32)):
+    i32, f32, bf16 = o.i32, o.f32, o.bf16
+    dtype, pool = qkv.dtype, k_pool.dtype
+    if device < 0 or (dtype is not bf16 and dtype is not f32):
         raise CheetahCudaError("qk_norm_rope: qkv must be a bf16 or f32 CUDA tensor")
-    if _elsewhere(device, stream):
+    if stream is not None or device != o.current_device():
         with _context(device, stream):
             return qk_norm_rope(qkv, q_heads, kv_heads, positions, slots, rope_cos, rope_sin, k_pool, v_pool, q_norm,
                                 k_norm, eps, q_out)
-    kv_dtype = _pool_dtype("qk_norm_rope", k_pool, v_pool)
-    pages, kvh, pt, D = k_pool.shape
-    T, dims = qkv.shape[0], qkv.dim()
+    shape = k_pool.shape
+    if len(shape) != 4 or shape != v_pool.shape or (pool is not bf16 and pool is not f32):
+        raise CheetahCudaError("qk_norm_rope: the pools must be bf16 or f32 [pages, kv_heads, page_tokens, head_dim] of one shape")
+    pages, kvh, pt, D = shape
+    T = qkv.shape[0]
     width = (q_heads + 2 * kv_heads) * D
-    inner = (qkv.stride(1) == D and qkv.stride(2) == 1) if dims == 3 else dims == 2 and qkv.stride(1) == 1
-    if not (T > 0 and kvh == kv_heads and q_heads > 0 and qkv.numel() == T * width and inner and (dims == 2 or qkv.shape[2] == D)):
+    strides = qkv.stride()
+    if not (T > 0 and kvh == kv_heads and q_heads > 0 and qkv.numel() == T * width
+            and (strides[1:] == (D, 1) and qkv.shape[2] == D or len(strides) == 2 and strides[1] == 1)):
         raise CheetahCudaError("qk_norm_rope: qkv must be [tokens, q_heads + 2 kv_heads, head_dim] with contiguous rows")
-    _check_tensors("qk_norm_rope", device, torch.int32, "positions slots", positions, slots)
-    _check_tensors("qk_norm_rope", device, torch.float32, "rope_cos rope_sin q_norm k_norm", rope_cos, rope_sin, q_norm, k_norm)
-    _check_tensors("qk_norm_rope", device, k_pool.dtype, "k_pool v_pool", k_pool, v_pool)
-    _check_tensors("qk_norm_rope", device, qkv.dtype, "q_out", q_out)
-    if not (positions.numel() == T and slots.numel() == T):
+    if not (_fits(positions, i32, device) and _fits(slots, i32, device) and _fits(rope_cos, f32, device)
+            and _fits(rope_sin, f32, device) and _fits(k_pool, pool, device) and _fits(v_pool, pool, device)
+            and (q_norm is None or _fits(q_norm, f32, device)) and (k_norm is None or _fits(k_norm, f32, device))
+            and (q_out is None or _fits(q_out, dtype, device))):
+        _refuse("qk_norm_rope", device, positions=(positions, i32), slots=(slots, i32), rope_cos=(rope_cos, f32),
+                rope_sin=(rope_sin, f32), k_pool=(k_pool, pool), v_pool=(v_pool, pool), q_norm=(q_norm, f32),
+                k_norm=(k_norm, f32), q_out=(q_out, dtype))
+    if positions.numel() != T or slots.numel() != T:
         raise CheetahCudaError("qk_norm_rope: positions and slots must hold one entry per row")
-    if not (rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape):
+    table = rope_cos.shape
+    if len(table) != 2 or table != rope_sin.shape:
         raise CheetahCudaError("qk_norm_rope: rope_cos and rope_sin must be [max_positions, rotary_dim/2]")
-    if not ((q_norm is None or q_norm.numel() == D) and (k_norm is None or k_norm.numel() == D)):
+    if (q_norm is not None and q_norm.numel() != D) or (k_norm is not None and k_norm.numel() != D):
         raise CheetahCudaError("qk_norm_rope: a norm weight must be [head_dim]")
-    if not (q_out is None or q_out.numel() == T * q_heads * D):
+    if q_out is None:
+        q_out = qkv.new_empty((T, q_heads, D))
+    elif q_out.numel() != T * q_heads * D:
         raise CheetahCudaError("qk_norm_rope: q_out must be [tokens, q_heads, head_dim]")
-    q = qkv.new_empty((T, q_heads, D)) if q_out is None else q_out
-    args = QkNormRopeArgs(qkv.data_ptr(), qkv.stride(0) if T > 1 else width,
-                          KV_F32 if qkv.dtype == torch.float32 else KV_BF16, kv_dtype,
-                          q_norm.data_ptr() if q_norm is not None else None,
-                          k_norm.data_ptr() if k_norm is not None else None, eps, rope_cos.data_ptr(),
-                          rope_sin.data_ptr(), rope_cos.shape[0], 2 * rope_cos.shape[1], positions.data_ptr(),
-                          slots.data_ptr(), T, q_heads, kv_heads, D, q.data_ptr(), k_pool.data_ptr(),
-                          v_pool.data_ptr(), pages, pt)
-    _check(lib().cheetah_cuda_op_qk_norm_rope(C.byref(args), _raw_stream(device)))
-    return q
+    args = QkNormRopeArgs(qkv.data_ptr(), strides[0] if T > 1 else width, KV_F32 if dtype is f32 else KV_BF16,
+                          KV_F32 if pool is f32 else KV_BF16, None if q_norm is None else q_norm.data_ptr(),
+                          None if k_norm is None else k_norm.data_ptr(), eps, rope_cos.data_ptr(), rope_sin.data_ptr(),
+                          table[0], 2 * table[1], positions.data_ptr(), slots.data_ptr(), T, q_heads, kv_heads, D,
+                          q_out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pages, pt)
+    if o.qk_norm_rope(args, o.raw_stream(device)):
+        _check(-1)
+    return q_out
 
 
 def tree_attention(q, k_pool, v_pool, page_table, seq_lens, row_starts, tree_mask, positions=None,
@@ -670,46 +695,53 @@ def tree_attention(q, k_pool, v_pool, page_table, seq_lens, row_starts, tree_mas
     (needed with a window). Rows behind the last sequence stay as `out` holds
     them. workspace: a uint8 tensor of `tree_attention_workspace` bytes that no
     overlapping call uses; None takes one from torch's allocator."""
-    import torch
+    o = _bound or _bind()
     device = q.get_device()
-    if not (device >= 0 and q.dim() == 3 and q.dtype == torch.bfloat16):
+    i32, bf16 = o.i32, o.bf16
+    if device < 0 or q.dtype is not bf16 or q.dim() != 3:
         raise CheetahCudaError("tree_attention: q must be a bf16 CUDA tensor [rows, q_heads, head_dim]")
-    if _elsewhere(device, stream):
+    if stream is not None or device != o.current_device():
         with _context(device, stream):
             return tree_attention(q, k_pool, v_pool, page_table, seq_lens, row_starts, tree_mask, positions,
                                   sliding_window, out, workspace)
     rows, qh, D = q.shape
-    if not (rows > 0 and q.stride(1) == D and q.stride(2) == 1):
+    strides = q.stride()
+    if rows < 1 or strides[1:] != (D, 1):
         raise CheetahCudaError("tree_attention: q must have contiguous rows")
-    if not (_pool_dtype("tree_attention", k_pool, v_pool) == KV_BF16 and k_pool.shape[3] == D):
-        raise CheetahCudaError("tree_attention: the pools must be bf16 and of q's head_dim")
-    pages, kvh, pt, _ = k_pool.shape
-    _check_tensors("tree_attention", device, torch.bfloat16, "k_pool v_pool out", k_pool, v_pool, out)
-    _check_tensors("tree_attention", device, torch.int32, "page_table seq_lens row_starts positions",
-                   page_table, seq_lens, row_starts, positions)
-    _check_tensors("tree_attention", device, torch.int64, "tree_mask", tree_mask)
-    _check_tensors("tree_attention", device, torch.uint8, "workspace", workspace)
+    shape = k_pool.shape
+    if len(shape) != 4 or shape != v_pool.shape or shape[3] != D:
+        raise CheetahCudaError("tree_attention: the pools must be bf16 [pages, kv_heads, page_tokens, head_dim] of q's head_dim")
+    if not (_fits(k_pool, bf16, device) and _fits(v_pool, bf16, device) and _fits(page_table, i32, device)
+            and _fits(seq_lens, i32, device) and _fits(row_starts, i32, device) and _fits(tree_mask, o.i64, device)
+            and (positions is None or _fits(positions, i32, device)) and (out is None or _fits(out, bf16, device))
+            and (workspace is None or _fits(workspace, o.u8, device))):
+        _refuse("tree_attention", device, k_pool=(k_pool, bf16), v_pool=(v_pool, bf16), page_table=(page_table, i32),
+                seq_lens=(seq_lens, i32), row_starts=(row_starts, i32), tree_mask=(tree_mask, o.i64),
+                positions=(positions, i32), out=(out, bf16), workspace=(workspace, o.u8))
     B = seq_lens.numel()
-    if not (page_table.dim() == 2 and page_table.shape[0] == B and row_starts.numel() == B + 1):
+    table, mask = page_table.shape, tree_mask.shape
+    if len(table) != 2 or table[0] != B or row_starts.numel() != B + 1:
         raise CheetahCudaError("tree_attention: page_table must be [batch, max_pages] and row_starts [batch + 1]")
-    if not (tree_mask.dim() == 2 and tree_mask.shape[0] == rows):
+    if len(mask) != 2 or mask[0] != rows:
         raise CheetahCudaError("tree_attention: tree_mask must be [rows, words]")
-    if not (positions is None or positions.numel() == rows):
+    if positions is not None and positions.numel() != rows:
         raise CheetahCudaError("tree_attention: positions must hold one entry per row")
-    if not (out is None or out.shape == q.shape):
-        raise CheetahCudaError("tree_attention: out must have q's shape")
-    if not (0 <= sliding_window < 2 ** 31):
+    if not 0 <= sliding_window < 2 ** 31:
         raise CheetahCudaError("tree_attention: sliding_window must be 0 .. 2^31-1")
+    if out is None:
+        out = o.empty_like(q) if strides[0] == qh * D else q.new_empty((rows, qh, D))
+    elif out.shape != q.shape:
+        raise CheetahCudaError("tree_attention: out must have q's shape")
     if workspace is None:
-        workspace = torch.empty(tree_attention_workspace(D, device), dtype=torch.uint8, device=q.device)
-    o = q.new_empty((rows, qh, D)) if out is None else out
-    args = TreeAttentionArgs(q.data_ptr(), q.stride(0) if rows > 1 else qh * D, rows, k_pool.data_ptr(),
-                             v_pool.data_ptr(), page_table.data_ptr(), page_table.shape[1], pages, pt,
-                             seq_lens.data_ptr(), row_starts.data_ptr(), B, tree_mask.data_ptr(),
-                             tree_mask.shape[1], positions.data_ptr() if positions is not None else None,
-                             sliding_window, qh, kvh, D, o.data_ptr(), workspace.data_ptr(), workspace.numel())
-    _check(lib().cheetah_cuda_op_tree_attention(C.byref(args), _raw_stream(device)))
-    return o
+        workspace = o.empty(tree_attention_workspace(D, device), dtype=o.u8, device=q.device)
+    args = TreeAttentionArgs(q.data_ptr(), strides[0] if rows > 1 else qh * D, rows, k_pool.data_ptr(), v_pool.data_ptr(),
+                             page_table.data_ptr(), table[1], shape[0], shape[2], seq_lens.data_ptr(),
+                             row_starts.data_ptr(), B, tree_mask.data_ptr(), mask[1],
+                             None if positions is None else positions.data_ptr(), sliding_window, qh, shape[1], D,
+                             out.data_ptr(), workspace.data_ptr(), workspace.numel())
+    if o.tree_attention(args, o.raw_stream(device)):
+        _check(-1)
+    return out
 
 
 _tree_workspace_bytes: dict = {}  # (device, head_dim) -> bytes, a property of the GPU
@@ -717,19 +749,18 @@ _tree_workspace_bytes: dict = {}  # (device, head_dim) -> bytes, a property of t
 
 def tree_attention_workspace(head_dim: int, device: Optional[int] = None) -> int:
     """Bytes of a `tree_attention` workspace on `device` (default: the current one)."""
-    import torch
     if device is None:
-        device = torch.cuda.current_device()
-    bytes_ = _tree_workspace_bytes.get((device, head_dim))
-    if bytes_ is None:
+        device = (_bound or _bind()).current_device()
+    size = _tree_workspace_bytes.get((device, head_dim))
+    if size is None:
         # Every field but head_dim is the least that passes the checks.
         args = TreeAttentionArgs(rows=1, max_pages_per_seq=1, num_pages=1, page_tokens=16, batch=1, mask_words=1,
                                  q_heads=1, kv_heads=1, head_dim=head_dim)
         n = C.c_size_t(0)
-        with torch.cuda.device(device):
+        with _context(device, None):
             _check(lib().cheetah_cuda_op_tree_attention_workspace(C.byref(args), C.byref(n)))
-        bytes_ = _tree_workspace_bytes[(device, head_dim)] = n.value
-    return bytes_
+        size = _tree_workspace_bytes[(device, head_dim)] = n.value
+    return size
 
 
 class TokenLogprobs(NamedTuple):
@@ -744,28 +775,31 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     """Log probability and rank of tokens[r] (int32) in row r of logits [rows,
     vocab] (f32 or bf16, rows may be strided), the row's entropy and its `top`
     likeliest tokens (`cheetah_cuda_op_token_logprobs`)."""
-    import torch
+    o = _bound or _bind()
     device = logits.get_device()
-    if not (device >= 0 and logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32)):
+    f32, dtype = o.f32, logits.dtype
+    if device < 0 or (dtype is not f32 and dtype is not o.bf16) or logits.dim() != 2:
         raise CheetahCudaError("token_logprobs: logits must be a bf16 or f32 CUDA tensor [rows, vocab]")
-    if _elsewhere(device, stream):
+    if stream is not None or device != o.current_device():
         with _context(device, stream):
             return token_logprobs(logits, tokens, top)
     rows, vocab = logits.shape
-    if not (rows > 0 and vocab > 0 and (logits.stride(1) == 1 or vocab == 1)):
+    strides = logits.stride()
+    if rows < 1 or vocab < 1 or (strides[1] != 1 and vocab > 1):
         raise CheetahCudaError("token_logprobs: logits must have contiguous rows")
-    _check_tensors("token_logprobs", device, torch.int32, "tokens", tokens)
-    if not (tokens.dim() == 1 and tokens.numel() == rows):
+    if not _fits(tokens, o.i32, device):
+        _refuse("token_logprobs", device, tokens=(tokens, o.i32))
+    if tokens.dim() != 1 or tokens.numel() != rows:
         raise CheetahCudaError("token_logprobs: tokens must be [rows]")
-    if not (0 <= top <= min(32, vocab)):
+    if not 0 <= top <= min(32, vocab):
         raise CheetahCudaError("token_logprobs: top must be at most 32 and at most vocab")
-    rank = torch.empty_like(tokens)
-    logprob = torch.empty_like(tokens, dtype=torch.float32)
-    entropy = torch.empty_like(logprob)
+    rank = o.empty_like(tokens)
+    logprob = o.empty_like(tokens, dtype=f32)
+    entropy = o.empty_like(logprob)
     ids, best = tokens.new_empty((rows, top)), logprob.new_empty((rows, top))
-    args = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
-                             KV_F32 if logits.dtype == torch.float32 else KV_BF16, rows, vocab,
-                             tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(), entropy.data_ptr(),
-                             ids.data_ptr() if top else None, best.data_ptr() if top else None)
-    _check(lib().cheetah_cuda_op_token_logprobs(C.byref(args), _raw_stream(device)))
+    args = TokenLogprobsArgs(logits.data_ptr(), strides[0] if rows > 1 else vocab, KV_F32 if dtype is f32 else KV_BF16,
+                             rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(),
+                             entropy.data_ptr(), ids.data_ptr() if top else None, best.data_ptr() if top else None)
+    if o.token_logprobs(args, o.raw_stream(device)):
+        _check(-1)
     return TokenLogprobs(logprob, entropy, rank, ids, best)
