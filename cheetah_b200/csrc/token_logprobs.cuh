@@ -4,8 +4,8 @@
 //   S = sum exp(x - m),  lse = m + log S,  log p_t = x_t - lse
 //   H = log S + sum (m - x) exp(x - m) / S   (both terms >= 0: no cancellation)
 //
-// with a running maximum per thread: moving m to m' multiplies S by f =
-// exp(m - m') and G = sum (x - m) exp(x - m) becomes f (G + (m - m') S).
+// with a reference m per thread: moving m to m' multiplies S by f = exp(m - m')
+// and G = sum (x - m) exp(x - m) becomes f (G + (m - m') S).
 //
 // Bound by memory where rows are many, by latency where they are few: a row
 // is split over a cluster of 1..16 CTAs that join their results in the first
@@ -15,9 +15,10 @@
 // of the CTA's part and one iteration reads the next line of every run, so
 // the first iteration samples the whole part. The `top`-th best of the
 // threads' first maxima is a lower bound of the part's `top`-th best value;
-// elements at or above it (about top * part / sample of them) go to a buffer,
-// from which each warp sorts its share in registers and the warps' lists are
-// merged pairwise. Where they do not fit (an adversarial order), the exact
+// elements at or above it go to a buffer, from which each warp sorts its share
+// in registers and the warps' lists are merged pairwise; done once after an
+// eighth of the part, this gives a closer bound for the rest (about 12 * top
+// candidates in all instead of 40 * top). Where they do not fit (an adversarial order), the exact
 // `top`-th key is found by a radix selection over the part instead, in 8 more
 // passes.
 #pragma once
@@ -28,13 +29,17 @@
 
 namespace cheetah {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / kWarp;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxCluster = 16;
 constexpr int kLpLoads = 4;        // 16-byte loads in flight per thread
 constexpr int kLpBuffer = 1024;    // candidates of a CTA
-constexpr float kLpFloor = -1.0e4f;  // exp of it is 0; keeps (x - m) * 0 finite
+constexpr int kLpAhead = 4;        // iterations asked for ahead of a sort
+constexpr float kLpLog2e = 1.4426950408889634f;
+constexpr float kLpFloor = -1.0e4f;  // 2^floor is 0; keeps t * 0 finite
+constexpr float kLpHeadroom = 8.0f;  // logits this far above a thread's reference move it
+constexpr float kLpFused = 1048576.0f;  // largest logit whose log2(e) multiple rounds to within 1/8
 
 struct LogprobParams {
     const void *logits;
@@ -69,8 +74,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// Running sums of a row part about the maximum m. A NaN or +inf logit makes s
-// NaN; a part without a logit above -inf has s = 0.
+// Sums of a row part about a logit m, in log2 units: s = sum 2^t, gap = sum t
+// 2^t with t = log2(e) (x - m). A NaN or +inf logit makes s NaN; a part
+// without a logit above -inf has s = 0.
 struct RowSums {
     float m, s, gap;
 
@@ -79,17 +85,19 @@ struct RowSums {
         s = gap = 0.0f;
     }
     __device__ __forceinline__ void raise(float to) {
-        const float d = max_nan(m - to, kLpFloor);
-        const float f = fast_exp2(d * 1.4426950408889634f);
-        gap = f * fmaf(d, s, gap);
+        const float t = max_nan((m - to) * kLpLog2e, kLpFloor);
+        const float f = fast_exp2(t);
+        gap = f * fmaf(t, s, gap);
         s *= f;
         m = to;
     }
+    // Any logit: every case is in order, for a few more operations.
     __device__ __forceinline__ void add(float x) {
-        const float d = max_nan(x - m, kLpFloor);
-        const float e = fast_exp2(d * 1.4426950408889634f);
+        if (x > m) raise(x);
+        const float t = max_nan((x - m) * kLpLog2e, kLpFloor);
+        const float e = fast_exp2(t);
         s += e;
-        gap = fmaf(d, e, gap);
+        gap = fmaf(t, e, gap);
     }
     __device__ __forceinline__ void join(const RowSums &o) {
         RowSums other = o;
@@ -100,6 +108,71 @@ struct RowSums {
         gap += other.gap;
     }
 };
+
+// The same sums as the stream over the row takes them: about a whole number r
+// of log2 units, exact in f32, so t = log2(e) x - r is one fused operation
+// with one rounding. r moves only when a logit lies kLpHeadroom above it. A
+// logit of -inf adds 0 to s but makes gap NaN, and logits beyond kLpFused have
+// no such r; then `blurred` is set and the part is summed once more, by add().
+struct StreamSums {
+    float r, s, gap, m, limit;
+    bool blurred;
+
+    __device__ __forceinline__ void init() {
+        r = s = gap = 0.0f;
+        m = limit = -INFINITY;
+        blurred = false;
+    }
+    __device__ __forceinline__ void move(float to_m) {
+        const float to = rintf(to_m * kLpLog2e);
+        const float shift = fmaxf(r - to, kLpFloor);
+        const float f = s > 0.0f ? fast_exp2(shift) : 0.0f;
+        gap = f * fmaf(shift, s, gap);
+        s *= f;
+        r = to;
+        m = to_m;
+        limit = to_m + kLpHeadroom;
+        blurred |= !(fabsf(to_m) < kLpFused);
+    }
+    __device__ __forceinline__ void add(float x) {
+        const float t = fmaf(x, kLpLog2e, -r);
+        const float e = fast_exp2(t);
+        s += e;
+        gap = fmaf(t, e, gap);
+    }
+    __device__ __forceinline__ RowSums about_m() {
+        RowSums o;
+        o.init();
+        if (m > -INFINITY) {
+            const float shift = -fmaf(m, kLpLog2e, -r);
+            const float f = fast_exp2(shift);
+            o.m = m;
+            o.s = s * f;
+            o.gap = f * fmaf(shift, s, gap);
+        }
+        blurred |= !(gap == gap);
+        return o;
+    }
+};
+
+// The larger of each half, as bf16.
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// 1 or 0 per half, and their sums.
+__device__ __forceinline__ uint32_t gt_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 
 template <typename T>
 struct LogitVec {
@@ -114,6 +187,34 @@ struct LogitVec {
             } else {
                 v[i] = __uint_as_float(w[i]);
             }
+        }
+    }
+    // The largest value of a vector (NaN left out); v: the vector widened.
+    static __device__ __forceinline__ float largest(const uint4 &raw, const float *v) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t m = max_bf16x2(max_bf16x2(raw.x, raw.y), max_bf16x2(raw.z, raw.w));
+            return fmaxf(bf16_lo(m), bf16_hi(m));
+        } else {
+            return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        }
+    }
+    // Value i of a vector.
+    static __device__ __forceinline__ float pick(const uint4 &raw, int i) {
+        const int word = i * (int)sizeof(T) / 4;
+        const uint32_t w = word < 2 ? (word == 0 ? raw.x : raw.y) : (word == 2 ? raw.z : raw.w);
+        if constexpr (sizeof(T) == 2) return (i & 1) ? bf16_hi(w) : bf16_lo(w);
+        else return __uint_as_float(w);
+    }
+    // How many values of a vector are above `than`.
+    static __device__ __forceinline__ int above(const uint4 &raw, const float *v, float than) {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t limit;
+            asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(limit) : "f"(than));  // a bf16 logit, or +inf: exact
+            const uint32_t n = add_bf16x2(add_bf16x2(gt_bf16x2(raw.x, limit), gt_bf16x2(raw.y, limit)),
+                                          add_bf16x2(gt_bf16x2(raw.z, limit), gt_bf16x2(raw.w, limit)));
+            return (int)(bf16_lo(n) + bf16_hi(n));
+        } else {
+            return (v[0] > than) + (v[1] > than) + (v[2] > than) + (v[3] > than);
         }
     }
     static __device__ __forceinline__ float one(const T *row, long long i) {
@@ -132,7 +233,7 @@ struct LogprobShared {
     int histogram[256];
     int count, need;
 };
-static_assert(kLpMaxTop <= kWarp && kLpMaxCluster <= kLpWarps, "a list is one key per lane, merged by a warp each");
+static_assert(kLpMaxTop <= kWarp && kLpMaxCluster <= 2 * kLpWarps, "a list is one key per lane, two are merged by a warp");
 
 // Bitonic steps over the warp's lanes; the best key ends in lane 0.
 __device__ __forceinline__ TopKey lane_exchange(TopKey k, int stride, bool best_low) {
@@ -179,7 +280,7 @@ __device__ __forceinline__ void pick_best(const TopKey *keys, int n, TopKey (*li
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobParams p) {
     namespace cg = cooperative_groups;
     using V = LogitVec<T>;
     constexpr int N = V::N;
@@ -202,6 +303,18 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     const int run = (lines + kLpWarps * kLpLoads - 1) / (kLpWarps * kLpLoads);
     // Vector of load j in iteration it (>= v1: none).
     auto vector_at = [&](int it, int j) -> int { return v0 + ((warp * kLpLoads + j) * run + it) * kWarp + lane; };
+    // Asks L2 for the lines of the coming iterations, so that DRAM keeps busy
+    // while the threads sort.
+    auto ask_ahead = [&](int it) {
+#pragma unroll 1
+        for (int a = it; a < min(it + kLpAhead, run); ++a) {
+#pragma unroll
+            for (int j = 0; j < kLpLoads; ++j) {
+                const int v = vector_at(a, j);
+                if (v < v1 && lane % 8 == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(vec + v));
+            }
+        }
+    };
     // The odd elements at the row's ends: one each for a few threads of the first CTA.
     int odd = -1;
     if (rank == 0) {
@@ -213,8 +326,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     const bool known = token >= 0 && token < p.vocab;
     const float chosen = known ? V::one(row, token) : INFINITY;
 
-    RowSums sums;
-    sums.init();
+    StreamSums stream;
+    stream.init();
     int above = 0;
     float tau = INFINITY;
     TopKey tau_key = ~0ull;
@@ -231,18 +344,19 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
             if (v >= v1) break;
             float x[N];
             V::widen(raw[j], x);
-            float mx = x[0];
+            const float mx = V::largest(raw[j], x);
+            if (mx > stream.limit) stream.move(mx);
 #pragma unroll
-            for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-            if (mx > sums.m) sums.raise(mx);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                sums.add(x[i]);
-                above += x[i] > chosen;
-            }
+            for (int i = 0; i < N; ++i) stream.add(x[i]);
+            above += V::above(raw[j], x, chosen);
             if (mx >= tau) {
-                for (int i = 0; i < N; ++i) {
-                    if (x[i] >= tau) push(x[i], head + v * N + i);
+                uint32_t near = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) near |= x[i] >= tau ? 1u << i : 0u;
+#pragma unroll 1
+                for (; near; near &= near - 1) {
+                    const int i = __ffs(near) - 1;
+                    push(V::pick(raw[j], i), head + v * N + i);
                 }
             }
         }
@@ -257,6 +371,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     uint4 raw[kLpLoads];
     load(raw, 0);
     if (p.top > 0) {
+        ask_ahead(1);
         TopKey mine = odd >= 0 ? top_key(V::one(row, odd), odd) : 0ull;
 #pragma unroll
         for (int j = 0; j < kLpLoads; ++j) {
@@ -264,27 +379,58 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
             if (run == 0 || v >= v1) break;
             float x[N];
             V::widen(raw[j], x);
+            const float mx = V::largest(raw[j], x);
+            int at = -1;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const TopKey key = x[i] == x[i] ? top_key(x[i], head + v * N + i) : 0ull;
-                mine = key > mine ? key : mine;
+            for (int i = N - 1; i >= 0; --i) {
+                if (x[i] == mx) at = i;
             }
+            const TopKey key = at >= 0 ? top_key(mx, head + v * N + at) : 0ull;
+            mine = key > mine ? key : mine;
         }
         sh.lists[warp][lane] = warp_sort(mine);
         merge_lists(sh.lists, kLpWarps);
         tau_key = sh.lists[0][p.top - 1];
         tau = tau_key ? top_key_value(tau_key) : -INFINITY;
     }
-    for (int it = 0; it < run; ++it) {
-        uint4 next[kLpLoads];
-        load(next, it + 1);
-        consume(raw, it);
+    auto stream_over = [&](int from, int to) {
+        for (int it = from; it < to; ++it) {
+            uint4 next[kLpLoads];
+            load(next, it + 1);
+            consume(raw, it);
 #pragma unroll
-        for (int j = 0; j < kLpLoads; ++j) raw[j] = next[j];
+            for (int j = 0; j < kLpLoads; ++j) raw[j] = next[j];
+        }
+    };
+    int done = 0;
+    if (p.top > 0 && run >= 8) {
+        // The best of an eighth of the part: a closer bound for the rest.
+        done = run / 8;
+        stream_over(0, done);
+        ask_ahead(done + 1);
+        __syncthreads();
+        const int count = sh.count;
+        if (count <= kLpBuffer) {
+            pick_best(sh.buffer, count, sh.lists);
+            if (tid < kWarp) sh.buffer[tid] = sh.lists[0][tid];
+            if (tid == 0) sh.count = min(count, kWarp);
+            const TopKey closer = sh.lists[0][p.top - 1];
+            if (closer > tau_key) {
+                tau_key = closer;
+                tau = top_key_value(closer);
+            }
+        }
+        __syncthreads();
+    }
+    stream_over(done, run);
+
+    RowSums sums = stream.about_m();
+    if (__syncthreads_or(stream.blurred)) {
+        sums.init();
+        for (int id = head + v0 * N + tid; id < head + v1 * N; id += kLpThreads) sums.add(V::one(row, id));
     }
     if (odd >= 0) {
         const float x = V::one(row, odd);
-        if (x > sums.m) sums.raise(x);
         sums.add(x);
         above += x > chosen;
         if (p.top > 0 && x >= tau) push(x, odd);
@@ -385,7 +531,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     if (tid == 0) {
         p.logprob[r] = bad || !known ? nan : (chosen - all.m) - log_s;
         if (p.rank) p.rank[r] = bad || !known ? 0 : 1 + count;
-        if (p.entropy) p.entropy[r] = bad ? nan : log_s - all.gap / all.s;
+        if (p.entropy) p.entropy[r] = bad ? nan : log_s - 0.69314718056f * (all.gap / all.s);
     }
     if (p.top > 0) {
         merge_lists(sh.joined, parts);

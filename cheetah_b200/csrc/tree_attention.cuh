@@ -54,6 +54,7 @@
 
 #include "attention_mma.cuh"
 #include "common.cuh"
+#include "pair.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
@@ -300,25 +301,6 @@ __device__ __noinline__ void patch_row(const TreeAttnParams &p, const TreeSegmen
     }
 }
 
-// Two f32 per instruction (sm_100's packed forms).
-__device__ __forceinline__ unsigned long long pair_f32(float lo, float hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpair_f32(unsigned long long v, float &lo, float &hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // Products of two bf16 pairs (exact for powers of two within range).
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;

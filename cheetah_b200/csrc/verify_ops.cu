@@ -80,8 +80,11 @@ int launch_qk(cheetah::QkNormRopeParams p, bool kv_bf16, cudaStream_t stream) {
     return 0;
 }
 
-// A cluster of CTAs per row: as many as keep every SM busy while each has at
-// least one full sample (kLpThreads threads x kLpLoads vectors) to read.
+// A cluster of CTAs per row: the number that leaves the busiest SM the least
+// (rows divide badly among 148 SMs, and one row fills 16). A part is charged 3%
+// for its join, 20% where it sorts too, and holds at least half a sample: 500
+// bf16 rows of 152064 take 36 us in two parts and 44 in one without
+// alternatives, 77 and 60 with twenty.
 int launch_logprobs(const cheetah::LogprobParams &p, bool bf16, cudaStream_t stream) {
     auto kernel = bf16 ? cheetah::token_logprobs_kernel<uint16_t> : cheetah::token_logprobs_kernel<float>;
     int device = 0;
@@ -89,7 +92,15 @@ int launch_logprobs(const cheetah::LogprobParams &p, bool bf16, cudaStream_t str
     const long long sms = cheetah::sm_count(device);
     const int sample = cheetah::kLpThreads * cheetah::kLpLoads * (bf16 ? 8 : 4);
     int parts = 1;
-    while (parts < cheetah::kLpMaxCluster && (long long)p.rows * parts * 2 <= sms && p.vocab / (parts * 2) >= sample / 2) parts *= 2;
+    double least = 0.0;
+    for (int n = 1; n <= cheetah::kLpMaxCluster && (n == 1 || p.vocab / n >= sample / 2); n *= 2) {
+        const long long busiest = ((long long)p.rows * n + sms - 1) / sms;
+        const double cost = (double)busiest / n * (1.0 + (p.top > 0 ? 0.2 : 0.03) * n);
+        if (n == 1 || cost < least) {
+            least = cost;
+            parts = n;
+        }
+    }
     CH_REQUIRE((uint64_t)p.rows * parts <= 0x7FFFFFFFull, "cheetah_cuda_op_token_logprobs: too many rows");
     if (parts > 8) CH_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t config = {};
