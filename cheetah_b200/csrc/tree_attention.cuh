@@ -82,7 +82,8 @@ struct TreeCfg {
     static constexpr int kTiles = 2 * kTile + kBufs * kTile;
     // Cost units of the shares: a key tile of an item with one Q tile (bound
     // by its loads) and with two (by the products and exponentials), and an
-    // item's beginning and end. Measured in halves of a one-tile key tile.
+    // item's beginning and end. Halves of a
+    // one-tile key tile's time, fitted to measured times.
     static constexpr int kOne = 2, kTwo = HD == 64 ? 4 : 3, kItem = HD == 64 ? 8 : 6;
     static constexpr int kMinShare = 4;
     static_assert(kMinShare >= kTwo, "every share holds a tile");
@@ -727,6 +728,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 }
                 s_phase ^= 1;
                 tc_fence_after();
+                // The first 64 scores are on their way during the other waits,
+                // the second 64 during the first's exponentials.
+                float sc[2][64];
+                if (warp_live) {
+                    tmem_ld32_nowait(s_addr, sc[0]);
+                    tmem_ld32_nowait(s_addr + 32, sc[0] + 32);
+                }
                 const int at = ring_at + tree_pos_v<C::kOwnP>(two, tile, T), buf = at % C::kBufs;
                 // V of this tile stays until this group's P is consumed, so
                 // its phase cannot have moved on.
@@ -737,6 +745,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     if (ok && i > 1) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.pv_done[grp]), pv_phase ^ 1));
                     pv_phase ^= 1;
                 }
+                tmem_wait_ld();
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t valid = sh.valid[buf];
@@ -745,16 +754,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1));
                 if (warp_live) {
                     const unsigned long long scale2 = pair_f32(p.scale_log2, p.scale_log2);
-#pragma unroll 1
+#pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float sc[64];
-                        tmem_ld32_nowait(s_addr + h * 64, sc);
-                        tmem_ld32_nowait(s_addr + h * 64 + 32, sc + 32);
-                        tmem_wait_ld();
-                        if (C::kOwnP && h == 1) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[grp]));
+                        if (h == 0) {
+                            tmem_ld32_nowait(s_addr + 64, sc[1]);
+                            tmem_ld32_nowait(s_addr + 96, sc[1] + 32);
+                        } else {
+                            tmem_wait_ld();
+                            if (C::kOwnP) {
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[grp]));
+                            }
                         }
                         if (masked) {
 #pragma unroll
@@ -763,7 +774,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                                                       (valid >> (4 * h + 2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
                                 const uint32_t seen = (h == 0 ? vis[c] : vis[2 + c]) & part;
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) sc[32 * c + k] = (seen >> k & 1) ? sc[32 * c + k] : -INFINITY;
+                                for (int k = 0; k < 32; ++k) sc[h][32 * c + k] = (seen >> k & 1) ? sc[h][32 * c + k] : -INFINITY;
                             }
                         }
                         // Exponentials about the present m, and the largest
@@ -775,7 +786,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                             // The first keys set m.
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) mx[k & 3] = max3(mx[k & 3], sc[2 * k], sc[2 * k + 1]);
+                            for (int k = 0; k < 32; ++k) mx[k & 3] = max3(mx[k & 3], sc[h][2 * k], sc[h][2 * k + 1]);
                             m_run = ceilf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
                         }
                         while (true) {
@@ -785,9 +796,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int k = 0; k < 32; ++k) {
-                                mx[k & 3] = max3(mx[k & 3], sc[2 * k], sc[2 * k + 1]);
+                                mx[k & 3] = max3(mx[k & 3], sc[h][2 * k], sc[h][2 * k + 1]);
                                 float e0, e1;
-                                unpair_f32(fma_pair(pair_f32(sc[2 * k], sc[2 * k + 1]), scale2, neg_m2), e0, e1);
+                                unpair_f32(fma_pair(pair_f32(sc[h][2 * k], sc[h][2 * k + 1]), scale2, neg_m2), e0, e1);
                                 e0 = fast_exp2(e0);
                                 e1 = fast_exp2(e1);
                                 sums[k & 3] = add_pair(sums[k & 3], pair_f32(e0, e1));
@@ -826,7 +837,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                             }
                         }
                         l_run += s0 + s1;
-                        // In S's columns, P's 32 are among the 64 just read.
+                        // In S's columns, P's 32 are among those read by now.
                         tmem_st16_nowait(p_addr + h * 32, w);
                         tmem_st16_nowait(p_addr + h * 32 + 16, w + 16);
                     }
@@ -1002,43 +1013,46 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const Tre
         const int tile = i / (p.tile_nodes * p.group);
         const int r = tile * kTreeRows + i - tile * p.tile_nodes * p.group;
         auto slot_of = [&](int k) -> int { return k == 0 ? 2 * c + s.first_slot : 2 * (c + k); };
-        float m = -INFINITY;
-#pragma unroll 4
-        for (int k = lane / block; k < s.parts; k += step) m = fmaxf(m, p.part_ml[slot_of(k) * 256 + r].x);
-        if (!few) {
-            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-        }
-        float l = 0.0f;
+        float m = -INFINITY, l = 0.0f;
         float4 o[kCols];
 #pragma unroll
         for (int j = 0; j < kCols; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // o, l about m join o2, l2 about m2, the later part second.
+        auto join = [&](float m2, float l2, const float4 (&o2)[kCols]) {
+            const float to = fmaxf(m, m2);
+            const float f = m == -INFINITY ? 0.0f : exp2f(m - to), f2 = m2 == -INFINITY ? 0.0f : exp2f(m2 - to);
+            m = to;
+            l = l * f + l2 * f2;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                o[j].x = o[j].x * f + o2[j].x * f2;
+                o[j].y = o[j].y * f + o2[j].y * f2;
+                o[j].z = o[j].z * f + o2[j].z * f2;
+                o[j].w = o[j].w * f + o2[j].w * f2;
+            }
+        };
 #pragma unroll 4
         for (int k = lane / block; k < s.parts; k += step) {
             const int slot = slot_of(k);
             const float2 ml = p.part_ml[slot * 256 + r];
-            const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
-            l = fmaf(ml.y, w, l);
+            float4 v[kCols];
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) {
-                const float4 v = p.part_o[((long long)slot * (HD / 4) + j * kTreeMergeWarps + warp) * 256 + r];
-                o[j].x = fmaf(v.x, w, o[j].x);
-                o[j].y = fmaf(v.y, w, o[j].y);
-                o[j].z = fmaf(v.z, w, o[j].z);
-                o[j].w = fmaf(v.w, w, o[j].w);
-            }
+            for (int j = 0; j < kCols; ++j) v[j] = p.part_o[((long long)slot * (HD / 4) + j * kTreeMergeWarps + warp) * 256 + r];
+            join(ml.x, ml.y, v);
         }
         if (!few) {
 #pragma unroll
             for (int x = 8; x < kWarp; x <<= 1) {
-                l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+                const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, x), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, x);
+                float4 v[kCols];
 #pragma unroll
                 for (int j = 0; j < kCols; ++j) {
-                    o[j].x += __shfl_xor_sync(0xFFFFFFFFu, o[j].x, x);
-                    o[j].y += __shfl_xor_sync(0xFFFFFFFFu, o[j].y, x);
-                    o[j].z += __shfl_xor_sync(0xFFFFFFFFu, o[j].z, x);
-                    o[j].w += __shfl_xor_sync(0xFFFFFFFFu, o[j].w, x);
+                    v[j].x = __shfl_xor_sync(0xFFFFFFFFu, o[j].x, x);
+                    v[j].y = __shfl_xor_sync(0xFFFFFFFFu, o[j].y, x);
+                    v[j].z = __shfl_xor_sync(0xFFFFFFFFu, o[j].z, x);
+                    v[j].w = __shfl_xor_sync(0xFFFFFFFFu, o[j].w, x);
                 }
+                join(m2, l2, v);
             }
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
