@@ -194,7 +194,8 @@ struct TreeShared {
     uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2], seg_done, exchange, drain;
     TreeSegment queue[kTreeQueue];
     uint32_t tmem;
-    int abort_flag, non_finite;
+    int abort_flag;
+    int non_finite[2];   // V values taken out of tiles: any, some of a tile of context alone
     uint32_t valid[12];  // per ring buffer: which 16-key parts of V hold loaded positions
     float2 ml[2][kTreeRows];
 };
@@ -249,7 +250,7 @@ __device__ __forceinline__ bool bf16_non_finite(uint32_t half) { return (half & 
 // One V row of a masked tile in shared memory: zero where it holds no
 // position, finite elsewhere (its non-finite values are noted for patch_row).
 template <int HD>
-__device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, bool holds) {
+__device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, bool holds, bool context) {
 #pragma unroll 1
     for (int c = 0; c < HD / 8; ++c) {
         // Each lane begins at another cell: the rows lie 128 bytes apart.
@@ -272,7 +273,8 @@ __device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, boo
             }
         }
         if (bad) {
-            *reinterpret_cast<volatile int *>(&sh.non_finite) = 1;
+            *reinterpret_cast<volatile int *>(&sh.non_finite[0]) = 1;
+            if (context) *reinterpret_cast<volatile int *>(&sh.non_finite[1]) = 1;
             __threadfence_block();  // flag before the zeros that hide it from the other group
             *cell = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -285,8 +287,10 @@ __device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, boo
 // products were left out of the MMAs.
 template <int HD>
 __device__ __noinline__ void patch_row(const TreeAttnParams &p, const TreeSegment &g, int row, int d0, int cols,
-                                       uint16_t *out, float *part) {
-    const int begin = p.window > 0 ? g.t0 * kTreeKeys : max(g.t0 * kTreeKeys, g.ctx / kTreeKeys * kTreeKeys);
+                                       uint16_t *out, float *part, bool context) {
+    // A tile of context alone was cleaned where a window or a page outside the
+    // pool masks it; where it was not, adding its values again changes nothing.
+    const int begin = context ? g.t0 * kTreeKeys : max(g.t0 * kTreeKeys, g.ctx / kTreeKeys * kTreeKeys);
     for (int p0 = begin; p0 < min(g.t1 * kTreeKeys, g.len); p0 += 32) {
         for (uint32_t rest = tree_visible(p, g, row, p0); rest; rest &= rest - 1) {
             const int pos = p0 + __ffs(rest) - 1;
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         mbar_init(smem_u32(&sh.exchange), 8);
         mbar_init(smem_u32(&sh.drain), 1);
         sh.abort_flag = 0;
-        sh.non_finite = 0;
+        sh.non_finite[0] = sh.non_finite[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -751,7 +755,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 const uint32_t valid = sh.valid[buf];
                 const bool masked = partial || valid != 0xFFu;
                 if (masked)
-                    tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1));
+                    tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1),
+                                     p0 + kTreeKeys <= ctx);
                 if (warp_live) {
                     const unsigned long long scale2 = pair_f32(p.scale_log2, p.scale_log2);
 #pragma unroll
@@ -921,8 +926,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 __syncwarp();  // patch_row reads what the warp has stored
                 if (live) {
                     if (slot >= 0 && (two || grp == 0)) p.part_ml[part_row] = make_float2(m, l);
-                    if (*reinterpret_cast<volatile int *>(&sh.non_finite))
-                        patch_row<HD>(p, g, row, d0, d1 - d0, out_row, slot >= 0 ? reinterpret_cast<float *>(part) : nullptr);
+                    if (*reinterpret_cast<volatile int *>(&sh.non_finite[0]))
+                        patch_row<HD>(p, g, row, d0, d1 - d0, out_row, slot >= 0 ? reinterpret_cast<float *>(part) : nullptr,
+                                      *reinterpret_cast<volatile int *>(&sh.non_finite[1]));
                 }
             }
             tc_fence_before();

@@ -336,6 +336,22 @@ def test_tree_attention_non_finite_cells_reach_only_the_rows_that_see_them(value
             assert torch.equal(out[i], want[i])
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,ctx", [(64, 400), (128, 400), (128, 9000)])
+def test_tree_attention_non_finite_context_beside_a_page_outside_the_pool(value, D, ctx):
+    """A context key that every row sees is non-finite, and the page before its
+    own lies outside the pool: the key still counts."""
+    case = Tree([ctx], [5], 8, 2, D, seed=23)
+    page = int(case.table[0, 3])
+    case.dev["page_table"][0, 2] = -1
+    case.dev["v_pool"][page, :, 5, ::3] = value
+    out = case.run()[:5].float()
+    hit = torch.zeros(D, dtype=torch.bool, device="cuda")
+    hit[::3] = True
+    assert bool((torch.isnan(out) if math.isnan(value) else out == value)[..., hit].all())
+    assert bool(torch.isfinite(out[..., ~hit]).all())
+
+
 def test_tree_attention_large_scores():
     """Scores of a few hundred: one weight is 1 and the others underflow."""
     case = Tree([300, 40], [10, 70], 14, 2, 64, seed=9, scale=40.0)
