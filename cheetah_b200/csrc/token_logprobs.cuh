@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     const int r = blockIdx.x / parts;
     const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
     if (tid == 0) sh.count = 0;
+    cluster.barrier_arrive();  // waited for before another CTA's shared memory is written
     pdl_wait();
     pdl_launch_dependents();
     const T *row = static_cast<const T *>(p.logits) + r * p.row_stride;
@@ -493,7 +494,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         }
     }
 
-    // Join the parts in the first CTA.
+    // Join the parts in the first CTA, which is running once all have arrived.
+    cluster.barrier_wait();
     LogprobShared *first = cluster.map_shared_rank(&sh, 0);
     if (tid == 0) {
         RowSums all;
