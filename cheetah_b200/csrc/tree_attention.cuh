@@ -477,7 +477,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                             split.nodes = g.nodes;
                             split.kvh = kvh;
                             split.first_slot = g.slot;
-                            split.parts = (unit - at + units - 1) / share - (int)blockIdx.x + 1;
+                            // Within the grid even if sequences share rows, which the units do not count on.
+                            split.parts = min((unit - at + units - 1) / share - (int)blockIdx.x + 1, (int)(gridDim.x - blockIdx.x));
                         }
                     }
                     unit += take;

@@ -260,6 +260,9 @@ static int check_tree_attention(const CheetahCudaTreeAttention *a) {
     CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens) && pool_in_range(a->max_pages_per_seq, a->page_tokens) &&
                    (uint64_t)a->num_pages * a->kv_heads * a->page_tokens <= 0x7FFFFFFFull,
                "cheetah_cuda_op_tree_attention: a pool holds 1 .. 2^31-1 rows of one head, a table row as many tokens");
+    // The end of a key tile is counted in 31 bits too.
+    CH_REQUIRE((uint64_t)a->max_pages_per_seq * a->page_tokens <= 0x7FFFFFFFull - cheetah::kTreeKeys,
+               "cheetah_cuda_op_tree_attention: a table row holds at most 2^31 - 129 tokens");
     CH_REQUIRE(a->mask_words > 0 && a->mask_words <= 16, "cheetah_cuda_op_tree_attention: mask_words must be 1..16");
     CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu, "cheetah_cuda_op_tree_attention: sliding_window is too large");
     // The kernel counts its cost units (at most 4 per key tile of an item, and
@@ -342,8 +345,9 @@ int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogprobs *a, void *stre
     CH_REQUIRE(a != nullptr && a->logits && a->tokens && a->logprob, "cheetah_cuda_op_token_logprobs: null argument");
     CH_REQUIRE(a->dtype == CHEETAH_CUDA_KV_BF16 || a->dtype == CHEETAH_CUDA_KV_F32,
                "cheetah_cuda_op_token_logprobs: unknown dtype");
-    CH_REQUIRE(a->rows > 0 && a->rows <= 0x7FFFFFFFu && a->vocab > 0 && a->vocab <= 0x7FFFFFFFu,
-               "cheetah_cuda_op_token_logprobs: empty shape");
+    CH_REQUIRE(a->rows > 0 && a->rows <= 0x7FFFFFFFu && a->vocab > 0, "cheetah_cuda_op_token_logprobs: empty shape");
+    // Ids and vector numbers are stepped through in 32 bits.
+    CH_REQUIRE(a->vocab <= (1u << 30), "cheetah_cuda_op_token_logprobs: vocab must be at most 2^30");
     CH_REQUIRE(a->top <= (uint32_t)cheetah::kLpMaxTop && a->top <= a->vocab,
                "cheetah_cuda_op_token_logprobs: top must be at most 32 and at most vocab");
     CH_REQUIRE(a->top == 0 || (a->top_ids && a->top_logprobs),

@@ -439,7 +439,7 @@ typedef struct CheetahCudaTreeAttention {
     const void *k_pool;        /* bf16 [num_pages][kv_heads][page_tokens][head_dim] */
     const void *v_pool;        /* same layout */
     const int32_t *page_table; /* [batch][max_pages_per_seq] */
-    uint32_t max_pages_per_seq;
+    uint32_t max_pages_per_seq; /* times page_tokens: at most 2^31 - 129 */
     uint32_t num_pages;
     uint32_t page_tokens;      /* a multiple of 16 */
     const int32_t *seq_lens;   /* [batch] */
@@ -472,7 +472,7 @@ typedef struct CheetahCudaTokenLogprobs {
     size_t row_stride;         /* elements between rows */
     int32_t dtype;             /* CHEETAH_CUDA_KV_F32 or _BF16 */
     uint32_t rows;
-    uint32_t vocab;
+    uint32_t vocab;            /* 1..2^30 */
     const int32_t *tokens;     /* [rows] */
     uint32_t top;              /* 0..32, at most vocab */
     float *logprob;            /* [rows] */

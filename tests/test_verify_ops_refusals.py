@@ -57,7 +57,8 @@ CASES = [
     (logprobs, dict(logits=None), "null"), (logprobs, dict(dtype=2), "dtype"), (logprobs, dict(rows=0), "empty"),
     (logprobs, dict(vocab=0), "empty"), (logprobs, dict(top=33), "top"), (logprobs, dict(vocab=1, top=2), "top"),
     (logprobs, dict(top_ids=None), "top_ids"), (logprobs, dict(row_stride=99), "overlap"),
-    (logprobs, dict(logits=P + 2), "aligned"),
+    (logprobs, dict(logits=P + 2), "aligned"), (logprobs, dict(vocab=(1 << 30) + 1, row_stride=1 << 31), "2^30"),
+    (tree, dict(max_pages_per_seq=(1 << 27) - 1), "table row"),
 ]
 
 
