@@ -194,8 +194,7 @@ struct TreeShared {
     uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2], seg_done, exchange, drain;
     TreeSegment queue[kTreeQueue];
     uint32_t tmem;
-    int abort_flag;
-    int non_finite[2];   // V values taken out of tiles: any, some of a tile of context alone
+    int abort_flag, non_finite;
     uint32_t valid[12];  // per ring buffer: which 16-key parts of V hold loaded positions
     float2 ml[2][kTreeRows];
 };
@@ -247,36 +246,48 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeAttnParams &p, const 
 
 __device__ __forceinline__ bool bf16_non_finite(uint32_t half) { return (half & 0x7F80u) == 0x7F80u; }
 
-// One V row of a masked tile in shared memory: zero where it holds no
-// position, finite elsewhere (its non-finite values are noted for patch_row).
+// acc + 0 * w: stays zero while the values are finite.
+__device__ __forceinline__ uint32_t probe_bf16x2(uint32_t w, uint32_t acc) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(acc));
+    return r;
+}
+
+// One V row of a masked tile in shared memory, of a key that some row does not
+// see: zero where it holds no position, finite elsewhere (its non-finite
+// values are noted for patch_row).
 template <int HD>
-__device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, bool holds, bool context) {
-#pragma unroll 1
-    for (int c = 0; c < HD / 8; ++c) {
-        // Each lane begins at another cell: the rows lie 128 bytes apart.
-        uint4 *cell = reinterpret_cast<uint4 *>(v_row + (c >> 3) * TreeCfg<HD>::kHalfBytes + ((c + threadIdx.x) & 7) * 16);
-        if (!holds) {
-            *cell = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-        }
-        uint32_t w[4] = {cell->x, cell->y, cell->z, cell->w};
-        bool bad = false;
+__device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, bool holds) {
+    // Each lane begins at another cell: the rows lie 128 bytes apart.
+    auto cell = [&](int c) -> uint4 & {
+        return *reinterpret_cast<uint4 *>(v_row + (c >> 3) * TreeCfg<HD>::kHalfBytes + ((c + threadIdx.x) & 7) * 16);
+    };
+    if (!holds) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            if (bf16_non_finite(w[x])) {
-                w[x] &= 0xFFFF0000u;
-                bad = true;
-            }
-            if (bf16_non_finite(w[x] >> 16)) {
-                w[x] &= 0x0000FFFFu;
-                bad = true;
-            }
+        for (int c = 0; c < HD / 8; ++c) cell(c) = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        uint32_t acc[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+            const uint4 v = cell(c);
+            acc[0] = probe_bf16x2(v.x, acc[0]);
+            acc[1] = probe_bf16x2(v.y, acc[1]);
+            acc[2] = probe_bf16x2(v.z, acc[2]);
+            acc[3] = probe_bf16x2(v.w, acc[3]);
         }
-        if (bad) {
-            *reinterpret_cast<volatile int *>(&sh.non_finite[0]) = 1;
-            if (context) *reinterpret_cast<volatile int *>(&sh.non_finite[1]) = 1;
-            __threadfence_block();  // flag before the zeros that hide it from the other group
-            *cell = make_uint4(w[0], w[1], w[2], w[3]);
+        if (!((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7FFF7FFFu)) return;
+        *reinterpret_cast<volatile int *>(&sh.non_finite) = 1;
+        __threadfence_block();  // flag before the zeros that hide it from the other group
+#pragma unroll 1
+        for (int c = 0; c < HD / 8; ++c) {
+            const uint4 v = cell(c);
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (bf16_non_finite(w[x])) w[x] &= 0xFFFF0000u;
+                if (bf16_non_finite(w[x] >> 16)) w[x] &= 0x0000FFFFu;
+            }
+            cell(c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -287,10 +298,10 @@ __device__ __forceinline__ void tree_clean_v(TreeShared &sh, uint8_t *v_row, boo
 // products were left out of the MMAs.
 template <int HD>
 __device__ __noinline__ void patch_row(const TreeAttnParams &p, const TreeSegment &g, int row, int d0, int cols,
-                                       uint16_t *out, float *part, bool context) {
-    // A tile of context alone was cleaned where a window or a page outside the
-    // pool masks it; where it was not, adding its values again changes nothing.
-    const int begin = context ? g.t0 * kTreeKeys : max(g.t0 * kTreeKeys, g.ctx / kTreeKeys * kTreeKeys);
+                                       uint16_t *out, float *part) {
+    // Without a window the context was left alone (adding its values again, in
+    // the tile of the first node, changes nothing).
+    const int begin = p.window > 0 ? g.t0 * kTreeKeys : max(g.t0 * kTreeKeys, g.ctx / kTreeKeys * kTreeKeys);
     for (int p0 = begin; p0 < min(g.t1 * kTreeKeys, g.len); p0 += 32) {
         for (uint32_t rest = tree_visible(p, g, row, p0); rest; rest &= rest - 1) {
             const int pos = p0 + __ffs(rest) - 1;
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         mbar_init(smem_u32(&sh.exchange), 8);
         mbar_init(smem_u32(&sh.drain), 1);
         sh.abort_flag = 0;
-        sh.non_finite[0] = sh.non_finite[1] = 0;
+        sh.non_finite = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -755,9 +766,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 tc_fence_after();
                 const uint32_t valid = sh.valid[buf];
                 const bool masked = partial || valid != 0xFFu;
-                if (masked)
-                    tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, p0 + r < g.len && (valid >> (r >> 4) & 1),
-                                     p0 + kTreeKeys <= ctx);
+                if (masked) {
+                    const bool holds = p0 + r < g.len && (valid >> (r >> 4) & 1);
+                    // Every row sees a context key, without a window.
+                    if (!holds || p.window > 0 || p0 + r >= ctx) tree_clean_v<HD>(sh, ring + buf * C::kTile + r * 128, holds);
+                }
                 if (warp_live) {
                     const unsigned long long scale2 = pair_f32(p.scale_log2, p.scale_log2);
 #pragma unroll
@@ -927,9 +940,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 __syncwarp();  // patch_row reads what the warp has stored
                 if (live) {
                     if (slot >= 0 && (two || grp == 0)) p.part_ml[part_row] = make_float2(m, l);
-                    if (*reinterpret_cast<volatile int *>(&sh.non_finite[0]))
-                        patch_row<HD>(p, g, row, d0, d1 - d0, out_row, slot >= 0 ? reinterpret_cast<float *>(part) : nullptr,
-                                      *reinterpret_cast<volatile int *>(&sh.non_finite[1]));
+                    if (*reinterpret_cast<volatile int *>(&sh.non_finite))
+                        patch_row<HD>(p, g, row, d0, d1 - d0, out_row, slot >= 0 ? reinterpret_cast<float *>(part) : nullptr);
                 }
             }
             tc_fence_before();
