@@ -405,7 +405,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     pdl_wait();
-    pdl_launch_dependents();
 
     int ring_at = 0;   // ring positions of the segments before
     int issued = 0;    // producers: tiles requested are at positions below this
@@ -960,6 +959,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    // The join may come up from here on; earlier its CTAs would take issue slots
+    // from the last softmax rows.
+    pdl_launch_dependents();
     if (sh.abort_flag) {
         // A wait gave up: let this CTA's copies and MMAs still in flight land
         // before its shared memory and TMEM are released (bounded waits).

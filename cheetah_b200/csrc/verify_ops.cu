@@ -144,7 +144,7 @@ int launch_tree_attention(const CUtensorMap &q_map, const CUtensorMap &k_map, co
     CH_CUDA_TRY(launch_ex(cheetah::tree_attention_kernel<HD>, dim3(ctas), dim3(cheetah::kTreeThreads), smem, stream, true,
                           q_map, k_map, v_map, p));
     CH_CUDA_TRY(launch_ex(cheetah::tree_merge_kernel<HD>, dim3(ctas * cheetah::kTreeMergeCtas), dim3(cheetah::kTreeMergeThreads),
-                          0, stream, false, p, ctas));
+                          0, stream, true, p, ctas));
     return 0;
 }
 
