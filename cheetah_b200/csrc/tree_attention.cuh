@@ -48,8 +48,21 @@
 // stay 0. A node's own non-finite V is zeroed there as well, and added to the
 // rows that do see it after the products (patch_row).
 //
+// Bounds and times (B200, the join included). One sequence, 708 keys, 14/2
+// heads of 64: 12.3 us, latency (attention 7, the join's launch 1, the join 4).
+// One sequence, 64 nodes at 32.7k keys: 28 us (265 TFLOP/s). 32 sequences of
+// 128 .. 8k keys with up to 16 nodes, 28/4 heads of 128: 65 us, 4.6 TB/s, bound
+// by the loads. 64 sequences of 3k .. 8k keys with 40 .. 64 nodes: 432 us, 634
+// TFLOP/s; there the chain S, softmax, PV of a tile (about 4400 cycles for the
+// two groups, of which the products are 2100 and the exponentials 2000) and
+// the clock under the power limit (1.62 of 1.96 GHz) bound it. S two jobs
+// ahead in 64-key tiles, with one MMA warp or one per group, was slower (470
+// .. 480 us: twice the waits, each 60 .. 200 cycles beside two busy warps per
+// scheduler), as was handing S and P over in halves (486 us).
+//
 // All mbarrier waits are bounded: on a timeout the CTA waits (bounded) for its
-// own copies and MMAs in flight, frees its TMEM and exits.
+// own copies and MMAs in flight, frees its TMEM and exits, and the join makes
+// every row NaN.
 #pragma once
 
 #include "attention_mma.cuh"
@@ -100,7 +113,7 @@ struct TreeCfg {
 struct TreeSplit {
     int row0, nodes, kvh;
     int first_slot;  // of the beginning; the other parts are slot 0 of the next CTAs
-    int parts;       // 0: nothing to join
+    int parts;       // 0: nothing to join; -1: the CTA gave up
     int pad[3];
 };
 
@@ -969,10 +982,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             if (q_issued > 0) mbar_wait(smem_u32(&sh.q_full), (q_issued - 1) & 1);
             for (int at = max(0, issued - C::kBufs); at < issued; ++at)
                 mbar_wait(smem_u32(&sh.full[at % C::kBufs]), (at / C::kBufs) & 1);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1 && elect_one()) {  // the lane that issued the MMAs
             umma_commit(smem_u32(&sh.drain));
             mbar_wait(smem_u32(&sh.drain), 0);
         }
+        if (threadIdx.x == kTreeThreads - 1) p.splits[blockIdx.x].parts = -1;  // the join makes the result NaN
         tc_fence_before();
         __syncthreads();
     }
@@ -1001,9 +1015,11 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const Tre
     pdl_wait();
     pdl_launch_dependents();
     int units = 0;
+    bool gave_up = false;
     if (tid < ctas) {
         const TreeSplit s = p.splits[tid];
         split_s[tid] = s;
+        gave_up = s.parts < 0;
         const int block = s.parts > kFew ? kWarp / 4 : kWarp;
         units = s.parts > 1 ? (s.nodes * p.group + block - 1) / block : 0;
     }
@@ -1016,7 +1032,12 @@ __global__ void __launch_bounds__(kTreeMergeThreads) tree_merge_kernel(const Tre
     __syncthreads();
     for (int w = 0; w < warp; ++w) units += warp_units[w];
     unit_end[tid] = units;
-    __syncthreads();
+    if (__syncthreads_or(gave_up)) {
+        const long long cells = (long long)min(max(p.row_starts[p.batch], 0), p.rows) * p.q_heads * HD;
+        for (long long i = (long long)blockIdx.x * kTreeMergeThreads + tid; i < cells; i += (long long)gridDim.x * kTreeMergeThreads)
+            p.out[i] = 0x7FC0u;
+        return;
+    }
     const int total = unit_end[kTreeMergeThreads - 1];
     for (int u = blockIdx.x; u < total; u += gridDim.x) {
         int c = 0, hi = kTreeMergeThreads - 1;
