@@ -9,8 +9,10 @@
 // it is rotated with, so the rotation needs no exchange and the norm only a
 // sum over the head's HD/2/VEC lanes; a warp takes several heads at a time and
 // walks over the heads of one row, whose cos/sin chunk and q weights it keeps
-// in registers. kQkUnroll heads' loads are issued before the first is used.
-// f32 arithmetic, one rounding to the output type.
+// in registers, with the loads of several head groups issued before the first
+// is used. f32 arithmetic, one rounding to the output type. 32768 rows of 28 + 2
+// * 4 heads of 128 in bf16 take 110 us (621 MB, 5.6 TB/s, 86% of a copy), 1021
+// such rows 6.2 us (3.1 TB/s), one row 1.8 us (latency).
 #pragma once
 
 #include "common.cuh"
@@ -18,7 +20,9 @@
 namespace cheetah {
 
 constexpr int kQkWarps = 4;
-constexpr int kQkUnroll = 3;
+// Head groups whose loads a warp issues together when it has many (110 us for
+// 32768 rows of 28 + 2 * 4 heads of 128; 3: 115, 4: 116, 9: 132).
+constexpr int kQkUnroll = 5;
 
 struct QkNormRopeParams {
     const void *qkv;
@@ -62,14 +66,16 @@ __device__ __forceinline__ void widen_chunk(const uint4 &raw, float (&v)[VEC]) {
     }
 }
 
-template <typename T, int VEC>
+// STREAM: the chunk will not be read while it could still lie in L2.
+template <typename T, int VEC, bool STREAM>
 __device__ __forceinline__ void store_chunk(void *base, long long at, const float (&v)[VEC]) {
     if constexpr (sizeof(T) == 2) {
         uint32_t w[VEC / 2];
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
         uint16_t *dst = static_cast<uint16_t *>(base) + at;
-        if constexpr (VEC == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (VEC == 8 && STREAM) __stcs(reinterpret_cast<uint4 *>(dst), make_uint4(w[0], w[1], w[2], w[3]));
+        else if constexpr (VEC == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
     } else {
         float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(base) + at);
@@ -78,7 +84,8 @@ __device__ __forceinline__ void store_chunk(void *base, long long at, const floa
     }
 }
 
-template <typename TIN, typename TKV, int HD>
+// U: head groups loaded together; 1 where a warp has only one.
+template <typename TIN, typename TKV, int HD, int U>
 __global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(const QkNormRopeParams p) {
     constexpr int VEC = 16 / sizeof(TIN);
     constexpr int kLanes = HD / 2 / VEC;        // lanes of a head
@@ -99,28 +106,13 @@ __global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(cons
     pdl_wait();
     pdl_launch_dependents();
     if (t >= p.tokens) return;
-    float wa[VEC], wb[VEC];
-    if (p.q_norm) {
-        load_floats(p.q_norm + da, wa);
-        load_floats(p.q_norm + db, wb);
-    }
-    const int pos = p.positions[t];
-    if (pos < 0 || pos >= p.max_positions) return;
-    const int slot = p.slots[t];
-    const int page = slot / p.page_tokens;
-    const bool cell_ok = slot >= 0 && page < p.num_pages;
-    float cs[VEC], sn[VEC];
-    if (turned) {
-        load_floats(p.rope_cos + (long long)pos * half + da, cs);
-        load_floats(p.rope_sin + (long long)pos * half + da, sn);
-    }
     const TIN *row = static_cast<const TIN *>(p.qkv) + t * p.qkv_stride;
     const int steps = (heads + kHeads - 1) / kHeads;
     const int step1 = min(steps, step0 + p.steps);
-    for (int s0 = step0; s0 < step1; s0 += kQkUnroll) {
-        uint4 raw[kQkUnroll][2];
+    uint4 raw[U][2];
+    auto load_heads = [&](int s0) {
 #pragma unroll
-        for (int u = 0; u < kQkUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int head = (s0 + u) * kHeads + sub;
             raw[u][0] = raw[u][1] = make_uint4(0u, 0u, 0u, 0u);
             if (s0 + u < step1 && head < heads) {
@@ -128,8 +120,31 @@ __global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(cons
                 raw[u][1] = __ldcs(reinterpret_cast<const uint4 *>(row + (long long)head * HD + db));
             }
         }
+    };
+    const int pos = p.positions[t];
+    const int slot = p.slots[t];
+    // Short rows are asked for together with their position (one row 2.06 ->
+    // 1.83 us); longer ones would hold too many registers meanwhile (32768 rows of
+    // 36 heads of 128: 134 instead of 110 us).
+    constexpr bool kEarly = U <= 3;
+    if (kEarly) load_heads(step0);
+    float wa[VEC], wb[VEC];
+    if (p.q_norm) {
+        load_floats(p.q_norm + da, wa);
+        load_floats(p.q_norm + db, wb);
+    }
+    if (pos < 0 || pos >= p.max_positions) return;
+    const int page = slot / p.page_tokens;
+    const bool cell_ok = slot >= 0 && page < p.num_pages;
+    float cs[VEC], sn[VEC];
+    if (turned) {
+        load_floats(p.rope_cos + (long long)pos * half + da, cs);
+        load_floats(p.rope_sin + (long long)pos * half + da, sn);
+    }
+    for (int s0 = step0; s0 < step1; s0 += U) {
+        if (!kEarly || s0 > step0) load_heads(s0);
 #pragma unroll
-        for (int u = 0; u < kQkUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             if (s0 + u >= step1) break;
             const int head = (s0 + u) * kHeads + sub;
             const bool is_q = head < p.q_heads;
@@ -172,14 +187,14 @@ __global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(cons
             }
             if (is_q) {
                 const long long at = ((long long)t * p.q_heads + head) * HD;
-                store_chunk<TIN>(p.q_out, at + da, a);
-                store_chunk<TIN>(p.q_out, at + db, b);
+                store_chunk<TIN, VEC, (U > 1)>(p.q_out, at + da, a);
+                store_chunk<TIN, VEC, (U > 1)>(p.q_out, at + db, b);
             } else if (cell_ok) {
                 const int kvh = is_k ? head - p.q_heads : head - p.q_heads - p.kv_heads;
                 const long long at = (((long long)page * p.kv_heads + kvh) * p.page_tokens + (slot - page * p.page_tokens)) * HD;
                 void *pool = is_k ? p.k_pool : p.v_pool;
-                store_chunk<TKV>(pool, at + da, a);
-                store_chunk<TKV>(pool, at + db, b);
+                store_chunk<TKV, VEC, (U > 1)>(pool, at + da, a);
+                store_chunk<TKV, VEC, (U > 1)>(pool, at + db, b);
             }
         }
     }

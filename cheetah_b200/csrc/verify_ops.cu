@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <atomic>
 #include <string>
+#include <type_traits>
 
 #include "cheetah_cuda.h"
 #include "common.cuh"
@@ -61,21 +62,30 @@ int make_q_map(CUtensorMap *map, const CheetahCudaTreeAttention &a, uint32_t gro
     return 0;
 }
 
-// Warps of a q/k norm call: a warp walks over a whole row where rows fill the
-// GPU (its cos/sin and weights are then read once), over one group of heads
-// where they do not.
+// Warps of a q/k norm call: a warp walks over a whole row where there are some
+// 48 head groups per SM (its cos/sin and weights are then read once), over one
+// group of heads where there are fewer and latency counts. 9 groups a row: 256
+// rows take 5.3 us whole and 2.7 in groups, 1021 rows 6.2 and 7.1, 4096 rows 17
+// and 30; 3 groups a row: 2048 rows 5.9 and 5.1, 4096 rows 6.2 and 9.1. Rows of
+// up to 3 groups have all their loads in flight with fewer registers (16384 of
+// them 23 us, with room for 5 groups 30).
 template <typename TIN, int HD>
 int launch_qk(cheetah::QkNormRopeParams p, bool kv_bf16, cudaStream_t stream) {
     constexpr int kHeads = cheetah::kWarp / (HD / 2 / (16 / (int)sizeof(TIN)));
     const int steps = (p.q_heads + 2 * p.kv_heads + kHeads - 1) / kHeads;
     int device = 0;
     CH_CUDA_TRY(cudaGetDevice(&device));
-    const long long fill = (long long)cheetah::sm_count(device) * 16;
-    p.steps = p.tokens >= fill ? steps : 1;
+    p.steps = (long long)p.tokens * steps >= 48ll * cheetah::sm_count(device) ? steps : 1;
     p.row_units = (steps + p.steps - 1) / p.steps;
     const uint64_t blocks = ((uint64_t)p.tokens * p.row_units + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
     CH_REQUIRE(blocks <= 0x7FFFFFFFull, "cheetah_cuda_op_qk_norm_rope: too many rows");
-    auto kernel = kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<TIN, uint16_t, HD> : cheetah::qk_norm_rope_rows_kernel<TIN, float, HD>;
+    auto pick = [&](auto u) {
+        constexpr int U = decltype(u)::value;
+        return kv_bf16 ? cheetah::qk_norm_rope_rows_kernel<TIN, uint16_t, HD, U> : cheetah::qk_norm_rope_rows_kernel<TIN, float, HD, U>;
+    };
+    auto kernel = p.steps == 1  ? pick(std::integral_constant<int, 1>())
+                  : p.steps <= 3 ? pick(std::integral_constant<int, 3>())
+                                 : pick(std::integral_constant<int, cheetah::kQkUnroll>());
     CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)blocks), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream, true, p));
     return 0;
 }
