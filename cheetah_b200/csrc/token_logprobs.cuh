@@ -12,18 +12,18 @@
 // one's shared memory, so a call is one launch and needs no workspace.
 //
 // One f32 row of 151936 with 5 alternatives takes 8.4 us (16 CTAs; latency),
-// 2048 such rows 208 us (6.0 TB/s), 500 bf16 rows of 152064 36 us without
-// alternatives and 57 us (2.7 TB/s) with twenty: there the operations per logit
-// bound it (about 8, and a logit is 2 bytes), and 500 rows leave a sixth of
-// the SMs' places empty.
+// 2048 such rows with one 208 .. 220 us (5.7 .. 6.0 TB/s), 500 bf16 rows of
+// 152064 36 us without alternatives and 54 us (2.8 TB/s) with twenty: there the
+// operations per logit bound it (about 8, and a logit is 2 bytes), the sorts,
+// and that 500 rows leave a sixth of the SMs' places empty.
 //
 // Alternatives. Each (warp, j) pair owns a contiguous run of 512-byte pieces
 // of the CTA's part and one iteration reads the next piece of every run, so
 // the first iteration samples the whole part. The `top`-th best of the
 // threads' first maxima is a lower bound of the part's `top`-th best value;
 // elements at or above it go to a buffer, from which each warp sorts its share
-// in registers and the warps' lists are merged pairwise; done once after an
-// eighth of the part, this gives a closer bound for the rest (about 12 * top
+// in registers and the warps' lists are merged pairwise; done once after a
+// quarter of the part, this gives a closer bound for the rest (about 13 * top
 // candidates in all instead of 40 * top). Where they do not fit (an
 // adversarial order), the exact `top`-th key is found by a radix selection over
 // the part instead, in 8 more passes.
@@ -42,6 +42,10 @@ constexpr int kLpMaxCluster = 16;
 constexpr int kLpLoads = 4;        // 16-byte loads in flight per thread
 constexpr int kLpBuffer = 1024;    // candidates of a CTA
 constexpr int kLpAhead = 4;        // iterations asked for ahead of a sort
+// From this many alternatives on a second bound pays for its sort: 500 bf16
+// rows of 152064 with twenty take 88 us without it, 57 with one after an eighth
+// and 54 after a quarter; 2048 f32 rows with one alternative 217 and 220.
+constexpr int kLpRefineTop = 4;
 constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr float kLpFloor = -1.0e4f;  // 2^floor is 0; keeps t * 0 finite
 constexpr float kLpHeadroom = 8.0f;  // logits this far above a thread's reference move it
@@ -410,9 +414,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         }
     };
     int done = 0;
-    if (p.top > 0 && run >= 8) {
-        // The best of an eighth of the part: a closer bound for the rest.
-        done = run / 8;
+    if (p.top >= kLpRefineTop && run >= 4) {
+        // The best of a quarter of the part: a closer bound for the rest.
+        done = (run + 2) / 4;
         stream_over(0, done);
         ask_ahead(done + 1);
         __syncthreads();
