@@ -35,11 +35,15 @@
 //              same), so a tile usually takes one pass over S: exponentials
 //              about the old m and the maximum beside them. O, l and P are
 //              rescaled, by a power of two, only when m moves.
-// With head_dim 64 TMEM has columns of its own for P, so S(i + 2) is computed
-// while the softmax of S(i) still runs; with head_dim 128 P takes S's columns
-// and S(i + 2) follows PV(i).
 // P is rounded to bf16 because the tensor cores multiply bf16; sums,
-// statistics and O stay f32.
+// statistics and O stay f32. Over many rows P's roundings add as much error as
+// the output's. A call of few rows, where one row with an unlucky rounding of
+// its largest weight shows, has time for a second product per tile (REST): what
+// bf16 leaves off, as bf16 again, is multiplied too (P to 2^-16 instead of
+// 2^-9), and the output is as exact as its own rounding.
+// With head_dim 64 TMEM has columns of its own for P, so without REST S(i + 2)
+// is computed while the softmax of S(i) still runs; otherwise P, or what it
+// leaves off, takes S's columns and S(i + 2) follows PV(i).
 //
 // Cells that a row must not see never reach it: their scores are replaced
 // before the softmax, and a tile that holds any (nodes, the end of the
@@ -49,7 +53,7 @@
 // rows that do see it after the products (patch_row).
 //
 // Bounds and times (B200, the join included). One sequence, 708 keys, 14/2
-// heads of 64: 12.3 us, latency (attention 7, the join's launch 1, the join 4).
+// heads of 64: 12.9 us, latency (attention 8, the join's launch 1, the join 4).
 // One sequence, 64 nodes at 32.7k keys: 28 us (265 TFLOP/s). 32 sequences of
 // 128 .. 8k keys with up to 16 nodes, 28/4 heads of 128: 65 us, 4.6 TB/s, bound
 // by the loads. 64 sequences of 3k .. 8k keys with 40 .. 64 nodes: 432 us, 634
@@ -106,6 +110,9 @@ struct TreeCfg {
     static constexpr uint32_t kOCol = 2 * kTreeKeys;
     static constexpr uint32_t kPCol = kOwnP ? kOCol + 2 * HD : 0;
     static constexpr uint32_t kPStep = kOwnP ? kTreeKeys / 2 : kTreeKeys;  // columns from P_A to P_B
+    static constexpr uint32_t kPHalf = kOwnP ? 32 : 64;                    // from the first 64 keys' to the rest's
+    // What bf16 leaves off of P, 32 columns of each half of S.
+    static constexpr uint32_t kRestCol = 32;
     static_assert((kOwnP ? kPCol + kTreeKeys : kOCol + 2 * HD) <= 512, "TMEM columns");
 };
 
@@ -342,6 +349,46 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// Exponentials of 64 scores about m as bf16 pairs, their sum (as two) and the
+// largest score. REST: the pairs, and what bf16 leaves off of them, go to TMEM
+// 16 at a time instead of to w (which would not fit the registers).
+template <bool REST>
+__device__ __forceinline__ float tree_exponentials(const float (&sc)[64], unsigned long long scale2, float neg_m, uint32_t (&w)[32],
+                                                   float &s0, float &s1, uint32_t p_addr, uint32_t rest_addr) {
+    const unsigned long long neg_m2 = pair_f32(neg_m, neg_m);
+    unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        uint32_t cut[16], rest[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const int k = 16 * c + x;
+            mx[k & 3] = max3(mx[k & 3], sc[2 * k], sc[2 * k + 1]);
+            float e0, e1;
+            unpair_f32(fma_pair(pair_f32(sc[2 * k], sc[2 * k + 1]), scale2, neg_m2), e0, e1);
+            e0 = fast_exp2(e0);
+            e1 = fast_exp2(e1);
+            sums[k & 3] = add_pair(sums[k & 3], pair_f32(e0, e1));
+            if constexpr (REST) {
+                // Cut off, not rounded, and the rest made larger by e 2^-23: it
+                // is positive like e, so an infinite V gives no inf - inf or 0 inf.
+                const uint32_t b0 = __float_as_uint(e0) & 0xFFFF0000u, b1 = __float_as_uint(e1) & 0xFFFF0000u;
+                cut[x] = b0 >> 16 | b1;
+                rest[x] = pack_bf16(fmaf(e0, 1.0f + 0x1p-23f, -__uint_as_float(b0)), fmaf(e1, 1.0f + 0x1p-23f, -__uint_as_float(b1)));
+            } else {
+                w[k] = pack_bf16(e0, e1);
+            }
+        }
+        if constexpr (REST) {
+            tmem_st16_nowait(p_addr + c * 16, cut);
+            tmem_st16_nowait(rest_addr + c * 16, rest);
+        }
+    }
+    unpair_f32(add_pair(add_pair(sums[0], sums[1]), add_pair(sums[2], sums[3])), s0, s1);
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
 // Stores 64 bytes of each lane's row (four 16-byte cells), with the four cells
 // of a row written by neighbouring lanes: lane l's v[j] becomes lane j's v[l]
 // among each four lanes, so a store covers 8 rows instead of 32.
@@ -370,11 +417,12 @@ __device__ __forceinline__ void store_rows4(uint16_t *dst, uint32_t (&v)[4][4], 
     }
 }
 
-template <int HD>
+template <int HD, bool REST>
 __global__ void __launch_bounds__(kTreeThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map, const TreeAttnParams p) {
     using C = TreeCfg<HD>;
+    constexpr bool kAhead = C::kOwnP && !REST;  // S(i + 2) before PV(i)
     constexpr uint32_t kIdescS = umma_idesc_bf16(kTreeRows, kTreeKeys);
     constexpr uint32_t kIdescPV = umma_idesc_bf16(kTreeRows, HD) | (1u << 16);  // V MN-major
     // The kernel's only shared memory, so it begins at a 1024-byte boundary
@@ -571,7 +619,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 uint32_t loaded = 0;
                 if (!is_v && seg == 0) load_q(g);
                 for (int i = 0; i < T; ++i) {
-                    const int at = ring_at + (is_v ? tree_pos_v<C::kOwnP>(two, i, T) : tree_pos_k<C::kOwnP>(two, i));
+                    const int at = ring_at + (is_v ? tree_pos_v<kAhead>(two, i, T) : tree_pos_k<kAhead>(two, i));
                     const int buf = at % C::kBufs;
                     const int box0 = (t0 + i) * boxes;
                     if (box0 >= first + kWarp) {
@@ -676,8 +724,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 if (leader) {
 #pragma unroll
                     for (int k = 0; k < kTreeKeys / 16; ++k) {
-                        umma_bf16_ta(tmem + C::kOCol + grp * HD, tmem + C::kPCol + grp * C::kPStep + k * 8, vd + (k * 2048 >> 4),
-                                     kIdescPV, (i > 1 || k > 0) ? 1u : 0u);
+                        umma_bf16_ta(tmem + C::kOCol + grp * HD, tmem + C::kPCol + grp * C::kPStep + (k >> 2) * C::kPHalf + (k & 3) * 8,
+                                     vd + (k * 2048 >> 4), kIdescPV, (i > 1 || k > 0) ? 1u : 0u);
+                    }
+                    if constexpr (REST) {
+#pragma unroll
+                        for (int k = 0; k < kTreeKeys / 16; ++k) {
+                            umma_bf16_ta(tmem + C::kOCol + grp * HD, tmem + grp * kTreeKeys + (k >> 2) * 64 + C::kRestCol + (k & 3) * 8,
+                                         vd + (k * 2048 >> 4), kIdescPV, 1u);
+                        }
                     }
                     if (C::kOwnP) umma_commit(smem_u32(&sh.pv_done[grp]));
                     if (!two || grp == 1) umma_commit(smem_u32(&sh.empty[v_buf]));
@@ -687,14 +742,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 return true;
             };
             // S(i + 2) goes into S(i)'s columns: once the softmax has read
-            // them, or, where P lies there, behind PV(i).
+            // them, or, where P or what it leaves off lies there, behind PV(i).
             auto free_s = [&](int i) -> bool { return wait(sh.s_free[i & 1], free_phase[i & 1]); };
             if (jobs > 0) {
                 ok = wait(sh.q_full, q_phase);
                 q_phase ^= 1;
                 if (ok) ok = issue_s(0) && (jobs < 2 || issue_s(1));
                 for (int i = 0; ok && i < jobs; ++i) {
-                    if (C::kOwnP) {
+                    if (kAhead) {
                         if (i + 2 < jobs) ok = free_s(i) && issue_s(i + 2);
                         free_phase[i & 1] ^= 1;
                         ok = ok && issue_pv(i);
@@ -763,7 +818,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     tmem_ld32_nowait(s_addr, sc[0]);
                     tmem_ld32_nowait(s_addr + 32, sc[0] + 32);
                 }
-                const int at = ring_at + tree_pos_v<C::kOwnP>(two, tile, T), buf = at % C::kBufs;
+                const int at = ring_at + tree_pos_v<kAhead>(two, tile, T), buf = at % C::kBufs;
                 // V of this tile stays until this group's P is consumed, so
                 // its phase cannot have moved on.
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sh.full[buf]), (at / C::kBufs) & 1));
@@ -787,12 +842,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     const unsigned long long scale2 = pair_f32(p.scale_log2, p.scale_log2);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (h == 0) {
+                        if (h == REST) {  // with REST the registers are needed until then
                             tmem_ld32_nowait(s_addr + 64, sc[1]);
                             tmem_ld32_nowait(s_addr + 96, sc[1] + 32);
-                        } else {
+                        }
+                        if (h == 1) {
                             tmem_wait_ld();
-                            if (C::kOwnP) {
+                            if (kAhead) {
                                 tc_fence_before();
                                 __syncwarp();
                                 if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[grp]));
@@ -822,21 +878,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                         }
                         while (true) {
                             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
-                            const unsigned long long neg_m2 = pair_f32(neg_m, neg_m);
-                            unsigned long long sums[4] = {0ull, 0ull, 0ull, 0ull};
-                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                mx[k & 3] = max3(mx[k & 3], sc[h][2 * k], sc[h][2 * k + 1]);
-                                float e0, e1;
-                                unpair_f32(fma_pair(pair_f32(sc[h][2 * k], sc[h][2 * k + 1]), scale2, neg_m2), e0, e1);
-                                e0 = fast_exp2(e0);
-                                e1 = fast_exp2(e1);
-                                sums[k & 3] = add_pair(sums[k & 3], pair_f32(e0, e1));
-                                w[k] = pack_bf16(e0, e1);
-                            }
-                            unpair_f32(add_pair(add_pair(sums[0], sums[1]), add_pair(sums[2], sums[3])), s0, s1);
-                            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                            const uint32_t p_part = p_addr + h * C::kPHalf, rest = s_addr + h * 64 + C::kRestCol;
+                            const float top = p.scale_log2 * tree_exponentials<REST>(sc[h], scale2, neg_m, w, s0, s1, p_part, rest);
                             const bool far = top > m_run + kTreeHeadroomLog2;
                             if (!__any_sync(0xFFFFFFFFu, far)) break;
                             // m is a whole number, so every rescaling is exact.
@@ -854,6 +897,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
                                     for (int k = 0; k < 16; ++k) pv[k] = __uint_as_float(mul_bf16x2(__float_as_uint(pv[k]), f2));
                                     tmem_st16(p_addr + c * 16, pv);
+                                    if (!REST) continue;
+                                    tmem_ld16(s_addr + C::kRestCol + c * 16, pv);
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) pv[k] = __uint_as_float(mul_bf16x2(__float_as_uint(pv[k]), f2));
+                                    tmem_st16(s_addr + C::kRestCol + c * 16, pv);
                                 }
                             }
                             if (i > 1) {
@@ -869,12 +917,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                         }
                         l_run += s0 + s1;
                         // In S's columns, P's 32 are among those read by now.
-                        tmem_st16_nowait(p_addr + h * 32, w);
-                        tmem_st16_nowait(p_addr + h * 32 + 16, w + 16);
+                        if (!REST) {
+                            tmem_st16_nowait(p_addr + h * C::kPHalf, w);
+                            tmem_st16_nowait(p_addr + h * C::kPHalf + 16, w + 16);
+                        }
                     }
                     tmem_wait_st();
                     tc_fence_before();
-                } else if (C::kOwnP && lane == 0) {
+                } else if (kAhead && lane == 0) {
                     mbar_arrive(smem_u32(&sh.s_free[grp]));
                 }
                 __syncwarp();

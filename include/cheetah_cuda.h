@@ -426,7 +426,9 @@ CHEETAH_CUDA_API int cheetah_cuda_op_qk_norm_rope(const CheetahCudaQkNormRope *a
  * cells a row does not see never reach it, non-finite ones included. Rows
  * from row_starts[batch] on stay as they were; a sequence with seq_lens[b] <
  * n gives zeros, and keys on a page outside the pool count as unseen. q and
- * the softmax weights are bf16 in the products, sums and statistics are f32.
+ * the softmax weights are bf16 in the products, the weights two bf16 parts
+ * where rows * q_heads <= 512; sums and statistics are f32. If a wait inside
+ * the kernel gives up, every row is NaN.
  *
  * `workspace` holds partial results between the two launches of a call:
  * cheetah_cuda_op_tree_attention_workspace says how many bytes (256-byte

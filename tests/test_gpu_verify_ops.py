@@ -352,6 +352,51 @@ def test_tree_attention_non_finite_context_beside_a_page_outside_the_pool(value,
     assert bool(torch.isfinite(out[..., ~hit]).all())
 
 
+# Calls of few rows (512 of all heads) multiply P in two parts; with rows behind
+# the last sequence the same trees run as a larger call does.
+
+@pytest.mark.parametrize("q_heads,kv_heads,D", HEADS)
+@pytest.mark.parametrize("ctx,nodes", [([0], [1]), ([700, 129], [3, 30]), ([1, 64, 300, 0], [1, 17, 40, 5]), ([5000], [12])])
+def test_tree_attention_as_a_larger_call(q_heads, kv_heads, D, ctx, nodes):
+    case = Tree(ctx, nodes, q_heads, kv_heads, D, seed=31, extra_rows=520)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tree_attention_masks_scores_and_cells_as_a_larger_call(D):
+    more = dict(q_heads=8, kv_heads=2, D=D, extra_rows=100)
+    for window in (5, 130):
+        case = Tree([200, 9], [7, 30], window=window, seed=32, **more)
+        case.check(case.run())
+    case = Tree([300, 40], [10, 70], seed=33, scale=40.0, **more)
+    case.check(case.run())
+    case = Tree([140, 50], [12, 9], seed=34, **more)
+    clean = case.run()
+    page, cell = int(case.table[0, 143 // 64]), 143 % 64
+    for pool in ("k_pool", "v_pool"):
+        case.dev[pool][page, :, cell] = math.inf
+    out = case.run()
+    for i in range(12):
+        if not case.seen[0][i][3]:
+            assert torch.equal(out[i], clean[i])
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,D", [(14, 2, 64), (8, 4, 128)])
+def test_tree_attention_of_few_rows_rounds_only_its_output(q_heads, kv_heads, D):
+    """P enters the products cut to bf16 (off by up to 2^-7) with the rest as
+    bf16 beside it (off by half a step of 2^-7): 2^-15, and 2^-23 added."""
+    case = Tree([700, 90], [8, 21], q_heads, kv_heads, D, seed=35)
+    out = case.run().cpu().double()
+    for b, i in ((0, 0), (0, 7), (1, 3), (1, 20)):
+        seen, r = case.visible(b, i), int(case.starts[b]) + i
+        for h in range(q_heads):
+            k, v = case.k[b][:, h // case.group], case.v[b][:, h // case.group]
+            want, tol = V.tree_row(case.q[r, h].double(), k, v, seen)
+            p = torch.softmax(k[seen] @ case.q[r, h].double() / math.sqrt(D), 0)
+            tol = tol - (p @ v[seen].abs()) * (2.0 ** -8 - 2.0 ** -15 - 2.0 ** -23) * 1.01
+            assert bool(((out[r, h] - want).abs() <= tol).all())
+
+
 def test_tree_attention_large_scores():
     """Scores of a few hundred: one weight is 1 and the others underflow."""
     case = Tree([300, 40], [10, 70], 14, 2, 64, seed=9, scale=40.0)
