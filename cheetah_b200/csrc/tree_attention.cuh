@@ -220,8 +220,8 @@ struct TreeShared {
 };
 
 template <int HD>
-constexpr size_t tree_attention_smem() { return (size_t)TreeCfg<HD>::kTiles + 3072; }
-static_assert(sizeof(TreeShared) <= 3072, "fits behind the tiles");
+constexpr size_t tree_attention_smem() { return (size_t)TreeCfg<HD>::kTiles + 3 * 1024; }
+static_assert(sizeof(TreeShared) <= 3 * 1024, "fits behind the tiles");
 
 // The role's next segment, once the scheduler has published it; false at the
 // end of the share or when a wait gave up (then *ok is false).
