@@ -204,8 +204,12 @@ int cheetah_cuda_op_page_slots(const CheetahCudaPageSlots *a, void *stream) {
     const bool wide = (long long)p.max_tokens > 2ll * cheetah::sm_count(device) * cheetah::kSlotThreads;
     const int vec = wide && aligned(a->positions, 16) && aligned(a->seq_ids, 16) && aligned(a->slots, 16) ? 4 : 1;
     auto kernel = vec == 4 ? cheetah::page_slots_kernel<4> : cheetah::page_slots_kernel<1>;
-    if (smem > 48 * 1024)
-        CH_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 48 * 1024) {
+        // What the largest batch needs, whatever this one does: the limit
+        // belongs to the kernel, and another thread may be about to launch it.
+        static std::atomic<uint64_t> done[2];
+        CH_CUDA_TRY(cheetah::allow_smem(kernel, (size_t)cheetah::kSlotMaxBatch * 3 * sizeof(int32_t), device, done[vec == 4]));
+    }
     const int per_block = cheetah::kSlotThreads * vec;
     const int blocks = (int)std::min<long long>(2 * cheetah::sm_count(device), ((long long)p.max_tokens + per_block - 1) / per_block);
     CH_CUDA_TRY(launch_ex(kernel, dim3(blocks), dim3(cheetah::kSlotThreads), smem, static_cast<cudaStream_t>(stream), true, p));

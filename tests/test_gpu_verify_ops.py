@@ -85,6 +85,37 @@ def test_page_slots_edges(name, cached, new, more):
     _check_slots(_slots_case(cached, new, 4, 16, **more))
 
 
+def test_page_slots_from_two_threads():
+    """Host threads whose batches need different amounts of shared memory call
+    at the same time (straight through the C-ABI, which runs without Python's
+    lock): neither call depends on what the other one asked for."""
+    import threading
+    from cheetah_b200 import runtime as R
+    call, failed = R.lib().cheetah_cuda_op_page_slots, []
+
+    def calls(batch):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            cached, new, table = i32([3] * batch), i32([1] * batch), torch.zeros(batch, 1, dtype=torch.int32, device="cuda")
+            free, free_count = i32(range(4)), i32([4])
+            outs = [torch.empty(n, dtype=torch.int32, device="cuda") for n in (batch + 1, batch, batch, batch, batch, 3)]
+        args = R.PageSlotsArgs(cached.data_ptr(), new.data_ptr(), free.data_ptr(), free_count.data_ptr(), 4, batch,
+                               table.data_ptr(), 1, 8, 16, batch, *[o.data_ptr() for o in outs])
+        for _ in range(20000):
+            if call(args, stream.cuda_stream):
+                failed.append((batch, R.lib().cheetah_cuda_last_error()))
+                break
+        stream.synchronize()
+        if outs[5].tolist() != [batch, 0, 0] or not bool((outs[2] == 3).all()):
+            failed.append((batch, "wrong rows"))
+    threads = [threading.Thread(target=calls, args=(batch,)) for batch in (4200, 16384)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
 # ---- qk_norm_rope -------------------------------------------------------------
 
 @pytest.mark.parametrize("q_heads,kv_heads,D,rotary", [(14, 2, 64, 64), (28, 4, 128, 128), (4, 4, 64, 32), (3, 1, 128, 16),
