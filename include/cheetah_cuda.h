@@ -427,8 +427,10 @@ CHEETAH_CUDA_API int cheetah_cuda_op_qk_norm_rope(const CheetahCudaQkNormRope *a
  * from row_starts[batch] on stay as they were; a sequence with seq_lens[b] <
  * n gives zeros, and keys on a page outside the pool count as unseen. q and
  * the softmax weights are bf16 in the products, the weights two bf16 parts
- * where rows * q_heads <= 512; sums and statistics are f32. If a wait inside
- * the kernel gives up, every row is NaN.
+ * where rows * q_heads <= 512 (rows behind the last sequence count); sums and
+ * statistics are f32. Values of at most 2^127 give finite results, whatever the
+ * scores; weights below 2^-87 of a row's largest may count as zero. If a wait
+ * inside the kernel gives up, every row is NaN.
  *
  * `workspace` holds partial results between the two launches of a call:
  * cheetah_cuda_op_tree_attention_workspace says how many bytes (256-byte

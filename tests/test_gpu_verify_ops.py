@@ -383,6 +383,38 @@ def test_tree_attention_non_finite_context_beside_a_page_outside_the_pool(value,
     assert bool(torch.isfinite(out[..., ~hit]).all())
 
 
+@pytest.mark.parametrize("extra_rows", [0, 520])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ctx,nodes", [(300, 12), (300, 40), (9000, 12)])
+def test_tree_attention_large_values(ctx, nodes, D, extra_rows):
+    """Values up to 2^127 and scores that rise after a row's first keys, by 20
+    log2 units and then by 60: the results are averages of the values, so they
+    are finite."""
+    case = Tree([ctx], [nodes], 8, 2, D, seed=36, extra_rows=extra_rows)
+    g = torch.Generator().manual_seed(37)
+    n = ctx + nodes
+    case.q = torch.zeros(case.rows, 8, D, dtype=torch.bfloat16)
+    case.q[:, :, 0] = 8.0
+    units = torch.full((n,), 20.0)  # the keys' scores
+    units[:64], units[ctx:] = 0.0, 0.0
+    for one in (20.0, 80.0):
+        units[n * 3 // 4] = one
+        k = torch.zeros(n, 2, D)
+        k[:, :, 0] = (units * math.log(2.0) * math.sqrt(D) / 8.0)[:, None]
+        v = (torch.rand(n, 2, D, generator=g) + 1.0) * 2.0 ** 126
+        v[:, :, 1::2] *= -1.0
+        k, v = k.bfloat16(), v.bfloat16()
+        case.k[0], case.v[0] = k.double(), v.double()
+        at = torch.arange(n)
+        page = torch.from_numpy(case.table[0])[at // 64].long().cuda()
+        case.dev["q"] = case.q.cuda()
+        case.dev["k_pool"][page, :, (at % 64).cuda()] = k.cuda()
+        case.dev["v_pool"][page, :, (at % 64).cuda()] = v.cuda()
+        out = case.run()
+        assert bool(torch.isfinite(out[:nodes].float()).all())
+        case.check(out)
+
+
 # Calls of few rows (512 of all heads) multiply P in two parts; with rows behind
 # the last sequence the same trees run as a larger call does.
 
