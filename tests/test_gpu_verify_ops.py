@@ -609,6 +609,54 @@ def test_token_logprobs_masked_and_broken_rows(dtype):
     _check_logprobs(x, [0, 5, 1, 2, 3, 4, 0, 7, -1, vocab], 8, dtype)
 
 
+@pytest.mark.parametrize("vocab", [300, 5000, 151936])
+@pytest.mark.parametrize("top", [0, 5])
+def test_token_logprobs_peaked_rows(vocab, top):
+    """Two logits at most count, the rest are 50 below. Then S = 1 + e^-d is
+    rounded twice at most (2^-24 each, in a thread and in the join), its log
+    once, and e^-d is off by 2^-20 of itself. The entropy adds a few terms of
+    at most 2 log2 units with one rounding each."""
+    from cheetah_b200 import runtime as R
+    gaps = [0.0, 0.5, 0.99, 1.01, 3.0, 7.99, 8.01, 12.0, 25.0]
+    places = [(3, vocab - 40), (vocab - 40, 3), (5, vocab // 2), (vocab // 2, vocab // 2 + 1), (vocab // 3, vocab - 1)]
+    for base in (0.0, 17.3, -40.2):
+        x = torch.full((len(gaps) * len(places), vocab), base - 50.0, dtype=torch.float64)
+        low, high = [], []
+        for i, d in enumerate(gaps):
+            for j, (a, b) in enumerate(places):
+                r = i * len(places) + j
+                x[r, a], x[r, b] = base, base + d
+                low.append(a)
+                high.append(b)
+        x = x.float()
+        exact = torch.log_softmax(x.double(), 1)
+        entropy = -(exact.exp() * exact).sum(1)
+        u = 2.0 ** -24
+        for tokens in (low, high):
+            got = R.token_logprobs(x.cuda(), i32(tokens), top=top)
+            want = exact.gather(1, torch.tensor(tokens)[:, None])[:, 0]
+            lp, h = got.logprob.cpu().double(), got.entropy.cpu().double()
+            assert bool((lp <= 0).all()) and bool((h >= 0).all())
+            tol = 3 * u + (1 - exact.max(1).values.exp()) * 2.0 ** -20 + 2 * u * want.abs()
+            assert bool(((lp - want).abs() <= tol).all()), float(((lp - want).abs() / tol).max())
+            assert bool(((h - entropy).abs() <= 15 * u + entropy * 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [700, 40000])
+def test_token_logprobs_signs(dtype, vocab):
+    """No log probability is above 0 and no entropy below, however far the
+    largest logit stands out and wherever it lies."""
+    from cheetah_b200 import runtime as R
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(1000, vocab, generator=g, device="cuda") * 0.3 - 12.0
+    at = torch.randint(0, vocab, (1000, 1), generator=g, device="cuda")
+    x.scatter_(1, at, torch.rand(1000, 1, generator=g, device="cuda") * 20.0)
+    x = x.to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+    got = R.token_logprobs(x, at[:, 0].int(), top=2)
+    assert bool((got.logprob <= 0).all()) and bool((got.top_logprobs <= 0).all()) and bool((got.entropy >= 0).all())
+
+
 def test_token_logprobs_strided_unaligned_rows():
     g = torch.Generator().manual_seed(4)
     for dtype in ("f32", "bf16"):
