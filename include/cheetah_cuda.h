@@ -399,7 +399,7 @@ typedef struct CheetahCudaQkNormRope {
     const float *rope_sin;
     uint32_t max_positions;
     uint32_t rotary_dim;       /* a multiple of 16, at most head_dim; later dimensions pass through */
-    const int32_t *positions;  /* [tokens] */
+    const int32_t *positions;  /* [tokens], absolute: a drafted node's is its sequence's cached length + its depth */
     const int32_t *slots;      /* [tokens] */
     uint32_t tokens;
     uint32_t q_heads;
@@ -451,7 +451,7 @@ typedef struct CheetahCudaTreeAttention {
     uint32_t batch;            /* 1..4096 */
     const uint64_t *tree_mask; /* [rows][mask_words] */
     uint32_t mask_words;       /* 1..16; nodes from 64*mask_words on are unseen by other rows and themselves */
-    const int32_t *positions;  /* [rows]; may be NULL without a window */
+    const int32_t *positions;  /* [rows], absolute as for the rotation; may be NULL without a window */
     uint32_t sliding_window;   /* 0 = full */
     uint32_t q_heads;
     uint32_t kv_heads;         /* q_heads / kv_heads: 1..32 */
