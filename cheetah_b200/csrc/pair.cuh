@@ -1,5 +1,5 @@
-// Two f32 per instruction: sm_100's packed add, multiply and fused
-// multiply-add on the halves of a 64-bit register.
+// Two f32 per instruction: sm_100's packed add and fused multiply-add on
+// the halves of a 64-bit register.
 #pragma once
 
 namespace cheetah {
@@ -20,11 +20,6 @@ __device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, uns
 __device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
     unsigned long long r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 
