@@ -30,14 +30,17 @@
 //   warps 4-11 two softmax groups, one thread per row: read the S row from
 //              TMEM 64 keys at a time, mask, exponentials, P as bf16 into
 //              TMEM (the A operand of PV is read from there). The reference m
-//              is a whole number of log2 units (P, l and O share it, so the
-//              quotient is the same) that moves only when a score lies 2^8
-//              above the one that set it, so a tile usually takes one pass
-//              over S: exponentials about the old m and the maximum beside
-//              them. O, l and P are rescaled, by a power of two, only when m
-//              moves. m lies so far above that score that the P of all keys
-//              sum to at most 1, whatever comes before the next move: O stays
-//              within the largest |v|, so finite values never overflow it.
+//              (P, l and O share it, so the quotient is the same) is set by
+//              the largest of a row's first scores and moves, by whole log2
+//              units, only when a score lies 2^8 above, so a tile usually
+//              takes one pass over S: exponentials about the old m and the
+//              maximum beside them. O, l and P are rescaled, by a power of
+//              two, only when m moves. m lies a whole number of units above
+//              that score, so its P is a power of two, which bf16 holds (a row
+//              that sees one key returns its value), and so far above that the
+//              P of all keys sum to at most 1, whatever comes before the next
+//              move: O stays within the largest |v|, so finite values never
+//              overflow it.
 // P is rounded to bf16 because the tensor cores multiply bf16; sums,
 // statistics and O stay f32. Over many rows P's roundings add as much error as
 // the output's. A call of few rows, where one row with an unlucky rounding of
@@ -796,9 +799,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             }
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             const int ctx = g.ctx;
-            // From a score to the m that it sets: the headroom, and log2 of
-            // the number of keys, rounded up.
-            const float rise = (float)(kTreeHeadroomLog2 + 32 - __clz(g.len - 1));
+            // From a score to the m that it sets: log2 of the number of keys,
+            // rounded up, and the headroom.
+            const float spread = (float)(32 - __clz(g.len - 1));
             float m_run = -INFINITY, l_run = 0.0f;
             for (int i = grp; i < jobs; i += 2) {
                 const int tile = two ? i >> 1 : i;
@@ -880,17 +883,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int k = 0; k < 32; ++k) mx[k & 3] = max3(mx[k & 3], sc[h][2 * k], sc[h][2 * k + 1]);
-                            m_run = ceilf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2) + rise;
+                            m_run = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2 + (spread + kTreeHeadroomLog2);
                         }
                         while (true) {
                             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
                             const uint32_t p_part = p_addr + h * C::kPHalf, rest = s_addr + h * 64 + C::kRestCol;
                             const float top = p.scale_log2 * tree_exponentials<REST>(sc[h], scale2, neg_m, w, s0, s1, p_part, rest);
-                            const bool far = top + (rise - kTreeHeadroomLog2) > m_run;
+                            const bool far = top + spread > m_run;
                             if (!__any_sync(0xFFFFFFFFu, far)) break;
-                            // m is a whole number, so every rescaling is exact.
-                            // (Rounding keeps order: then `far` is false.)
-                            const float m_new = far ? ceilf(top) + rise : m_run;
+                            // By a whole number, so every rescaling is exact,
+                            // and to where `far` is false (from -inf, where the
+                            // first keys are unseen: to the score itself).
+                            float m_new = m_run;
+                            if (far) {
+                                // (Once more: a register less outside.)
+                                const float to = top + (float)(kTreeHeadroomLog2 + 32 - __clz(g.len - 1));
+                                m_new = fmaxf(m_run + ceilf(to - m_run), to);
+                            }
                             const float f = m_new == m_run ? 1.0f : exp2f(m_run - m_new);
                             m_run = m_new;
                             l_run *= f;

@@ -444,6 +444,21 @@ def test_tree_attention_masks_scores_and_cells_as_a_larger_call(D):
             assert torch.equal(out[i], clean[i])
 
 
+@pytest.mark.parametrize("extra_rows", [0, 520])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tree_attention_rows_that_see_one_key_return_its_value(D, extra_rows):
+    """The only weight of a row is 1 whatever its rounding, in small calls and
+    in large ones: nodes that see themselves alone, over an empty context."""
+    def masks(rng, n):
+        return np.eye(n, dtype=bool)
+    case = Tree([0, 0], [30, 9], 8, 2, D, masks=masks, seed=38, extra_rows=extra_rows)
+    out = case.run().cpu()
+    for b, n in enumerate(case.nodes):
+        for i in range(n):
+            value = case.v[b][i].bfloat16().repeat_interleave(case.group, 0)
+            assert torch.equal(out[int(case.starts[b]) + i], value), (b, i)
+
+
 @pytest.mark.parametrize("q_heads,kv_heads,D", [(14, 2, 64), (8, 4, 128)])
 def test_tree_attention_of_few_rows_rounds_only_its_output(q_heads, kv_heads, D):
     """P enters the products cut to bf16 (off by up to 2^-7) with the rest as
