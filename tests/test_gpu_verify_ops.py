@@ -313,6 +313,22 @@ def test_tree_attention_long_and_wide():
     case.check(case.run())
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,D", [(17, 1, 64), (24, 1, 128), (31, 1, 128), (32, 1, 64), (64, 2, 128)])
+def test_tree_attention_wide_groups(q_heads, kv_heads, D):
+    case = Tree([300, 0, 129], [9, 20, 1], q_heads, kv_heads, D, seed=q_heads)
+    case.check(case.run())
+    case = Tree([130], [11], q_heads, kv_heads, D, window=70, seed=q_heads)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,D,window", [(14, 2, 64, 0), (8, 4, 128, 0), (4, 4, 64, 100)])
+def test_tree_attention_as_many_nodes_as_a_mask_holds(q_heads, kv_heads, D, window):
+    """1024 nodes of one sequence, as a tree and as a prompt chunk (a chain)."""
+    case = Tree([77, 5], [1024, 3], q_heads, kv_heads, D, window=window, seed=41)
+    case.check(case.run())
+    case = Tree([200], [1000], q_heads, kv_heads, D, seed=42, masks=lambda rng, n: np.tril(np.ones((n, n), bool)))
+    case.check(case.run())
+
 def test_tree_attention_many_sequences():
     rng = np.random.default_rng(8)
     case = Tree(rng.integers(0, 200, 300).tolist(), rng.integers(0, 4, 300).tolist(), 14, 2, 64, seed=8)
@@ -555,6 +571,33 @@ def test_tree_attention_on_other_streams_and_in_graphs():
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert torch.equal(o, w)
+
+
+def test_tree_attention_join_after_a_wait_that_gave_up(tmp_path):
+    """The join alone, on a list of split items in which one CTA has given up:
+    every row is NaN, those behind the last sequence stay. Without one that has,
+    and without anything to join, it writes nothing."""
+    import ctypes as C
+    import subprocess
+    from pathlib import Path
+    from cheetah_b200 import build
+    here = Path(__file__).resolve().parent
+    lib = tmp_path / "tree_join.so"
+    subprocess.run([build.nvcc(), *build.ARCH_FLAGS, "-O1", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-I", str(build.CSRC),
+                    "-I", str(build.INCLUDE), "--expt-relaxed-constexpr", "-o", str(lib), str(here / "tree_join_entry.cu")],
+                   check=True, capture_output=True, timeout=300)
+    join = C.CDLL(str(lib)).tree_join
+    rows, q_heads, ctas = 20, 3, 5
+    starts = i32([0, 4, 13])
+    splits = torch.zeros(32 * ctas, dtype=torch.uint8, device="cuda")
+    for parts, given_up in (([0, 0, -1, 0, 0], True), ([0, 1, 0, 1, 0], False), ([-1] * 5, True)):
+        out = torch.full((rows, q_heads, 64), 2.5, dtype=torch.bfloat16, device="cuda")
+        rc = join((C.c_int * ctas)(*parts), ctas, C.c_void_p(starts.data_ptr()), 2, rows, q_heads, C.c_void_p(splits.data_ptr()),
+                  C.c_void_p(out.data_ptr()), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert rc == 0
+        assert bool(torch.isnan(out[:13]).all()) if given_up else bool((out[:13] == 2.5).all())
+        assert bool((out[13:] == 2.5).all())
 
 
 # ---- token_logprobs -----------------------------------------------------------
