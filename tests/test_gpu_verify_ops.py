@@ -169,6 +169,54 @@ def test_qk_norm_rope(q_heads, kv_heads, D, rotary, dtype, kv_dtype, tokens, nor
     assert torch.equal(v_pool.cpu(), want_v)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,D,rotary,dtype,kv_dtype,tokens", [
+    (14, 2, 64, 64, "bf16", "bf16", 2501), (28, 4, 128, 128, "bf16", "bf16", 901), (14, 2, 64, 32, "f32", "bf16", 1503),
+    (4, 1, 128, 128, "f32", "f32", 2407), (3, 1, 64, 64, "bf16", "f32", 7205), (32, 8, 64, 64, "bf16", "bf16", 1301)])
+def test_qk_norm_rope_rows_that_a_warp_walks_over(q_heads, kv_heads, D, rotary, dtype, kv_dtype, tokens):
+    """So many rows that a warp takes all heads of one, up to three groups of
+    them and more; some rows are skipped and some append nothing."""
+    from cheetah_b200 import runtime as R
+    types = {"bf16": torch.bfloat16, "f32": torch.float32}
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    heads, pt, max_pos = q_heads + 2 * kv_heads, 16, 70
+    pages = -(-tokens // pt) + 2
+    x = torch.randn(tokens, heads, D, generator=g, device="cuda").to(types[dtype])
+    slots = torch.randperm(pages * pt, generator=g, device="cuda")[:tokens].to(torch.int32)
+    positions = torch.randint(0, max_pos, (tokens,), generator=g, device="cuda").to(torch.int32)
+    positions[::7], slots[::5] = -1, pages * pt
+    angle = torch.rand(max_pos, rotary // 2, generator=g, device="cuda") * 6.0
+    cos, sin = angle.cos(), angle.sin()
+    w = [1.0 + 0.3 * torch.randn(D, generator=g, device="cuda") for _ in range(2)]
+    pools = [torch.randn(pages, kv_heads, pt, D, generator=g, device="cuda").to(types[kv_dtype]) for _ in range(2)]
+    k_pool, v_pool = pools[0].clone(), pools[1].clone()
+    q_out = torch.full((tokens, q_heads, D), 7.0, dtype=types[dtype], device="cuda")
+    R.qk_norm_rope(x, q_heads, kv_heads, positions, slots, cos, sin, k_pool, v_pool, q_norm=w[0], k_norm=w[1], eps=1e-5, q_out=q_out)
+
+    # The formula in 64 bits, and the magnitudes that its last addition joins.
+    at = positions.long().clamp(min=0)
+    c, s = cos.double()[at][:, None], sin.double()[at][:, None]
+    y = x[:, :q_heads + kv_heads].double()
+    weight = torch.cat([w[0].expand(q_heads, D), w[1].expand(kv_heads, D)]).double()
+    y = y * (weight / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-5))
+    half = rotary // 2
+    z, mag = y.clone(), y.abs()
+    a, b = y[..., :half], y[..., half:rotary]
+    z[..., :half], z[..., half:rotary] = a * c - b * s, b * c + a * s
+    mag[..., :half], mag[..., half:rotary] = (a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()
+    f32 = (D / 2 + 10) * 2.0 ** -24
+    step = {"bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+    live = positions >= 0
+    q, zq = q_out.double(), z[:, :q_heads]
+    assert bool(((q - zq).abs() <= mag[:, :q_heads] * f32 + zq.abs() * step[dtype] + 1e-30)[live].all())
+    assert bool((q[~live] == 7.0).all())
+    kept = live & (slots < pages * pt)
+    page, cell = slots[kept].long() // pt, slots[kept].long() % pt
+    zk, mk = z[kept, q_heads:], mag[kept, q_heads:]
+    assert bool(((k_pool[page, :, cell].double() - zk).abs() <= mk * f32 + zk.abs() * step[kv_dtype] + 1e-30).all())
+    pools[0][page, :, cell] = k_pool[page, :, cell]
+    pools[1][page, :, cell] = x[kept, q_heads + kv_heads:].to(types[kv_dtype])
+    assert torch.equal(k_pool, pools[0]) and torch.equal(v_pool, pools[1])  # cells not named: unchanged
+
 def test_qk_norm_rope_large_values_and_zero_rows():
     """A zero row stays zero, values near the type's limits keep their scale,
     a non-finite value stays in its own head."""
@@ -312,6 +360,14 @@ def test_tree_attention_long_and_wide():
     case = Tree([5000, 1], [130, 257], 28, 4, 128, seed=4)
     case.check(case.run())
 
+
+def test_tree_attention_as_many_sequences_as_a_call_takes():
+    rng = np.random.default_rng(9)
+    case = Tree(rng.integers(0, 150, 4096).tolist(), rng.integers(0, 2, 4096).tolist(), 4, 2, 64, page_tokens=16, seed=9)
+    case.check(case.run())
+    # All but the last without rows.
+    case = Tree([3] * 4095 + [200], [0] * 4095 + [5], 4, 2, 128, page_tokens=16, seed=10)
+    case.check(case.run())
 
 @pytest.mark.parametrize("q_heads,kv_heads,D", [(17, 1, 64), (24, 1, 128), (31, 1, 128), (32, 1, 64), (64, 2, 128)])
 def test_tree_attention_wide_groups(q_heads, kv_heads, D):
