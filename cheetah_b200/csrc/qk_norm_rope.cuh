@@ -66,7 +66,9 @@ __device__ __forceinline__ void widen_chunk(const uint4 &raw, float (&v)[VEC]) {
     }
 }
 
-// STREAM: the chunk will not be read while it could still lie in L2.
+// STREAM: the chunk is the first to leave L2. A long call's rows are gone before
+// the attention reads them; a short call's (1021 rows are under 20 MB) still lie
+// there while L2 has room.
 template <typename T, int VEC, bool STREAM>
 __device__ __forceinline__ void store_chunk(void *base, long long at, const float (&v)[VEC]) {
     if constexpr (sizeof(T) == 2) {

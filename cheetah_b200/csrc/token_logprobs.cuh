@@ -13,9 +13,9 @@
 // is split over a cluster of 1..16 CTAs that join their results in the first
 // one's shared memory, so a call is one launch and needs no workspace.
 //
-// One f32 row of 151936 with 5 alternatives takes 8.4 us (16 CTAs; latency),
-// 2048 such rows with one 208 .. 220 us (5.7 .. 6.0 TB/s), 500 bf16 rows of
-// 152064 36 us without alternatives and 54 us (2.8 TB/s) with twenty: there the
+// One f32 row of 151936 with 5 alternatives takes 8.7 us (16 CTAs; latency),
+// 2048 such rows with one 214 .. 218 us (5.7 .. 5.8 TB/s), 500 bf16 rows of
+// 152064 38 us without alternatives and 55 us (2.8 TB/s) with twenty: there the
 // operations per logit bound it (about 8, and a logit is 2 bytes), the sorts,
 // and that 500 rows leave a sixth of the SMs' places empty.
 //

@@ -45,8 +45,8 @@
 // statistics and O stay f32. Over many rows P's roundings add as much error as
 // the output's. A call of few rows, where one row with an unlucky rounding of
 // its largest weight shows, has time for a second product per tile (REST): what
-// bf16 leaves off, as bf16 again, is multiplied too (P to 2^-16 instead of
-// 2^-9), and the output is as exact as its own rounding.
+// bf16 leaves off, as bf16 again, is multiplied too (P to 2^-15 instead of
+// 2^-8), and the output is as exact as its own rounding.
 // With head_dim 64 TMEM has columns of its own for P, so without REST S(i + 2)
 // is computed while the softmax of S(i) still runs; otherwise P, or what it
 // leaves off, takes S's columns and S(i + 2) follows PV(i).
@@ -59,11 +59,11 @@
 // rows that do see it after the products (patch_row).
 //
 // Bounds and times (B200, the join included). One sequence, 708 keys, 14/2
-// heads of 64: 12.9 us, latency (attention 8, the join's launch 1, the join 4).
-// One sequence, 64 nodes at 32.7k keys: 28 us (265 TFLOP/s). 32 sequences of
-// 128 .. 8k keys with up to 16 nodes, 28/4 heads of 128: 65 us, 4.6 TB/s, bound
-// by the loads. 64 sequences of 3k .. 8k keys with 40 .. 64 nodes: 432 us, 634
-// TFLOP/s; there the chain S, softmax, PV of a tile (about 4400 cycles for the
+// heads of 64: 12.5 .. 13 us, latency (attention 8, the join's launch 1, the join
+// 4). One sequence, 64 nodes at 32.7k keys: 28 us (267 TFLOP/s). 32 sequences of
+// 128 .. 8k keys with up to 16 nodes, 28/4 heads of 128: 66 us, 4.5 TB/s, bound
+// by the loads. 64 sequences of 3k .. 8k keys with 40 .. 64 nodes: 433 .. 445 us,
+// 625 TFLOP/s; there the chain S, softmax, PV of a tile (about 4400 cycles for the
 // two groups, of which the products are 2100 and the exponentials 2000) and
 // the clock under the power limit (1.62 of 1.96 GHz) bound it. S two jobs
 // ahead in 64-key tiles, with one MMA warp or one per group, was slower (470

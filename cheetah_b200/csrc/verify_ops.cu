@@ -93,8 +93,8 @@ int launch_qk(cheetah::QkNormRopeParams p, bool kv_bf16, cudaStream_t stream) {
 // A cluster of CTAs per row: the number that leaves the busiest SM the least
 // (rows divide badly among 148 SMs, and one row fills 16). A part is charged 3%
 // for its join, 20% where it sorts too, and holds at least half a sample: 500
-// bf16 rows of 152064 take 36 us in two parts and 44 in one without
-// alternatives, 77 and 60 with twenty.
+// bf16 rows of 152064 take 37.5 us in two parts and 39.6 in one without
+// alternatives, 59.2 and 55.4 with twenty.
 int launch_logprobs(const cheetah::LogprobParams &p, bool bf16, cudaStream_t stream) {
     auto kernel = bf16 ? cheetah::token_logprobs_kernel<uint16_t> : cheetah::token_logprobs_kernel<float>;
     int device = 0;

@@ -352,7 +352,8 @@ CHEETAH_CUDA_API int cheetah_cuda_op_decode_attention_noalloc(const CheetahCudaD
  * A slot is page * page_tokens + the position within the page.
  *
  * A sequence is refused where a length is negative or its positions pass the
- * table's width (it then counts as no rows), where its rows pass max_tokens, or
+ * table's width (it then counts as no rows), where its rows pass max_tokens
+ * (every later sequence is then refused too, with rows or without), or
  * where its pages pass the end of the free list (every later sequence that
  * needs a page is then refused too). A refused sequence takes no page, its
  * table row stays, seq_lens is 0 and its rows hold position and slot -1. Rows
