@@ -23,7 +23,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libcheetah_cuda.so"
 
-SOURCES = ["cheetah_cuda.cu", "verify_ops.cu", "store.cpp"]
+SOURCES = ["cheetah_cuda.cu", "verify_ops.cu", "kv8_ops.cu", "store.cpp"]
 HEADERS = ["common.cuh", "gemv.cuh", "attention.cuh", "kernels_misc.cuh", "store.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,53 @@
+// The 8-bit cache format: e4m3 codes, and one f32 scale for the kKv8Block cells
+// of a block and KV head. value = code * scale.
+#pragma once
+
+#include <stdint.h>
+
+namespace cheetah {
+
+constexpr int kKv8Block = 16;
+constexpr int kKv8LeastLog2 = -64;  // log2 of the smallest scale that an append sets
+
+// Four e4m3 codes of f32 values (nearest, ties to even; NaN stays NaN). Values
+// beyond 448 become 448.
+__device__ __forceinline__ uint32_t pack_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+    return pack_e4m3x2(a, b) | pack_e4m3x2(c, d) << 16;
+}
+
+// Two e4m3 codes (the low half of w) as an f16 pair: exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
+    return r;
+}
+__device__ __forceinline__ void unpack_e4m3x4(uint32_t w, float (&v)[4]) {
+    const uint32_t lo = e4m3x2_to_f16x2(w), hi = e4m3x2_to_f16x2(w >> 16);
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(v[0]), "=f"(v[1]) : "r"(lo));
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(v[2]), "=f"(v[3]) : "r"(hi));
+}
+
+// f32 that any narrower format rounds as it would round x: cut off, and the last
+// bit set where that left something off (it can then not lie on a tie). A
+// non-finite value becomes NaN, which has no code but NaN.
+__device__ __forceinline__ float round_to_odd(double x) {
+    const float f = __double2float_rz(x);
+    const uint32_t bits = __float_as_uint(f);
+    if ((bits & 0x7F800000u) == 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    return (double)f == x ? f : __uint_as_float(bits | 1u);
+}
+
+// The smallest power of two, 2^kKv8LeastLog2 at least, whose 448-fold reaches the
+// magnitude whose f32 bits these are.
+__device__ __forceinline__ float kv8_scale_for(uint32_t top_bits) {
+    // 448 = 1.75 * 2^8.
+    const int e = (int)(top_bits >> 23) - 127 - 8 + ((top_bits & 0x7FFFFFu) > 0x600000u);
+    return __uint_as_float((uint32_t)(max(e, kKv8LeastLog2) + 127) << 23);
+}
+
+}  // namespace cheetah

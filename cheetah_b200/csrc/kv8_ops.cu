@@ -1,0 +1,279 @@
+// The op entries of a step over an 8-bit cache (include/cheetah_cuda.h): q/k
+// norm with rotation and 8-bit append, reading back, attention, and the test of
+// drafted tokens. Each checks its arguments, launches on the caller's stream and
+// keeps nothing.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <string>
+#include <type_traits>
+
+#include "attention_kv8.cuh"
+#include "cheetah_cuda.h"
+#include "common.cuh"
+#include "kv8_append.cuh"
+#include "kv8_read.cuh"
+#include "launch.cuh"
+#include "verify_drafts.cuh"
+
+using cheetah::launch_ex;
+
+static_assert(cheetah::kKv8Block == CHEETAH_CUDA_KV8_BLOCK, "cells that share a scale");
+
+namespace {
+
+bool aligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// A pool's slots, and its rows of one head, are numbered in 32 bits.
+bool pool_in_range(uint32_t num_pages, uint32_t page_tokens, uint32_t kv_heads) {
+    return num_pages > 0 && page_tokens > 0 && page_tokens % CHEETAH_CUDA_KV8_BLOCK == 0 &&
+           (uint64_t)num_pages * page_tokens * kv_heads <= 0x7FFFFFFFull;
+}
+
+// Rows among which a warp looks for blocks to append: one where there are few
+// rows, each its own block perhaps, and latency counts; sixteen where prompts
+// fill whole blocks.
+constexpr uint32_t kAppendFewRows = 2048;
+
+template <typename TIN, int HD>
+int launch_append(cheetah::Kv8AppendParams p, cudaStream_t stream) {
+    constexpr int kHeads = cheetah::kWarp / (HD / 2 / (16 / (int)sizeof(TIN)));
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    // Warps of the q rows as for qk_norm_rope (verify_ops.cu).
+    const int steps = (p.q.q_heads + kHeads - 1) / kHeads;
+    p.q.steps = (long long)p.q.tokens * steps >= 48ll * cheetah::sm_count(device) ? steps : 1;
+    p.q.row_units = (steps + p.q.steps - 1) / p.q.steps;
+    p.q_blocks = ((long long)p.q.tokens * p.q.row_units + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
+    p.group_rows = (uint32_t)p.q.tokens <= kAppendFewRows ? 1 : cheetah::kKv8MaxGroup;
+    const long long groups = ((long long)p.q.tokens + p.group_rows - 1) / p.group_rows;
+    const long long kv_blocks = (groups * 2 * p.kv_heads + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
+    CH_REQUIRE(p.q_blocks + kv_blocks <= 0x7FFFFFFFll, "cheetah_cuda_op_qk_norm_rope_kv8: too many rows");
+    auto kernel = p.q.steps == 1  ? cheetah::qk_norm_rope_kv8_kernel<TIN, HD, 1>
+                  : p.q.steps <= 3 ? cheetah::qk_norm_rope_kv8_kernel<TIN, HD, 3>
+                                   : cheetah::qk_norm_rope_kv8_kernel<TIN, HD, cheetah::kQkUnroll>;
+    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)(p.q_blocks + kv_blocks)), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream,
+                          true, p));
+    return 0;
+}
+
+template <typename TOUT, int HD>
+int launch_read(const cheetah::Kv8ReadParams &p, cudaStream_t stream) {
+    const long long per_block = cheetah::kKv8ReadThreads * cheetah::kKv8ReadLoads;
+    const long long blocks = (p.chunks + per_block - 1) / per_block;
+    CH_REQUIRE(blocks <= 0x7FFFFFFFll, "cheetah_cuda_op_kv8_read: too many rows");
+    CH_CUDA_TRY(launch_ex(cheetah::kv8_read_kernel<TOUT, HD>, dim3((unsigned)blocks), dim3(cheetah::kKv8ReadThreads), 0, stream, true, p));
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cheetah_cuda_op_qk_norm_rope_kv8(const CheetahCudaQkNormRopeKv8 *a, void *stream) {
+    CH_REQUIRE(a != nullptr && a->qkv && a->rope_cos && a->rope_sin && a->positions && a->slots && a->q_out &&
+                   a->k_codes && a->v_codes && a->k_scales && a->v_scales,
+               "cheetah_cuda_op_qk_norm_rope_kv8: null argument");
+    CH_REQUIRE(a->dtype == CHEETAH_CUDA_KV_BF16 || a->dtype == CHEETAH_CUDA_KV_F32,
+               "cheetah_cuda_op_qk_norm_rope_kv8: unknown dtype");
+    CH_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "cheetah_cuda_op_qk_norm_rope_kv8: head_dim must be 64 or 128");
+    CH_REQUIRE(a->rotary_dim > 0 && a->rotary_dim % 16 == 0 && a->rotary_dim <= a->head_dim,
+               "cheetah_cuda_op_qk_norm_rope_kv8: rotary_dim must be a multiple of 16 up to head_dim");
+    CH_REQUIRE(a->tokens > 0 && a->tokens <= 0x7FFFFFFFu && a->max_positions > 0 && a->max_positions <= 0x7FFFFFFFu,
+               "cheetah_cuda_op_qk_norm_rope_kv8: empty shape");
+    CH_REQUIRE(a->q_heads > 0 && a->kv_heads > 0 && a->q_heads <= 1024 && a->kv_heads <= 1024,
+               "cheetah_cuda_op_qk_norm_rope_kv8: head counts must be 1..1024");
+    CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens, 1),
+               "cheetah_cuda_op_qk_norm_rope_kv8: a pool holds 1 .. 2^31-1 tokens, in pages of a multiple of 16");
+    const bool bf16 = a->dtype == CHEETAH_CUDA_KV_BF16;
+    const size_t heads = (size_t)a->q_heads + 2 * (size_t)a->kv_heads;
+    CH_REQUIRE(a->qkv_stride >= heads * a->head_dim && a->qkv_stride % (bf16 ? 8 : 4) == 0 &&
+                   a->qkv_stride < ((size_t)1 << 40),
+               "cheetah_cuda_op_qk_norm_rope_kv8: qkv rows must not overlap and must be 16-byte aligned");
+    CH_REQUIRE(aligned(a->qkv, 16) && aligned(a->q_out, 16) && aligned(a->k_codes, 16) && aligned(a->v_codes, 16) &&
+                   aligned(a->rope_cos, 16) && aligned(a->rope_sin, 16) && aligned(a->q_norm, 16) && aligned(a->k_norm, 16) &&
+                   aligned(a->k_scales, 4) && aligned(a->v_scales, 4),
+               "cheetah_cuda_op_qk_norm_rope_kv8: buffers must be 16-byte aligned, the scales 4-byte");
+    cheetah::Kv8AppendParams p = {};
+    p.q.qkv = a->qkv;
+    p.q.qkv_stride = (long long)a->qkv_stride;
+    p.q.q_norm = a->q_norm;
+    p.q.k_norm = a->k_norm;
+    p.q.eps = a->eps;
+    p.q.rope_cos = a->rope_cos;
+    p.q.rope_sin = a->rope_sin;
+    p.q.max_positions = (int)a->max_positions;
+    p.q.rotary_dim = (int)a->rotary_dim;
+    p.q.positions = a->positions;
+    p.q.slots = a->slots;
+    p.q.tokens = (int)a->tokens;
+    p.q.q_heads = (int)a->q_heads;
+    p.q.kv_heads = 0;
+    p.q.q_out = a->q_out;
+    p.q.num_pages = (int)a->num_pages;
+    p.q.page_tokens = (int)a->page_tokens;
+    p.kv_heads = (int)a->kv_heads;
+    p.k_codes = static_cast<uint8_t *>(a->k_codes);
+    p.v_codes = static_cast<uint8_t *>(a->v_codes);
+    p.k_scales = a->k_scales;
+    p.v_scales = a->v_scales;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->head_dim == 64) return bf16 ? launch_append<uint16_t, 64>(p, st) : launch_append<float, 64>(p, st);
+    return bf16 ? launch_append<uint16_t, 128>(p, st) : launch_append<float, 128>(p, st);
+}
+
+int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *a, void *stream) {
+    CH_REQUIRE(a != nullptr && a->k_codes && a->v_codes && a->k_scales && a->v_scales && a->slots && a->k_out && a->v_out,
+               "cheetah_cuda_op_kv8_read: null argument");
+    CH_REQUIRE(a->dtype == CHEETAH_CUDA_KV_BF16 || a->dtype == CHEETAH_CUDA_KV_F32, "cheetah_cuda_op_kv8_read: unknown dtype");
+    CH_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "cheetah_cuda_op_kv8_read: head_dim must be 64 or 128");
+    CH_REQUIRE(a->tokens > 0 && a->tokens <= 0x7FFFFFFFu, "cheetah_cuda_op_kv8_read: empty shape");
+    CH_REQUIRE(a->kv_heads > 0 && a->kv_heads <= 1024, "cheetah_cuda_op_kv8_read: kv_heads must be 1..1024");
+    CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens, 1),
+               "cheetah_cuda_op_kv8_read: a pool holds 1 .. 2^31-1 tokens, in pages of a multiple of 16");
+    CH_REQUIRE(aligned(a->k_codes, 16) && aligned(a->v_codes, 16) && aligned(a->k_out, 16) && aligned(a->v_out, 16) &&
+                   aligned(a->k_scales, 4) && aligned(a->v_scales, 4),
+               "cheetah_cuda_op_kv8_read: buffers must be 16-byte aligned, the scales 4-byte");
+    cheetah::Kv8ReadParams p = {};
+    p.k_codes = static_cast<const uint8_t *>(a->k_codes);
+    p.v_codes = static_cast<const uint8_t *>(a->v_codes);
+    p.k_scales = a->k_scales;
+    p.v_scales = a->v_scales;
+    p.num_pages = (int)a->num_pages;
+    p.page_tokens = (int)a->page_tokens;
+    p.slots = a->slots;
+    p.chunks = (long long)a->tokens * a->kv_heads * (a->head_dim / 8);
+    p.kv_heads = (int)a->kv_heads;
+    p.k_out = a->k_out;
+    p.v_out = a->v_out;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool bf16 = a->dtype == CHEETAH_CUDA_KV_BF16;
+    if (a->head_dim == 64) return bf16 ? launch_read<uint16_t, 64>(p, st) : launch_read<float, 64>(p, st);
+    return bf16 ? launch_read<uint16_t, 128>(p, st) : launch_read<float, 128>(p, st);
+}
+
+static int check_attention_kv8(const CheetahCudaAttentionKv8 *a) {
+    CH_REQUIRE(a != nullptr, "cheetah_cuda_op_attention_kv8: null argument");
+    CH_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "cheetah_cuda_op_attention_kv8: head_dim must be 64 or 128");
+    CH_REQUIRE(a->kv_heads > 0 && a->q_heads > 0 && a->q_heads % a->kv_heads == 0 && a->q_heads / a->kv_heads <= 32 &&
+                   a->q_heads <= 1024,
+               "cheetah_cuda_op_attention_kv8: q_heads must be a multiple of kv_heads (group <= 32)");
+    CH_REQUIRE(a->batch > 0 && a->batch <= 4096, "cheetah_cuda_op_attention_kv8: batch must be 1..4096");
+    CH_REQUIRE(a->rows > 0 && a->rows <= (1u << 24), "cheetah_cuda_op_attention_kv8: rows must be 1..2^24");
+    CH_REQUIRE(pool_in_range(a->num_pages, a->page_tokens, a->kv_heads) && pool_in_range(a->max_pages_per_seq, a->page_tokens, 1),
+               "cheetah_cuda_op_attention_kv8: a pool holds 1 .. 2^31-1 rows of one head, a table row as many tokens, in "
+               "pages of a multiple of 16");
+    // The end of a key tile is counted in 31 bits too.
+    CH_REQUIRE((uint64_t)a->max_pages_per_seq * a->page_tokens <= 0x7FFFFFFFull - 128,
+               "cheetah_cuda_op_attention_kv8: a table row holds at most 2^31 - 129 tokens");
+    CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu && a->sinks <= 0x7FFFFFFFu,
+               "cheetah_cuda_op_attention_kv8: sliding_window or sinks is too large");
+    return 0;
+}
+
+int cheetah_cuda_op_attention_kv8_workspace(const CheetahCudaAttentionKv8 *a, size_t *bytes) {
+    CH_REQUIRE(bytes != nullptr, "cheetah_cuda_op_attention_kv8_workspace: null argument");
+    if (check_attention_kv8(a) != 0) return -1;
+    *bytes = 256;
+    return 0;
+}
+
+int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream) {
+    if (check_attention_kv8(a) != 0) return -1;
+    CH_REQUIRE(a->q && a->k_codes && a->v_codes && a->k_scales && a->v_scales && a->page_table && a->seq_lens &&
+                   a->row_starts && a->out && a->workspace,
+               "cheetah_cuda_op_attention_kv8: null argument");
+    CH_REQUIRE(a->q_stride >= (size_t)a->q_heads * a->head_dim && a->q_stride % 8 == 0 && a->q_stride < ((size_t)1 << 32),
+               "cheetah_cuda_op_attention_kv8: q rows must not overlap and must be 16-byte aligned");
+    CH_REQUIRE(aligned(a->q, 16) && aligned(a->k_codes, 16) && aligned(a->v_codes, 16) && aligned(a->out, 16) &&
+                   aligned(a->k_scales, 4) && aligned(a->v_scales, 4) && aligned(a->workspace, 256),
+               "cheetah_cuda_op_attention_kv8: q, out and the codes must be 16-byte aligned, the scales 4-byte, the workspace "
+               "256-byte");
+    CH_REQUIRE(a->workspace_bytes >= 256, "cheetah_cuda_op_attention_kv8: the workspace is too small");
+    cheetah::Kv8AttnParams p = {};
+    p.q = static_cast<const uint16_t *>(a->q);
+    p.q_stride = (long long)a->q_stride;
+    p.k_codes = static_cast<const uint8_t *>(a->k_codes);
+    p.v_codes = static_cast<const uint8_t *>(a->v_codes);
+    p.k_scales = a->k_scales;
+    p.v_scales = a->v_scales;
+    p.page_table = a->page_table;
+    p.max_pages = (int)a->max_pages_per_seq;
+    p.num_pages = (int)a->num_pages;
+    p.page_tokens = (int)a->page_tokens;
+    p.seq_lens = a->seq_lens;
+    p.row_starts = a->row_starts;
+    p.batch = (int)a->batch;
+    p.rows = (int)a->rows;
+    p.window = (int)a->sliding_window;
+    p.sinks = (int)a->sinks;
+    p.q_heads = (int)a->q_heads;
+    p.kv_heads = (int)a->kv_heads;
+    p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
+    p.out = static_cast<uint16_t *>(a->out);
+    auto kernel = a->head_dim == 64 ? cheetah::attention_kv8_simple_kernel<64> : cheetah::attention_kv8_simple_kernel<128>;
+    CH_CUDA_TRY(launch_ex(kernel, dim3(a->rows * a->q_heads), dim3(cheetah::kKv8SimpleWarps * cheetah::kWarp), 0,
+                          static_cast<cudaStream_t>(stream), true, p));
+    return 0;
+}
+
+int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream) {
+    CH_REQUIRE(a != nullptr && a->target_probs && a->tokens && a->row_starts && a->accept_u && a->sample_u && a->accepted &&
+                   a->out_tokens,
+               "cheetah_cuda_op_verify_drafts: null argument");
+    CH_REQUIRE(a->rows > 0 && a->rows <= 0x7FFFFFFFu && a->vocab > 0 && a->vocab <= (1u << 30),
+               "cheetah_cuda_op_verify_drafts: rows must be positive and vocab 1..2^30");
+    CH_REQUIRE(a->batch > 0 && a->batch <= 65535, "cheetah_cuda_op_verify_drafts: batch must be 1..65535");
+    CH_REQUIRE((a->target_stride >= a->vocab || a->rows == 1) && a->target_stride < ((size_t)1 << 40) &&
+                   (a->draft_probs == nullptr ||
+                    ((a->draft_stride >= a->vocab || a->rows == 1) && a->draft_stride < ((size_t)1 << 40))),
+               "cheetah_cuda_op_verify_drafts: rows must not overlap");
+    CH_REQUIRE(aligned(a->target_probs, 4) && aligned(a->draft_probs, 4),
+               "cheetah_cuda_op_verify_drafts: probabilities must be aligned to their type");
+    cheetah::VerifyDraftsParams p = {};
+    p.target = a->target_probs;
+    p.draft = a->draft_probs;
+    p.target_stride = (long long)a->target_stride;
+    p.draft_stride = (long long)a->draft_stride;
+    p.rows = (int)a->rows;
+    p.vocab = (int)a->vocab;
+    p.tokens = a->tokens;
+    p.row_starts = a->row_starts;
+    p.batch = (int)a->batch;
+    p.accept_u = a->accept_u;
+    p.sample_u = a->sample_u;
+    p.accepted = a->accepted;
+    p.out_tokens = a->out_tokens;
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    // Parts of a row: enough CTAs for two on every SM, each with two chunks at least.
+    const long long vecs = ((long long)a->vocab + 6) / 4;
+    p.parts = 1;
+    while (p.parts < cheetah::kVdMaxCluster && (long long)a->batch * p.parts * 2 <= 2ll * cheetah::sm_count(device) &&
+           vecs >= 4ll * p.parts * cheetah::kVdThreads) {
+        p.parts *= 2;
+    }
+    p.chunk_vecs = cheetah::kVdThreads;
+    while ((vecs + p.chunk_vecs - 1) / p.chunk_vecs > (long long)cheetah::kVdMaxChunks * p.parts) p.chunk_vecs *= 2;
+    auto kernel = cheetah::verify_drafts_kernel;
+    if (p.parts > 8) CH_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(a->batch * (uint32_t)p.parts));
+    config.blockDim = dim3(cheetah::kVdThreads);
+    config.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 2;
+    CH_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+    return 0;
+}
+
+}  // extern "C"

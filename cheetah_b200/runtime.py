@@ -129,6 +129,44 @@ class TokenLogprobsArgs(C.Structure):
     ]
 
 
+class QkNormRopeKv8Args(C.Structure):
+    _fields_ = [
+        ("qkv", C.c_void_p), ("qkv_stride", C.c_size_t), ("dtype", C.c_int32), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+        ("eps", C.c_float), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("max_positions", C.c_uint32),
+        ("rotary_dim", C.c_uint32), ("positions", C.c_void_p), ("slots", C.c_void_p), ("tokens", C.c_uint32),
+        ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("q_out", C.c_void_p),
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("num_pages", C.c_uint32), ("page_tokens", C.c_uint32),
+    ]
+
+
+class Kv8ReadArgs(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("num_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("slots", C.c_void_p), ("tokens", C.c_uint32),
+        ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("dtype", C.c_int32), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+    ]
+
+
+class AttentionKv8Args(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("q_stride", C.c_size_t), ("rows", C.c_uint32), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p),
+        ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("page_table", C.c_void_p), ("max_pages_per_seq", C.c_uint32),
+        ("num_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("seq_lens", C.c_void_p), ("row_starts", C.c_void_p),
+        ("batch", C.c_uint32), ("sliding_window", C.c_uint32), ("sinks", C.c_uint32), ("q_heads", C.c_uint32),
+        ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("out", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class VerifyDraftsArgs(C.Structure):
+    _fields_ = [
+        ("target_probs", C.c_void_p), ("target_stride", C.c_size_t), ("draft_probs", C.c_void_p), ("draft_stride", C.c_size_t),
+        ("rows", C.c_uint32), ("vocab", C.c_uint32), ("tokens", C.c_void_p), ("row_starts", C.c_void_p), ("batch", C.c_uint32),
+        ("accept_u", C.c_void_p), ("sample_u", C.c_void_p), ("accepted", C.c_void_p), ("out_tokens", C.c_void_p),
+    ]
+
+
 # Every symbol include/cheetah_cuda.h declares, with its ctypes signature.
 _P, _S, _I = C.c_void_p, C.c_size_t, C.c_int
 SIGNATURES = {
@@ -175,6 +213,11 @@ SIGNATURES = {
     "cheetah_cuda_op_tree_attention_workspace": (_I, [C.POINTER(TreeAttentionArgs), C.POINTER(_S)]),
     "cheetah_cuda_op_tree_attention": (_I, [C.POINTER(TreeAttentionArgs), _P]),
     "cheetah_cuda_op_token_logprobs": (_I, [C.POINTER(TokenLogprobsArgs), _P]),
+    "cheetah_cuda_op_qk_norm_rope_kv8": (_I, [C.POINTER(QkNormRopeKv8Args), _P]),
+    "cheetah_cuda_op_kv8_read": (_I, [C.POINTER(Kv8ReadArgs), _P]),
+    "cheetah_cuda_op_attention_kv8_workspace": (_I, [C.POINTER(AttentionKv8Args), C.POINTER(_S)]),
+    "cheetah_cuda_op_attention_kv8": (_I, [C.POINTER(AttentionKv8Args), _P]),
+    "cheetah_cuda_op_verify_drafts": (_I, [C.POINTER(VerifyDraftsArgs), _P]),
 }
 
 _lib: Optional[C.CDLL] = None
@@ -545,9 +588,10 @@ class _Bound:
         self.raw_stream = torch._C._cuda_getCurrentRawStream
         self.empty, self.empty_like = torch.empty, torch.empty_like
         self.i32, self.i64, self.u8 = torch.int32, torch.int64, torch.uint8
-        self.bf16, self.f32 = torch.bfloat16, torch.float32
+        self.bf16, self.f32, self.e4m3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
         handle = lib()
-        for name in ("page_slots", "qk_norm_rope", "tree_attention", "token_logprobs"):
+        for name in ("page_slots", "qk_norm_rope", "tree_attention", "token_logprobs", "qk_norm_rope_kv8", "kv8_read",
+                     "attention_kv8", "verify_drafts"):
             setattr(self, name, getattr(handle, "cheetah_cuda_op_" + name))
 
 
@@ -803,3 +847,236 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     if o.token_logprobs(args, o.raw_stream(device)):
         _check(-1)
     return TokenLogprobs(logprob, entropy, rank, ids, best)
+
+
+# ---- a cache held in 8 bits, and the test of drafted tokens ---------------
+#
+# Codes are float8_e4m3fn tensors [pages, kv_heads, page_tokens, head_dim], the
+# scales f32 [pages, kv_heads, page_tokens / 16]: one for 16 cells of a head.
+
+KV8_BLOCK = 16
+
+
+def _kv8_pool(o, op: str, device: int, k_codes, v_codes, k_scales, v_scales):
+    """The shape of an 8-bit pool, once its four tensors are found in order."""
+    shape = k_codes.shape
+    if len(shape) != 4 or shape != v_codes.shape or shape[2] % KV8_BLOCK:
+        raise CheetahCudaError(f"{op}: the codes must be [pages, kv_heads, page_tokens, head_dim] of one shape, "
+                               f"page_tokens a multiple of {KV8_BLOCK}")
+    if not (_fits(k_codes, o.e4m3, device) and _fits(v_codes, o.e4m3, device) and _fits(k_scales, o.f32, device)
+            and _fits(v_scales, o.f32, device)):
+        _refuse(op, device, k_codes=(k_codes, o.e4m3), v_codes=(v_codes, o.e4m3), k_scales=(k_scales, o.f32),
+                v_scales=(v_scales, o.f32))
+    blocks = (shape[0], shape[1], shape[2] // KV8_BLOCK)
+    if k_scales.shape != blocks or v_scales.shape != blocks:
+        raise CheetahCudaError(f"{op}: the scales must be [pages, kv_heads, page_tokens / {KV8_BLOCK}]")
+    return shape
+
+
+def qk_norm_rope_kv8(qkv, q_heads: int, kv_heads: int, positions, slots, rope_cos, rope_sin, k_codes, v_codes, k_scales,
+                     v_scales, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, stream=None):
+    """`qk_norm_rope` with K/V appended in 8 bits (`cheetah_cuda_op_qk_norm_rope_kv8`):
+    a block whose first cell is among `slots` gets a new scale, another one the
+    larger of its own and what the new cells need. The rows of one block lie
+    within 32 rows of each other. Returns q_out [T, q_heads, D]."""
+    o = _bound or _bind()
+    device = qkv.get_device()
+    i32, f32 = o.i32, o.f32
+    dtype = qkv.dtype
+    if device < 0 or (dtype is not o.bf16 and dtype is not f32):
+        raise CheetahCudaError("qk_norm_rope_kv8: qkv must be a bf16 or f32 CUDA tensor")
+    if stream is not None or device != o.current_device():
+        with _context(device, stream):
+            return qk_norm_rope_kv8(qkv, q_heads, kv_heads, positions, slots, rope_cos, rope_sin, k_codes, v_codes,
+                                    k_scales, v_scales, q_norm, k_norm, eps, q_out)
+    pages, kvh, pt, D = _kv8_pool(o, "qk_norm_rope_kv8", device, k_codes, v_codes, k_scales, v_scales)
+    T = qkv.shape[0]
+    width = (q_heads + 2 * kv_heads) * D
+    strides = qkv.stride()
+    if not (T > 0 and kvh == kv_heads and q_heads > 0 and qkv.numel() == T * width
+            and (strides[1:] == (D, 1) and qkv.shape[2] == D or len(strides) == 2 and strides[1] == 1)):
+        raise CheetahCudaError("qk_norm_rope_kv8: qkv must be [tokens, q_heads + 2 kv_heads, head_dim] with contiguous rows")
+    if not (_fits(positions, i32, device) and _fits(slots, i32, device) and _fits(rope_cos, f32, device)
+            and _fits(rope_sin, f32, device) and (q_norm is None or _fits(q_norm, f32, device))
+            and (k_norm is None or _fits(k_norm, f32, device)) and (q_out is None or _fits(q_out, dtype, device))):
+        _refuse("qk_norm_rope_kv8", device, positions=(positions, i32), slots=(slots, i32), rope_cos=(rope_cos, f32),
+                rope_sin=(rope_sin, f32), q_norm=(q_norm, f32), k_norm=(k_norm, f32), q_out=(q_out, dtype))
+    if positions.numel() != T or slots.numel() != T:
+        raise CheetahCudaError("qk_norm_rope_kv8: positions and slots must hold one entry per row")
+    table = rope_cos.shape
+    if len(table) != 2 or table != rope_sin.shape:
+        raise CheetahCudaError("qk_norm_rope_kv8: rope_cos and rope_sin must be [max_positions, rotary_dim/2]")
+    if (q_norm is not None and q_norm.numel() != D) or (k_norm is not None and k_norm.numel() != D):
+        raise CheetahCudaError("qk_norm_rope_kv8: a norm weight must be [head_dim]")
+    if q_out is None:
+        q_out = qkv.new_empty((T, q_heads, D))
+    elif q_out.numel() != T * q_heads * D:
+        raise CheetahCudaError("qk_norm_rope_kv8: q_out must be [tokens, q_heads, head_dim]")
+    args = QkNormRopeKv8Args(qkv.data_ptr(), strides[0] if T > 1 else width, KV_F32 if dtype is f32 else KV_BF16,
+                             None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                             eps, rope_cos.data_ptr(), rope_sin.data_ptr(), table[0], 2 * table[1], positions.data_ptr(),
+                             slots.data_ptr(), T, q_heads, kv_heads, D, q_out.data_ptr(), k_codes.data_ptr(),
+                             v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, pt)
+    if o.qk_norm_rope_kv8(args, o.raw_stream(device)):
+        _check(-1)
+    return q_out
+
+
+def kv8_read(k_codes, v_codes, k_scales, v_scales, slots, dtype=None, k_out=None, v_out=None, stream=None):
+    """Cells `slots` (int32 [T]) of an 8-bit cache as rows (k, v) [T, kv_heads,
+    head_dim] of `dtype`, bf16 (default) or f32 (`cheetah_cuda_op_kv8_read`).
+    Slots outside the pool give zeros."""
+    o = _bound or _bind()
+    device = k_codes.get_device()
+    if device < 0:
+        raise CheetahCudaError("kv8_read: k_codes must be a CUDA tensor")
+    if stream is not None or device != o.current_device():
+        with _context(device, stream):
+            return kv8_read(k_codes, v_codes, k_scales, v_scales, slots, dtype, k_out, v_out)
+    pages, kvh, pt, D = _kv8_pool(o, "kv8_read", device, k_codes, v_codes, k_scales, v_scales)
+    if dtype is None:
+        dtype = o.bf16 if k_out is None else k_out.dtype
+    if dtype is not o.bf16 and dtype is not o.f32:
+        raise CheetahCudaError("kv8_read: dtype must be bf16 or f32")
+    if not (_fits(slots, o.i32, device) and (k_out is None or _fits(k_out, dtype, device))
+            and (v_out is None or _fits(v_out, dtype, device))):
+        _refuse("kv8_read", device, slots=(slots, o.i32), k_out=(k_out, dtype), v_out=(v_out, dtype))
+    T = slots.numel()
+    if T < 1 or slots.dim() != 1:
+        raise CheetahCudaError("kv8_read: slots must be [tokens]")
+    if k_out is None:
+        k_out = o.empty((T, kvh, D), dtype=dtype, device=slots.device)
+    if v_out is None:
+        v_out = o.empty_like(k_out)
+    if k_out.numel() != T * kvh * D or v_out.numel() != T * kvh * D:
+        raise CheetahCudaError("kv8_read: k_out and v_out must be [tokens, kv_heads, head_dim]")
+    args = Kv8ReadArgs(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, pt,
+                       slots.data_ptr(), T, kvh, D, KV_F32 if dtype is o.f32 else KV_BF16, k_out.data_ptr(), v_out.data_ptr())
+    if o.kv8_read(args, o.raw_stream(device)):
+        _check(-1)
+    return k_out, v_out
+
+
+def attention_kv8(q, k_codes, v_codes, k_scales, v_scales, page_table, seq_lens, row_starts, sliding_window: int = 0,
+                  sinks: int = 0, out=None, workspace=None, stream=None):
+    """Causal attention of a batch's new rows over an 8-bit cache
+    (`cheetah_cuda_op_attention_kv8`). q [rows, q_heads, D] bf16 (rows may be
+    strided); page_table int32 [B, max_pages]; seq_lens int32 [B] (its rows
+    included); row_starts int32 [B + 1]. With a sliding window the first `sinks`
+    positions stay visible. Rows behind the last sequence stay as `out` holds
+    them. workspace: a uint8 tensor of `attention_kv8_workspace` bytes that no
+    overlapping call uses; None takes one from torch's allocator."""
+    o = _bound or _bind()
+    device = q.get_device()
+    i32, bf16 = o.i32, o.bf16
+    if device < 0 or q.dtype is not bf16 or q.dim() != 3:
+        raise CheetahCudaError("attention_kv8: q must be a bf16 CUDA tensor [rows, q_heads, head_dim]")
+    if stream is not None or device != o.current_device():
+        with _context(device, stream):
+            return attention_kv8(q, k_codes, v_codes, k_scales, v_scales, page_table, seq_lens, row_starts, sliding_window,
+                                 sinks, out, workspace)
+    rows, qh, D = q.shape
+    strides = q.stride()
+    if rows < 1 or strides[1:] != (D, 1):
+        raise CheetahCudaError("attention_kv8: q must have contiguous rows")
+    shape = _kv8_pool(o, "attention_kv8", device, k_codes, v_codes, k_scales, v_scales)
+    if shape[3] != D:
+        raise CheetahCudaError("attention_kv8: the pool must have q's head_dim")
+    if not (_fits(page_table, i32, device) and _fits(seq_lens, i32, device) and _fits(row_starts, i32, device)
+            and (out is None or _fits(out, bf16, device)) and (workspace is None or _fits(workspace, o.u8, device))):
+        _refuse("attention_kv8", device, page_table=(page_table, i32), seq_lens=(seq_lens, i32), row_starts=(row_starts, i32),
+                out=(out, bf16), workspace=(workspace, o.u8))
+    B = seq_lens.numel()
+    table = page_table.shape
+    if len(table) != 2 or table[0] != B or row_starts.numel() != B + 1:
+        raise CheetahCudaError("attention_kv8: page_table must be [batch, max_pages] and row_starts [batch + 1]")
+    if not (0 <= sliding_window < 2 ** 31 and 0 <= sinks < 2 ** 31):
+        raise CheetahCudaError("attention_kv8: sliding_window and sinks must be 0 .. 2^31-1")
+    if out is None:
+        out = o.empty_like(q) if strides[0] == qh * D else q.new_empty((rows, qh, D))
+    elif out.shape != q.shape:
+        raise CheetahCudaError("attention_kv8: out must have q's shape")
+    if workspace is None:
+        workspace = o.empty(attention_kv8_workspace(D, device), dtype=o.u8, device=q.device)
+    args = AttentionKv8Args(q.data_ptr(), strides[0] if rows > 1 else qh * D, rows, k_codes.data_ptr(), v_codes.data_ptr(),
+                            k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), table[1], shape[0], shape[2],
+                            seq_lens.data_ptr(), row_starts.data_ptr(), B, sliding_window, sinks, qh, shape[1], D,
+                            out.data_ptr(), workspace.data_ptr(), workspace.numel())
+    if o.attention_kv8(args, o.raw_stream(device)):
+        _check(-1)
+    return out
+
+
+_kv8_workspace_bytes: dict = {}  # (device, head_dim) -> bytes, a property of the GPU
+
+
+def attention_kv8_workspace(head_dim: int, device: Optional[int] = None) -> int:
+    """Bytes of an `attention_kv8` workspace on `device` (default: the current one)."""
+    if device is None:
+        device = (_bound or _bind()).current_device()
+    size = _kv8_workspace_bytes.get((device, head_dim))
+    if size is None:
+        # Every field but head_dim is the least that passes the checks.
+        args = AttentionKv8Args(rows=1, max_pages_per_seq=1, num_pages=1, page_tokens=KV8_BLOCK, batch=1, q_heads=1,
+                                kv_heads=1, head_dim=head_dim)
+        n = C.c_size_t(0)
+        with _context(device, None):
+            _check(lib().cheetah_cuda_op_attention_kv8_workspace(C.byref(args), C.byref(n)))
+        size = _kv8_workspace_bytes[(device, head_dim)] = n.value
+    return size
+
+
+class DraftVerdict(NamedTuple):
+    accepted: object  # int32 [batch]: drafts kept; -1 for a sequence without rows
+    tokens: object    # int32 [rows]: a sequence's kept drafts, its next token, then -1
+
+
+def verify_drafts(target_probs, draft_probs, tokens, row_starts, accept_u, sample_u, out_tokens=None,
+                  stream=None) -> DraftVerdict:
+    """Which drafted tokens the target keeps and the token that follows them
+    (`cheetah_cuda_op_verify_drafts`). target_probs f32 [rows, vocab] and
+    draft_probs the same or None (certain drafts), rows may be strided: row r's
+    is the distribution of the token behind tokens[r] (int32 [rows], a
+    sequence's last token and its drafts); row_starts int32 [B + 1]; accept_u
+    f32 [rows] and sample_u f32 [B], uniform in [0, 1). Rows behind the last
+    sequence stay as `out_tokens` holds them."""
+    o = _bound or _bind()
+    device = target_probs.get_device()
+    f32, i32 = o.f32, o.i32
+    if device < 0 or target_probs.dtype is not f32 or target_probs.dim() != 2:
+        raise CheetahCudaError("verify_drafts: target_probs must be an f32 CUDA tensor [rows, vocab]")
+    if stream is not None or device != o.current_device():
+        with _context(device, stream):
+            return verify_drafts(target_probs, draft_probs, tokens, row_starts, accept_u, sample_u, out_tokens)
+    rows, vocab = target_probs.shape
+    strides = target_probs.stride()
+    if rows < 1 or vocab < 1 or (strides[1] != 1 and vocab > 1):
+        raise CheetahCudaError("verify_drafts: target_probs must have contiguous rows")
+    draft_stride = 0
+    if draft_probs is not None:
+        if draft_probs.dtype is not f32 or draft_probs.get_device() != device or draft_probs.shape != target_probs.shape:
+            raise CheetahCudaError("verify_drafts: draft_probs must be f32 [rows, vocab] on the target's device")
+        draft_strides = draft_probs.stride()
+        if draft_strides[1] != 1 and vocab > 1:
+            raise CheetahCudaError("verify_drafts: draft_probs must have contiguous rows")
+        draft_stride = draft_strides[0] if rows > 1 else vocab
+    if not (_fits(tokens, i32, device) and _fits(row_starts, i32, device) and _fits(accept_u, f32, device)
+            and _fits(sample_u, f32, device) and (out_tokens is None or _fits(out_tokens, i32, device))):
+        _refuse("verify_drafts", device, tokens=(tokens, i32), row_starts=(row_starts, i32), accept_u=(accept_u, f32),
+                sample_u=(sample_u, f32), out_tokens=(out_tokens, i32))
+    B = sample_u.numel()
+    if tokens.numel() != rows or accept_u.numel() != rows or row_starts.numel() != B + 1:
+        raise CheetahCudaError("verify_drafts: tokens and accept_u must hold one entry per row, sample_u one per sequence, "
+                               "row_starts one more")
+    if out_tokens is None:
+        out_tokens = o.empty_like(tokens)
+    elif out_tokens.numel() != rows:
+        raise CheetahCudaError("verify_drafts: out_tokens must be [rows]")
+    accepted = o.empty_like(sample_u, dtype=i32)
+    args = VerifyDraftsArgs(target_probs.data_ptr(), strides[0] if rows > 1 else vocab,
+                            None if draft_probs is None else draft_probs.data_ptr(), draft_stride, rows, vocab,
+                            tokens.data_ptr(), row_starts.data_ptr(), B, accept_u.data_ptr(), sample_u.data_ptr(),
+                            accepted.data_ptr(), out_tokens.data_ptr())
+    if o.verify_drafts(args, o.raw_stream(device)):
+        _check(-1)
+    return DraftVerdict(accepted, out_tokens)

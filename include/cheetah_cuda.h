@@ -488,6 +488,157 @@ typedef struct CheetahCudaTokenLogprobs {
 } CheetahCudaTokenLogprobs;
 CHEETAH_CUDA_API int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogprobs *args, void *stream);
 
+/* ---- A key/value cache held in 8 bits, and the test of drafted tokens ----
+ *
+ * The entries below run a serving step over a paged cache of half the bytes:
+ * codes are e4m3 (4 exponent bits, 3 of mantissa, no infinity) in the layout of
+ * the 16-bit pools, and the CHEETAH_CUDA_KV8_BLOCK cells of a block (an aligned
+ * run within a page) share one f32 scale per KV head, K and V apart: the value
+ * of a cell is code * scale. Rows, sequences and slots are those of
+ * cheetah_cuda_op_page_slots. All are asynchronous on `stream` (a stream of
+ * the current device), allocate nothing, keep nothing between calls and may be
+ * captured into a graph. No counterpart in the reference (its cache is f32). */
+#define CHEETAH_CUDA_KV8_BLOCK 16
+
+/* cheetah_cuda_op_qk_norm_rope with an append in 8 bits. A block's cells are
+ * filled from its first one on: where a call names the block's first cell its
+ * scale is set anew, else it becomes the larger of the one it has and what the
+ * new cells need, and the cells ahead of the first new one keep their values,
+ * rounded again where the scale grew; other cells keep their codes. What cells
+ * need is the smallest power of two, at least 2^-64, whose 448-fold reaches
+ * their largest finite magnitude. Codes are the nearest e4m3 values (ties to
+ * even) of exact quotients, k itself computed in 64 bits; a NaN or an infinity
+ * becomes the NaN code. The slots of one call must be distinct and the rows of
+ * one block within 32 rows of each other (as page_slots numbers them); cells of
+ * a block that breaks this have undefined values. Rows whose position or slot
+ * is out of range are treated as there. */
+typedef struct CheetahCudaQkNormRopeKv8 {
+    const void *qkv;           /* [tokens][q_heads + 2*kv_heads][head_dim]: q, k, v heads of a row */
+    size_t qkv_stride;         /* elements between rows */
+    int32_t dtype;             /* of qkv and q_out: CHEETAH_CUDA_KV_BF16 or _F32 */
+    const float *q_norm;       /* [head_dim] or NULL: q is not normalised */
+    const float *k_norm;       /* [head_dim] or NULL */
+    float eps;
+    const float *rope_cos;     /* [max_positions][rotary_dim/2] */
+    const float *rope_sin;
+    uint32_t max_positions;
+    uint32_t rotary_dim;       /* a multiple of 16, at most head_dim; later dimensions pass through */
+    const int32_t *positions;  /* [tokens] */
+    const int32_t *slots;      /* [tokens] */
+    uint32_t tokens;
+    uint32_t q_heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;         /* 64 or 128 */
+    void *q_out;               /* [tokens][q_heads][head_dim] */
+    void *k_codes;             /* e4m3 [num_pages][kv_heads][page_tokens][head_dim] */
+    void *v_codes;
+    float *k_scales;           /* [num_pages][kv_heads][page_tokens/16] */
+    float *v_scales;
+    uint32_t num_pages;
+    uint32_t page_tokens;      /* a multiple of 16 */
+} CheetahCudaQkNormRopeKv8;
+CHEETAH_CUDA_API int cheetah_cuda_op_qk_norm_rope_kv8(const CheetahCudaQkNormRopeKv8 *args, void *stream);
+
+/* Cells of an 8-bit cache, by slot, as bf16 or f32 rows (one rounding of code *
+ * scale). A slot outside the pool gives zeros. */
+typedef struct CheetahCudaKv8Read {
+    const void *k_codes;       /* e4m3 [num_pages][kv_heads][page_tokens][head_dim] */
+    const void *v_codes;
+    const float *k_scales;     /* [num_pages][kv_heads][page_tokens/16] */
+    const float *v_scales;
+    uint32_t num_pages;
+    uint32_t page_tokens;      /* a multiple of 16 */
+    const int32_t *slots;      /* [tokens]; repeated ones are allowed */
+    uint32_t tokens;
+    uint32_t kv_heads;
+    uint32_t head_dim;         /* 64 or 128 */
+    int32_t dtype;             /* of the outputs: CHEETAH_CUDA_KV_BF16 or _F32 */
+    void *k_out;               /* [tokens][kv_heads][head_dim] */
+    void *v_out;
+} CheetahCudaKv8Read;
+CHEETAH_CUDA_API int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *args, void *stream);
+
+/* Causal attention of a batch's new rows over an 8-bit cache. Sequence b has n
+ * = row_starts[b+1] - row_starts[b] rows (one for a decode step, several for
+ * drafted tokens, many for a prompt chunk) and seq_lens[b] cached positions,
+ * the last n of which are its rows' own K/V. The row at position i sees the
+ * positions j <= i; with a sliding window only those above i - sliding_window
+ * and the first `sinks` ones. Positions on a page outside the pool count as
+ * unseen, and a row that sees nothing gives zeros. Cells that a row does not
+ * see never reach it, NaN codes and scales of blocks that hold none of its
+ * positions included. Rows from row_starts[batch] on stay as they were; a
+ * sequence with seq_lens[b] < n gives zeros. Scales must be positive where a
+ * row sees the block. Sums and statistics are f32; the softmax weights, times
+ * V's scale, enter the products as two e4m3 parts (about 8 bits, as bf16
+ * holds, down to 2^-17 of a row's largest such product). If a wait inside the
+ * kernel gives up, every row is NaN.
+ *
+ * `workspace` holds partial results between the launches of a call:
+ * cheetah_cuda_op_attention_kv8_workspace says how many bytes (256-byte
+ * aligned; the contents need no initialisation and are garbage afterwards).
+ * Calls that may overlap on the GPU, graphs included, each need their own. */
+typedef struct CheetahCudaAttentionKv8 {
+    const void *q;             /* bf16 [rows][q_heads][head_dim], RoPE applied */
+    size_t q_stride;           /* elements between rows, a multiple of 8 */
+    uint32_t rows;             /* rows of q and out: at least row_starts[batch] */
+    const void *k_codes;       /* e4m3 [num_pages][kv_heads][page_tokens][head_dim] */
+    const void *v_codes;
+    const float *k_scales;     /* [num_pages][kv_heads][page_tokens/16] */
+    const float *v_scales;
+    const int32_t *page_table; /* [batch][max_pages_per_seq] */
+    uint32_t max_pages_per_seq; /* times page_tokens: at most 2^31 - 129 */
+    uint32_t num_pages;
+    uint32_t page_tokens;      /* a multiple of 16 */
+    const int32_t *seq_lens;   /* [batch] */
+    const int32_t *row_starts; /* [batch+1], ascending from 0 */
+    uint32_t batch;            /* 1..4096 */
+    uint32_t sliding_window;   /* 0 = full */
+    uint32_t sinks;            /* first positions that a window leaves visible */
+    uint32_t q_heads;
+    uint32_t kv_heads;         /* q_heads / kv_heads: 1..32 */
+    uint32_t head_dim;         /* 64 or 128 */
+    void *out;                 /* bf16 [rows][q_heads][head_dim] */
+    void *workspace;
+    size_t workspace_bytes;
+} CheetahCudaAttentionKv8;
+CHEETAH_CUDA_API int cheetah_cuda_op_attention_kv8_workspace(const CheetahCudaAttentionKv8 *args, size_t *bytes);
+CHEETAH_CUDA_API int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *args, void *stream);
+
+/* Which drafted tokens a target model keeps, and the token that follows them,
+ * from given random numbers, so that the tokens are distributed as the
+ * target's own. The rows of sequence b are its step's input tokens: the last
+ * one that it had, then its drafts. Row r's distributions are of the token of
+ * row r + 1: with p = target_probs[r], q = draft_probs[r] and x = tokens[r+1]
+ * the draft is kept while accept_u[r] * q(x) < p(x) (an exact comparison). At
+ * the first that is not, the next token is drawn from the positive part of p -
+ * q (from p where that is zero throughout); behind the last draft from the last
+ * row's p. Drawn: the first token at which the running sum of the weights, in
+ * 64 bits, passes sample_u[b] times their sum, or else the last one of positive
+ * weight. Without draft_probs a draft is certain: q(x) = 1. NaN and negative
+ * probabilities count as 0, a draft outside the vocabulary is not kept (it
+ * counts as drawn from q with p(x) = 0). A row whose weights sum to 0 or to no
+ * finite number gives token -1.
+ *
+ * out_tokens holds, for each row of a sequence, its kept drafts, the next
+ * token, then -1; rows from row_starts[batch] on stay as they were. accepted
+ * is the number of drafts kept, -1 for a sequence without rows. */
+typedef struct CheetahCudaVerifyDrafts {
+    const float *target_probs; /* [rows][vocab] */
+    size_t target_stride;      /* elements between rows */
+    const float *draft_probs;  /* [rows][vocab] or NULL; a sequence's last row is not read */
+    size_t draft_stride;
+    uint32_t rows;
+    uint32_t vocab;            /* 1..2^30 */
+    const int32_t *tokens;     /* [rows] the step's input tokens */
+    const int32_t *row_starts; /* [batch+1], ascending from 0 */
+    uint32_t batch;            /* 1..65535 */
+    const float *accept_u;     /* [rows] in [0, 1) */
+    const float *sample_u;     /* [batch] in [0, 1) */
+    int32_t *accepted;         /* [batch] */
+    int32_t *out_tokens;       /* [rows] */
+} CheetahCudaVerifyDrafts;
+CHEETAH_CUDA_API int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
