@@ -1,16 +1,63 @@
-// Causal attention of a batch's new rows over an 8-bit paged cache.
+// Causal attention of a batch's new rows over an 8-bit paged cache: what its
+// kernels share.
 //
 //   o_i = sum_j softmax_j(q_i . k_j / sqrt(D)) v_j,   k_j = kc_j ks,  v_j = vc_j vs
 //
-// with e4m3 codes and one scale per 16 cells and head.
+// with e4m3 codes and one scale per 16 cells and head, in one pass over the keys
+// with a running reference m and sum (log2 units, t_j = log2(e)/sqrt(D) q . k_j):
+//   l = sum_j 2^(t_j - m),   o' = sum_j (2^(t_j - m) vs) vc_j,   o = o' / l.
 //
-// A warp takes every fourth key of one row and head.
+// The codes are multiplied as they are (tcgen05 kind::f8f6f4). What meets them
+// is split into e4m3 parts that are multiplied one after the other: q, over a
+// power of two of its row, into two (exact for elements within 2^-10 of the
+// row's largest, else off by 2^-18 of that), the weights times V's scale into
+// two as well (2^-8, as bf16 holds, down to the smallest step of e4m3). K's scale
+// joins the factor of the scores. m follows t_j + log2(vs), so the weights fill
+// e4m3's range however V's scales differ.
+//
+// Work. An item is a run of rows of one (sequence, KV head): nodes (new tokens)
+// times the query heads of the group, so K and V are read once for all of them.
+// Its key tiles (128 keys) are those of the first `sinks` positions and from the
+// window's begin to its last row's position. The tiles of all items lie on one
+// axis that is cut into equal shares, one per CTA, one CTA per SM: ragged
+// batches and a single long sequence fill the GPU alike. An item cut by a share's
+// end leaves partial (o, m, l) in the workspace, and the merge joins them,
+// always in the same order.
+//
+// Cells that a row must not see never reach it: their weights are 0, and a V cell
+// that holds no position, or a NaN that some row does not see, is zeroed in shared
+// memory first, where 0 times NaN would not stay 0; the rows that do see it are
+// made NaN at the end (kv8_patch).
+//
+// All mbarrier waits are bounded: on a timeout the CTA waits (bounded) for its
+// own copies and MMAs in flight, frees its TMEM and exits, and the merge makes
+// every row NaN.
 #pragma once
+
+#include <limits.h>
 
 #include "common.cuh"
 #include "kv8.cuh"
+#include "pair.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
 
 namespace cheetah {
+
+constexpr int kKv8Keys = 128;     // keys per tile
+constexpr int kKv8MaxCtas = 256;  // CTAs of a launch that a merge can list
+constexpr int kKv8Queue = 4;      // segments the scheduler may be ahead
+// Weights are scaled to at most 2^kKv8TopLog2 when a row's reference is set, and
+// it moves when one would pass 2^kKv8RoomLog2 times that (e4m3 ends at 448).
+constexpr float kKv8TopLog2 = 7.0f, kKv8RoomLog2 = 1.75f;
+
+// What a split item needs to be joined, written by the CTA that begins it.
+struct Kv8Split {
+    int row0, nodes, kvh;
+    int first_slot;  // of the beginning; the other parts are slot 0 of the next CTAs
+    int parts;       // 0: nothing to join; -1: the CTA gave up
+    int pad[3];
+};
 
 struct Kv8AttnParams {
     const uint16_t *q;
@@ -18,81 +65,398 @@ struct Kv8AttnParams {
     const uint8_t *k_codes, *v_codes;
     const float *k_scales, *v_scales;
     const int32_t *page_table;
-    int max_pages, num_pages, page_tokens;
+    int max_pages, num_pages, page_tokens, box_keys;
     const int32_t *seq_lens, *row_starts;
     int batch, rows, window, sinks;
-    int q_heads, kv_heads;
+    int q_heads, kv_heads, group;
+    int item_nodes;    // new tokens of an item at most
     float scale_log2;
     uint16_t *out;
+    Kv8Split *splits;  // [CTAs]
+    float *part_o;     // [CTAs][2][rows of an item][HD] unnormalised
+    float2 *part_ml;   // [CTAs][2][rows of an item]
 };
 
-constexpr int kKv8SimpleWarps = 4;
+// A run of tiles [t0, t1) of one item.
+struct Kv8Segment {
+    int row0, nodes;    // the item's rows of q
+    int pos0;           // position of the first
+    int len;            // cached positions within the table
+    int b, kvh;
+    int t0, t1;
+    int sink_tiles, skip;  // tile t >= sink_tiles covers the keys of tile t + skip
+    int low;            // the first key that its first row sees in the window
+    int jobs;           // tiles (0: rows to be zeroed; -1: no more segments)
+    int slot;           // workspace slot of a part; -1: the segment is its whole item
+    __device__ __forceinline__ int key0(int t) const { return (t < sink_tiles ? t : t + skip) * kKv8Keys; }
+};
 
+struct Kv8Seq {
+    int row0, n, ctx, len, items;
+};
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnParams &p, int b) {
+    Kv8Seq s;
+    const int r0 = p.row_starts[b], r1 = p.row_starts[b + 1], len = p.seq_lens[b];
+    s.row0 = min(max(r0, 0), p.rows);
+    s.n = max(min(r1, p.rows) - s.row0, 0);
+    s.ctx = len - s.n;
+    s.len = (int)min((long long)len, (long long)p.max_pages * p.page_tokens);
+    s.items = (s.n + p.item_nodes - 1) / p.item_nodes;
+    return s;
+}
+// Tiles of item j of a sequence.
+struct Kv8Range {
+    int tiles, sink_tiles, skip, low;
+};
+__device__ __forceinline__ Kv8Range kv8_range(const Kv8AttnParams &p, const Kv8Seq &s, int j) {
+    Kv8Range r = {1, 0, 0, 0};
+    if (s.ctx < 0) return r;  // without room for its rows: one tile that writes zeros
+    const int node0 = j * p.item_nodes, nodes = min(s.n - node0, p.item_nodes);
+    r.low = p.window > 0 ? max(0, s.ctx + node0 - p.window + 1) : 0;
+    const int lo = r.low / kKv8Keys, hi = (min(s.ctx + node0 + nodes, s.len) + kKv8Keys - 1) / kKv8Keys;
+    r.sink_tiles = min((p.sinks + (kKv8Keys - 1LL)) / kKv8Keys, (long long)lo);
+    r.skip = lo - r.sink_tiles;
+    r.tiles = max(1, r.sink_tiles + max(hi - lo, 0));
+    return r;
+}
+// Cost units of one KV head of a sequence: its items' tiles, and ITEM for each
+// item's beginning and end.
+template <int ITEM>
+__device__ __forceinline__ int kv8_head_units(const Kv8AttnParams &p, const Kv8Seq &s) {
+    int units = 0;
+    for (int j = 0; j < s.items; ++j) units += ITEM + kv8_range(p, s, j).tiles;
+    return units;
+}
+
+// The share of this CTA, segment by segment. Called by a whole warp, whose lanes
+// then hold the same state.
+template <int ITEM, int MIN_SHARE>
+struct Kv8Walk {
+    int b, j, kvh, left, unit, at, share, count;
+    Kv8Seq s;
+    Kv8Split split;
+
+    __device__ __forceinline__ void init(const Kv8AttnParams &p) {
+        const int lane = threadIdx.x % kWarp;
+        int total = 0, mine = 0;
+        for (int i = lane; i < p.batch; i += kWarp) {
+            const int units = kv8_head_units<ITEM>(p, kv8_seq(p, i)) * p.kv_heads;
+            if (i == lane) mine = units;
+            total += units;
+        }
+        total = __reduce_add_sync(0xFFFFFFFFu, total);
+        share = max(MIN_SHARE, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+        const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
+        int start = -1, before = 0;
+        at = 0;
+        for (int b0 = 0; b0 < p.batch && start < 0 && u0 < total; b0 += kWarp) {
+            const int i = b0 + lane;
+            const int units = b0 == 0 ? mine : (i < p.batch ? kv8_head_units<ITEM>(p, kv8_seq(p, i)) * p.kv_heads : 0);
+            int end = units;
+#pragma unroll
+            for (int o = 1; o < kWarp; o <<= 1) {
+                const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
+                if (lane >= o) end += up;
+            }
+            end += before;
+            const uint32_t here = __ballot_sync(0xFFFFFFFFu, end - units <= u0 && u0 < end);
+            if (here) {
+                start = b0 + __ffs(here) - 1;
+                at = u0 - __shfl_sync(0xFFFFFFFFu, end - units, __ffs(here) - 1);
+            }
+            before = __shfl_sync(0xFFFFFFFFu, end, kWarp - 1);
+        }
+        b = start;
+        left = min(share, total - u0);
+        unit = u0;
+        j = kvh = count = 0;
+        split = Kv8Split{};
+        if (left > 0) {
+            s = kv8_seq(p, b);
+            const int head = kv8_head_units<ITEM>(p, s);
+            kvh = at / head;
+            at -= kvh * head;
+            while (true) {
+                const int units = ITEM + kv8_range(p, s, j).tiles;
+                if (at < units) break;
+                at -= units;
+                ++j;
+            }
+        }
+    }
+    __device__ __forceinline__ Kv8Segment next(const Kv8AttnParams &p) {
+        Kv8Segment g = {};
+        g.jobs = -1;
+        while (left > 0) {
+            const Kv8Range r = kv8_range(p, s, j);
+            const int units = ITEM + r.tiles;
+            const int take = min(left, units - at);
+            // Tiles of this piece; an item's first ITEM units hold none.
+            const int t0 = max(at - ITEM, 0), t1 = max(at + take - ITEM, 0);
+            if (t1 > t0) {
+                const bool whole = t1 - t0 == r.tiles;
+                const int node0 = j * p.item_nodes;
+                g.row0 = s.row0 + node0;
+                g.nodes = min(s.n - node0, p.item_nodes);
+                g.pos0 = s.ctx + node0;
+                g.len = s.len;
+                g.b = b;
+                g.kvh = kvh;
+                g.t0 = t0;
+                g.t1 = t1;
+                g.sink_tiles = r.sink_tiles;
+                g.skip = r.skip;
+                g.low = r.low;
+                g.jobs = s.ctx < 0 ? 0 : t1 - t0;
+                g.slot = whole ? -1 : (count == 0 ? 0 : 1);
+                if (t0 == 0 && !whole) {
+                    split.row0 = g.row0;
+                    split.nodes = g.nodes;
+                    split.kvh = kvh;
+                    split.first_slot = g.slot;
+                    // Within the grid even if sequences share rows, which the units do not count on.
+                    split.parts = min((unit - at + units - 1) / share - (int)blockIdx.x + 1, (int)(gridDim.x - blockIdx.x));
+                }
+                ++count;
+            }
+            unit += take;
+            left -= take;
+            at += take;
+            if (at == units) {
+                at = 0;
+                if (++j == s.items) {
+                    j = 0;
+                    ++kvh;
+                }
+                while (left > 0 && kvh >= (s.items > 0 ? p.kv_heads : 0)) {  // the next sequence with rows
+                    if (++b >= p.batch) {
+                        left = 0;
+                        break;
+                    }
+                    s = kv8_seq(p, b);
+                    kvh = 0;
+                }
+            }
+            if (t1 > t0) break;
+        }
+        return g;
+    }
+};
+
+__device__ __forceinline__ uint32_t kv8_low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+
+// The pool rows of a segment's boxes (runs of box_keys keys on one page), 32 of
+// them at a time, one per lane; -1: not loaded. A tile's boxes never straddle
+// the 32 (a multiple of 1, 2, 4 and 8).
+struct Kv8Boxes {
+    int first, row;
+    uint32_t loaded;
+    __device__ __forceinline__ void init() {
+        first = INT_MIN;
+        row = -1;
+        loaded = 0;
+    }
+    __device__ __forceinline__ void reach(const Kv8AttnParams &p, const Kv8Segment &g, int box0) {
+        if (first != INT_MIN && box0 >= first && box0 < first + kWarp) return;
+        first = box0;
+        row = -1;
+        const long long pos = (long long)(box0 + (int)(threadIdx.x % kWarp)) * p.box_keys;
+        if (pos < min(g.len, g.pos0 + g.nodes) && (pos + p.box_keys > g.low || pos < p.sinks)) {
+            const int col = (int)pos / p.page_tokens;
+            const int page = p.page_table[(long long)g.b * p.max_pages + col];
+            if (page >= 0 && page < p.num_pages) row = (page * p.kv_heads + g.kvh) * p.page_tokens + ((int)pos - col * p.page_tokens);
+        }
+        loaded = __ballot_sync(0xFFFFFFFFu, row >= 0);
+    }
+};
+
+// 16 bf16 elements of q (cell `c` of a row that `cells` neighbouring lanes hold)
+// as two e4m3 parts of x / scale in rows `row` and `row_lo` of K-major tiles; the
+// scale is a power of two of the row's largest element. All lanes of a warp call.
 template <int HD>
-__global__ void __launch_bounds__(kKv8SimpleWarps *kWarp) attention_kv8_simple_kernel(const Kv8AttnParams p) {
-    constexpr int V = HD / kWarp;
-    __shared__ float part_s[kKv8SimpleWarps][HD + 2];
+__device__ __forceinline__ float kv8_split_q(const uint4 (&raw)[2], uint8_t *tile, uint8_t *tile_lo, int row, int row_lo, int c) {
+    constexpr int kCells = HD / 16;
+    float x[16];
+    const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[2 * i] = bf16_lo(w[i]);
+        x[2 * i + 1] = bf16_hi(w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (fabsf(x[i]) < INFINITY) top = fmaxf(top, fabsf(x[i]));
+        else x[i] = NAN;  // an infinity has no code
+    }
+#pragma unroll
+    for (int o = kCells / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float scale = kv8_scale_for(__float_as_uint(top)), inv = 1.0f / scale;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float v[4], h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = x[4 * i + k] * inv;
+        hi[i] = pack_e4m3x4(v[0], v[1], v[2], v[3]);
+        unpack_e4m3x4(hi[i], h);
+        lo[i] = pack_e4m3x4(v[0] - h[0], v[1] - h[1], v[2] - h[2], v[3] - h[3]);
+    }
+    *reinterpret_cast<uint4 *>(tile + e4m3_tile_offset<HD>(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(tile_lo + e4m3_tile_offset<HD>(row_lo, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    return scale;
+}
+
+// cp.async of one f32, and an arrival on an mbarrier once the lane's copies so
+// far have landed (counted among its arrivals).
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Whether a word holds a NaN code.
+__device__ __forceinline__ uint32_t e4m3_nan_bits(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// One V row of a tile in shared memory: zero where it holds no position, else
+// its NaN codes zeroed and noted for kv8_patch.
+template <int HD>
+__device__ __forceinline__ void kv8_clean_v(uint8_t *v_row, bool holds, int *non_finite) {
+    constexpr int kCells = HD / 16;
+    // Each lane begins at another cell: the rows lie 64 or 128 bytes apart.
+    auto cell = [&](int c) -> uint4 & { return *reinterpret_cast<uint4 *>(v_row + ((c + threadIdx.x) % kCells) * 16); };
+    if (!holds) {
+#pragma unroll
+        for (int c = 0; c < kCells; ++c) cell(c) = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int c = 0; c < kCells; ++c) {
+            const uint4 v = cell(c);
+            bad |= e4m3_nan_bits(v.x) | e4m3_nan_bits(v.y) | e4m3_nan_bits(v.z) | e4m3_nan_bits(v.w);
+        }
+        if (!bad) return;
+        *reinterpret_cast<volatile int *>(non_finite) = 1;
+        __threadfence_block();  // flag before the zeros that hide it from other warps
+#pragma unroll 1
+        for (int c = 0; c < kCells; ++c) {
+            const uint4 v = cell(c);
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[x] &= ~((e4m3_nan_bits(w[x]) >> 7) * 0xFFu);
+            cell(c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Whether a row at `pos` sees key j (pages aside).
+__device__ __forceinline__ bool kv8_sees(const Kv8AttnParams &p, int pos, int j) {
+    return j <= pos && (p.window == 0 || j > (long long)pos - p.window || j < p.sinks);
+}
+
+// Whether dimension d of a V row that the row at `pos` sees, and that kv8_clean_v
+// may have changed, is NaN: keys of the segment's tiles that one of its rows sees
+// and another does not, those of its own positions and of the window's edge.
+__device__ __noinline__ bool kv8_patch(const Kv8AttnParams &p, const Kv8Segment &g, int head_dim, int pos, int d) {
+    const int last = g.pos0 + g.nodes - 1;
+    for (int part = p.window > 0 ? 0 : 1; part < 2; ++part) {
+        const int begin = part == 0 ? max(g.low, p.sinks) : g.pos0 + 1;
+        const int end = part == 0 ? min(g.pos0, last - p.window) : last;  // the last of them
+        for (int j = begin; j <= min(end, g.len - 1); ++j) {
+            const int tile = j / kKv8Keys, t = tile < g.sink_tiles ? tile : tile - g.skip;
+            if (t < g.t0 || t >= g.t1 || !kv8_sees(p, pos, j)) continue;
+            const int page = p.page_table[(long long)g.b * p.max_pages + j / p.page_tokens];
+            if (page < 0 || page >= p.num_pages) continue;
+            const long long cell = ((long long)page * p.kv_heads + g.kvh) * p.page_tokens + j % p.page_tokens;
+            if ((p.v_codes[cell * head_dim + d] & 0x7F) == 0x7F) return true;
+        }
+    }
+    return false;
+}
+
+// Joins the parts of the items that shares cut: o = sum_k 2^(m_k - m) o_k / sum_k
+// 2^(m_k - m) l_k, in a fixed order. A block per kKv8MergeRows rows of one split
+// item; its warps take every eighth part and join through shared memory.
+constexpr int kKv8MergeThreads = 256, kKv8MergeRows = 4;
+
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(kKv8MergeThreads) kv8_merge_kernel(const Kv8AttnParams p, int ctas) {
+    constexpr int kWarps = kKv8MergeThreads / kWarp, V = HD / kWarp;
+    static_assert(kKv8MaxCtas <= kKv8MergeThreads, "a thread per listed CTA");
+    __shared__ float o_s[kWarps][kKv8MergeRows][HD];
+    __shared__ float2 ml_s[kWarps][kKv8MergeRows];
     const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-    const int row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads;
     pdl_wait();
     pdl_launch_dependents();
-    if (row >= p.row_starts[p.batch]) return;
-    int b = 0, hi = p.batch - 1;
-    while (b < hi) {
-        const int mid = (b + hi) / 2;
-        if (p.row_starts[mid + 1] > row) hi = mid;
-        else b = mid + 1;
+    const Kv8Split s = p.splits[blockIdx.x];
+    const bool gave_up = (int)threadIdx.x < ctas && p.splits[threadIdx.x].parts < 0;
+    if (__syncthreads_or(gave_up)) {
+        const long long cells = (long long)min(max(p.row_starts[p.batch], 0), p.rows) * p.q_heads * HD;
+        const long long step = (long long)gridDim.x * gridDim.y * kKv8MergeThreads;
+        for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kKv8MergeThreads + threadIdx.x; i < cells; i += step) p.out[i] = 0x7FC0u;
+        return;
     }
-    const int n = p.row_starts[b + 1] - p.row_starts[b], len = p.seq_lens[b];
-    const int pos = len - n + row - p.row_starts[b];
-    const int kvh = head / (p.q_heads / p.kv_heads);
-    float q[V], o[V], m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < V; ++i) {
-        q[i] = bf16_to_f32(p.q[row * p.q_stride + head * HD + lane * V + i]) * p.scale_log2;
-        o[i] = 0.0f;
+    const int i0 = blockIdx.y * kKv8MergeRows, rows = s.nodes * p.group;
+    if (s.parts <= 1 || i0 >= rows) return;
+    float m[kKv8MergeRows], l[kKv8MergeRows], o[kKv8MergeRows][V];
+#pragma unroll
+    for (int i = 0; i < kKv8MergeRows; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < V; ++x) o[i][x] = 0.0f;
     }
-    const long long limit = (long long)p.max_pages * p.page_tokens;
-    const int end = len < n ? 0 : (int)min((long long)pos + 1, limit);
-    for (int j = warp; j < end; j += kKv8SimpleWarps) {
-        if (p.window > 0 && j >= p.sinks && j <= pos - p.window) continue;
-        const int col = j / p.page_tokens, at = j - col * p.page_tokens;
-        const int page = p.page_table[(long long)b * p.max_pages + col];
-        if (page < 0 || page >= p.num_pages) continue;
-        const long long h = (long long)page * p.kv_heads + kvh;
-        const long long cell = (h * p.page_tokens + at) * HD + lane * V, block = h * (p.page_tokens / kKv8Block) + at / kKv8Block;
-        float s = 0.0f, v[V];
-        for (int i = 0; i < V; i += 2) {
-            float f[4];
-            unpack_e4m3x4(*reinterpret_cast<const uint16_t *>(p.k_codes + cell + i), f);
-            s += q[i] * f[0] + q[i + 1] * f[1];
-            unpack_e4m3x4(*reinterpret_cast<const uint16_t *>(p.v_codes + cell + i), f);
-            v[i] = f[0] * p.v_scales[block];
-            v[i + 1] = f[1] * p.v_scales[block];
+    auto join = [&](int i, float m2, float l2, const float (&o2)[V]) {
+        const float to = fmaxf(m[i], m2);
+        const float f = m[i] == -INFINITY ? 0.0f : exp2f(m[i] - to), f2 = m2 == -INFINITY ? 0.0f : exp2f(m2 - to);
+        m[i] = to;
+        l[i] = l[i] * f + l2 * f2;
+#pragma unroll
+        for (int x = 0; x < V; ++x) o[i][x] = o[i][x] * f + o2[x] * f2;
+    };
+#pragma unroll 2
+    for (int k = warp; k < s.parts; k += kWarps) {
+        const long long slot = k == 0 ? 2 * blockIdx.x + s.first_slot : 2 * (blockIdx.x + k);
+        float o2[kKv8MergeRows][V];
+        float2 ml[kKv8MergeRows];
+#pragma unroll
+        for (int i = 0; i < kKv8MergeRows; ++i) {
+            const long long row = slot * ROWS + min(i0 + i, rows - 1);
+            ml[i] = p.part_ml[row];
+#pragma unroll
+            for (int x = 0; x < V; ++x) o2[i][x] = p.part_o[row * HD + x * kWarp + lane];
         }
-        s = warp_sum(s) * p.k_scales[block];
-        const float to = fmaxf(m, s);
-        const float f = exp2f(m - to), e = exp2f(s - to);
-        m = to;
-        l = l * f + e;
-        for (int i = 0; i < V; ++i) o[i] = o[i] * f + e * v[i];
+#pragma unroll
+        for (int i = 0; i < kKv8MergeRows; ++i) join(i, ml[i].x, ml[i].y, o2[i]);
     }
-    for (int i = 0; i < V; ++i) part_s[warp][lane * V + i] = o[i];
-    if (lane == 0) {
-        part_s[warp][HD] = m;
-        part_s[warp][HD + 1] = l;
+#pragma unroll
+    for (int i = 0; i < kKv8MergeRows; ++i) {
+#pragma unroll
+        for (int x = 0; x < V; ++x) o_s[warp][i][x * kWarp + lane] = o[i][x];
+        if (lane == 0) ml_s[warp][i] = make_float2(m[i], l[i]);
     }
     __syncthreads();
-    if (warp != 0) return;
-    float top = -INFINITY, sum = 0.0f;
-    for (int w = 0; w < kKv8SimpleWarps; ++w) top = fmaxf(top, part_s[w][HD]);
-    for (int i = 0; i < V; ++i) o[i] = 0.0f;
-    for (int w = 0; w < kKv8SimpleWarps; ++w) {
-        const float f = part_s[w][HD] == -INFINITY ? 0.0f : exp2f(part_s[w][HD] - top);
-        sum += f * part_s[w][HD + 1];
-        for (int i = 0; i < V; ++i) o[i] += f * part_s[w][lane * V + i];
+    for (int x = threadIdx.x; x < kKv8MergeRows * HD / 2; x += kKv8MergeThreads) {
+        const int i = x / (HD / 2), d = x % (HD / 2) * 2;
+        if (i0 + i >= rows) break;
+        float top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w][i].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = ml_s[w][i].x == -INFINITY ? 0.0f : exp2f(ml_s[w][i].x - top);
+            sum += f * ml_s[w][i].y;
+            a += f * o_s[w][i][d];
+            b += f * o_s[w][i][d + 1];
+        }
+        const float inv = sum == 0.0f ? 0.0f : exp2f(-kKv8TopLog2) / sum;
+        const int node = (i0 + i) / p.group, h = (i0 + i) - node * p.group;
+        uint32_t w2;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w2) : "f"(b * inv), "f"(a * inv));
+        *reinterpret_cast<uint32_t *>(p.out + ((long long)(s.row0 + node) * p.q_heads + s.kvh * p.group + h) * HD + d) = w2;
     }
-    for (int i = 0; i < V; ++i)
-        p.out[((long long)row * p.q_heads + head) * HD + lane * V + i] = f32_to_bf16_rne(sum == 0.0f ? 0.0f : o[i] / sum);
 }
 
 }  // namespace cheetah

@@ -26,10 +26,12 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
     return r;
 }
+__device__ __forceinline__ void unpack_e4m3x2(uint32_t w, float &a, float &b) {
+    asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}" : "=f"(a), "=f"(b) : "r"(e4m3x2_to_f16x2(w)));
+}
 __device__ __forceinline__ void unpack_e4m3x4(uint32_t w, float (&v)[4]) {
-    const uint32_t lo = e4m3x2_to_f16x2(w), hi = e4m3x2_to_f16x2(w >> 16);
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(v[0]), "=f"(v[1]) : "r"(lo));
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(v[2]), "=f"(v[3]) : "r"(hi));
+    unpack_e4m3x2(w, v[0], v[1]);
+    unpack_e4m3x2(w >> 16, v[2], v[3]);
 }
 
 // f32 that any narrower format rounds as it would round x: cut off, and the last

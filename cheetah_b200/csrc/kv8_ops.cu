@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "attention_kv8.cuh"
+#include "attention_kv8_few.cuh"
 #include "cheetah_cuda.h"
 #include "common.cuh"
 #include "kv8_append.cuh"
@@ -66,6 +67,56 @@ int launch_read(const cheetah::Kv8ReadParams &p, cudaStream_t stream) {
     const long long blocks = (p.chunks + per_block - 1) / per_block;
     CH_REQUIRE(blocks <= 0x7FFFFFFFll, "cheetah_cuda_op_kv8_read: too many rows");
     CH_CUDA_TRY(launch_ex(cheetah::kv8_read_kernel<TOUT, HD>, dim3((unsigned)blocks), dim3(cheetah::kKv8ReadThreads), 0, stream, true, p));
+    return 0;
+}
+
+// 2D map over a pool's codes viewed as [rows][head_dim]: boxes of `box_rows` rows
+// of one page, swizzled over a row.
+int make_codes_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t head_dim, uint32_t box_rows) {
+    auto encode = cheetah::tensor_map_encoder();
+    CH_REQUIRE(encode != nullptr, "CUDA backend: cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[2] = {head_dim, rows};
+    cuuint64_t strides[1] = {(cuuint64_t)head_dim};
+    cuuint32_t box[2] = {head_dim, box_rows};
+    cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CH_REQUIRE(r == CUDA_SUCCESS, "CUDA backend: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return 0;
+}
+
+int attention_ctas(int device) { return std::min(cheetah::sm_count(device), cheetah::kKv8MaxCtas); }
+
+// Workspace of an attention call of `ctas` CTAs: two parts each, of up to
+// kPartRows rows.
+constexpr int kPartRows = 32;
+struct AttentionWorkspace {
+    size_t splits, ml, o, bytes;
+};
+AttentionWorkspace attention_workspace(int ctas, uint32_t head_dim) {
+    auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+    AttentionWorkspace w;
+    w.splits = 0;
+    w.ml = up(ctas * sizeof(cheetah::Kv8Split));
+    w.o = w.ml + up((size_t)ctas * 2 * kPartRows * sizeof(float2));
+    w.bytes = w.o + (size_t)ctas * 2 * kPartRows * head_dim * sizeof(float);
+    return w;
+}
+
+template <int HD, int R>
+int launch_attention_few(const CUtensorMap &k_map, const CUtensorMap &v_map, cheetah::Kv8AttnParams p, int device, int ctas,
+                         cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t smem = cheetah::kv8_few_smem<HD, R>();
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    p.item_nodes = R / p.group;
+    CH_CUDA_TRY(cheetah::allow_smem(cheetah::attention_kv8_few_kernel<HD, R>, smem, device, done));
+    CH_CUDA_TRY(launch_ex(cheetah::attention_kv8_few_kernel<HD, R>, dim3(ctas), dim3(cheetah::Kv8Few<HD, R>::kThreads), smem,
+                          stream, true, k_map, v_map, p));
+    CH_CUDA_TRY(launch_ex(cheetah::kv8_merge_kernel<HD, R>, dim3(ctas, R / cheetah::kKv8MergeRows), dim3(cheetah::kKv8MergeThreads),
+                          0, stream, true, p, ctas));
     return 0;
 }
 
@@ -171,13 +222,20 @@ static int check_attention_kv8(const CheetahCudaAttentionKv8 *a) {
                "cheetah_cuda_op_attention_kv8: a table row holds at most 2^31 - 129 tokens");
     CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu && a->sinks <= 0x7FFFFFFFu,
                "cheetah_cuda_op_attention_kv8: sliding_window or sinks is too large");
+    // The kernel counts its cost units (a key tile each, and a few per item) in
+    // 31 bits.
+    const uint64_t items = ((uint64_t)a->rows / (8 / std::min(8u, a->q_heads / a->kv_heads)) + a->batch) * a->kv_heads;
+    const uint64_t tiles = (uint64_t)a->max_pages_per_seq * a->page_tokens / cheetah::kKv8Keys + 1;
+    CH_REQUIRE(items * (tiles + 8) <= 0x7FFFFFFFull, "cheetah_cuda_op_attention_kv8: too many rows and cached positions");
     return 0;
 }
 
 int cheetah_cuda_op_attention_kv8_workspace(const CheetahCudaAttentionKv8 *a, size_t *bytes) {
     CH_REQUIRE(bytes != nullptr, "cheetah_cuda_op_attention_kv8_workspace: null argument");
     if (check_attention_kv8(a) != 0) return -1;
-    *bytes = 256;
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    *bytes = attention_workspace(attention_ctas(device), a->head_dim).bytes;
     return 0;
 }
 
@@ -192,7 +250,13 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
                    aligned(a->k_scales, 4) && aligned(a->v_scales, 4) && aligned(a->workspace, 256),
                "cheetah_cuda_op_attention_kv8: q, out and the codes must be 16-byte aligned, the scales 4-byte, the workspace "
                "256-byte");
-    CH_REQUIRE(a->workspace_bytes >= 256, "cheetah_cuda_op_attention_kv8: the workspace is too small");
+    int device = 0;
+    CH_CUDA_TRY(cudaGetDevice(&device));
+    const int ctas = attention_ctas(device);
+    const AttentionWorkspace w = attention_workspace(ctas, a->head_dim);
+    CH_REQUIRE(a->workspace_bytes >= w.bytes,
+               "cheetah_cuda_op_attention_kv8: the workspace holds " + std::to_string(a->workspace_bytes) + " of " +
+                   std::to_string(w.bytes) + " bytes");
     cheetah::Kv8AttnParams p = {};
     p.q = static_cast<const uint16_t *>(a->q);
     p.q_stride = (long long)a->q_stride;
@@ -214,10 +278,30 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
     p.kv_heads = (int)a->kv_heads;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
     p.out = static_cast<uint16_t *>(a->out);
-    auto kernel = a->head_dim == 64 ? cheetah::attention_kv8_simple_kernel<64> : cheetah::attention_kv8_simple_kernel<128>;
-    CH_CUDA_TRY(launch_ex(kernel, dim3(a->rows * a->q_heads), dim3(cheetah::kKv8SimpleWarps * cheetah::kWarp), 0,
-                          static_cast<cudaStream_t>(stream), true, p));
-    return 0;
+    p.group = (int)(a->q_heads / a->kv_heads);
+    p.box_keys = a->page_tokens % 128 == 0 ? 128 : (a->page_tokens % 64 == 0 ? 64 : (a->page_tokens % 32 == 0 ? 32 : 16));
+    uint8_t *ws = static_cast<uint8_t *>(a->workspace);
+    p.splits = reinterpret_cast<cheetah::Kv8Split *>(ws + w.splits);
+    p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
+    p.part_o = reinterpret_cast<float *>(ws + w.o);
+    CUtensorMap k_map, v_map;
+    const uint64_t pool_rows = (uint64_t)a->num_pages * a->kv_heads * a->page_tokens;
+    if (make_codes_map(&k_map, a->k_codes, pool_rows, a->head_dim, (uint32_t)p.box_keys) != 0 ||
+        make_codes_map(&v_map, a->v_codes, pool_rows, a->head_dim, (uint32_t)p.box_keys) != 0) {
+        return -1;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const uint64_t rows = (uint64_t)((a->rows + a->batch - 1) / a->batch) * p.group;
+    const int least = p.group <= 8 ? 8 : (p.group <= 16 ? 16 : 32);
+    const int r = std::max(least, rows <= 8 ? 8 : (rows <= 16 ? 16 : 32));
+    if (a->head_dim == 64) {
+        return r == 8    ? launch_attention_few<64, 8>(k_map, v_map, p, device, ctas, st)
+               : r == 16 ? launch_attention_few<64, 16>(k_map, v_map, p, device, ctas, st)
+                         : launch_attention_few<64, 32>(k_map, v_map, p, device, ctas, st);
+    }
+    return r == 8    ? launch_attention_few<128, 8>(k_map, v_map, p, device, ctas, st)
+           : r == 16 ? launch_attention_few<128, 16>(k_map, v_map, p, device, ctas, st)
+                     : launch_attention_few<128, 32>(k_map, v_map, p, device, ctas, st);
 }
 
 int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream) {

@@ -56,6 +56,47 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, u
         : "memory");
 }
 
+// kind::f8f6f4, A = B = e4m3, D = f32 (both K-major unless a transpose bit, 15
+// for A and 16 for B, is added): 32 k per instruction.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// 8-bit tiles whose rows are 128 bytes (128-byte swizzle) or 64 bytes (64-byte
+// swizzle), K-major or MN-major (one atom along MN): 8-row atoms lie 8 rows apart.
+template <int ROW_BYTES>
+__device__ __forceinline__ uint64_t umma_smem_desc_e4m3(uint32_t addr) {
+    static_assert(ROW_BYTES == 64 || ROW_BYTES == 128, "a row is one swizzle span");
+    uint64_t desc = 0;
+    desc |= (uint64_t)((addr >> 4) & 0x3FFF);
+    desc |= (uint64_t)1 << 16;
+    desc |= (uint64_t)(8 * ROW_BYTES >> 4) << 32;
+    desc |= (uint64_t)1 << 46;
+    desc |= (uint64_t)(ROW_BYTES == 128 ? 2 : 4) << 61;
+    return desc;
+}
+// Offset of 16-byte chunk `chunk` of row `row` in such a tile.
+template <int ROW_BYTES>
+__device__ __forceinline__ int e4m3_tile_offset(int row, int chunk) {
+    return row * ROW_BYTES + ((chunk ^ (ROW_BYTES == 128 ? row & 7 : row >> 1 & 3)) << 4);
+}
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A from TMEM: row = lane, four codes of consecutive k per column.
+__device__ __forceinline__ void umma_e4m3_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -116,6 +157,22 @@ __device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t addr, uint32_t at
     desc |= (uint64_t)1 << 46;
     desc |= (uint64_t)2 << 61;
     return desc;
+}
+
+// 8 columns, without the wait.
+__device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, float *v) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st8_nowait(uint32_t taddr, const float *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+                 "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, float *v) {
