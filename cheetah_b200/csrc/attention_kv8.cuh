@@ -29,6 +29,8 @@
 // memory first, where 0 times NaN would not stay 0; the rows that do see it are
 // made NaN at the end (kv8_patch).
 //
+// Shares, splits of items and the list of parts are those of tree_attention.cuh.
+//
 // All mbarrier waits are bounded: on a timeout the CTA waits (bounded) for its
 // own copies and MMAs in flight, frees its TMEM and exits, and the merge makes
 // every row NaN.
@@ -41,23 +43,16 @@
 #include "pair.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
+#include "tree_attention.cuh"
 
 namespace cheetah {
 
 constexpr int kKv8Keys = 128;     // keys per tile
-constexpr int kKv8MaxCtas = 256;  // CTAs of a launch that a merge can list
+constexpr int kKv8MaxCtas = kTreeMaxCtas;
 constexpr int kKv8Queue = 4;      // segments the scheduler may be ahead
 // Weights are scaled to at most 2^kKv8TopLog2 when a row's reference is set, and
 // it moves when one would pass 2^kKv8RoomLog2 times that (e4m3 ends at 448).
 constexpr float kKv8TopLog2 = 7.0f, kKv8RoomLog2 = 1.75f;
-
-// What a split item needs to be joined, written by the CTA that begins it.
-struct Kv8Split {
-    int row0, nodes, kvh;
-    int first_slot;  // of the beginning; the other parts are slot 0 of the next CTAs
-    int parts;       // 0: nothing to join; -1: the CTA gave up
-    int pad[3];
-};
 
 struct Kv8AttnParams {
     const uint16_t *q;
@@ -70,9 +65,10 @@ struct Kv8AttnParams {
     int batch, rows, window, sinks;
     int q_heads, kv_heads, group;
     int item_nodes;    // new tokens of an item at most
+    int tile_nodes;    // and of one of its row tiles (few rows: the item's)
     float scale_log2;
     uint16_t *out;
-    Kv8Split *splits;  // [CTAs]
+    TreeSplit *splits;  // [CTAs]
     float *part_o;     // [CTAs][2][rows of an item][HD] unnormalised
     float2 *part_ml;   // [CTAs][2][rows of an item]
 };
@@ -119,39 +115,50 @@ __device__ __forceinline__ Kv8Range kv8_range(const Kv8AttnParams &p, const Kv8S
     r.tiles = max(1, r.sink_tiles + max(hi - lo, 0));
     return r;
 }
-// Cost units of one KV head of a sequence: its items' tiles, and ITEM for each
-// item's beginning and end.
-template <int ITEM>
-__device__ __forceinline__ int kv8_head_units(const Kv8AttnParams &p, const Kv8Seq &s) {
-    int units = 0;
-    for (int j = 0; j < s.items; ++j) units += ITEM + kv8_range(p, s, j).tiles;
-    return units;
-}
+// Cost units of a kernel: ITEM for an item's beginning and end, ONE or TWO for a
+// key tile, by its row tiles. A share holds MIN_SHARE at least, which hold a tile.
+template <int ITEM_, int ONE, int TWO, int MIN_SHARE_>
+struct Kv8Cost {
+    static constexpr int ITEM = ITEM_, MIN_SHARE = MIN_SHARE_;
+    static_assert(MIN_SHARE >= TWO && TWO >= ONE, "every share holds a tile");
+    static __device__ __forceinline__ int tile(const Kv8AttnParams &p, const Kv8Seq &s, int j) {
+        return s.n - j * p.item_nodes > p.tile_nodes ? TWO : ONE;
+    }
+    static __device__ __forceinline__ int item(const Kv8AttnParams &p, const Kv8Seq &s, int j) {
+        return ITEM + kv8_range(p, s, j).tiles * tile(p, s, j);
+    }
+    // Of one KV head of a sequence.
+    static __device__ __forceinline__ int head(const Kv8AttnParams &p, const Kv8Seq &s) {
+        int units = 0;
+        for (int j = 0; j < s.items; ++j) units += item(p, s, j);
+        return units;
+    }
+};
 
 // The share of this CTA, segment by segment. Called by a whole warp, whose lanes
 // then hold the same state.
-template <int ITEM, int MIN_SHARE>
+template <typename Cost>
 struct Kv8Walk {
     int b, j, kvh, left, unit, at, share, count;
     Kv8Seq s;
-    Kv8Split split;
+    TreeSplit split;
 
     __device__ __forceinline__ void init(const Kv8AttnParams &p) {
         const int lane = threadIdx.x % kWarp;
         int total = 0, mine = 0;
         for (int i = lane; i < p.batch; i += kWarp) {
-            const int units = kv8_head_units<ITEM>(p, kv8_seq(p, i)) * p.kv_heads;
+            const int units = Cost::head(p, kv8_seq(p, i)) * p.kv_heads;
             if (i == lane) mine = units;
             total += units;
         }
         total = __reduce_add_sync(0xFFFFFFFFu, total);
-        share = max(MIN_SHARE, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+        share = max(Cost::MIN_SHARE, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
         const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
         int start = -1, before = 0;
         at = 0;
         for (int b0 = 0; b0 < p.batch && start < 0 && u0 < total; b0 += kWarp) {
             const int i = b0 + lane;
-            const int units = b0 == 0 ? mine : (i < p.batch ? kv8_head_units<ITEM>(p, kv8_seq(p, i)) * p.kv_heads : 0);
+            const int units = b0 == 0 ? mine : (i < p.batch ? Cost::head(p, kv8_seq(p, i)) * p.kv_heads : 0);
             int end = units;
 #pragma unroll
             for (int o = 1; o < kWarp; o <<= 1) {
@@ -170,14 +177,14 @@ struct Kv8Walk {
         left = min(share, total - u0);
         unit = u0;
         j = kvh = count = 0;
-        split = Kv8Split{};
+        split = TreeSplit{};
         if (left > 0) {
             s = kv8_seq(p, b);
-            const int head = kv8_head_units<ITEM>(p, s);
+            const int head = Cost::head(p, s);
             kvh = at / head;
             at -= kvh * head;
             while (true) {
-                const int units = ITEM + kv8_range(p, s, j).tiles;
+                const int units = Cost::item(p, s, j);
                 if (at < units) break;
                 at -= units;
                 ++j;
@@ -189,10 +196,10 @@ struct Kv8Walk {
         g.jobs = -1;
         while (left > 0) {
             const Kv8Range r = kv8_range(p, s, j);
-            const int units = ITEM + r.tiles;
+            const int cost = Cost::tile(p, s, j), units = Cost::ITEM + r.tiles * cost;
             const int take = min(left, units - at);
             // Tiles of this piece; an item's first ITEM units hold none.
-            const int t0 = max(at - ITEM, 0), t1 = max(at + take - ITEM, 0);
+            const int t0 = max(at - Cost::ITEM, 0) / cost, t1 = max(at + take - Cost::ITEM, 0) / cost;
             if (t1 > t0) {
                 const bool whole = t1 - t0 == r.tiles;
                 const int node0 = j * p.item_nodes;
@@ -316,6 +323,52 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// A producer warp's part of a segment: its K tiles, or its V tiles and the scales of
+// both, into a ring of [stage][K, V]. The scales go with V, whose stage is free only
+// once the weights that need them are multiplied. False if a wait gave up.
+template <int HD, int STAGES>
+__device__ __forceinline__ bool kv8_load_tiles(const Kv8AttnParams &p, const Kv8Segment &g, bool is_v, const CUtensorMap *map, uint64_t *full,
+                                               uint64_t *empty, uint8_t *ring, float (*scales)[16], uint32_t *valid_of, int tile_at,
+                                               int &issued) {
+    const int lane = threadIdx.x % kWarp, boxes = kKv8Keys / p.box_keys;
+    Kv8Boxes box;
+    box.init();
+    for (int t = g.t0; t < g.t0 + g.jobs; ++t) {
+        const int at = tile_at + t - g.t0, buf = at % STAGES;
+        const int box0 = g.key0(t) / p.box_keys;
+        box.reach(p, g, box0);
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[buf]), ((at / STAGES) & 1) ^ 1))) return false;
+        const uint32_t good = (box.loaded >> (box0 - box.first)) & kv8_low_bits(boxes);
+        const uint32_t bar = smem_u32(&full[buf]);
+        const uint32_t dst = smem_u32(ring + (2 * buf + is_v) * kKv8Keys * HD);
+        if (is_v) {
+            // Scales: lanes 0..7 K's of a block each, 8..15 V's.
+            const int block = lane & 7, x = block * kKv8Block / p.box_keys;
+            const int row = __shfl_sync(0xFFFFFFFFu, box.row, (box0 - box.first + x) & 31);
+            if (lane < 16 && row >= 0) {
+                const int at_block = row / kKv8Block + block - x * (p.box_keys / kKv8Block);
+                cp_async4(smem_u32(&scales[buf][lane]), (lane < 8 ? p.k_scales : p.v_scales) + at_block);
+            }
+            cp_async_arrive(bar);
+            if (lane == 0) {
+                uint32_t valid = 0;
+                for (int i = 0; i < boxes; ++i) {
+                    if (good >> i & 1) valid |= kv8_low_bits(8 / boxes) << (i * (8 / boxes));
+                }
+                valid_of[buf] = valid;
+            }
+        }
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(good) * p.box_keys * HD));
+        __syncwarp();
+        for (int x = 0; x < boxes; ++x) {
+            const int row = __shfl_sync(0xFFFFFFFFu, box.row, box0 - box.first + x);
+            if (lane == 0 && row >= 0) tma_load_2d(dst + x * p.box_keys * HD, map, 0, row, bar);
+        }
+        issued = at + 1;
+    }
+    return true;
+}
+
 // Whether a word holds a NaN code.
 __device__ __forceinline__ uint32_t e4m3_nan_bits(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
@@ -390,7 +443,7 @@ __global__ void __launch_bounds__(kKv8MergeThreads) kv8_merge_kernel(const Kv8At
     const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
     pdl_wait();
     pdl_launch_dependents();
-    const Kv8Split s = p.splits[blockIdx.x];
+    const TreeSplit s = p.splits[blockIdx.x];
     const bool gave_up = (int)threadIdx.x < ctas && p.splits[threadIdx.x].parts < 0;
     if (__syncthreads_or(gave_up)) {
         const long long cells = (long long)min(max(p.row_starts[p.batch], 0), p.rows) * p.q_heads * HD;

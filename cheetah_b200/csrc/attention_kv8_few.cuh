@@ -32,7 +32,7 @@ struct Kv8Few {
     static constexpr uint32_t kOCol = kGroups * 2 * R;
     static constexpr uint32_t kCols = kGroups * 4 * R <= 128 ? 128 : 256;
     static_assert(kGroups * 4 * R <= (int)kCols, "TMEM columns");
-    static constexpr int kItem = 2, kMinShare = 6;
+    using Cost = Kv8Cost<2, 1, 1, 6>;
     static constexpr int kDims = HD == 128 ? 32 : 16;               // dimensions (lanes) of a warp's part of O^T
 };
 
@@ -45,7 +45,7 @@ struct Kv8FewShared {
     uint32_t tmem;
     int abort_flag, non_finite;
     uint32_t valid[STAGES];          // per V tile: which 16-key blocks hold loaded positions
-    float scales[STAGES][16];        // K's, then V's
+    alignas(16) float scales[STAGES][16];  // K's, then V's
     alignas(16) float q_scale[2][R];
     int far[GROUPS][4];
     float top[GROUPS][4][R];         // maxima, at a segment's end sums
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
     int tile_at = 0;   // tiles of the segments before
     int issued = 0;    // producers: tiles requested
     if (warp == 3) {
-        Kv8Walk<C::kItem, C::kMinShare> walk;
+        Kv8Walk<typename C::Cost> walk;
         walk.init(p);
         int q_count = 0;  // segments with q
         for (int seg = 0;; ++seg) {
@@ -178,46 +178,10 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
     } else if (warp < 2) {
         const bool is_v = warp == 1;
         const CUtensorMap *map = is_v ? &v_map : &k_map;
-        const int boxes = kKv8Keys / p.box_keys;
         uint64_t *full = is_v ? sh.v_full : sh.k_full, *empty = is_v ? sh.v_empty : sh.k_empty;
         for (int seg = 0; next(seg); ++seg) {
             const Kv8Segment &g = sh.queue[seg % kKv8Queue];
-            Kv8Boxes box;
-            box.init();
-            for (int t = g.t0; t < g.t0 + g.jobs; ++t) {
-                const int at = tile_at + t - g.t0, buf = at % kStages;
-                const int box0 = g.key0(t) / p.box_keys;
-                box.reach(p, g, box0);
-                ok = wait(empty[buf], ((at / kStages) & 1) ^ 1);
-                if (!ok) break;
-                const uint32_t good = (box.loaded >> (box0 - box.first)) & kv8_low_bits(boxes);
-                const uint32_t bar = smem_u32(&full[buf]);
-                const uint32_t dst = smem_u32(ring + (2 * buf + is_v) * C::kTile);
-                if (is_v) {
-                    // Scales: lanes 0..7 K's of a block each, 8..15 V's.
-                    const int block = lane & 7, x = block * kKv8Block / p.box_keys;
-                    const int row = __shfl_sync(0xFFFFFFFFu, box.row, (box0 - box.first + x) & 31);
-                    if (lane < 16 && row >= 0) {
-                        const int at_block = row / kKv8Block + block - x * (p.box_keys / kKv8Block);
-                        cp_async4(smem_u32(&sh.scales[buf][lane]), (lane < 8 ? p.k_scales : p.v_scales) + at_block);
-                    }
-                    cp_async_arrive(bar);
-                    if (lane == 0) {
-                        uint32_t valid = 0;
-                        for (int i = 0; i < boxes; ++i) {
-                            if (good >> i & 1) valid |= kv8_low_bits(8 / boxes) << (i * (8 / boxes));
-                        }
-                        sh.valid[buf] = valid;
-                    }
-                }
-                if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(good) * p.box_keys * HD));
-                __syncwarp();
-                for (int x = 0; x < boxes; ++x) {
-                    const int row = __shfl_sync(0xFFFFFFFFu, box.row, box0 - box.first + x);
-                    if (lane == 0 && row >= 0) tma_load_2d(dst + x * p.box_keys * HD, map, 0, row, bar);
-                }
-                issued = at + 1;
-            }
+            ok = kv8_load_tiles<HD, kStages>(p, g, is_v, map, full, empty, ring, sh.scales, sh.valid, tile_at, issued);
             if (!ok) break;
             tile_at += g.jobs;
             release(seg);

@@ -1,6 +1,6 @@
 // q/k norm, rotation and the append of K and V to an 8-bit cache, in one launch:
-// the first CTAs take the q heads as qk_norm_rope does, the others the K and V
-// heads block by block of the cache.
+// some CTAs take the q heads as qk_norm_rope does, the others the K and V heads
+// block by block of the cache.
 //
 //   y = rotate(x * (1/sqrt(mean(x^2) + eps) * w)),   s = 2^ceil(log2(max|y| / 448)),
 //   code = e4m3(y / s)
@@ -8,21 +8,26 @@
 // with one s for the cells of a block (kKv8Block) and head. Bound by memory
 // where rows are many and by latency where they are few.
 //
-// A warp takes the new rows of one (block, head, K or V): up to 16 of them stay
-// in registers between the maximum and the codes, so a row is read once. Which
-// rows share a block is found from the slots of the 31 rows on either side: the
-// first of them leads, its warp takes all. Only a block that holds earlier cells
-// is read, and only its scale unless that grows; then the codes ahead of the new
-// ones are rounded again.
+// A CTA looks among kv8_append's `group_rows` rows for blocks of one head of K or V:
+// the first row that has a block leads (which rows share one is found from the
+// slots of the 31 rows on either side). A warp holds kRows rows in registers
+// between the maximum and the codes, so a row is read once: blocks with no more new
+// rows than that are dealt out to the warps, the others are taken by all four
+// together. Only a block that holds earlier cells is read, and only its scale unless
+// that grows; then the codes ahead of the new ones are rounded again.
 //
 // Codes decide between neighbours 1/8 or 1/16 apart, so a value next to the
-// border of two must not be moved over it by a rounding: k is computed in 64 bits,
-// reduced to f32 so that no second rounding shows (round_to_odd), and divided by
-// a power of two.
+// border of two must not be moved over it by a rounding. k is computed in f32 with
+// a bound on its error; where the values a bound below and above differ in their
+// codes (one in 10^4 does) or in the block's scale, or where f32 would not hold an
+// intermediate, the rows at hand are computed again in 64 bits, reduced to f32 so
+// that no second rounding shows (round_to_odd). Quotients by a power of two are
+// exact. All of k in 64 bits took 243 us for 32768 rows of 28 + 2 * 4 heads of 128.
 #pragma once
 
 #include "common.cuh"
 #include "kv8.cuh"
+#include "pair.cuh"
 #include "qk_norm_rope.cuh"
 
 namespace cheetah {
@@ -30,8 +35,9 @@ namespace cheetah {
 struct Kv8AppendParams {
     QkNormRopeParams q;      // the q heads (no KV heads), and what K shares with them
     int kv_heads;
-    long long q_blocks;      // CTAs that take q
-    int group_rows;          // rows among which a warp looks for blocks to take
+    long long kv_blocks;     // CTAs that append; the others take q
+    int group_rows;          // rows among which a CTA looks for blocks to take
+    int parts;               // heads of K and V that it takes of them
     uint8_t *k_codes, *v_codes;
     float *k_scales, *v_scales;
 };
@@ -42,26 +48,77 @@ constexpr int kKv8MaxGroup = 16;
 template <typename TIN, int HD>
 struct Kv8Cfg {
     static constexpr int kVec = 16 / sizeof(TIN);
-    static constexpr int kLanes = HD / 2 / kVec;      // lanes of a row: two chunks each
-    static constexpr int kRows = kWarp / kLanes;      // rows a warp takes at a time
-    static constexpr int kSteps = kKv8Block / kRows;
+    static constexpr int kLanes = HD / 2 / kVec;                  // lanes of a row: two chunks each
+    static constexpr int kSide = kWarp / kLanes;                  // rows side by side in a warp
+    static constexpr int kSteps = kKv8Block > kSide * kQkWarps ? kKv8Block / (kSide * kQkWarps) : 1;
+    static constexpr int kRows = kSide * kSteps;                  // rows of a warp
+};
+
+// Of a block: f32 bits of an upper bound of the largest magnitude and of the most
+// that a value is off by, and the largest magnitude found in 64 bits where those
+// leave the scale open.
+struct Kv8Top {
+    uint32_t top, off, exact;
 };
 
 struct Kv8Members {
-    int block[kKv8MaxGroup + 2 * kKv8Reach + 2];  // cache block of each row around; -1: not appended
-    int row[kKv8Block], cell[kKv8Block];          // of the block at hand
+    int block[kKv8MaxGroup + 2 * kKv8Reach];   // cache block of each row around; -1: not appended
+    int row[kQkWarps][kKv8Block], cell[kQkWarps][kKv8Block];  // of the block at hand
+    Kv8Top top[3];                             // of the blocks that all warps take, in turn
 };
 
 __device__ __forceinline__ void store_codes(uint8_t *dst, const uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]); }
 __device__ __forceinline__ void store_codes(uint8_t *dst, const uint32_t (&w)[1]) { *reinterpret_cast<uint32_t *>(dst) = w[0]; }
 
-// The `count` rows of one block listed in m, of one K or V head.
-template <typename TIN, int HD, bool IS_K>
-__device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const Kv8Members &m, int block, int count, int first, int kvh) {
+// Quotients by `scale` in 64 bits, rounded to odd, of the two chunks of a row that
+// a lane has: of k (is_k), or of the values as they are. All lanes of a warp call;
+// `at` is the offset into the rotary table, or negative.
+template <typename TIN, int HD>
+__device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint4 r0, uint4 r1, int da, int db, long long at, float scale,
+                                       float *out) {
     using C = Kv8Cfg<TIN, HD>;
     constexpr int VEC = C::kVec;
+    float wide[2][VEC];
+    widen_chunk<TIN>(r0, wide[0]);
+    widen_chunk<TIN>(r1, wide[1]);
+    const bool normed = is_k && p.q.k_norm != nullptr;
+    double inv = 1.0;
+    if (normed) {
+        double ss = 0.0;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) ss = fma((double)wide[0][x], (double)wide[0][x], fma((double)wide[1][x], (double)wide[1][x], ss));
+#pragma unroll
+        for (int o = C::kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        inv = 1.0 / sqrt(ss * (1.0 / HD) + (double)p.q.eps);
+    }
+#pragma unroll 1
+    for (int x = 0; x < VEC; ++x) {
+        double a = (double)wide[0][x], b = (double)wide[1][x];
+        if (normed) {
+            a *= inv * (double)p.q.k_norm[da + x];
+            b *= inv * (double)p.q.k_norm[db + x];
+        }
+        if (is_k && at >= 0) {
+            const double t = a, cs = (double)p.q.rope_cos[at + x], sn = (double)p.q.rope_sin[at + x];
+            a = t * cs - b * sn;
+            b = b * cs + t * sn;
+        }
+        out[x] = round_to_odd(a / (double)scale);
+        out[VEC + x] = round_to_odd(b / (double)scale);
+    }
+}
+
+// The `count` rows of one block listed in rows and cells, of parts [part0, part1)
+// (K's heads, then V's), one after the other with the next one's loads under
+// way. all: this warp has kRows of them and the other warps the rest.
+template <typename TIN, int HD>
+__device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const int *rows, const int *cell_of, Kv8Top *tops, int &turn,
+                                                 int block, int count, int first, int part0, int part1, bool all) {
+    using C = Kv8Cfg<TIN, HD>;
+    constexpr int VEC = C::kVec, kSide = C::kSide, kSteps = C::kSteps;
     const int lane = threadIdx.x % kWarp;
-    const int c = lane % C::kLanes, sub = lane / C::kLanes;
+    const int first_row = all ? threadIdx.x / kWarp * C::kRows : 0;
+    const int c = lane % C::kLanes, sub = first_row + lane / C::kLanes;
     const int half = p.q.rotary_dim / 2;
     // As qk_norm_rope_rows: the chunks that are rotated against each other, or
     // the halves of what passes through.
@@ -69,158 +126,321 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
     const int rest = c * VEC - half;
     const int da = turned ? c * VEC : 2 * half + rest;
     const int db = turned ? half + c * VEC : 2 * half + (HD - 2 * half) / 2 + rest;
-    const int head = p.q.q_heads + (IS_K ? 0 : p.kv_heads) + kvh;
-    const TIN *base = static_cast<const TIN *>(p.q.qkv) + (long long)head * HD;
-    uint4 raw[C::kSteps][2];
+    const int blocks_per_page = p.q.page_tokens / kKv8Block;
+    const int page = block / blocks_per_page, at_block = block - page * blocks_per_page;
+    const TIN *src[kSteps];
+    long long rope_at[kSteps];  // -1: not rotated
+    int cell[kSteps];
 #pragma unroll
-    for (int s = 0; s < C::kSteps; ++s) {
-        const int i = s * C::kRows + sub;
-        raw[s][0] = raw[s][1] = make_uint4(0u, 0u, 0u, 0u);
+    for (int s = 0; s < kSteps; ++s) {
+        const int i = s * kSide + sub;
+        src[s] = nullptr;
+        rope_at[s] = -1;
+        cell[s] = 0;
         if (i < count) {
-            const TIN *row = base + m.row[i] * p.q.qkv_stride;
-            raw[s][0] = __ldcs(reinterpret_cast<const uint4 *>(row + da));
-            raw[s][1] = __ldcs(reinterpret_cast<const uint4 *>(row + db));
+            src[s] = static_cast<const TIN *>(p.q.qkv) + rows[i] * p.q.qkv_stride + (long long)p.q.q_heads * HD;
+            cell[s] = cell_of[i];
+            if (turned && part0 < p.kv_heads) rope_at[s] = (long long)p.q.positions[rows[i]] * half + da;
         }
     }
-    const int blocks_per_page = p.q.page_tokens / kKv8Block;
-    const int page = block / blocks_per_page, part = block - page * blocks_per_page;
-    const long long head_at = (long long)page * p.kv_heads + kvh;
-    float *scale_at = (IS_K ? p.k_scales : p.v_scales) + head_at * blocks_per_page + part;
-    uint8_t *cells = (IS_K ? p.k_codes : p.v_codes) + (head_at * p.q.page_tokens + part * kKv8Block) * HD;
-    const float old = first > 0 ? *scale_at : 0.0f;
-
-    float z[C::kSteps][2 * VEC];
-    uint32_t top = 0;
+    auto load = [&](int part, uint4 (&r)[kSteps][2]) {
 #pragma unroll
-    for (int s = 0; s < C::kSteps; ++s) {
-        float a[VEC], b[VEC];
-        widen_chunk<TIN>(raw[s][0], a);
-        widen_chunk<TIN>(raw[s][1], b);
-        if (IS_K && s * C::kRows < count) {
-            double ya[VEC], yb[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                ya[i] = (double)a[i];
-                yb[i] = (double)b[i];
+        for (int s = 0; s < kSteps; ++s) {
+            r[s][0] = r[s][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (src[s] != nullptr) {
+                r[s][0] = __ldcs(reinterpret_cast<const uint4 *>(src[s] + (long long)part * HD + da));
+                r[s][1] = __ldcs(reinterpret_cast<const uint4 *>(src[s] + (long long)part * HD + db));
             }
-            if (p.q.k_norm != nullptr) {
-                double ss = 0.0;
+        }
+    };
+    auto scale_of = [&](int part) -> float * {
+        const bool k = part < p.kv_heads;
+        return (k ? p.k_scales : p.v_scales) + ((long long)page * p.kv_heads + (k ? part : part - p.kv_heads)) * blocks_per_page + at_block;
+    };
+    uint4 raw[kSteps][2], next_raw[kSteps][2];
+    load(part0, next_raw);
+    float next_old = first > 0 ? *scale_of(part0) : 0.0f;
+    // cos, sin and -sin of two elements at a time (1, 0, 0 where nothing turns),
+    // and the largest of their magnitudes.
+    constexpr int kPairs = VEC / 2;
+    using Pair = unsigned long long;
+    Pair cs[kSteps][kPairs], sn[kSteps][kPairs], neg_sn[kSteps][kPairs];
+    float turn_max[kSteps];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) ss = fma(ya[i], ya[i], fma(yb[i], yb[i], ss));
+    for (int s = 0; s < kSteps; ++s) {
+        float cv[VEC], sv[VEC];
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) {
+            cv[x] = 1.0f;
+            sv[x] = 0.0f;
+        }
+        if (rope_at[s] >= 0) {
+            load_floats(p.q.rope_cos + rope_at[s], cv);
+            load_floats(p.q.rope_sin + rope_at[s], sv);
+        }
+        turn_max[s] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kPairs; ++x) {
+            cs[s][x] = pair_f32(cv[2 * x], cv[2 * x + 1]);
+            sn[s][x] = pair_f32(sv[2 * x], sv[2 * x + 1]);
+            neg_sn[s][x] = pair_f32(-sv[2 * x], -sv[2 * x + 1]);
+            turn_max[s] = fmaxf(fmaxf(turn_max[s], fmaxf(fabsf(cv[2 * x]), fabsf(cv[2 * x + 1]))), fmaxf(fabsf(sv[2 * x]), fabsf(sv[2 * x + 1])));
+        }
+    }
+#pragma unroll 1
+    for (int part = part0; part < part1; ++part) {
+        const bool is_k = part < p.kv_heads;
+        const float old = next_old;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            raw[s][0] = next_raw[s][0];
+            raw[s][1] = next_raw[s][1];
+        }
+        if (part + 1 < part1) {
+            load(part + 1, next_raw);
+            if (first > 0) next_old = *scale_of(part + 1);
+        }
+        // Values (chunk a, then b), and what both of a pair of turned ones are off by
+        // in units of kOff: cos and sin of |a| + |b| at most. Squares and sums lose 11
+        // steps of 2^-24 (20 additions, halved by the root), the root 3, products 3,
+        // the rotation and the bound itself 6: below 32 of them.
+        constexpr float kOff = 0x1p-19f;
+        Pair z[kSteps][2 * kPairs], off[kSteps][kPairs];
+        auto exact = [&](int s, float scale) {  // all lanes of a warp
+            float t[2 * VEC];
+            kv8_exact<TIN, HD>(p, is_k, raw[s][0], raw[s][1], da, db, rope_at[s], scale, t);
+#pragma unroll
+            for (int x = 0; x < 2 * kPairs; ++x) z[s][x] = pair_f32(t[2 * x], t[2 * x + 1]);
+#pragma unroll
+            for (int x = 0; x < kPairs; ++x) off[s][x] = 0ull;
+        };
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            float wide[2][VEC];
+            widen_chunk<TIN>(raw[s][0], wide[0]);
+            widen_chunk<TIN>(raw[s][1], wide[1]);
+#pragma unroll
+            for (int x = 0; x < kPairs; ++x) {
+                z[s][x] = pair_f32(wide[0][2 * x], wide[0][2 * x + 1]);
+                z[s][kPairs + x] = pair_f32(wide[1][2 * x], wide[1][2 * x + 1]);
+                off[s][x] = 0ull;
+            }
+            if (!is_k) continue;
+            bool plain = true;
+            if (p.q.k_norm != nullptr) {
+                Pair ss2 = 0ull;
+#pragma unroll
+                for (int x = 0; x < 2 * kPairs; ++x) ss2 = fma_pair(z[s][x], z[s][x], ss2);
+                float ss, ss_hi;
+                unpair_f32(ss2, ss, ss_hi);
+                ss += ss_hi;
 #pragma unroll
                 for (int o = C::kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-                const double inv = 1.0 / sqrt(ss * (1.0 / HD) + (double)p.q.eps);
+                const float mean = ss * (1.0f / HD) + p.q.eps;
+                plain = mean > 0x1p-100f && mean < 0x1p100f;  // no square was lost
+                const float inv = rsqrtf(mean);
+                const Pair inv2 = pair_f32(inv, inv);
                 float wa[VEC], wb[VEC];
                 load_floats(p.q.k_norm + da, wa);
                 load_floats(p.q.k_norm + db, wb);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    ya[i] *= inv * (double)wa[i];
-                    yb[i] *= inv * (double)wb[i];
+                for (int x = 0; x < kPairs; ++x) {
+                    z[s][x] = mul_pair(z[s][x], mul_pair(inv2, pair_f32(wa[2 * x], wa[2 * x + 1])));
+                    z[s][kPairs + x] = mul_pair(z[s][kPairs + x], mul_pair(inv2, pair_f32(wb[2 * x], wb[2 * x + 1])));
                 }
             }
-            const int i = s * C::kRows + sub;
-            if (turned && i < count) {
-                const long long at = (long long)p.q.positions[m.row[i]] * half + da;
-                float cs[VEC], sn[VEC];
-                load_floats(p.q.rope_cos + at, cs);
-                load_floats(p.q.rope_sin + at, sn);
+            float most = 0.0f;
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) {
-                    const double t = ya[x];
-                    ya[x] = t * (double)cs[x] - yb[x] * (double)sn[x];
-                    yb[x] = yb[x] * (double)cs[x] + t * (double)sn[x];
+            for (int x = 0; x < kPairs; ++x) {
+                const Pair a = z[s][x], b = z[s][kPairs + x];
+                float a0, a1, b0, b1;
+                unpair_f32(a, a0, a1);
+                unpair_f32(b, b0, b1);
+                const float o0 = fabsf(a0) + fabsf(b0), o1 = fabsf(a1) + fabsf(b1);
+                off[s][x] = pair_f32(o0, o1);
+                most = fmaxf(most, fmaxf(o0, o1));
+                z[s][x] = fma_pair(a, cs[s][x], mul_pair(b, neg_sn[s][x]));
+                z[s][kPairs + x] = fma_pair(b, cs[s][x], mul_pair(a, sn[s][x]));
+            }
+            // (A NaN is no lost value: it stays one. An infinity makes `most` one.)
+            plain = plain && most * turn_max[s] < 0x1p100f;
+            if (__any_sync(0xFFFFFFFFu, src[s] != nullptr && !plain)) exact(s, 1.0f);
+        }
+        // f32 bits of the largest finite magnitude.
+        auto largest = [&]() -> uint32_t {
+            float most = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int x = 0; x < 2 * kPairs; ++x) {
+                    float v0, v1;
+                    unpair_f32(z[s][x], v0, v1);
+                    most = fmaxf(most, fmaxf(fabsf(v0), fabsf(v1)));
                 }
             }
+            if (__any_sync(0xFFFFFFFFu, most == INFINITY)) {
+                most = 0.0f;
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) {
-                a[x] = round_to_odd(ya[x]);
-                b[x] = round_to_odd(yb[x]);
+                for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                    for (int x = 0; x < 2 * kPairs; ++x) {
+                        float v[2];
+                        unpair_f32(z[s][x], v[0], v[1]);
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            if (fabsf(v[y]) < INFINITY) most = fmaxf(most, fabsf(v[y]));
+                            else v[y] = NAN;  // an infinity has no code
+                        }
+                        z[s][x] = pair_f32(v[0], v[1]);
+                    }
+                }
+            }
+            return __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+        };
+        uint32_t top = largest(), most_off = 0;
+        if (is_k) {
+            float most = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int x = 0; x < kPairs; ++x) {
+                    float v0, v1;
+                    unpair_f32(off[s][x], v0, v1);
+                    most = fmaxf(most, fmaxf(v0, v1) * turn_max[s]);
+                }
+            }
+            most_off = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+        }
+        Kv8Top *top_s = &tops[turn % 3], *next_top_s = &tops[(turn + 1) % 3];
+        ++turn;
+        if (all) {
+            if (lane == 0) {
+                atomicMax(&top_s->top, top);
+                if (is_k) atomicMax(&top_s->off, most_off);
+            }
+            if (threadIdx.x == 0) *next_top_s = Kv8Top{0u, 0u, 0u};  // read two parts ago, written next after this barrier
+            __syncthreads();
+            top = top_s->top;
+            most_off = top_s->off;
+        }
+        float need = kv8_scale_for(top);
+        if (is_k) {
+            const float gap = __uint_as_float(most_off) * kOff, at = __uint_as_float(top);
+            if (!(gap < INFINITY) || kv8_scale_for(__float_as_uint(at + gap)) != kv8_scale_for(__float_as_uint(fmaxf(at - gap, 0.0f)))) {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) exact(s, 1.0f);
+                top = largest();
+                if (all) {
+                    if (lane == 0) atomicMax(&top_s->exact, top);
+                    __syncthreads();
+                    top = top_s->exact;
+                }
+                need = kv8_scale_for(top);
             }
         }
+        const long long head_at = (long long)page * p.kv_heads + (is_k ? part : part - p.kv_heads);
+        uint8_t *cells = (is_k ? p.k_codes : p.v_codes) + (head_at * p.q.page_tokens + at_block * kKv8Block) * HD;
+        const float scale = old > need && old < INFINITY ? old : need;
+        if (first > 0 && scale != old) {
+            const double ratio = (double)old / (double)scale;
+            uint4 *held = reinterpret_cast<uint4 *>(cells);
+#pragma unroll 1
+            for (int x = all ? threadIdx.x : lane; x < first * (HD / 16); x += all ? kQkWarps * kWarp : kWarp) {
+                const uint4 was = held[x];
+                uint32_t w[4] = {was.x, was.y, was.z, was.w};
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) {
-            z[s][x] = a[x];
-            z[s][VEC + x] = b[x];
-            const uint32_t ma = __float_as_uint(a[x]) & 0x7FFFFFFFu, mb = __float_as_uint(b[x]) & 0x7FFFFFFFu;
-            if (ma < 0x7F800000u) top = max(top, ma);
-            if (mb < 0x7F800000u) top = max(top, mb);
+                for (int k = 0; k < 4; ++k) {
+                    float v[4];
+                    unpack_e4m3x4(w[k], v);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) v[y] = round_to_odd((double)v[y] * ratio);
+                    w[k] = pack_e4m3x4(v[0], v[1], v[2], v[3]);
+                }
+                held[x] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
-    }
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    const float need = kv8_scale_for(top);
-    const float scale = old > need && old < INFINITY ? old : need;
-    if (first > 0 && scale != old) {
-        const double ratio = (double)old / (double)scale;
-        uint4 *held = reinterpret_cast<uint4 *>(cells);
-        for (int x = lane; x < first * (HD / 16); x += kWarp) {
-            const uint4 was = held[x];
-            uint32_t w[4] = {was.x, was.y, was.z, was.w};
+        if (lane == 0 && first_row == 0 && scale != old) *scale_of(part) = scale;
+        // Products by a power of two are exact; a scale that was not set here may be
+        // none, and is divided by in 64 bits.
+        const uint32_t scale_bits = __float_as_uint(scale);
+        const bool power = (scale_bits & 0x7FFFFFu) == 0 && scale_bits >= 0x00800000u;
+        const float inv = __uint_as_float((254u << 23) - scale_bits);  // of a power of two: exponents add up to 254
+        const Pair inv2 = pair_f32(inv, inv), minus2 = pair_f32(-1.0f, -1.0f);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+        for (int s = 0; s < kSteps; ++s) {
+            uint32_t w[2 * VEC / 4];
+            auto pack = [&](Pair lo, Pair hi) -> uint32_t {
                 float v[4];
-                unpack_e4m3x4(w[k], v);
+                unpair_f32(lo, v[0], v[1]);
+                unpair_f32(hi, v[2], v[3]);
+                return pack_e4m3x4(v[0], v[1], v[2], v[3]);
+            };
+            bool same = power;
+            if (is_k) {
+                const float unit = inv * (kOff * turn_max[s]);
+                const Pair unit2 = pair_f32(unit, unit);
+                Pair e[kPairs];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) v[y] = round_to_odd((double)v[y] * ratio);
-                w[k] = pack_e4m3x4(v[0], v[1], v[2], v[3]);
+                for (int x = 0; x < kPairs; ++x) e[x] = mul_pair(off[s][x], unit2);
+#pragma unroll
+                for (int k = 0; k < 2 * VEC / 4; ++k) {
+                    const Pair v0 = mul_pair(z[s][2 * k], inv2), v1 = mul_pair(z[s][2 * k + 1], inv2);
+                    const Pair e0 = e[2 * k % kPairs], e1 = e[(2 * k + 1) % kPairs];
+                    w[k] = pack(add_pair(v0, e0), add_pair(v1, e1));
+                    same = same && w[k] == pack(fma_pair(e0, minus2, v0), fma_pair(e1, minus2, v1));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(mul_pair(z[s][2 * k], inv2), mul_pair(z[s][2 * k + 1], inv2));
             }
-            held[x] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
-    if (lane == 0 && scale != old) *scale_at = scale;
-    // Exact but where a scale that was not set here is no power of two.
-    const bool power = (__float_as_uint(scale) & 0x7FFFFFu) == 0;
-    const float inv = 1.0f / scale;
+            if (__any_sync(0xFFFFFFFFu, !same)) {
+                exact(s, scale);
 #pragma unroll
-    for (int s = 0; s < C::kSteps; ++s) {
-        const int i = s * C::kRows + sub;
-        if (i >= count) continue;
-        uint8_t *cell = cells + m.cell[i] * HD;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float v[VEC];
-#pragma unroll
-            for (int x = 0; x < VEC; ++x) {
-                const float y = z[s][h * VEC + x];
-                v[x] = power ? y * inv : y / scale;
-                if ((__float_as_uint(y) & 0x7F800000u) == 0x7F800000u) v[x] = __uint_as_float(0x7FC00000u);
+                for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(z[s][2 * k], z[s][2 * k + 1]);
             }
-            uint32_t w[VEC / 4];
+            if (src[s] == nullptr) continue;
+            uint8_t *dst = cells + cell[s] * HD;
+            uint32_t half_w[VEC / 4];
 #pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) w[k] = pack_e4m3x4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-            store_codes(cell + (h ? db : da), w);
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int k = 0; k < VEC / 4; ++k) half_w[k] = w[h * (VEC / 4) + k];
+                store_codes(dst + (h ? db : da), half_w);
+            }
         }
     }
 }
 
 template <typename TIN, int HD, int U>
-__global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_kv8_kernel(const Kv8AppendParams p) {
-    if ((long long)blockIdx.x < p.q_blocks) {
-        qk_norm_rope_rows<TIN, TIN, HD, U>(p.q, blockIdx.x);
+__global__ void __launch_bounds__(kQkWarps *kWarp, 4) qk_norm_rope_kv8_kernel(const Kv8AppendParams p) {
+    // The CTAs that append lie evenly among those that take q: their long chains of
+    // dependent steps run beside loads and stores that bound the rest.
+    const long long unit = blockIdx.x * p.kv_blocks / gridDim.x;
+    if ((blockIdx.x + 1) * p.kv_blocks / gridDim.x == unit) {
+        qk_norm_rope_rows<TIN, TIN, HD, U>(p.q, blockIdx.x - unit);
         return;
     }
-    __shared__ Kv8Members members[kQkWarps];
-    const int lane = threadIdx.x % kWarp;
-    Kv8Members &m = members[threadIdx.x / kWarp];
-    const long long unit = ((long long)blockIdx.x - p.q_blocks) * kQkWarps + threadIdx.x / kWarp;
-    const int part = (int)(unit % (2 * p.kv_heads));
-    const long long first_row = unit / (2 * p.kv_heads) * p.group_rows;
+    __shared__ Kv8Members m;
+    const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+    const int splits = (2 * p.kv_heads + p.parts - 1) / p.parts;  // of a group's parts
+    const int part0 = (int)(unit % splits) * p.parts, part1 = min(part0 + p.parts, 2 * p.kv_heads);
+    const int r0 = (int)(unit / splits * p.group_rows);
     pdl_wait();
     pdl_launch_dependents();
-    if (first_row >= p.q.tokens) return;
-    const int r0 = (int)first_row;
     const int group = min(p.group_rows, p.q.tokens - r0);
     const int slots_end = p.q.num_pages * p.q.page_tokens;  // at most 2^31 - 1
-    for (int i = lane; i < group + 2 * kKv8Reach; i += kWarp) {
-        const long long t = (long long)r0 - kKv8Reach + i;
+    static_assert(kKv8MaxGroup + 2 * kKv8Reach <= kQkWarps * kWarp, "a thread per row around");
+    if ((int)threadIdx.x < group + 2 * kKv8Reach) {
+        const long long t = (long long)r0 - kKv8Reach + threadIdx.x;
         int block = -1;
         if (t >= 0 && t < p.q.tokens) {
             const int slot = p.q.slots[t], pos = p.q.positions[t];
             if (slot >= 0 && slot < slots_end && pos >= 0 && pos < p.q.max_positions) block = slot / kKv8Block;
         }
-        m.block[i] = block;
+        m.block[threadIdx.x] = block;
     }
-    __syncwarp();
+    if (threadIdx.x < 3) m.top[threadIdx.x] = Kv8Top{0u, 0u, 0u};
+    __syncthreads();
     bool leads = false;
     if (lane < group) {
         const int mine = m.block[lane + kKv8Reach];
@@ -229,25 +449,28 @@ __global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_kv8_kernel(const
         for (int j = 0; j < kKv8Reach; ++j) again |= m.block[lane + j] == mine;
         leads = mine >= 0 && !again;
     }
+    using C = Kv8Cfg<TIN, HD>;
+    int nth = 0, turn = 0, alone = 0;  // blocks of one warp so far, maxima of all warps
     for (uint32_t left = __ballot_sync(0xFFFFFFFFu, leads); left; left &= left - 1) {
         const int at = __ffs(left) - 1 + kKv8Reach;
         const int block = m.block[at];
         // The rows of the block and their cells (16 at most: cells are distinct).
         const bool mine = m.block[at + lane] == block;  // at + lane stays within the group's reach
         const uint32_t all = __ballot_sync(0xFFFFFFFFu, mine);
+        const int count = min(__popc(all), kKv8Block);
+        const bool together = count > C::kRows;
+        if (!together && nth++ % kQkWarps != warp) continue;
         const int ordinal = __popc(all & ((1u << lane) - 1u));
         int cell = kKv8Block;
         if (mine && ordinal < kKv8Block) {
             const int t = r0 + at - kKv8Reach + lane;
             cell = p.q.slots[t] % kKv8Block;
-            m.row[ordinal] = t;
-            m.cell[ordinal] = cell;
+            m.row[warp][ordinal] = t;
+            m.cell[warp][ordinal] = cell;
         }
         const int first = (int)__reduce_min_sync(0xFFFFFFFFu, (uint32_t)cell);
         __syncwarp();
-        const int count = min(__popc(all), kKv8Block);
-        if (part < p.kv_heads) kv8_append_block<TIN, HD, true>(p, m, block, count, first, part);
-        else kv8_append_block<TIN, HD, false>(p, m, block, count, first, part - p.kv_heads);
+        kv8_append_block<TIN, HD>(p, m.row[warp], m.cell[warp], m.top, together ? turn : alone, block, count, first, part0, part1, together);
         __syncwarp();  // before the lists are written again
     }
 }

@@ -13,6 +13,7 @@
 
 #include "attention_kv8.cuh"
 #include "attention_kv8_few.cuh"
+#include "attention_kv8_many.cuh"
 #include "cheetah_cuda.h"
 #include "common.cuh"
 #include "kv8_append.cuh"
@@ -34,11 +35,6 @@ bool pool_in_range(uint32_t num_pages, uint32_t page_tokens, uint32_t kv_heads) 
            (uint64_t)num_pages * page_tokens * kv_heads <= 0x7FFFFFFFull;
 }
 
-// Rows among which a warp looks for blocks to append: one where there are few
-// rows, each its own block perhaps, and latency counts; sixteen where prompts
-// fill whole blocks.
-constexpr uint32_t kAppendFewRows = 2048;
-
 template <typename TIN, int HD>
 int launch_append(cheetah::Kv8AppendParams p, cudaStream_t stream) {
     constexpr int kHeads = cheetah::kWarp / (HD / 2 / (16 / (int)sizeof(TIN)));
@@ -48,15 +44,20 @@ int launch_append(cheetah::Kv8AppendParams p, cudaStream_t stream) {
     const int steps = (p.q.q_heads + kHeads - 1) / kHeads;
     p.q.steps = (long long)p.q.tokens * steps >= 48ll * cheetah::sm_count(device) ? steps : 1;
     p.q.row_units = (steps + p.q.steps - 1) / p.q.steps;
-    p.q_blocks = ((long long)p.q.tokens * p.q.row_units + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
-    p.group_rows = (uint32_t)p.q.tokens <= kAppendFewRows ? 1 : cheetah::kKv8MaxGroup;
+    const long long q_blocks = ((long long)p.q.tokens * p.q.row_units + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
+    // Rows among which a CTA looks for blocks, and how many of their heads it takes:
+    // sixteen and all where that gives every SM two CTAs, else four, and as many
+    // heads as leave some four CTAs for every SM.
+    const long long sms = cheetah::sm_count(device), parts = 2ll * p.kv_heads;
+    p.group_rows = p.q.tokens >= 2 * sms * cheetah::kKv8MaxGroup ? cheetah::kKv8MaxGroup : 4;
     const long long groups = ((long long)p.q.tokens + p.group_rows - 1) / p.group_rows;
-    const long long kv_blocks = (groups * 2 * p.kv_heads + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
-    CH_REQUIRE(p.q_blocks + kv_blocks <= 0x7FFFFFFFll, "cheetah_cuda_op_qk_norm_rope_kv8: too many rows");
+    p.parts = p.group_rows == 4 ? (int)std::min(parts, std::max(1ll, groups * parts / (4 * sms))) : (int)parts;
+    p.kv_blocks = groups * ((parts + p.parts - 1) / p.parts);
+    CH_REQUIRE(q_blocks + p.kv_blocks <= 0x7FFFFFFFll, "cheetah_cuda_op_qk_norm_rope_kv8: too many rows");
     auto kernel = p.q.steps == 1  ? cheetah::qk_norm_rope_kv8_kernel<TIN, HD, 1>
                   : p.q.steps <= 3 ? cheetah::qk_norm_rope_kv8_kernel<TIN, HD, 3>
                                    : cheetah::qk_norm_rope_kv8_kernel<TIN, HD, cheetah::kQkUnroll>;
-    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)(p.q_blocks + kv_blocks)), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream,
+    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)(q_blocks + p.kv_blocks)), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream,
                           true, p));
     return 0;
 }
@@ -89,19 +90,19 @@ int make_codes_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t h
 
 int attention_ctas(int device) { return std::min(cheetah::sm_count(device), cheetah::kKv8MaxCtas); }
 
-// Workspace of an attention call of `ctas` CTAs: two parts each, of up to
-// kPartRows rows.
-constexpr int kPartRows = 32;
+// Workspace of an attention call of `ctas` CTAs: two parts each, of up to two
+// row tiles.
 struct AttentionWorkspace {
     size_t splits, ml, o, bytes;
 };
 AttentionWorkspace attention_workspace(int ctas, uint32_t head_dim) {
     auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+    constexpr int kRows = 2 * cheetah::kManyRows;
     AttentionWorkspace w;
     w.splits = 0;
-    w.ml = up(ctas * sizeof(cheetah::Kv8Split));
-    w.o = w.ml + up((size_t)ctas * 2 * kPartRows * sizeof(float2));
-    w.bytes = w.o + (size_t)ctas * 2 * kPartRows * head_dim * sizeof(float);
+    w.ml = up(ctas * sizeof(cheetah::TreeSplit));
+    w.o = w.ml + up((size_t)ctas * 2 * kRows * sizeof(float2));
+    w.bytes = w.o + (size_t)ctas * 2 * kRows * head_dim * sizeof(float);
     return w;
 }
 
@@ -111,12 +112,41 @@ int launch_attention_few(const CUtensorMap &k_map, const CUtensorMap &v_map, che
     static std::atomic<uint64_t> done{0};
     constexpr size_t smem = cheetah::kv8_few_smem<HD, R>();
     static_assert(smem <= 232448, "shared memory of a CTA");
-    p.item_nodes = R / p.group;
+    p.item_nodes = p.tile_nodes = R / p.group;
     CH_CUDA_TRY(cheetah::allow_smem(cheetah::attention_kv8_few_kernel<HD, R>, smem, device, done));
     CH_CUDA_TRY(launch_ex(cheetah::attention_kv8_few_kernel<HD, R>, dim3(ctas), dim3(cheetah::Kv8Few<HD, R>::kThreads), smem,
                           stream, true, k_map, v_map, p));
     CH_CUDA_TRY(launch_ex(cheetah::kv8_merge_kernel<HD, R>, dim3(ctas, R / cheetah::kKv8MergeRows), dim3(cheetah::kKv8MergeThreads),
                           0, stream, true, p, ctas));
+    return 0;
+}
+
+template <int HD>
+int launch_attention_many(const CUtensorMap &k_map, const CUtensorMap &v_map, cheetah::Kv8AttnParams p, int device, int ctas,
+                          cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t smem = cheetah::kv8_many_smem<HD>();
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    p.tile_nodes = cheetah::kManyRows / p.group;
+    p.item_nodes = 2 * p.tile_nodes;
+    CH_CUDA_TRY(cheetah::allow_smem(cheetah::attention_kv8_many_kernel<HD>, smem, device, done));
+    CH_CUDA_TRY(launch_ex(cheetah::attention_kv8_many_kernel<HD>, dim3(ctas), dim3(cheetah::kManyThreads), smem, stream, true, k_map,
+                          v_map, p));
+    // Parts lie and are listed as tree attention's.
+    cheetah::TreeAttnParams t = {};
+    t.row_starts = p.row_starts;
+    t.batch = p.batch;
+    t.rows = p.rows;
+    t.q_heads = p.q_heads;
+    t.kv_heads = p.kv_heads;
+    t.group = p.group;
+    t.tile_nodes = p.tile_nodes;
+    t.out = p.out;
+    t.splits = p.splits;
+    t.part_o = reinterpret_cast<float4 *>(p.part_o);
+    t.part_ml = p.part_ml;
+    CH_CUDA_TRY(launch_ex(cheetah::tree_merge_kernel<HD>, dim3(ctas * cheetah::kTreeMergeCtas), dim3(cheetah::kTreeMergeThreads), 0,
+                          stream, true, t, ctas));
     return 0;
 }
 
@@ -226,7 +256,7 @@ static int check_attention_kv8(const CheetahCudaAttentionKv8 *a) {
     // 31 bits.
     const uint64_t items = ((uint64_t)a->rows / (8 / std::min(8u, a->q_heads / a->kv_heads)) + a->batch) * a->kv_heads;
     const uint64_t tiles = (uint64_t)a->max_pages_per_seq * a->page_tokens / cheetah::kKv8Keys + 1;
-    CH_REQUIRE(items * (tiles + 8) <= 0x7FFFFFFFull, "cheetah_cuda_op_attention_kv8: too many rows and cached positions");
+    CH_REQUIRE(items * (3 * tiles + 8) <= 0x7FFFFFFFull, "cheetah_cuda_op_attention_kv8: too many rows and cached positions");
     return 0;
 }
 
@@ -281,7 +311,7 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
     p.group = (int)(a->q_heads / a->kv_heads);
     p.box_keys = a->page_tokens % 128 == 0 ? 128 : (a->page_tokens % 64 == 0 ? 64 : (a->page_tokens % 32 == 0 ? 32 : 16));
     uint8_t *ws = static_cast<uint8_t *>(a->workspace);
-    p.splits = reinterpret_cast<cheetah::Kv8Split *>(ws + w.splits);
+    p.splits = reinterpret_cast<cheetah::TreeSplit *>(ws + w.splits);
     p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
     p.part_o = reinterpret_cast<float *>(ws + w.o);
     CUtensorMap k_map, v_map;
@@ -292,6 +322,9 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint64_t rows = (uint64_t)((a->rows + a->batch - 1) / a->batch) * p.group;
+    if (rows > 32)
+        return a->head_dim == 64 ? launch_attention_many<64>(k_map, v_map, p, device, ctas, st)
+                                 : launch_attention_many<128>(k_map, v_map, p, device, ctas, st);
     const int least = p.group <= 8 ? 8 : (p.group <= 16 ? 16 : 32);
     const int r = std::max(least, rows <= 8 ? 8 : (rows <= 16 ? 16 : 32));
     if (a->head_dim == 64) {
@@ -333,10 +366,10 @@ int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream
     p.out_tokens = a->out_tokens;
     int device = 0;
     CH_CUDA_TRY(cudaGetDevice(&device));
-    // Parts of a row: enough CTAs for two on every SM, each with two chunks at least.
+    // Parts of a row: up to six CTAs for every SM, each with two chunks at least.
     const long long vecs = ((long long)a->vocab + 6) / 4;
     p.parts = 1;
-    while (p.parts < cheetah::kVdMaxCluster && (long long)a->batch * p.parts * 2 <= 2ll * cheetah::sm_count(device) &&
+    while (p.parts < cheetah::kVdMaxCluster && (long long)a->batch * p.parts <= 3ll * cheetah::sm_count(device) &&
            vecs >= 4ll * p.parts * cheetah::kVdThreads) {
         p.parts *= 2;
     }
