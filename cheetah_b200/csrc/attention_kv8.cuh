@@ -5,7 +5,7 @@
 //
 // with e4m3 codes and one scale per 16 cells and head, in one pass over the keys
 // with a running reference m and sum (log2 units, t_j = log2(e)/sqrt(D) q . k_j):
-//   l = sum_j 2^(t_j - m),   o' = sum_j (2^(t_j - m) vs) vc_j,   o = o' / l.
+//   w_j = 2^(t_j + log2(vs) - m),   o' = sum_j w_j vc_j,   l = sum_j w_j / vs,   o = o' / l.
 //
 // The codes are multiplied as they are (tcgen05 kind::f8f6f4). What meets them
 // is split into e4m3 parts that are multiplied one after the other: q, over a
@@ -144,21 +144,26 @@ struct Kv8Walk {
     TreeSplit split;
 
     __device__ __forceinline__ void init(const Kv8AttnParams &p) {
+        // A lane per sequence; the units of the first kKept * 32 stay in registers.
+        constexpr int kKept = 4;
         const int lane = threadIdx.x % kWarp;
-        int total = 0, mine = 0;
-        for (int i = lane; i < p.batch; i += kWarp) {
-            const int units = Cost::head(p, kv8_seq(p, i)) * p.kv_heads;
-            if (i == lane) mine = units;
-            total += units;
+        auto units_of = [&](int i) -> int { return i < p.batch ? Cost::head(p, kv8_seq(p, i)) * p.kv_heads : 0; };
+        int kept[kKept], total = 0;
+        Kv8Seq first[kKept];
+#pragma unroll
+        for (int k = 0; k < kKept; ++k) first[k] = kv8_seq(p, min(lane + k * kWarp, p.batch - 1));  // loads side by side
+#pragma unroll
+        for (int k = 0; k < kKept; ++k) {
+            kept[k] = lane + k * kWarp < p.batch ? Cost::head(p, first[k]) * p.kv_heads : 0;
+            total += kept[k];
         }
+        for (int i = lane + kKept * kWarp; i < p.batch; i += kWarp) total += units_of(i);
         total = __reduce_add_sync(0xFFFFFFFFu, total);
         share = max(Cost::MIN_SHARE, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
         const int u0 = (int)min((long long)blockIdx.x * share, (long long)total);
         int start = -1, before = 0;
         at = 0;
-        for (int b0 = 0; b0 < p.batch && start < 0 && u0 < total; b0 += kWarp) {
-            const int i = b0 + lane;
-            const int units = b0 == 0 ? mine : (i < p.batch ? Cost::head(p, kv8_seq(p, i)) * p.kv_heads : 0);
+        auto look = [&](int b0, int units) {
             int end = units;
 #pragma unroll
             for (int o = 1; o < kWarp; o <<= 1) {
@@ -172,6 +177,13 @@ struct Kv8Walk {
                 at = u0 - __shfl_sync(0xFFFFFFFFu, end - units, __ffs(here) - 1);
             }
             before = __shfl_sync(0xFFFFFFFFu, end, kWarp - 1);
+        };
+        if (u0 < total) {
+#pragma unroll
+            for (int k = 0; k < kKept; ++k) {
+                if (start < 0) look(k * kWarp, kept[k]);
+            }
+            for (int b0 = kKept * kWarp; b0 < p.batch && start < 0; b0 += kWarp) look(b0, units_of(b0 + lane));
         }
         b = start;
         left = min(share, total - u0);
@@ -314,6 +326,64 @@ __device__ __forceinline__ float kv8_split_q(const uint4 (&raw)[2], uint8_t *til
     return scale;
 }
 
+// The same for one row by a whole warp, a lane with HD / 32 elements; `src` is the
+// row of q, or nullptr for zeros.
+template <int HD>
+__device__ __forceinline__ float kv8_split_row(const uint16_t *src, uint8_t *tile, int row, int row_lo) {
+    constexpr int V = HD / kWarp;  // 4 or 2
+    const int lane = threadIdx.x % kWarp;
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = 0u;
+    if (src != nullptr) {
+        if constexpr (V == 4) {
+            const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(src) + lane);
+            w[0] = raw.x;
+            w[1] = raw.y;
+        } else {
+            w[0] = __ldg(reinterpret_cast<const uint32_t *>(src) + lane);
+        }
+    }
+    float x[V];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        x[i] = i % 2 == 0 ? bf16_lo(w[i / 2]) : bf16_hi(w[i / 2]);
+        const uint32_t mag = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+        if (mag < 0x7F800000u) top = max(top, mag);
+        else x[i] = NAN;  // an infinity has no code
+    }
+    const float scale = kv8_scale_for(__reduce_max_sync(0xFFFFFFFFu, top));
+    const float inv = __uint_as_float((254u << 23) - __float_as_uint(scale));  // of a power of two
+    uint32_t hi[V / 2], lo[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        const float a = x[2 * i] * inv, b = x[2 * i + 1] * inv;
+        hi[i] = pack_e4m3x2(a, b);
+        float ha, hb;
+        unpack_e4m3x2(hi[i], ha, hb);
+        lo[i] = pack_e4m3x2(a - ha, b - hb);
+    }
+    const int at = lane * V % 16, c = lane * V / 16;
+    uint8_t *dst = tile + e4m3_tile_offset<HD>(row, c) + at, *dst_lo = tile + e4m3_tile_offset<HD>(row_lo, c) + at;
+    if constexpr (V == 4) {
+        *reinterpret_cast<uint32_t *>(dst) = hi[0] | hi[1] << 16;
+        *reinterpret_cast<uint32_t *>(dst_lo) = lo[0] | lo[1] << 16;
+    } else {
+        *reinterpret_cast<uint16_t *>(dst) = (uint16_t)hi[0];
+        *reinterpret_cast<uint16_t *>(dst_lo) = (uint16_t)lo[0];
+    }
+    return scale;
+}
+
+__device__ __forceinline__ void st_shared_u8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+
+__device__ __forceinline__ float kv8_log2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // cp.async of one f32, and an arrival on an mbarrier once the lane's copies so
 // far have landed (counted among its arrivals).
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
@@ -324,12 +394,12 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
 }
 
 // A producer warp's part of a segment: its K tiles, or its V tiles and the scales of
-// both, into a ring of [stage][K, V]. The scales go with V, whose stage is free only
-// once the weights that need them are multiplied. False if a wait gave up.
-template <int HD, int STAGES>
-__device__ __forceinline__ bool kv8_load_tiles(const Kv8AttnParams &p, const Kv8Segment &g, bool is_v, const CUtensorMap *map, uint64_t *full,
-                                               uint64_t *empty, uint8_t *ring, float (*scales)[16], uint32_t *valid_of, int tile_at,
-                                               int &issued) {
+// both, into a ring of tiles `step` bytes apart. The scales go with V, whose stage is
+// free only once the weights that need them are multiplied. False if a wait gave up.
+template <int HD, int STAGES, bool IS_V>
+__device__ __forceinline__ bool kv8_load_tiles(const Kv8AttnParams &p, const Kv8Segment &g, const CUtensorMap *map, uint64_t *full,
+                                               uint64_t *empty, uint8_t *ring, int step, float (*scales)[16], uint32_t *valid_of,
+                                               int tile_at, int &issued) {
     const int lane = threadIdx.x % kWarp, boxes = kKv8Keys / p.box_keys;
     Kv8Boxes box;
     box.init();
@@ -340,8 +410,8 @@ __device__ __forceinline__ bool kv8_load_tiles(const Kv8AttnParams &p, const Kv8
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[buf]), ((at / STAGES) & 1) ^ 1))) return false;
         const uint32_t good = (box.loaded >> (box0 - box.first)) & kv8_low_bits(boxes);
         const uint32_t bar = smem_u32(&full[buf]);
-        const uint32_t dst = smem_u32(ring + (2 * buf + is_v) * kKv8Keys * HD);
-        if (is_v) {
+        const uint32_t dst = smem_u32(ring + buf * step);
+        if (IS_V) {
             // Scales: lanes 0..7 K's of a block each, 8..15 V's.
             const int block = lane & 7, x = block * kKv8Block / p.box_keys;
             const int row = __shfl_sync(0xFFFFFFFFu, box.row, (box0 - box.first + x) & 31);
@@ -504,7 +574,7 @@ __global__ void __launch_bounds__(kKv8MergeThreads) kv8_merge_kernel(const Kv8At
             a += f * o_s[w][i][d];
             b += f * o_s[w][i][d + 1];
         }
-        const float inv = sum == 0.0f ? 0.0f : exp2f(-kKv8TopLog2) / sum;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int node = (i0 + i) / p.group, h = (i0 + i) - node * p.group;
         uint32_t w2;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w2) : "f"(b * inv), "f"(a * inv));

@@ -142,10 +142,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     } else if (warp < 2) {
         const bool is_v = warp == 1;
         const CUtensorMap *map = is_v ? &v_map : &k_map;
-        uint64_t *full = is_v ? sh.v_full : sh.k_full, *empty = is_v ? sh.v_empty : sh.k_empty;
         for (int seg = 0; next(seg); ++seg) {
             const Kv8Segment &g = sh.queue[seg % kKv8Queue];
-            ok = kv8_load_tiles<HD, kStages>(p, g, is_v, map, full, empty, ring, sh.scales, sh.valid, tile_at, issued);
+            ok = is_v ? kv8_load_tiles<HD, kStages, true>(p, g, map, sh.v_full, sh.v_empty, ring + C::kTile, 2 * C::kTile, sh.scales, sh.valid, tile_at, issued)
+                      : kv8_load_tiles<HD, kStages, false>(p, g, map, sh.k_full, sh.k_empty, ring, 2 * C::kTile, nullptr, nullptr, tile_at, issued);
             if (!ok) break;
             tile_at += g.jobs;
             release(seg);
