@@ -60,7 +60,8 @@ struct Kv8AttnParams {
     const uint8_t *k_codes, *v_codes;
     const float *k_scales, *v_scales;
     const int32_t *page_table;
-    int max_pages, num_pages, page_tokens, box_keys;
+    int max_pages, num_pages, page_tokens;
+    int box_shift;     // log2 of the keys of a TMA box: 4 .. 7
     const int32_t *seq_lens, *row_starts;
     int batch, rows, window, sinks;
     int q_heads, kv_heads, group;
@@ -264,28 +265,21 @@ struct Kv8Walk {
 
 __device__ __forceinline__ uint32_t kv8_low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
 
-// The pool rows of a segment's boxes (runs of box_keys keys on one page), 32 of
+// The pool rows of a segment's boxes (runs of 2^box_shift keys on one page), 32 of
 // them at a time, one per lane; -1: not loaded. A tile's boxes never straddle
 // the 32 (a multiple of 1, 2, 4 and 8).
 struct Kv8Boxes {
     int first, row;
-    uint32_t loaded;
-    __device__ __forceinline__ void init() {
-        first = INT_MIN;
-        row = -1;
-        loaded = 0;
-    }
     __device__ __forceinline__ void reach(const Kv8AttnParams &p, const Kv8Segment &g, int box0) {
-        if (first != INT_MIN && box0 >= first && box0 < first + kWarp) return;
+        if (box0 >= first && box0 < first + kWarp) return;
         first = box0;
         row = -1;
-        const long long pos = (long long)(box0 + (int)(threadIdx.x % kWarp)) * p.box_keys;
-        if (pos < min(g.len, g.pos0 + g.nodes) && (pos + p.box_keys > g.low || pos < p.sinks)) {
+        const long long pos = (long long)(box0 + (int)(threadIdx.x % kWarp)) << p.box_shift;
+        if (pos < min(g.len, g.pos0 + g.nodes) && (pos + (1 << p.box_shift) > g.low || pos < p.sinks)) {
             const int col = (int)pos / p.page_tokens;
             const int page = p.page_table[(long long)g.b * p.max_pages + col];
             if (page >= 0 && page < p.num_pages) row = (page * p.kv_heads + g.kvh) * p.page_tokens + ((int)pos - col * p.page_tokens);
         }
-        loaded = __ballot_sync(0xFFFFFFFFu, row >= 0);
     }
 };
 
@@ -384,15 +378,6 @@ __device__ __forceinline__ float kv8_log2(float x) {
     return y;
 }
 
-// cp.async of one f32, and an arrival on an mbarrier once the lane's copies so
-// far have landed (counted among its arrivals).
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-
 // A producer warp's part of a segment: its K tiles, or its V tiles and the scales of
 // both, into a ring of tiles `step` bytes apart. The scales go with V, whose stage is
 // free only once the weights that need them are multiplied. False if a wait gave up.
@@ -400,41 +385,49 @@ template <int HD, int STAGES, bool IS_V>
 __device__ __forceinline__ bool kv8_load_tiles(const Kv8AttnParams &p, const Kv8Segment &g, const CUtensorMap *map, uint64_t *full,
                                                uint64_t *empty, uint8_t *ring, int step, float (*scales)[16], uint32_t *valid_of,
                                                int tile_at, int &issued) {
-    const int lane = threadIdx.x % kWarp, boxes = kKv8Keys / p.box_keys;
+    const int lane = threadIdx.x % kWarp, shift = p.box_shift, boxes = kKv8Keys >> shift;
+    const uint32_t box_bytes = (uint32_t)HD << shift;
+    // Scales: lanes 0..7 K's of a block each, 8..15 V's; `x` is the block's box.
+    const int block = lane & 7, x = block >> (shift - 4), in_box = block & ((1 << (shift - 4)) - 1);
+    const float *scale_of = lane < 8 ? p.k_scales : p.v_scales;
     Kv8Boxes box;
-    box.init();
-    for (int t = g.t0; t < g.t0 + g.jobs; ++t) {
-        const int at = tile_at + t - g.t0, buf = at % STAGES;
-        const int box0 = g.key0(t) / p.box_keys;
+    box.first = INT_MIN / 2;
+    box.row = -1;
+    int buf = tile_at % STAGES, box0 = 0, row = -1;
+    uint32_t phase = (tile_at / STAGES) & 1, valid = 0;
+    float scale = 0.0f;
+    // The next tile's boxes, and this lane's scale of it, on its way while others wait.
+    auto look = [&](int t) {
+        box0 = g.key0(t) >> shift;
         box.reach(p, g, box0);
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[buf]), ((at / STAGES) & 1) ^ 1))) return false;
-        const uint32_t good = (box.loaded >> (box0 - box.first)) & kv8_low_bits(boxes);
+        row = __shfl_sync(0xFFFFFFFFu, box.row, (box0 - box.first + x) & 31);  // of this lane's block
+        valid = __ballot_sync(0xFFFFFFFFu, row >= 0) & 0xFFu;
+        if (IS_V && lane < 16 && row >= 0) scale = __ldg(scale_of + row / kKv8Block + in_box);
+    };
+    const int t1 = g.t0 + g.jobs;
+    if (g.jobs > 0) look(g.t0);
+    for (int t = g.t0; t < t1; ++t) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[buf]), phase ^ 1))) return false;
         const uint32_t bar = smem_u32(&full[buf]);
+        // (The phase ends with the arrival below: it waits for these bytes as well.)
         const uint32_t dst = smem_u32(ring + buf * step);
+        for (int i = 0; i < boxes; ++i) {
+            const int box_row = __shfl_sync(0xFFFFFFFFu, box.row, box0 - box.first + i);
+            if (lane == 0 && box_row >= 0) tma_load_2d(dst + i * box_bytes, map, 0, box_row, bar);
+        }
         if (IS_V) {
-            // Scales: lanes 0..7 K's of a block each, 8..15 V's.
-            const int block = lane & 7, x = block * kKv8Block / p.box_keys;
-            const int row = __shfl_sync(0xFFFFFFFFu, box.row, (box0 - box.first + x) & 31);
-            if (lane < 16 && row >= 0) {
-                const int at_block = row / kKv8Block + block - x * (p.box_keys / kKv8Block);
-                cp_async4(smem_u32(&scales[buf][lane]), (lane < 8 ? p.k_scales : p.v_scales) + at_block);
-            }
-            cp_async_arrive(bar);
-            if (lane == 0) {
-                uint32_t valid = 0;
-                for (int i = 0; i < boxes; ++i) {
-                    if (good >> i & 1) valid |= kv8_low_bits(8 / boxes) << (i * (8 / boxes));
-                }
-                valid_of[buf] = valid;
-            }
+            if (lane < 16) scales[buf][lane] = scale;
+            if (lane == 0) valid_of[buf] = valid;
+            __syncwarp();
         }
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(good) * p.box_keys * HD));
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(valid) * kKv8Block * HD);
         __syncwarp();
-        for (int x = 0; x < boxes; ++x) {
-            const int row = __shfl_sync(0xFFFFFFFFu, box.row, box0 - box.first + x);
-            if (lane == 0 && row >= 0) tma_load_2d(dst + x * p.box_keys * HD, map, 0, row, bar);
+        ++issued;
+        if (++buf == STAGES) {
+            buf = 0;
+            phase ^= 1;
         }
-        issued = at + 1;
+        if (t + 1 < t1) look(t + 1);
     }
     return true;
 }

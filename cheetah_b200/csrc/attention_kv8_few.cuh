@@ -75,7 +75,7 @@ constexpr size_t kv8_few_smem() {
 // max of a warp's values (NaN ignored).
 __device__ __forceinline__ float kv8_warp_max(float v) {
     float r;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
 
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
             mbar_init(smem_u32(&sh.s_done[i]), 1);
         }
         for (int i = 0; i < kStagesV; ++i) {
-            mbar_init(smem_u32(&sh.v_full[i]), 1 + kWarp);
+            mbar_init(smem_u32(&sh.v_full[i]), 1);
             mbar_init(smem_u32(&sh.o_done[i]), 1);
         }
         for (int i = 0; i < kKv8Queue; ++i) {
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh.q_full[i]), kGroups * 4);
-            mbar_init(smem_u32(&sh.q_empty[i]), 1 + kGroups * 4);
+            mbar_init(smem_u32(&sh.q_empty[i]), kGroups * 4);
         }
         for (int g = 0; g < kGroups; ++g) {
             for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sh.p_full[g][i]), 4);
@@ -216,7 +216,6 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
 #pragma unroll
                     for (int k = 0; k < HD / 32; ++k) umma_e4m3(tmem + s_at * 2 * R, kd + 2 * k, q_desc + 2 * k, kIdescS, k > 0 ? 1u : 0u);
                     umma_commit(smem_u32(&sh.s_done[k_buf]));
-                    if (s_left == 0) umma_commit(smem_u32(&sh.q_empty[q_count & 1]));
                 }
                 __syncwarp();
                 s_at += 2;
@@ -348,6 +347,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                     r1 = n1 * p.group;
                 }
                 const float log_vs = kv8_log2(vs);
+                __syncwarp();  // the loads from TMEM are the whole warp's
                 float arg[R];
                 // arg without sub, S in steps of 16 rows at most.
                 constexpr int kStep = R < 16 ? R : 16;

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = 0; i < kStages; ++i) {
             mbar_init(smem_u32(&sh.k_full[i]), 1);
             mbar_init(smem_u32(&sh.k_empty[i]), 1);
-            mbar_init(smem_u32(&sh.v_full[i]), 1 + kWarp);
+            mbar_init(smem_u32(&sh.v_full[i]), 1);
             mbar_init(smem_u32(&sh.v_empty[i]), 1);
         }
         for (int i = 0; i < kKv8Queue; ++i) {

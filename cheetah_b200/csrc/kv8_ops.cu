@@ -309,15 +309,15 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)a->head_dim);
     p.out = static_cast<uint16_t *>(a->out);
     p.group = (int)(a->q_heads / a->kv_heads);
-    p.box_keys = a->page_tokens % 128 == 0 ? 128 : (a->page_tokens % 64 == 0 ? 64 : (a->page_tokens % 32 == 0 ? 32 : 16));
+    p.box_shift = a->page_tokens % 128 == 0 ? 7 : (a->page_tokens % 64 == 0 ? 6 : (a->page_tokens % 32 == 0 ? 5 : 4));
     uint8_t *ws = static_cast<uint8_t *>(a->workspace);
     p.splits = reinterpret_cast<cheetah::TreeSplit *>(ws + w.splits);
     p.part_ml = reinterpret_cast<float2 *>(ws + w.ml);
     p.part_o = reinterpret_cast<float *>(ws + w.o);
     CUtensorMap k_map, v_map;
     const uint64_t pool_rows = (uint64_t)a->num_pages * a->kv_heads * a->page_tokens;
-    if (make_codes_map(&k_map, a->k_codes, pool_rows, a->head_dim, (uint32_t)p.box_keys) != 0 ||
-        make_codes_map(&v_map, a->v_codes, pool_rows, a->head_dim, (uint32_t)p.box_keys) != 0) {
+    if (make_codes_map(&k_map, a->k_codes, pool_rows, a->head_dim, 1u << p.box_shift) != 0 ||
+        make_codes_map(&v_map, a->v_codes, pool_rows, a->head_dim, 1u << p.box_shift) != 0) {
         return -1;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);

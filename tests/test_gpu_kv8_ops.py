@@ -367,6 +367,14 @@ def test_attention_of_a_long_context(rows):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("q_heads,kvh,D,batch", [(7, 1, 128, 160), (14, 2, 64, 40), (16, 1, 128, 40), (32, 1, 64, 24)])
+def test_attention_rings_go_round(q_heads, kvh, D, batch):
+    """So many key tiles to a CTA that its rings of tiles go round several times."""
+    rng = np.random.default_rng(batch)
+    c = Attend(batch, (rng.integers(0, 9000, batch) * (160 / batch)).astype(int).clip(max=18000).tolist(), [1] * batch, q_heads, kvh, D, 64)
+    c.check(c.run(), sample=range(0, batch, 7))
+
+
 def test_attention_codes_of_every_size():
     """Any code and scales that vary over several powers of two: weights and V's scale together set what a row resolves."""
     for seed, rows in ((1, 1), (2, 4), (3, 70)):
