@@ -1,5 +1,5 @@
 // q/k norm, rotation and the append of K and V to an 8-bit cache, in one launch:
-// some CTAs take the q heads as qk_norm_rope does, the others the K and V heads
+// some CTAs take the q heads, the others the K and V heads
 // block by block of the cache.
 //
 //   y = rotate(x * (1/sqrt(mean(x^2) + eps) * w)),   s = 2^ceil(log2(max|y| / 448)),
@@ -35,7 +35,7 @@ namespace cheetah {
 struct Kv8AppendParams {
     QkNormRopeParams q;      // the q heads (no KV heads), and what K shares with them
     int kv_heads;
-    long long kv_blocks;     // CTAs that append; the others take q
+    uint32_t kv_blocks, every;  // CTAs that append, and of how many one does; the others take q
     int group_rows;          // rows among which a CTA looks for blocks to take
     int parts;               // heads of K and V that it takes of them
     uint8_t *k_codes, *v_codes;
@@ -70,6 +70,138 @@ struct Kv8Members {
 __device__ __forceinline__ void store_codes(uint8_t *dst, const uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]); }
 __device__ __forceinline__ void store_codes(uint8_t *dst, const uint32_t (&w)[1]) { *reinterpret_cast<uint32_t *>(dst) = w[0]; }
 
+// VEC elements of a 16-byte chunk as f32 pairs.
+template <typename T, int VEC>
+__device__ __forceinline__ void widen_pairs(const uint4 &raw, unsigned long long *v) {
+    float f[VEC];
+    widen_chunk<T>(raw, f);
+#pragma unroll
+    for (int x = 0; x < VEC / 2; ++x) v[x] = pair_f32(f[2 * x], f[2 * x + 1]);
+}
+
+// Mean of the squares of a row, of which each of LANES lanes has N pairs.
+template <int HD, int LANES, int N>
+__device__ __forceinline__ float kv8_mean_square(const unsigned long long *v) {
+    unsigned long long sum = 0ull;
+#pragma unroll
+    for (int x = 0; x < N; ++x) sum = fma_pair(v[x], v[x], sum);
+    float lo, hi;
+    unpair_f32(sum, lo, hi);
+    lo += hi;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) lo += __shfl_xor_sync(0xFFFFFFFFu, lo, o);
+    return lo * (1.0f / HD);
+}
+
+// The rotation of a lane's two chunks at a row's position, the norm's weights
+// multiplied into it: (a, b) -> (a wa c - b wb s, b wb c + a wa s). Two elements at a
+// time; computed once for all heads of the row.
+template <int VEC>
+struct Kv8Turn {
+    unsigned long long wac[VEC / 2], wbs[VEC / 2], wbc[VEC / 2], was[VEC / 2];  // wbs is negative
+    float largest;
+
+    __device__ __forceinline__ void load(const QkNormRopeParams &p, const float *norm, long long at, int da, int db) {
+        float c[VEC], s[VEC], wa[VEC], wb[VEC];
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) {
+            c[x] = wa[x] = wb[x] = 1.0f;
+            s[x] = 0.0f;
+        }
+        if (at >= 0) {
+            load_floats(p.rope_cos + at, c);
+            load_floats(p.rope_sin + at, s);
+        }
+        if (norm != nullptr) {
+            load_floats(norm + da, wa);
+            load_floats(norm + db, wb);
+        }
+        largest = 0.0f;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) largest = fmaxf(largest, fmaxf(fabsf(wa[x]), fabsf(wb[x])) * fmaxf(fabsf(c[x]), fabsf(s[x])));
+#pragma unroll
+        for (int x = 0; x < VEC / 2; ++x) {
+            wac[x] = pair_f32(wa[2 * x] * c[2 * x], wa[2 * x + 1] * c[2 * x + 1]);
+            wbs[x] = pair_f32(-wb[2 * x] * s[2 * x], -wb[2 * x + 1] * s[2 * x + 1]);
+            wbc[x] = pair_f32(wb[2 * x] * c[2 * x], wb[2 * x + 1] * c[2 * x + 1]);
+            was[x] = pair_f32(wa[2 * x] * s[2 * x], wa[2 * x + 1] * s[2 * x + 1]);
+        }
+    }
+    __device__ __forceinline__ void apply(unsigned long long *v) const {
+#pragma unroll
+        for (int x = 0; x < VEC / 2; ++x) {
+            const unsigned long long a = v[x], b = v[VEC / 2 + x];
+            v[x] = fma_pair(a, wac[x], mul_pair(b, wbs[x]));
+            v[VEC / 2 + x] = fma_pair(b, wbc[x], mul_pair(a, was[x]));
+        }
+    }
+};
+
+// The q heads of a row: as qk_norm_rope_rows, with the rotation's numbers and the
+// weights multiplied once per row and two elements per operation.
+template <typename TIN, int HD, int U>
+__device__ __forceinline__ void kv8_q_rows(const QkNormRopeParams &p, uint32_t block) {
+    using C = Kv8Cfg<TIN, HD>;
+    constexpr int VEC = C::kVec, kLanes = C::kLanes, kHeads = C::kSide, kPairs = VEC / 2;
+    const int lane = threadIdx.x % kWarp;
+    const int c = lane % kLanes, sub = lane / kLanes;
+    const uint32_t unit = block * kQkWarps + threadIdx.x / kWarp;  // (the host keeps it below 2^31)
+    const int t = (int)(p.row_units == 1 ? unit : unit / (uint32_t)p.row_units);
+    const int step0 = (int)(unit - (uint32_t)t * (uint32_t)p.row_units) * p.steps;
+    const int half = p.rotary_dim / 2;
+    const bool turned = c * VEC < half;
+    const int rest = c * VEC - half;
+    const int da = turned ? c * VEC : 2 * half + rest;
+    const int db = turned ? half + c * VEC : 2 * half + (HD - 2 * half) / 2 + rest;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (t >= p.tokens) return;
+    const TIN *row = static_cast<const TIN *>(p.qkv) + t * p.qkv_stride;
+    const int step1 = min((p.q_heads + kHeads - 1) / kHeads, step0 + p.steps);
+    uint4 raw[U][2];
+    auto load_heads = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int head = (s0 + u) * kHeads + sub;
+            raw[u][0] = raw[u][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (s0 + u < step1 && head < p.q_heads) {
+                raw[u][0] = __ldcs(reinterpret_cast<const uint4 *>(row + (long long)head * HD + da));
+                raw[u][1] = __ldcs(reinterpret_cast<const uint4 *>(row + (long long)head * HD + db));
+            }
+        }
+    };
+    load_heads(step0);
+    const int pos = p.positions[t];
+    if (pos < 0 || pos >= p.max_positions) return;
+    Kv8Turn<VEC> turn;
+    turn.load(p, p.q_norm, turned ? (long long)pos * half + da : -1, da, db);
+    for (int s0 = step0; s0 < step1; s0 += U) {
+        if (s0 > step0) load_heads(s0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u >= step1) break;
+            const int head = (s0 + u) * kHeads + sub;
+            unsigned long long v[2 * kPairs];
+            widen_pairs<TIN, VEC>(raw[u][0], v);
+            widen_pairs<TIN, VEC>(raw[u][1], v + kPairs);
+            float inv = 1.0f;
+            if (p.q_norm != nullptr) inv = rsqrtf(kv8_mean_square<HD, kLanes, 2 * kPairs>(v) + p.eps);
+            turn.apply(v);
+            if (head >= p.q_heads) continue;
+            float a[VEC], b[VEC];
+#pragma unroll
+            for (int x = 0; x < kPairs; ++x) {
+                const unsigned long long inv2 = pair_f32(inv, inv);
+                unpair_f32(mul_pair(v[x], inv2), a[2 * x], a[2 * x + 1]);
+                unpair_f32(mul_pair(v[kPairs + x], inv2), b[2 * x], b[2 * x + 1]);
+            }
+            const long long at = ((long long)t * p.q_heads + head) * HD;
+            store_chunk<TIN, VEC, (U > 1)>(p.q_out, at + da, a);
+            store_chunk<TIN, VEC, (U > 1)>(p.q_out, at + db, b);
+        }
+    }
+}
+
 // Quotients by `scale` in 64 bits, rounded to odd, of the two chunks of a row that
 // a lane has: of k (is_k), or of the values as they are. All lanes of a warp call;
 // `at` is the offset into the rotary table, or negative.
@@ -82,6 +214,9 @@ __device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint
     widen_chunk<TIN>(r0, wide[0]);
     widen_chunk<TIN>(r1, wide[1]);
     const bool normed = is_k && p.q.k_norm != nullptr;
+    const uint32_t bits = __float_as_uint(scale);
+    const bool power = (bits & 0x7FFFFFu) == 0 && bits >= 0x00800000u;
+    const double by = (double)__uint_as_float((254u << 23) - bits);  // 1 / scale, where that is a power of two
     double inv = 1.0;
     if (normed) {
         double ss = 0.0;
@@ -103,8 +238,8 @@ __device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint
             a = t * cs - b * sn;
             b = b * cs + t * sn;
         }
-        out[x] = round_to_odd(a / (double)scale);
-        out[VEC + x] = round_to_odd(b / (double)scale);
+        out[x] = round_to_odd(power ? a * by : a / (double)scale);
+        out[VEC + x] = round_to_odd(power ? b * by : b / (double)scale);
     }
 }
 
@@ -160,32 +295,14 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
     uint4 raw[kSteps][2], next_raw[kSteps][2];
     load(part0, next_raw);
     float next_old = first > 0 ? *scale_of(part0) : 0.0f;
-    // cos, sin and -sin of two elements at a time (1, 0, 0 where nothing turns),
-    // and the largest of their magnitudes.
+    // k's rotation with the norm's weights in it (Kv8Turn), and the largest of its
+    // magnitudes.
     constexpr int kPairs = VEC / 2;
     using Pair = unsigned long long;
-    Pair cs[kSteps][kPairs], sn[kSteps][kPairs], neg_sn[kSteps][kPairs];
-    float turn_max[kSteps];
+    Kv8Turn<VEC> turns[kSteps];
+    if (part0 < p.kv_heads) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        float cv[VEC], sv[VEC];
-#pragma unroll
-        for (int x = 0; x < VEC; ++x) {
-            cv[x] = 1.0f;
-            sv[x] = 0.0f;
-        }
-        if (rope_at[s] >= 0) {
-            load_floats(p.q.rope_cos + rope_at[s], cv);
-            load_floats(p.q.rope_sin + rope_at[s], sv);
-        }
-        turn_max[s] = 0.0f;
-#pragma unroll
-        for (int x = 0; x < kPairs; ++x) {
-            cs[s][x] = pair_f32(cv[2 * x], cv[2 * x + 1]);
-            sn[s][x] = pair_f32(sv[2 * x], sv[2 * x + 1]);
-            neg_sn[s][x] = pair_f32(-sv[2 * x], -sv[2 * x + 1]);
-            turn_max[s] = fmaxf(fmaxf(turn_max[s], fmaxf(fabsf(cv[2 * x]), fabsf(cv[2 * x + 1]))), fmaxf(fabsf(sv[2 * x]), fabsf(sv[2 * x + 1])));
-        }
+        for (int s = 0; s < kSteps; ++s) turns[s].load(p.q, p.q.k_norm, rope_at[s], da, db);
     }
 #pragma unroll 1
     for (int part = part0; part < part1; ++part) {
@@ -200,12 +317,14 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
             load(part + 1, next_raw);
             if (first > 0) next_old = *scale_of(part + 1);
         }
-        // Values (chunk a, then b), and what both of a pair of turned ones are off by
-        // in units of kOff: cos and sin of |a| + |b| at most. Squares and sums lose 11
-        // steps of 2^-24 (20 additions, halved by the root), the root 3, products 3,
-        // the rotation and the bound itself 6: below 32 of them.
+        // Values over the row's factor (chunk a, then b), and what both of a pair of
+        // turned ones are off by in units of kOff: the rotation's largest number of |a|
+        // + |b| at most. Squares and sums lose 11 steps of 2^-24 (20 additions, halved
+        // by the root), the root 3, weights, rotation and factor 4, the bound itself and
+        // what is added to it 4: below 32 of them.
         constexpr float kOff = 0x1p-19f;
         Pair z[kSteps][2 * kPairs], off[kSteps][kPairs];
+        float factor[kSteps];
         auto exact = [&](int s, float scale) {  // all lanes of a warp
             float t[2 * VEC];
             kv8_exact<TIN, HD>(p, is_k, raw[s][0], raw[s][1], da, db, rope_at[s], scale, t);
@@ -213,57 +332,34 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
             for (int x = 0; x < 2 * kPairs; ++x) z[s][x] = pair_f32(t[2 * x], t[2 * x + 1]);
 #pragma unroll
             for (int x = 0; x < kPairs; ++x) off[s][x] = 0ull;
+            factor[s] = 1.0f;
         };
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            float wide[2][VEC];
-            widen_chunk<TIN>(raw[s][0], wide[0]);
-            widen_chunk<TIN>(raw[s][1], wide[1]);
-#pragma unroll
-            for (int x = 0; x < kPairs; ++x) {
-                z[s][x] = pair_f32(wide[0][2 * x], wide[0][2 * x + 1]);
-                z[s][kPairs + x] = pair_f32(wide[1][2 * x], wide[1][2 * x + 1]);
-                off[s][x] = 0ull;
-            }
+            widen_pairs<TIN, VEC>(raw[s][0], z[s]);
+            widen_pairs<TIN, VEC>(raw[s][1], z[s] + kPairs);
+            factor[s] = 1.0f;
             if (!is_k) continue;
             bool plain = true;
             if (p.q.k_norm != nullptr) {
-                Pair ss2 = 0ull;
-#pragma unroll
-                for (int x = 0; x < 2 * kPairs; ++x) ss2 = fma_pair(z[s][x], z[s][x], ss2);
-                float ss, ss_hi;
-                unpair_f32(ss2, ss, ss_hi);
-                ss += ss_hi;
-#pragma unroll
-                for (int o = C::kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-                const float mean = ss * (1.0f / HD) + p.q.eps;
+                const float mean = kv8_mean_square<HD, C::kLanes, 2 * kPairs>(z[s]) + p.q.eps;
                 plain = mean > 0x1p-100f && mean < 0x1p100f;  // no square was lost
-                const float inv = rsqrtf(mean);
-                const Pair inv2 = pair_f32(inv, inv);
-                float wa[VEC], wb[VEC];
-                load_floats(p.q.k_norm + da, wa);
-                load_floats(p.q.k_norm + db, wb);
-#pragma unroll
-                for (int x = 0; x < kPairs; ++x) {
-                    z[s][x] = mul_pair(z[s][x], mul_pair(inv2, pair_f32(wa[2 * x], wa[2 * x + 1])));
-                    z[s][kPairs + x] = mul_pair(z[s][kPairs + x], mul_pair(inv2, pair_f32(wb[2 * x], wb[2 * x + 1])));
-                }
+                factor[s] = rsqrtf(mean);
             }
             float most = 0.0f;
 #pragma unroll
             for (int x = 0; x < kPairs; ++x) {
-                const Pair a = z[s][x], b = z[s][kPairs + x];
                 float a0, a1, b0, b1;
-                unpair_f32(a, a0, a1);
-                unpair_f32(b, b0, b1);
+                unpair_f32(z[s][x], a0, a1);
+                unpair_f32(z[s][kPairs + x], b0, b1);
                 const float o0 = fabsf(a0) + fabsf(b0), o1 = fabsf(a1) + fabsf(b1);
                 off[s][x] = pair_f32(o0, o1);
                 most = fmaxf(most, fmaxf(o0, o1));
-                z[s][x] = fma_pair(a, cs[s][x], mul_pair(b, neg_sn[s][x]));
-                z[s][kPairs + x] = fma_pair(b, cs[s][x], mul_pair(a, sn[s][x]));
             }
+            turns[s].apply(z[s]);
             // (A NaN is no lost value: it stays one. An infinity makes `most` one.)
-            plain = plain && most * turn_max[s] < 0x1p100f;
+            most *= turns[s].largest;
+            plain = plain && most < 0x1p100f && most * factor[s] < 0x1p100f;
             if (__any_sync(0xFFFFFFFFu, src[s] != nullptr && !plain)) exact(s, 1.0f);
         }
         // f32 bits of the largest finite magnitude.
@@ -271,12 +367,14 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
             float most = 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
+                float row = 0.0f;
 #pragma unroll
                 for (int x = 0; x < 2 * kPairs; ++x) {
                     float v0, v1;
                     unpair_f32(z[s][x], v0, v1);
-                    most = fmaxf(most, fmaxf(fabsf(v0), fabsf(v1)));
+                    row = fmaxf(row, fmaxf(fabsf(v0), fabsf(v1)));
                 }
+                most = fmaxf(most, row * factor[s]);
             }
             if (__any_sync(0xFFFFFFFFu, most == INFINITY)) {
                 most = 0.0f;
@@ -288,7 +386,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
                         unpair_f32(z[s][x], v[0], v[1]);
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            if (fabsf(v[y]) < INFINITY) most = fmaxf(most, fabsf(v[y]));
+                            if (fabsf(v[y]) < INFINITY) most = fmaxf(most, fabsf(v[y]) * factor[s]);
                             else v[y] = NAN;  // an infinity has no code
                         }
                         z[s][x] = pair_f32(v[0], v[1]);
@@ -302,12 +400,14 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
             float most = 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
+                float row = 0.0f;
 #pragma unroll
                 for (int x = 0; x < kPairs; ++x) {
                     float v0, v1;
                     unpair_f32(off[s][x], v0, v1);
-                    most = fmaxf(most, fmaxf(v0, v1) * turn_max[s]);
+                    row = fmaxf(row, fmaxf(v0, v1));
                 }
+                most = fmaxf(most, row * (turns[s].largest * factor[s]));
             }
             most_off = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
         }
@@ -365,7 +465,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
         const uint32_t scale_bits = __float_as_uint(scale);
         const bool power = (scale_bits & 0x7FFFFFu) == 0 && scale_bits >= 0x00800000u;
         const float inv = __uint_as_float((254u << 23) - scale_bits);  // of a power of two: exponents add up to 254
-        const Pair inv2 = pair_f32(inv, inv), minus2 = pair_f32(-1.0f, -1.0f);
+        const Pair minus2 = pair_f32(-1.0f, -1.0f);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             uint32_t w[2 * VEC / 4];
@@ -376,22 +476,24 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
                 return pack_e4m3x4(v[0], v[1], v[2], v[3]);
             };
             bool same = power;
+            const float by = factor[s] * inv;
+            const Pair by2 = pair_f32(by, by);
             if (is_k) {
-                const float unit = inv * (kOff * turn_max[s]);
+                const float unit = by * (kOff * turns[s].largest);
                 const Pair unit2 = pair_f32(unit, unit);
                 Pair e[kPairs];
 #pragma unroll
                 for (int x = 0; x < kPairs; ++x) e[x] = mul_pair(off[s][x], unit2);
 #pragma unroll
                 for (int k = 0; k < 2 * VEC / 4; ++k) {
-                    const Pair v0 = mul_pair(z[s][2 * k], inv2), v1 = mul_pair(z[s][2 * k + 1], inv2);
+                    const Pair v0 = mul_pair(z[s][2 * k], by2), v1 = mul_pair(z[s][2 * k + 1], by2);
                     const Pair e0 = e[2 * k % kPairs], e1 = e[(2 * k + 1) % kPairs];
                     w[k] = pack(add_pair(v0, e0), add_pair(v1, e1));
                     same = same && w[k] == pack(fma_pair(e0, minus2, v0), fma_pair(e1, minus2, v1));
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(mul_pair(z[s][2 * k], inv2), mul_pair(z[s][2 * k + 1], inv2));
+                for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(mul_pair(z[s][2 * k], by2), mul_pair(z[s][2 * k + 1], by2));
             }
             if (__any_sync(0xFFFFFFFFu, !same)) {
                 exact(s, scale);
@@ -413,18 +515,19 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
 
 template <typename TIN, int HD, int U>
 __global__ void __launch_bounds__(kQkWarps *kWarp, 4) qk_norm_rope_kv8_kernel(const Kv8AppendParams p) {
-    // The CTAs that append lie evenly among those that take q: their long chains of
-    // dependent steps run beside loads and stores that bound the rest.
-    const long long unit = blockIdx.x * p.kv_blocks / gridDim.x;
-    if ((blockIdx.x + 1) * p.kv_blocks / gridDim.x == unit) {
-        qk_norm_rope_rows<TIN, TIN, HD, U>(p.q, blockIdx.x - unit);
+    // The CTAs that append lie among those that take q, one to every `every`: their
+    // long chains of dependent steps run beside loads and stores that bound the rest.
+    const uint32_t unit = blockIdx.x / p.every;
+    if (unit >= p.kv_blocks || unit * p.every != blockIdx.x) {
+        kv8_q_rows<TIN, HD, U>(p.q, blockIdx.x - min(unit + (unit * p.every < blockIdx.x), p.kv_blocks));
         return;
     }
     __shared__ Kv8Members m;
     const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-    const int splits = (2 * p.kv_heads + p.parts - 1) / p.parts;  // of a group's parts
-    const int part0 = (int)(unit % splits) * p.parts, part1 = min(part0 + p.parts, 2 * p.kv_heads);
-    const int r0 = (int)(unit / splits * p.group_rows);
+    const uint32_t splits = (2 * p.kv_heads + p.parts - 1) / p.parts;  // of a group's parts
+    const uint32_t rows_at = splits == 1 ? unit : unit / splits;
+    const int part0 = (int)(unit - rows_at * splits) * p.parts, part1 = min(part0 + p.parts, 2 * p.kv_heads);
+    const int r0 = (int)rows_at * p.group_rows;
     pdl_wait();
     pdl_launch_dependents();
     const int group = min(p.group_rows, p.q.tokens - r0);

@@ -52,12 +52,15 @@ int launch_append(cheetah::Kv8AppendParams p, cudaStream_t stream) {
     p.group_rows = p.q.tokens >= 2 * sms * cheetah::kKv8MaxGroup ? cheetah::kKv8MaxGroup : 4;
     const long long groups = ((long long)p.q.tokens + p.group_rows - 1) / p.group_rows;
     p.parts = p.group_rows == 4 ? (int)std::min(parts, std::max(1ll, groups * parts / (4 * sms))) : (int)parts;
-    p.kv_blocks = groups * ((parts + p.parts - 1) / p.parts);
-    CH_REQUIRE(q_blocks + p.kv_blocks <= 0x7FFFFFFFll, "cheetah_cuda_op_qk_norm_rope_kv8: too many rows");
+    const long long kv_blocks = groups * ((parts + p.parts - 1) / p.parts), blocks = q_blocks + kv_blocks;
+    // Warps are numbered in 31 bits.
+    CH_REQUIRE(blocks <= 0x7FFFFFFFll / cheetah::kQkWarps, "cheetah_cuda_op_qk_norm_rope_kv8: too many rows");
+    p.kv_blocks = (uint32_t)kv_blocks;
+    p.every = (uint32_t)(blocks / kv_blocks);
     auto kernel = p.q.steps == 1  ? cheetah::qk_norm_rope_kv8_kernel<TIN, HD, 1>
                   : p.q.steps <= 3 ? cheetah::qk_norm_rope_kv8_kernel<TIN, HD, 3>
                                    : cheetah::qk_norm_rope_kv8_kernel<TIN, HD, cheetah::kQkUnroll>;
-    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)(q_blocks + p.kv_blocks)), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream,
+    CH_CUDA_TRY(launch_ex(kernel, dim3((unsigned)blocks), dim3(cheetah::kQkWarps * cheetah::kWarp), 0, stream,
                           true, p));
     return 0;
 }

@@ -86,16 +86,15 @@ __device__ __forceinline__ void store_chunk(void *base, long long at, const floa
     }
 }
 
-// U: head groups loaded together; 1 where a warp has only one. block: of the
-// CTAs that share the rows.
+// U: head groups loaded together; 1 where a warp has only one.
 template <typename TIN, typename TKV, int HD, int U>
-__device__ __forceinline__ void qk_norm_rope_rows(const QkNormRopeParams &p, long long block) {
+__global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(const QkNormRopeParams p) {
     constexpr int VEC = 16 / sizeof(TIN);
     constexpr int kLanes = HD / 2 / VEC;        // lanes of a head
     constexpr int kHeads = kWarp / kLanes;      // heads a warp takes at a time
     const int lane = threadIdx.x % kWarp;
     const int c = lane % kLanes, sub = lane / kLanes;
-    const long long unit = block * kQkWarps + threadIdx.x / kWarp;
+    const long long unit = (long long)blockIdx.x * kQkWarps + threadIdx.x / kWarp;
     const int t = (int)(unit / p.row_units);
     const int step0 = (int)(unit % p.row_units) * p.steps;
     const int heads = p.q_heads + 2 * p.kv_heads;
@@ -201,11 +200,6 @@ __device__ __forceinline__ void qk_norm_rope_rows(const QkNormRopeParams &p, lon
             }
         }
     }
-}
-
-template <typename TIN, typename TKV, int HD, int U>
-__global__ void __launch_bounds__(kQkWarps *kWarp) qk_norm_rope_rows_kernel(const QkNormRopeParams p) {
-    qk_norm_rope_rows<TIN, TKV, HD, U>(p, blockIdx.x);
 }
 
 }  // namespace cheetah
