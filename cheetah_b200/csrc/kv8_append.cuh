@@ -8,13 +8,13 @@
 // with one s for the cells of a block (kKv8Block) and head. Bound by memory
 // where rows are many and by latency where they are few.
 //
-// A CTA looks among kv8_append's `group_rows` rows for blocks of one head of K or V:
-// the first row that has a block leads (which rows share one is found from the
-// slots of the 31 rows on either side). A warp holds kRows rows in registers
-// between the maximum and the codes, so a row is read once: blocks with no more new
-// rows than that are dealt out to the warps, the others are taken by all four
-// together. Only a block that holds earlier cells is read, and only its scale unless
-// that grows; then the codes ahead of the new ones are rounded again.
+// A CTA looks among `group_rows` rows for blocks: the first row that has a block leads
+// (which rows share one is found from the slots of the 31 rows on either side). A
+// warp holds kRows rows in registers between the maximum and the codes, so a row is
+// read once. The rows of short blocks lie side by side in a warp, each warp taking
+// other heads; a longer block all four warps take together, head by head. Only a
+// block that holds earlier cells is read, and only its scale unless that grows; then
+// the codes ahead of the new ones are rounded again.
 //
 // Codes decide between neighbours 1/8 or 1/16 apart, so a value next to the
 // border of two must not be moved over it by a rounding. k is computed in f32 with
@@ -63,12 +63,34 @@ struct Kv8Top {
 
 struct Kv8Members {
     int block[kKv8MaxGroup + 2 * kKv8Reach];   // cache block of each row around; -1: not appended
-    int row[kQkWarps][kKv8Block], cell[kQkWarps][kKv8Block];  // of the block at hand
-    Kv8Top top[3];                             // of the blocks that all warps take, in turn
+    int row[kQkWarps][kKv8Block], cell[kQkWarps][kKv8Block];  // of the rows at hand
+    int of[kQkWarps][kKv8Block];               // and, of short blocks, which block it is and its first new cell
+    Kv8Top top[3][kQkWarps];                   // of the parts that teams of warps take, in turn
 };
 
 __device__ __forceinline__ void store_codes(uint8_t *dst, const uint32_t (&w)[2]) { *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]); }
 __device__ __forceinline__ void store_codes(uint8_t *dst, const uint32_t (&w)[1]) { *reinterpret_cast<uint32_t *>(dst) = w[0]; }
+
+// Four codes times a power of two.
+__device__ __forceinline__ uint32_t kv8_rescale(uint32_t codes, float ratio) {
+    float v[4];
+    unpack_e4m3x4(codes, v);
+    return pack_e4m3x4(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
+}
+// Sixteen codes times old / scale, whatever these are.
+__device__ __noinline__ uint4 kv8_rescale_exact(uint4 codes, float old, float scale) {
+    const double ratio = (double)old / (double)scale;
+    uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+        float v[4];
+        unpack_e4m3x4(w[k], v);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] = round_to_odd((double)v[y] * ratio);
+        w[k] = pack_e4m3x4(v[0], v[1], v[2], v[3]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // VEC elements of a 16-byte chunk as f32 pairs.
 template <typename T, int VEC>
@@ -243,16 +265,22 @@ __device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint
     }
 }
 
-// The `count` rows of one block listed in rows and cells, of parts [part0, part1)
-// (K's heads, then V's), one after the other with the next one's loads under
-// way. all: this warp has kRows of them and the other warps the rest.
+// The `count` rows listed in rows and cells, of every part_step'th of parts [part0,
+// part1) (K's heads, then V's), one after the other with the next one's loads under
+// way. team > 0: they are one block's, as many warps have kRows each, and every warp
+// of the CTA is here (with as many parts: part0 may lie past the end). Else they
+// are all rows of one or several blocks (mixed: a row in a warp's side, kSide at
+// most); block and first are the lane's.
 template <typename TIN, int HD>
-__device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const int *rows, const int *cell_of, Kv8Top *tops, int &turn,
-                                                 int block, int count, int first, int part0, int part1, bool all) {
+__device__ __forceinline__ void kv8_append_rows(const Kv8AppendParams &p, const int *rows, const int *cell_of, Kv8Top (*tops)[kQkWarps], int &turn,
+                                                int block, int count, int first, int part0, int part1, int part_step, int team, bool mixed) {
     using C = Kv8Cfg<TIN, HD>;
     constexpr int VEC = C::kVec, kSide = C::kSide, kSteps = C::kSteps;
     const int lane = threadIdx.x % kWarp;
-    const int first_row = all ? threadIdx.x / kWarp * C::kRows : 0;
+    const bool all = team > 0;
+    const int warp = threadIdx.x / kWarp, in_team = all ? warp % team : 0, first_row = in_team * C::kRows;
+    // Of a warp whose part lies past the end, only the barriers.
+    const int rounds = (part1 - (all ? part0 - warp / team : part0) + part_step - 1) / part_step;
     const int c = lane % C::kLanes, sub = first_row + lane / C::kLanes;
     const int half = p.q.rotary_dim / 2;
     // As qk_norm_rope_rows: the chunks that are rotated against each other, or
@@ -261,6 +289,12 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
     const int rest = c * VEC - half;
     const int da = turned ? c * VEC : 2 * half + rest;
     const int db = turned ? half + c * VEC : 2 * half + (HD - 2 * half) / 2 + rest;
+    // Whether this lane's side has the first listed row of its block.
+    bool leader = true;
+    if (mixed) {
+        const int before = __shfl_up_sync(0xFFFFFFFFu, block, C::kLanes);
+        leader = block >= 0 && (lane < C::kLanes || before != block);
+    }
     const int blocks_per_page = p.q.page_tokens / kKv8Block;
     const int page = block / blocks_per_page, at_block = block - page * blocks_per_page;
     const TIN *src[kSteps];
@@ -272,7 +306,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
         src[s] = nullptr;
         rope_at[s] = -1;
         cell[s] = 0;
-        if (i < count) {
+        if (i < count && part0 < part1) {
             src[s] = static_cast<const TIN *>(p.q.qkv) + rows[i] * p.q.qkv_stride + (long long)p.q.q_heads * HD;
             cell[s] = cell_of[i];
             if (turned && part0 < p.kv_heads) rope_at[s] = (long long)p.q.positions[rows[i]] * half + da;
@@ -294,7 +328,8 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
     };
     uint4 raw[kSteps][2], next_raw[kSteps][2];
     load(part0, next_raw);
-    float next_old = first > 0 ? *scale_of(part0) : 0.0f;
+    const bool holds = first > 0 && (!mixed || src[0] != nullptr);
+    float next_old = holds && part0 < part1 ? *scale_of(part0) : 0.0f;
     // k's rotation with the norm's weights in it (Kv8Turn), and the largest of its
     // magnitudes.
     constexpr int kPairs = VEC / 2;
@@ -305,7 +340,9 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
         for (int s = 0; s < kSteps; ++s) turns[s].load(p.q, p.q.k_norm, rope_at[s], da, db);
     }
 #pragma unroll 1
-    for (int part = part0; part < part1; ++part) {
+    for (int round = 0; round < rounds; ++round) {
+        const int part = min(part0 + round * part_step, part1 - 1);
+        const bool live = part0 + round * part_step < part1;
         const bool is_k = part < p.kv_heads;
         const float old = next_old;
 #pragma unroll
@@ -313,9 +350,9 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
             raw[s][0] = next_raw[s][0];
             raw[s][1] = next_raw[s][1];
         }
-        if (part + 1 < part1) {
-            load(part + 1, next_raw);
-            if (first > 0) next_old = *scale_of(part + 1);
+        if (part + part_step < part1) {
+            load(part + part_step, next_raw);
+            if (holds) next_old = *scale_of(part + part_step);
         }
         // Values over the row's factor (chunk a, then b), and what both of a pair of
         // turned ones are off by in units of kOff: the rotation's largest number of |a|
@@ -362,6 +399,19 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
             plain = plain && most < 0x1p100f && most * factor[s] < 0x1p100f;
             if (__any_sync(0xFFFFFFFFu, src[s] != nullptr && !plain)) exact(s, 1.0f);
         }
+        // The largest of the lanes whose rows are of this lane's block.
+        auto among = [&](uint32_t v) -> uint32_t {
+            if (!mixed) return __reduce_max_sync(0xFFFFFFFFu, v);
+#pragma unroll
+            for (int o = 1; o < C::kLanes; o <<= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+            uint32_t most = v;
+#pragma unroll
+            for (int o = C::kLanes; o < kWarp; o += C::kLanes) {
+                const uint32_t theirs = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+                if (__shfl_xor_sync(0xFFFFFFFFu, block, o) == block) most = max(most, theirs);
+            }
+            return most;
+        };
         // f32 bits of the largest finite magnitude.
         auto largest = [&]() -> uint32_t {
             float most = 0.0f;
@@ -393,7 +443,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
                     }
                 }
             }
-            return __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+            return among(__float_as_uint(most));
         };
         uint32_t top = largest(), most_off = 0;
         if (is_k) {
@@ -409,57 +459,56 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
                 }
                 most = fmaxf(most, row * (turns[s].largest * factor[s]));
             }
-            most_off = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+            most_off = among(__float_as_uint(most));
         }
-        Kv8Top *top_s = &tops[turn % 3], *next_top_s = &tops[(turn + 1) % 3];
-        ++turn;
+        Kv8Top *top_s = &tops[turn % 3][all ? warp / team : 0], *next_top_s = &tops[(turn + 1) % 3][warp];
+        turn += all;  // (the same in every warp)
         if (all) {
             if (lane == 0) {
                 atomicMax(&top_s->top, top);
                 if (is_k) atomicMax(&top_s->off, most_off);
             }
-            if (threadIdx.x == 0) *next_top_s = Kv8Top{0u, 0u, 0u};  // read two parts ago, written next after this barrier
+            if (lane == 0) *next_top_s = Kv8Top{0u, 0u, 0u};  // read two rounds ago, written next after this barrier
             __syncthreads();
             top = top_s->top;
             most_off = top_s->off;
         }
         float need = kv8_scale_for(top);
+        bool redone = false;
         if (is_k) {
             const float gap = __uint_as_float(most_off) * kOff, at = __uint_as_float(top);
-            if (!(gap < INFINITY) || kv8_scale_for(__float_as_uint(at + gap)) != kv8_scale_for(__float_as_uint(fmaxf(at - gap, 0.0f)))) {
+            const bool open = !(gap < INFINITY) || kv8_scale_for(__float_as_uint(at + gap)) != kv8_scale_for(__float_as_uint(fmaxf(at - gap, 0.0f)));
+            if (__any_sync(0xFFFFFFFFu, open)) {  // (not mixed: all lanes of the block)
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) exact(s, 1.0f);
                 top = largest();
-                if (all) {
-                    if (lane == 0) atomicMax(&top_s->exact, top);
-                    __syncthreads();
-                    top = top_s->exact;
-                }
+                if (all && lane == 0) atomicMax(&top_s->exact, top);
                 need = kv8_scale_for(top);
+                redone = true;
             }
         }
+        // (Every warp is here: another team's block may be open, and parts be of K and V.)
+        if (all && __syncthreads_or(redone) && redone) need = kv8_scale_for(top_s->exact);
         const long long head_at = (long long)page * p.kv_heads + (is_k ? part : part - p.kv_heads);
         uint8_t *cells = (is_k ? p.k_codes : p.v_codes) + (head_at * p.q.page_tokens + at_block * kKv8Block) * HD;
         const float scale = old > need && old < INFINITY ? old : need;
-        if (first > 0 && scale != old) {
-            const double ratio = (double)old / (double)scale;
+        // Who rounds held cells again: the team, the warp, or the block's first row's
+        // lanes (a mixed block's rows are neighbours).
+        const int held_at = all ? in_team * kWarp + lane : (mixed ? c : lane);
+        const int held_step = all ? team * kWarp : (mixed ? C::kLanes : kWarp);
+        if (first > 0 && scale != old && leader && live) {
+            // The quotient of two powers of two, and a code times it, are exact in f32.
+            const bool powers = ((__float_as_uint(old) | __float_as_uint(scale)) & 0x007FFFFFu) == 0 && old > 0.0f;
+            const float ratio = old / scale;
             uint4 *held = reinterpret_cast<uint4 *>(cells);
 #pragma unroll 1
-            for (int x = all ? threadIdx.x : lane; x < first * (HD / 16); x += all ? kQkWarps * kWarp : kWarp) {
+            for (int x = held_at; x < first * (HD / 16); x += held_step) {
                 const uint4 was = held[x];
-                uint32_t w[4] = {was.x, was.y, was.z, was.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float v[4];
-                    unpack_e4m3x4(w[k], v);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) v[y] = round_to_odd((double)v[y] * ratio);
-                    w[k] = pack_e4m3x4(v[0], v[1], v[2], v[3]);
-                }
-                held[x] = make_uint4(w[0], w[1], w[2], w[3]);
+                held[x] = powers ? make_uint4(kv8_rescale(was.x, ratio), kv8_rescale(was.y, ratio), kv8_rescale(was.z, ratio), kv8_rescale(was.w, ratio))
+                                 : kv8_rescale_exact(was, old, scale);
             }
         }
-        if (lane == 0 && first_row == 0 && scale != old) *scale_of(part) = scale;
+        if ((mixed ? c == 0 && leader : lane == 0 && in_team == 0) && scale != old && live) *scale_of(part) = scale;
         // Products by a power of two are exact; a scale that was not set here may be
         // none, and is divided by in 64 bits.
         const uint32_t scale_bits = __float_as_uint(scale);
@@ -500,7 +549,7 @@ __device__ __forceinline__ void kv8_append_block(const Kv8AppendParams &p, const
 #pragma unroll
                 for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(z[s][2 * k], z[s][2 * k + 1]);
             }
-            if (src[s] == nullptr) continue;
+            if (src[s] == nullptr || !live) continue;
             uint8_t *dst = cells + cell[s] * HD;
             uint32_t half_w[VEC / 4];
 #pragma unroll
@@ -542,7 +591,7 @@ __global__ void __launch_bounds__(kQkWarps *kWarp, 4) qk_norm_rope_kv8_kernel(co
         }
         m.block[threadIdx.x] = block;
     }
-    if (threadIdx.x < 3) m.top[threadIdx.x] = Kv8Top{0u, 0u, 0u};
+    if (threadIdx.x < 3 * kQkWarps) m.top[threadIdx.x / kQkWarps][threadIdx.x % kQkWarps] = Kv8Top{0u, 0u, 0u};
     __syncthreads();
     bool leads = false;
     if (lane < group) {
@@ -553,27 +602,52 @@ __global__ void __launch_bounds__(kQkWarps *kWarp, 4) qk_norm_rope_kv8_kernel(co
         leads = mine >= 0 && !again;
     }
     using C = Kv8Cfg<TIN, HD>;
-    int nth = 0, turn = 0, alone = 0;  // blocks of one warp so far, maxima of all warps
-    for (uint32_t left = __ballot_sync(0xFFFFFFFFu, leads); left; left &= left - 1) {
-        const int at = __ffs(left) - 1 + kKv8Reach;
-        const int block = m.block[at];
-        // The rows of the block and their cells (16 at most: cells are distinct).
-        const bool mine = m.block[at + lane] == block;  // at + lane stays within the group's reach
-        const uint32_t all = __ballot_sync(0xFFFFFFFFu, mine);
-        const int count = min(__popc(all), kKv8Block);
-        const bool together = count > C::kRows;
-        if (!together && nth++ % kQkWarps != warp) continue;
-        const int ordinal = __popc(all & ((1u << lane) - 1u));
-        int cell = kKv8Block;
-        if (mine && ordinal < kKv8Block) {
-            const int t = r0 + at - kKv8Reach + lane;
-            cell = p.q.slots[t] % kKv8Block;
-            m.row[warp][ordinal] = t;
-            m.cell[warp][ordinal] = cell;
+    int turn = 0;
+    int *row_s = m.row[warp], *cell_s = m.cell[warp], *of_s = m.of[warp];
+    // The rows of short blocks are gathered side by side in a warp, and each warp
+    // takes other heads of them; of a longer block teams of warps do.
+    uint32_t left = __ballot_sync(0xFFFFFFFFu, leads);
+    while (left) {
+        int rows = 0, block = -1, first = 0;
+        bool mixed = true;
+        while (left) {
+            const int at = __ffs(left) - 1 + kKv8Reach;
+            block = m.block[at];
+            // The rows of the block and their cells (16 at most: cells are distinct).
+            const bool mine = m.block[at + lane] == block;  // at + lane stays within the group's reach
+            const uint32_t all = __ballot_sync(0xFFFFFFFFu, mine);
+            const int count = min(__popc(all), kKv8Block);
+            if (rows > 0 && rows + count > C::kSide) break;
+            left &= left - 1;
+            const int ordinal = rows + __popc(all & ((1u << lane) - 1u));
+            int cell = kKv8Block;
+            if (mine && ordinal < kKv8Block) {
+                const int t = r0 + at - kKv8Reach + lane;
+                cell = p.q.slots[t] % kKv8Block;
+                row_s[ordinal] = t;
+                cell_s[ordinal] = cell;
+            }
+            first = (int)__reduce_min_sync(0xFFFFFFFFu, (uint32_t)cell);
+            if (mine && ordinal < kKv8Block) of_s[ordinal] = at << 8 | first;
+            rows += count;
+            if (rows >= C::kSide) {
+                mixed = rows == C::kSide;
+                break;
+            }
         }
-        const int first = (int)__reduce_min_sync(0xFFFFFFFFu, (uint32_t)cell);
         __syncwarp();
-        kv8_append_block<TIN, HD>(p, m.row[warp], m.cell[warp], m.top, together ? turn : alone, block, count, first, part0, part1, together);
+        int team = 0, from = part0 + warp, step = kQkWarps;
+        if (mixed) {
+            const int side = lane / C::kLanes;
+            block = side < rows ? m.block[of_s[side] >> 8] : -1;
+            first = side < rows ? of_s[side] & 0xFF : 0;
+        } else if (rows > C::kRows) {
+            team = rows > 2 * C::kRows ? kQkWarps : 2;
+            from = part0 + warp / team;
+            step = kQkWarps / team;
+        }
+        if (team > 0 || from < part1)
+            kv8_append_rows<TIN, HD>(p, row_s, cell_s, m.top, turn, block, rows, first, from, part1, step, team, mixed);
         __syncwarp();  // before the lists are written again
     }
 }

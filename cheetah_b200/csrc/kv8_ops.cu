@@ -45,13 +45,14 @@ int launch_append(cheetah::Kv8AppendParams p, cudaStream_t stream) {
     p.q.steps = (long long)p.q.tokens * steps >= 48ll * cheetah::sm_count(device) ? steps : 1;
     p.q.row_units = (steps + p.q.steps - 1) / p.q.steps;
     const long long q_blocks = ((long long)p.q.tokens * p.q.row_units + cheetah::kQkWarps - 1) / cheetah::kQkWarps;
-    // Rows among which a CTA looks for blocks, and how many of their heads it takes:
-    // sixteen and all where that gives every SM two CTAs, else four, and as many
-    // heads as leave some four CTAs for every SM.
+    // Rows among which a CTA looks for blocks: sixteen where that gives every SM two
+    // CTAs, else four. Their heads are shared by as many CTAs as there is room for
+    // beside q's (four on an SM), each with four at least, one for each of its warps.
     const long long sms = cheetah::sm_count(device), parts = 2ll * p.kv_heads;
     p.group_rows = p.q.tokens >= 2 * sms * cheetah::kKv8MaxGroup ? cheetah::kKv8MaxGroup : 4;
     const long long groups = ((long long)p.q.tokens + p.group_rows - 1) / p.group_rows;
-    p.parts = p.group_rows == 4 ? (int)std::min(parts, std::max(1ll, groups * parts / (4 * sms))) : (int)parts;
+    const long long splits = std::max(1ll, std::min((parts + cheetah::kQkWarps - 1) / cheetah::kQkWarps, (4 * sms - q_blocks) / groups));
+    p.parts = (int)((parts + splits - 1) / splits);
     const long long kv_blocks = groups * ((parts + p.parts - 1) / p.parts), blocks = q_blocks + kv_blocks;
     // Warps are numbered in 31 bits.
     CH_REQUIRE(blocks <= 0x7FFFFFFFll / cheetah::kQkWarps, "cheetah_cuda_op_qk_norm_rope_kv8: too many rows");
