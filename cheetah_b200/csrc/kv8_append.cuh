@@ -224,12 +224,13 @@ __device__ __forceinline__ void kv8_q_rows(const QkNormRopeParams &p, uint32_t b
     }
 }
 
-// Quotients by `scale` in 64 bits, rounded to odd, of the two chunks of a row that
-// a lane has: of k (is_k), or of the values as they are. All lanes of a warp call;
-// `at` is the offset into the rotary table, or negative.
+// Quotients by `scale` in 64 bits, rounded to odd, of those elements of the two
+// chunks that a lane has of a row whose bit is set (chunk b's from bit VEC on): of k
+// (is_k), or of the values as they are. All lanes of a warp call; `at` is the offset
+// into the rotary table, or negative.
 template <typename TIN, int HD>
 __device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint4 r0, uint4 r1, int da, int db, long long at, float scale,
-                                       float *out) {
+                                       uint32_t which, float *out) {
     using C = Kv8Cfg<TIN, HD>;
     constexpr int VEC = C::kVec;
     float wide[2][VEC];
@@ -241,27 +242,32 @@ __device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint
     const double by = (double)__uint_as_float((254u << 23) - bits);  // 1 / scale, where that is a power of two
     double inv = 1.0;
     if (normed) {
-        double ss = 0.0;
+        double ss[2] = {0.0, 0.0};
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) ss = fma((double)wide[0][x], (double)wide[0][x], fma((double)wide[1][x], (double)wide[1][x], ss));
+        for (int x = 0; x < VEC; ++x) {
+            ss[0] = fma((double)wide[0][x], (double)wide[0][x], ss[0]);
+            ss[1] = fma((double)wide[1][x], (double)wide[1][x], ss[1]);
+        }
+        ss[0] += ss[1];
 #pragma unroll
-        for (int o = C::kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-        inv = 1.0 / sqrt(ss * (1.0 / HD) + (double)p.q.eps);
+        for (int o = C::kLanes / 2; o > 0; o >>= 1) ss[0] += __shfl_xor_sync(0xFFFFFFFFu, ss[0], o);
+        inv = 1.0 / sqrt(ss[0] * (1.0 / HD) + (double)p.q.eps);
     }
 #pragma unroll 1
-    for (int x = 0; x < VEC; ++x) {
-        double a = (double)wide[0][x], b = (double)wide[1][x];
+    for (; which; which &= which - 1) {
+        const int i = __ffs(which) - 1, x = i % VEC;
+        const bool second = i >= VEC;
+        // This element and the one that it is turned with.
+        double a = (double)wide[second][x], b = (double)wide[!second][x];
         if (normed) {
-            a *= inv * (double)p.q.k_norm[da + x];
-            b *= inv * (double)p.q.k_norm[db + x];
+            a *= inv * (double)p.q.k_norm[(second ? db : da) + x];
+            b *= inv * (double)p.q.k_norm[(second ? da : db) + x];
         }
         if (is_k && at >= 0) {
-            const double t = a, cs = (double)p.q.rope_cos[at + x], sn = (double)p.q.rope_sin[at + x];
-            a = t * cs - b * sn;
-            b = b * cs + t * sn;
+            const double cs = (double)p.q.rope_cos[at + x], sn = (double)p.q.rope_sin[at + x];
+            a = a * cs + b * (second ? sn : -sn);
         }
-        out[x] = round_to_odd(power ? a * by : a / (double)scale);
-        out[VEC + x] = round_to_odd(power ? b * by : b / (double)scale);
+        out[i] = round_to_odd(power ? a * by : a / (double)scale);
     }
 }
 
@@ -364,7 +370,7 @@ __device__ __forceinline__ void kv8_append_rows(const Kv8AppendParams &p, const 
         float factor[kSteps];
         auto exact = [&](int s, float scale) {  // all lanes of a warp
             float t[2 * VEC];
-            kv8_exact<TIN, HD>(p, is_k, raw[s][0], raw[s][1], da, db, rope_at[s], scale, t);
+            kv8_exact<TIN, HD>(p, is_k, raw[s][0], raw[s][1], da, db, rope_at[s], scale, (1u << 2 * VEC) - 1u, t);
 #pragma unroll
             for (int x = 0; x < 2 * kPairs; ++x) z[s][x] = pair_f32(t[2 * x], t[2 * x + 1]);
 #pragma unroll
@@ -524,7 +530,7 @@ __device__ __forceinline__ void kv8_append_rows(const Kv8AppendParams &p, const 
                 unpair_f32(hi, v[2], v[3]);
                 return pack_e4m3x4(v[0], v[1], v[2], v[3]);
             };
-            bool same = power;
+            uint32_t open = power ? 0u : (1u << 2 * VEC) - 1u;  // elements whose code is not decided yet
             const float by = factor[s] * inv;
             const Pair by2 = pair_f32(by, by);
             if (is_k) {
@@ -538,16 +544,29 @@ __device__ __forceinline__ void kv8_append_rows(const Kv8AppendParams &p, const 
                     const Pair v0 = mul_pair(z[s][2 * k], by2), v1 = mul_pair(z[s][2 * k + 1], by2);
                     const Pair e0 = e[2 * k % kPairs], e1 = e[(2 * k + 1) % kPairs];
                     w[k] = pack(add_pair(v0, e0), add_pair(v1, e1));
-                    same = same && w[k] == pack(fma_pair(e0, minus2, v0), fma_pair(e1, minus2, v1));
+                    const uint32_t differ = w[k] ^ pack(fma_pair(e0, minus2, v0), fma_pair(e1, minus2, v1));
+                    if (differ) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) open |= (differ >> (8 * y) & 0xFFu ? 1u : 0u) << (4 * k + y);
+                    }
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(mul_pair(z[s][2 * k], by2), mul_pair(z[s][2 * k + 1], by2));
             }
-            if (__any_sync(0xFFFFFFFFu, !same)) {
-                exact(s, scale);
+            if (__any_sync(0xFFFFFFFFu, open)) {
+                float t[2 * VEC];
+                uint32_t codes[2 * VEC / 4];
+                kv8_exact<TIN, HD>(p, is_k, raw[s][0], raw[s][1], da, db, rope_at[s], scale, open, t);
 #pragma unroll
-                for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = pack(z[s][2 * k], z[s][2 * k + 1]);
+                for (int k = 0; k < 2 * VEC / 4; ++k) codes[k] = w[k];
+#pragma unroll 1
+                for (; open; open &= open - 1) {
+                    const int i = __ffs(open) - 1;
+                    reinterpret_cast<uint8_t *>(codes)[i] = (uint8_t)pack_e4m3x2(t[i], t[i]);
+                }
+#pragma unroll
+                for (int k = 0; k < 2 * VEC / 4; ++k) w[k] = codes[k];
             }
             if (src[s] == nullptr || !live) continue;
             uint8_t *dst = cells + cell[s] * HD;
