@@ -11,7 +11,7 @@
 // is split into e4m3 parts that are multiplied one after the other: q, over a
 // power of two of its row, into two (exact for elements within 2^-10 of the
 // row's largest, else off by 2^-18 of that), the weights times V's scale into
-// two as well (2^-8, as bf16 holds, down to the smallest step of e4m3). K's scale
+// two as well (2^-8, as bf16 holds, or 2^-15 of the row's largest). K's scale
 // joins the factor of the scores. m follows t_j + log2(vs), so the weights fill
 // e4m3's range however V's scales differ.
 //
@@ -50,9 +50,11 @@ namespace cheetah {
 constexpr int kKv8Keys = 128;     // keys per tile
 constexpr int kKv8MaxCtas = kTreeMaxCtas;
 constexpr int kKv8Queue = 4;      // segments the scheduler may be ahead
-// Weights are scaled to at most 2^kKv8TopLog2 when a row's reference is set, and
-// it moves when one would pass 2^kKv8RoomLog2 times that (e4m3 ends at 448).
-constexpr float kKv8TopLog2 = 7.0f, kKv8RoomLog2 = 1.75f;
+// Weights are scaled to at most 2^kKv8TopLog2 when a row's reference is set, and it
+// moves when one would pass 2^kKv8RoomLog2 times that (e4m3 ends at 448 = 2^8.8). A
+// move costs a pass over O, and in 32 rows one moves soon: with 7 and 1.75 nearly
+// every tile of a prompt had one.
+constexpr float kKv8TopLog2 = 6.0f, kKv8RoomLog2 = 2.75f;
 
 struct Kv8AttnParams {
     const uint16_t *q;

@@ -449,10 +449,8 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                     const float w0 = fast_exp2(arg[r]), w1 = fast_exp2(arg[r + 1]);
                     l[r] = fmaf(w0, inv_vs, l[r]);
                     l[r + 1] = fmaf(w1, inv_vs, l[r + 1]);
-                    const uint32_t hi = pack_e4m3x2(w0, w1);
-                    float h0, h1;
-                    unpack_e4m3x2(hi, h0, h1);
-                    const uint32_t lo = pack_e4m3x2(w0 - h0, w1 - h1);
+                    uint32_t hi, lo;
+                    split_e4m3x2(w0, w1, hi, lo);
                     const uint32_t at0 = p_row[r % 8] + p_at + r / 8 * 1024, at1 = p_row[(r + 1) % 8] + p_at + (r + 1) / 8 * 1024;
                     st_shared_u8(at0, hi);
                     st_shared_u8(at1, hi >> 8);

@@ -26,10 +26,6 @@ constexpr int kManyRows = 128;
 // As kTreeLeanRegs, kTreeSoftmaxRegs: 128 x 64 + 256 x 216 is below 384 x 168.
 constexpr int kManyLeanRegs = 64, kManySoftmaxRegs = 216;
 static_assert(128 * kManyLeanRegs + 256 * kManySoftmaxRegs <= kManyThreads * 168, "register split");
-// The first part is cut by arithmetic that knows no subnormal codes; one bit more
-// of range makes up for it.
-constexpr float kManyTopLog2 = 8.0f, kManyRoomLog2 = 0.75f;
-
 template <int HD>
 struct Kv8Many {
     static constexpr int kTile = kKv8Keys * HD;   // one K or V tile, or one part of a Q tile
@@ -59,9 +55,6 @@ template <int HD>
 constexpr size_t kv8_many_smem() {
     return (size_t)Kv8Many<HD>::kBytes + ((sizeof(Kv8ManyShared<Kv8Many<HD>::kStages>) + 127) & ~size_t(127));
 }
-
-// e rounded to 4 bits of significand (ties away from zero), the first part of a weight.
-__device__ __forceinline__ float kv8_cut(float e) { return __uint_as_float((__float_as_uint(e) + 0x00080000u) & 0xFFF00000u); }
 
 template <int HD>
 __global__ void __launch_bounds__(kManyThreads, 1)
@@ -336,7 +329,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             top = fmaxf(top, fmaf(fmaxf(mx[0], mx[1]), factor[4 * half + b], add[4 * half + b]));
                         }
                     }
-                    const bool far = top > m_run + kManyRoomLog2;
+                    const bool far = top > m_run + kKv8RoomLog2;
                     if (__any_sync(0xFFFFFFFFu, far)) {
                         const float m_new = far ? ceilf(top) : m_run;
                         const float f = far ? exp2f(m_run - m_new) : 1.0f;  // 0 from -inf
@@ -354,7 +347,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             }
                         }
                     }
-                    const float base = kManyTopLog2 - (m_run == -INFINITY ? 0.0f : m_run);
+                    const float base = kKv8TopLog2 - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll
                     for (int half = 1; half >= 0; --half) {
                         if (half == 0) load(0);
@@ -368,19 +361,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                 unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll
                                 for (int x = 0; x < 4; ++x) {
-                                    float e[4], cut[4];
+                                    uint32_t part[2][2];
 #pragma unroll
                                     for (int y = 0; y < 2; ++y) {
                                         const int k = 16 * at16 + 4 * x + 2 * y;
-                                        unpair_f32(fma_pair(pair_f32(s[k], s[k + 1]), f2, a2), e[2 * y], e[2 * y + 1]);
-                                        e[2 * y] = fast_exp2(e[2 * y]);
-                                        e[2 * y + 1] = fast_exp2(e[2 * y + 1]);
-                                        sums[y] = add_pair(sums[y], pair_f32(e[2 * y], e[2 * y + 1]));
-                                        cut[2 * y] = kv8_cut(e[2 * y]);
-                                        cut[2 * y + 1] = kv8_cut(e[2 * y + 1]);
+                                        float e0, e1;
+                                        unpair_f32(fma_pair(pair_f32(s[k], s[k + 1]), f2, a2), e0, e1);
+                                        e0 = fast_exp2(e0);
+                                        e1 = fast_exp2(e1);
+                                        sums[y] = add_pair(sums[y], pair_f32(e0, e1));
+                                        split_e4m3x2(e0, e1, part[0][y], part[1][y]);
                                     }
-                                    hi[4 * h + x] = pack_e4m3x4(cut[0], cut[1], cut[2], cut[3]);
-                                    lo[4 * h + x] = pack_e4m3x4(e[0] - cut[0], e[1] - cut[1], e[2] - cut[2], e[3] - cut[3]);
+                                    hi[4 * h + x] = part[0][0] | part[0][1] << 16;
+                                    lo[4 * h + x] = part[1][0] | part[1][1] << 16;
                                 }
                                 float s0, s1;
                                 unpair_f32(add_pair(sums[0], sums[1]), s0, s1);

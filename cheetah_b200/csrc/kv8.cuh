@@ -26,6 +26,21 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
     return r;
 }
+// Two values as two e4m3 parts each, hi + lo: through f16, in which what hi leaves
+// off is exact.
+__device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    uint16_t h, l;
+    asm("{\n\t.reg .b32 w, r;\n\t"
+        "cvt.rn.f16x2.f32 w, %3, %2;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 %0, w;\n\t"
+        "cvt.rn.f16x2.e4m3x2 r, %0;\n\t"
+        "sub.f16x2 w, w, r;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 %1, w;\n\t}"
+        : "=h"(h), "=h"(l)
+        : "f"(a), "f"(b));
+    hi = h;
+    lo = l;
+}
 __device__ __forceinline__ void unpack_e4m3x2(uint32_t w, float &a, float &b) {
     asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}" : "=f"(a), "=f"(b) : "r"(e4m3x2_to_f16x2(w)));
 }

@@ -570,7 +570,7 @@ CHEETAH_CUDA_API int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *args, vo
  * sequence with seq_lens[b] < n gives zeros. Scales must be positive where a
  * row sees the block. Sums and statistics are f32; the softmax weights, times
  * V's scale, enter the products as two e4m3 parts (about 8 bits, as bf16
- * holds, down to 2^-17 of a row's largest such product). If a wait inside the
+ * holds, or 2^-15 of a row's largest such product). If a wait inside the
  * kernel gives up, every row is NaN.
  *
  * `workspace` holds partial results between the launches of a call:

@@ -85,8 +85,9 @@ def attend(q, k, v, v_codes, v_scales, seen):
     exponential, rescaling) on either side of the quotient. Weights enter the
     second product times V's scale as two e4m3 parts: off by 2^-8 of themselves
     (a part is off by 2^-4 of what it rounds), or by half the codes' smallest
-    step, 2^-10, where the row's largest lies at 2^6 or above: 2^-16 of that, times
-    the code of V. The sum over L keys L 2^-23; the output 2^-8 of the value."""
+    step, 2^-10, where the row's largest lies at 2^5 or above (a row's reference is
+    set so that the largest of it lies in (2^5, 2^6], and moves before one passes
+    2^8.75): 2^-15 of that, times the code of V. The sum over L keys L 2^-23; the output 2^-8 of the value."""
     D = q.shape[1]
     s = (q @ k.T / math.sqrt(D)).masked_fill(~seen, -math.inf)
     p = torch.softmax(s, 1)
@@ -95,7 +96,7 @@ def attend(q, k, v, v_codes, v_scales, seen):
     sums = torch.where(seen, (q.abs() @ k.abs().T) * D * 2.0 ** -23
                        + q.abs().amax(1, keepdim=True) * k.abs().sum(1) * 2.0 ** -19, torch.zeros_like(p)).amax(1, keepdim=True)
     delta = sums / math.sqrt(D) + 2.0 ** -20
-    step = (p * v_scales).amax(1, keepdim=True) * 2.0 ** -16 * (seen.double() @ v_codes.abs())
+    step = (p * v_scales).amax(1, keepdim=True) * 2.0 ** -15 * (seen.double() @ v_codes.abs())
     return o, (mag * (2.0 ** -8 + 2 * delta + k.shape[0] * 2.0 ** -23) + step) * 1.01 + o.abs() * 2.0 ** -8
 
 
