@@ -14,6 +14,14 @@
 // differences nearly, and a running sum over 10^5 weights in f32 would move the
 // borders between tokens by more than many of them are wide. A sum's order is
 // fixed by the launch's shape.
+//
+// A short call is a chain of dependent reads (the starts, the tokens, their
+// probabilities, the row, the sums' exchange, one chunk again): 7.8 us for one
+// sequence of 5 rows over 151936 tokens, 7.5 us for 8. With many sequences it is
+// bytes, of reads whose latency the lanes must cover: 96 sequences over 152064
+// tokens, 58 MB of p and up to as much of q, take 23.3 us. Four vectors of each row
+// in flight per lane beat two (33.8 us) and eight (29.3 us, whose registers leave
+// two CTAs an SM).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -26,7 +34,8 @@ constexpr int kVdThreads = 256;
 constexpr int kVdWarps = kVdThreads / kWarp;
 constexpr int kVdMaxCluster = 16;
 constexpr int kVdMaxChunks = 1024;  // of a CTA
-constexpr int kVdLoads = 2;         // vectors of p (and of q) in flight per lane
+constexpr int kVdLoads = 4;         // vectors of p (and of q) in flight per lane
+constexpr int kVdResident = 3;      // CTAs of an SM that run at once
 
 struct VerifyDraftsParams {
     const float *target, *draft;
@@ -104,7 +113,7 @@ __device__ __forceinline__ double vd_warp_scan(double v) {
     return v;
 }
 
-__global__ void __launch_bounds__(kVdThreads) verify_drafts_kernel(const VerifyDraftsParams p) {
+__global__ void __launch_bounds__(kVdThreads, kVdResident) verify_drafts_kernel(const VerifyDraftsParams p) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ double chunk_sum[kVdMaxChunks];
