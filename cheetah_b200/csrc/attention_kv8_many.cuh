@@ -9,13 +9,18 @@
 // and 1 load K and V tiles, warp 2 issues the MMAs, warp 3 cuts the share into
 // segments, warps 4-11 are two softmax groups with a row per thread. With two row
 // tiles the groups share each key tile, with one they take alternate key tiles and
-// join at the end.
+// join at the end. An item of up to 64 (32) rows fills its tile with two (four)
+// copies of them: each copy weighs a half (quarter) of a tile's keys, the others'
+// weights being 0 in its rows, and the copies join as the groups do. So the four warps
+// of a group always share the softmax; the products cost what they cost anyway.
 //
 // A block's 16 keys share their scales: the scores' factor is one number per row
 // and block, and log2 of V's scale is added to the exponents, so a weight is one
 // fused operation and one exponential; the sum l takes a block's weights divided by
 // its scale again.
 #pragma once
+
+#include <type_traits>
 
 #include "attention_kv8.cuh"
 
@@ -214,7 +219,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + lane_off + grp * kKv8Keys;
         const uint32_t o_addr = tmem + lane_off + C::kOCol + grp * HD;
-        const int node_of_r = r / p.group, head_of_r = r % p.group;
         uint32_t s_phase = 0, done_phase = 0, x_phase = 0;
         for (int seg = 0; next(seg); ++seg) {
             const Kv8Segment &g = sh.queue[seg % kKv8Queue];
@@ -222,11 +226,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const bool two = g.nodes > p.tile_nodes;
             const int jobs = two ? 2 * tiles : tiles;
             const int tile_node = two ? grp * p.tile_nodes : 0;  // first of this group's rows
+            // The copies of its rows that the tile holds, one after the other; this
+            // thread has row `item_row` and, of every key tile, keys `key_part` * part_rows on.
+            const int rows = min(g.nodes, p.tile_nodes) * p.group;
+            const int part_rows = rows <= 32 ? 32 : (rows <= 64 ? 64 : kManyRows);
+            const int item_row = r & (part_rows - 1), key_part = r / part_rows;
+            const int node_of_r = item_row / p.group, head_of_r = item_row % p.group;
             const int node = tile_node + node_of_r;
             const bool live = node_of_r < p.tile_nodes && node < g.nodes;
             uint16_t *out_row = p.out + ((long long)(g.row0 + node) * p.q_heads + g.kvh * p.group + head_of_r) * HD;
             if (jobs == 0) {
-                if (live && (two || grp == 0)) {
+                if (live && key_part == 0 && (two || grp == 0)) {
 #pragma unroll
                     for (int i = 0; i < HD / 8; ++i) reinterpret_cast<uint4 *>(out_row)[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
@@ -241,7 +251,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const int c = lane % kCells;
 #pragma unroll 2
                 for (int i = 0; i < kWarp; i += kRowsAt) {
-                    const int x = quad * 32 + i + lane / kCells, n = x / p.group, h = x - n * p.group;
+                    const int x = quad * 32 + i + lane / kCells, y = x & (part_rows - 1), n = y / p.group, h = y - n * p.group;
                     uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
                     if (n < p.tile_nodes && tile_node + n < g.nodes) {
                         const uint4 *src = reinterpret_cast<const uint4 *>(p.q + (long long)(g.row0 + tile_node + n) * p.q_stride +
@@ -287,46 +297,46 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     if (!holds || j > first_pos || (p.window > 0 && j >= p.sinks && j <= last_pos - (long long)p.window))
                         kv8_clean_v<HD>(ring + (2 * buf + 1) * C::kTile + r * HD, holds, &sh.non_finite);
                 }
-                // Scales: lane b % 8 works out log2 and the inverse of V's for block b.
+                // log2 and the inverse of V's scales: lane b % 8 works out those of block b.
                 const float vs = sh.scales[buf][8 + (lane & 7)];
                 const float my_log = __log2f(vs), my_inv = 1.0f / vs;
-                const float4 ks4[2] = {*reinterpret_cast<const float4 *>(&sh.scales[buf][0]), *reinterpret_cast<const float4 *>(&sh.scales[buf][4])};
-                const float ks[8] = {ks4[0].x, ks4[0].y, ks4[0].z, ks4[0].w, ks4[1].x, ks4[1].y, ks4[1].z, ks4[1].w};
                 ok = wait(sh.s_full[grp], s_phase);
                 if (!ok) break;
                 s_phase ^= 1;
                 tc_fence_after();
-                if (warp_live) {
-                    // Scores of 64 keys at a time: the maxima of both halves first, then
-                    // the weights of the second and, read once more, of the first.
-                    float s[64];
-                    float factor[8], add[8];
-                    auto load = [&](int half) {
-                        tmem_ld32_nowait(s_addr + 64 * half, s);
-                        tmem_ld32_nowait(s_addr + 64 * half + 32, s + 32);
+                // Keys [k0, k0 + KEYS) of the tile: their maximum first, then their weights.
+                // Scores are read 64 keys at a time; of 128, the first half twice.
+                auto weigh = [&](auto keys, const int k0, const uint32_t (&vis)[decltype(keys)::value / 32]) {
+                    constexpr int KEYS = decltype(keys)::value, kPieces = KEYS > 64 ? 2 : 1, kPiece = KEYS / kPieces;
+                    float s[kPiece];
+                    float factor[KEYS / 16], add[KEYS / 16];
+                    auto load = [&](int piece) {
+#pragma unroll
+                        for (int c = 0; c < kPiece / 32; ++c) tmem_ld32_nowait(s_addr + k0 + kPiece * piece + 32 * c, s + 32 * c);
                         tmem_wait_ld();
                         if (masked) {
 #pragma unroll
-                            for (int k = 0; k < 64; ++k) s[k] = ((half == 0 ? vis[k / 32] : vis[2 + k / 32]) >> (k % 32) & 1) ? s[k] : -INFINITY;
+                            for (int k = 0; k < kPiece; ++k) s[k] = (vis[piece * (kPiece / 32) + k / 32] >> (k % 32) & 1) ? s[k] : -INFINITY;
                         }
                     };
 #pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        factor[b] = q_scale * ks[b];
-                        add[b] = __shfl_sync(0xFFFFFFFFu, my_log, b);
+                    for (int b = 0; b < KEYS / 16; ++b) {
+                        factor[b] = q_scale * sh.scales[buf][k0 / 16 + b];
+                        add[b] = __shfl_sync(0xFFFFFFFFu, my_log, k0 / 16 + b);
                         // Scales of a block that the row sees nothing of may be anything.
                         if (masked && (vis[b / 2] >> (b % 2 * 16) & 0xFFFFu) == 0) factor[b] = 1.0f, add[b] = 0.0f;
                     }
                     float top = -INFINITY;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        load(half);
+                    for (int piece = 0; piece < kPieces; ++piece) {
+                        load(piece);
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {
+                        for (int b = 0; b < kPiece / 16; ++b) {
                             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                             for (int k = 0; k < 8; ++k) mx[k & 1] = max3(mx[k & 1], s[16 * b + 2 * k], s[16 * b + 2 * k + 1]);
-                            top = fmaxf(top, fmaf(fmaxf(mx[0], mx[1]), factor[4 * half + b], add[4 * half + b]));
+                            const int all = piece * (kPiece / 16) + b;
+                            top = fmaxf(top, fmaf(fmaxf(mx[0], mx[1]), factor[all], add[all]));
                         }
                     }
                     const bool far = top > m_run + kKv8RoomLog2;
@@ -347,16 +357,27 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             }
                         }
                     }
+                    if constexpr (KEYS < kKv8Keys) {
+                        // The other copies' keys count nothing here.
+                        float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int c = 0; c < kKv8Keys; c += 32) {
+                            if (c >= k0 && c < k0 + KEYS) continue;
+                            const uint32_t at = s_addr + C::kHalfCol * (c / 64) + c % 64 / 4;
+                            tmem_st8_nowait(at, zero);
+                            tmem_st8_nowait(at + C::kLoCol, zero);
+                        }
+                    }
                     const float base = kKv8TopLog2 - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll
-                    for (int half = 1; half >= 0; --half) {
-                        if (half == 0) load(0);
+                    for (int piece = kPieces - 1; piece >= 0; --piece) {
+                        if (piece < kPieces - 1) load(piece);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
+                        for (int c = 0; c < kPiece / 32; ++c) {
                             uint32_t hi[8], lo[8];
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const int at16 = 2 * c + h, b = 4 * half + at16;
+                                const int at16 = 2 * c + h, b = piece * (kPiece / 16) + at16;
                                 const unsigned long long f2 = pair_f32(factor[b], factor[b]), a2 = pair_f32(add[b] + base, add[b] + base);
                                 unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll
@@ -377,16 +398,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                 }
                                 float s0, s1;
                                 unpair_f32(add_pair(sums[0], sums[1]), s0, s1);
-                                const float inv = __shfl_sync(0xFFFFFFFFu, my_inv, b);
+                                const float inv = __shfl_sync(0xFFFFFFFFu, my_inv, k0 / 16 + b);
                                 const bool any = !masked || (vis[b / 2] >> (16 * h) & 0xFFFFu) != 0;
                                 l_run = any ? fmaf(s0 + s1, inv, l_run) : l_run;
                             }
-                            tmem_st8_nowait(s_addr + C::kHalfCol * half + 8 * c, reinterpret_cast<const float *>(hi));
-                            tmem_st8_nowait(s_addr + C::kHalfCol * half + C::kLoCol + 8 * c, reinterpret_cast<const float *>(lo));
+                            const int key = k0 + kPiece * piece + 32 * c;
+                            const uint32_t at = s_addr + C::kHalfCol * (key / 64) + key % 64 / 4;
+                            tmem_st8_nowait(at, reinterpret_cast<const float *>(hi));
+                            tmem_st8_nowait(at + C::kLoCol, reinterpret_cast<const float *>(lo));
                         }
                     }
                     tmem_wait_st();
                     tc_fence_before();
+                };
+                if (warp_live) {
+                    if (part_rows == kManyRows) weigh(std::integral_constant<int, 128>{}, 0, vis);
+                    else if (part_rows == 64) weigh(std::integral_constant<int, 64>{}, 64 * key_part, {key_part ? vis[2] : vis[0], key_part ? vis[3] : vis[1]});
+                    else weigh(std::integral_constant<int, 32>{}, 32 * key_part, {key_part & 2 ? (key_part & 1 ? vis[3] : vis[2]) : (key_part & 1 ? vis[1] : vis[0])});
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[grp]));
@@ -407,11 +435,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 ok = wait(sh.exchange, x_phase);
                 if (!ok) break;
                 x_phase ^= 1;
-                const float2 other = sh.ml[grp ^ 1][r];
-                m = fmaxf(m_run, other.x);
+                // (Copies of a row are part_rows apart.)
+                m = -INFINITY;
+#pragma unroll 1
+                for (int x = item_row; x < kManyRows; x += part_rows) m = fmaxf(m, fmaxf(sh.ml[0][x].x, sh.ml[1][x].x));
+                l = 0.0f;
+#pragma unroll 1
+                for (int x = item_row; x < 2 * kManyRows; x += part_rows) {
+                    const float2 ml = sh.ml[x / kManyRows][x % kManyRows];
+                    l += ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m) * ml.y;
+                }
+                const float m_other = sh.ml[grp ^ 1][r].x;
                 w_own = m_run == -INFINITY ? 0.0f : exp2f(m_run - m);
-                w_other = other.x == -INFINITY ? 0.0f : exp2f(other.x - m);
-                l = l_run * w_own + other.y * w_other;
+                w_other = m_other == -INFINITY ? 0.0f : exp2f(m_other - m);
             }
             if (warp_live) {
                 const bool joined = !two && jobs > 1;
@@ -420,15 +456,68 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const uint32_t other_addr = tmem + lane_off + C::kOCol + (grp ^ 1) * HD;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const int slot = g.slot;
-                const long long part_row = (long long)(2 * blockIdx.x + max(slot, 0)) * 256 + (two ? grp * kManyRows : 0) + r;
+                const long long part_row = (long long)(2 * blockIdx.x + max(slot, 0)) * 256 + (two ? grp * kManyRows : 0) + item_row;
                 float4 *part = reinterpret_cast<float4 *>(p.part_o) + (part_row / 256) * (HD / 4) * 256 + part_row % 256;
                 const uint32_t live_mask = __ballot_sync(0xFFFFFFFFu, live);
                 const bool patch = *reinterpret_cast<volatile int *>(&sh.non_finite) != 0;
                 // Two row tiles: every column of the own row. One: group A finishes
                 // the first half of the columns, B the second.
                 const int d0 = two ? 0 : grp * (HD / 2), d1 = two ? HD : d0 + HD / 2;
+                if (part_rows < kManyRows) {
+                    // The copies' parts meet in q's place, as [column][row].
+                    float *meet = reinterpret_cast<float *>(q_s);
 #pragma unroll 1
-                for (int c = d0; c < d1; c += 32) {
+                    for (int c = d0; c < d1; c += 16) {
+                        float ov[16];
+                        tmem_ld16(own + c, ov);
+                        if (joined) {
+                            float ox[16];
+                            tmem_ld16(other_addr + c, ox);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) ov[k] = ov[k] * w_own + ox[k] * w_other;
+                        } else {
+                            // (Only group A has accumulated.)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) ov[k] *= grp == 0 ? w_own : w_other;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) meet[(c + k) * kManyRows + r] = ov[k];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.exchange));
+                    ok = wait(sh.exchange, x_phase);
+                    if (!ok) break;
+                    x_phase ^= 1;
+                    // A thread finishes its row's share of its group's columns, 8 at a time.
+                    const int share = HD / 2 * part_rows / kManyRows;
+#pragma unroll 1
+                    for (int c = d0 + key_part * share; live && c < d0 + (key_part + 1) * share; c += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+#pragma unroll 1
+                        for (int x = item_row; x < kManyRows; x += part_rows) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) v[k] += meet[(c + k) * kManyRows + x];
+                        }
+                        if (patch) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                if (kv8_patch(p, g, HD, pos, c + k)) v[k] = NAN;
+                            }
+                        }
+                        if (slot >= 0) {
+                            part[(c / 4) * 256] = make_float4(v[0], v[1], v[2], v[3]);
+                            part[(c / 4 + 1) * 256] = make_float4(v[4], v[5], v[6], v[7]);
+                        } else {
+                            *reinterpret_cast<uint4 *>(out_row + c) =
+                                make_uint4(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv),
+                                           pack_bf16(v[4] * inv, v[5] * inv), pack_bf16(v[6] * inv, v[7] * inv));
+                        }
+                    }
+                }
+#pragma unroll 1
+                for (int c = part_rows < kManyRows ? d1 : d0; c < d1; c += 32) {
                     float ov[32];
                     if (joined) {
                         float ox[32];
@@ -463,7 +552,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         store_rows4(out_row + c, v, live_mask);
                     }
                 }
-                if (live && slot >= 0 && (two || grp == 0)) p.part_ml[part_row] = make_float2(m, l);
+                if (live && slot >= 0 && key_part == 0 && (two || grp == 0)) p.part_ml[part_row] = make_float2(m, l);
             }
             tc_fence_before();
             // Neither accumulator may be overwritten before both are read, and
