@@ -285,11 +285,11 @@ struct Kv8Boxes {
     }
 };
 
-// 16 bf16 elements of q (cell `c` of a row that `cells` neighbouring lanes hold)
-// as two e4m3 parts of x / scale in rows `row` and `row_lo` of K-major tiles; the
-// scale is a power of two of the row's largest element. All lanes of a warp call.
+// 16 bf16 elements of q (of a row that HD / 16 neighbouring lanes hold) as two e4m3
+// parts of x / scale; the scale is a power of two of the row's largest element. All
+// lanes of a warp call.
 template <int HD>
-__device__ __forceinline__ float kv8_split_q(const uint4 (&raw)[2], uint8_t *tile, uint8_t *tile_lo, int row, int row_lo, int c) {
+__device__ __forceinline__ float kv8_split_q(const uint4 (&raw)[2], uint4 &part_hi, uint4 &part_lo) {
     constexpr int kCells = HD / 16;
     float x[16];
     const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
@@ -317,8 +317,8 @@ __device__ __forceinline__ float kv8_split_q(const uint4 (&raw)[2], uint8_t *til
         unpack_e4m3x4(hi[i], h);
         lo[i] = pack_e4m3x4(v[0] - h[0], v[1] - h[1], v[2] - h[2], v[3] - h[3]);
     }
-    *reinterpret_cast<uint4 *>(tile + e4m3_tile_offset<HD>(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4 *>(tile_lo + e4m3_tile_offset<HD>(row_lo, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    part_hi = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    part_lo = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     return scale;
 }
 

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + lane_off + grp * kKv8Keys;
         const uint32_t o_addr = tmem + lane_off + C::kOCol + grp * HD;
-        uint32_t s_phase = 0, done_phase = 0, x_phase = 0;
+        uint32_t q_phase = 0, s_phase = 0, done_phase = 0, x_phase = 0;
         for (int seg = 0; next(seg); ++seg) {
             const Kv8Segment &g = sh.queue[seg % kKv8Queue];
             const int tiles = g.jobs;
@@ -243,30 +243,49 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 release(seg);
                 continue;
             }
-            // q of this group's rows in two parts: a lane has 16 elements of a row at
-            // a time. (Its tile's last product of the segment before is done.)
+            // q of this group's rows in two parts: a lane has 16 elements of a row at a
+            // time, a warp a quarter of the rows, for all copies; four loads are in flight
+            // per lane. (Its tile's last product of the segment before is done.)
             {
-                constexpr int kCells = HD / 16, kRowsAt = kWarp / kCells;
+                constexpr int kCells = HD / 16, kRowsAt = kWarp / kCells, kLoads = 4;
                 uint8_t *tile = q_s + 2 * grp * C::kTile;
-                const int c = lane % kCells;
-#pragma unroll 2
-                for (int i = 0; i < kWarp; i += kRowsAt) {
-                    const int x = quad * 32 + i + lane / kCells, y = x & (part_rows - 1), n = y / p.group, h = y - n * p.group;
-                    uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-                    if (n < p.tile_nodes && tile_node + n < g.nodes) {
-                        const uint4 *src = reinterpret_cast<const uint4 *>(p.q + (long long)(g.row0 + tile_node + n) * p.q_stride +
-                                                                           (long long)(g.kvh * p.group + h) * HD + c * 16);
-                        raw[0] = __ldg(src);
-                        raw[1] = __ldg(src + 1);
+                const int c = lane % kCells, first = quad * (part_rows / 4), end = first + part_rows / 4;
+                const uint16_t *q = p.q + (long long)(g.row0 + tile_node) * p.q_stride + (long long)g.kvh * p.group * HD + c * 16;
+#pragma unroll 1
+                for (int y0 = first + lane / kCells; y0 - lane / kCells < end; y0 += kLoads * kRowsAt) {
+                    uint4 raw[kLoads][2];
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        const int y = y0 + i * kRowsAt, n = y / p.group, h = y - n * p.group;
+                        raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+                        if (y < end && n < p.tile_nodes && tile_node + n < g.nodes) {
+                            const uint4 *src = reinterpret_cast<const uint4 *>(q + n * p.q_stride + h * HD);
+                            raw[i][0] = __ldg(src);
+                            raw[i][1] = __ldg(src + 1);
+                        }
                     }
-                    const float scale = kv8_split_q<HD>(raw, tile, tile + C::kTile, x, x, c);
-                    if (c == 0) sh.ml[grp][x].x = scale * p.scale_log2;
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        const int y = y0 + i * kRowsAt;
+                        if (y - lane / kCells >= end) break;  // (the whole warp)
+                        uint4 hi, lo;
+                        const float scale = kv8_split_q<HD>(raw[i], hi, lo);
+                        for (int x = y; x < kManyRows; x += part_rows) {
+                            const uint32_t at = e4m3_tile_offset<HD>(x, c);
+                            *reinterpret_cast<uint4 *>(tile + at) = hi;
+                            *reinterpret_cast<uint4 *>(tile + C::kTile + at) = lo;
+                        }
+                        if (c == 0) sh.ml[grp][y].x = scale * p.scale_log2;
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[grp]));
+                ok = wait(sh.q_full[grp], q_phase);
+                if (!ok) break;
+                q_phase ^= 1;
             }
-            const float q_scale = sh.ml[grp][r].x;
+            const float q_scale = sh.ml[grp][item_row].x;
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             // Positions of this row, and of this group's first and last.
             const int pos = g.pos0 + node, first_pos = g.pos0 + tile_node, len = g.len;
