@@ -23,17 +23,18 @@ namespace cheetah {
 
 template <int HD, int R>
 struct Kv8Few {
-    static constexpr int kGroups = R == 32 ? 2 : 3;
+    static_assert(R == 8 || R == 16, "more rows are the other kernel's");
+    static constexpr int kGroups = 3;
     static constexpr int kThreads = 128 + kGroups * 128;
     static constexpr int kTile = kKv8Keys * HD;                     // one K or V tile
-    static constexpr int kAhead = R == 32 ? 1 : 2;                  // tiles of weights that a group may be ahead of their product
+    static constexpr int kAhead = 2;                                // tiles of weights that a group may be ahead of their product
     static constexpr int kP = 2 * R * kKv8Keys;                     // the weights of a tile
     static constexpr int kPX = kGroups * kAhead * kP;               // at a segment's end the groups' O
     static constexpr int kRowsX = kPX / (kGroups * HD * 4) < R ? kPX / (kGroups * HD * 4) : R;  // rows of them at a time
     static constexpr int kQ = 2 * R * HD;                           // q's parts, one segment's
     // V tiles stay until their weights are there, K tiles only for S: the ring of V
     // is the deeper one.
-    static constexpr int kStagesK = (R == 8 ? 6 : R == 16 ? 5 : 4) * (128 / HD), kStagesV = (R == 16 ? 6 : 7) * (128 / HD);
+    static constexpr int kStagesK = (R == 8 ? 6 : 5) * (128 / HD), kStagesV = (R == 8 ? 7 : 6) * (128 / HD);
     // S products ahead of the weights': within the places of S, and such that a
     // barrier's next phase can only end once its group has waited for the last: S of
     // tile x + kStagesK follows the weights of tile x, the products of tile x +
@@ -349,23 +350,16 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                 const float log_vs = kv8_log2(vs);
                 __syncwarp();  // the loads from TMEM are the whole warp's
                 float arg[R];
-                // arg without sub, S in steps of 16 rows at most.
-                constexpr int kStep = R < 16 ? R : 16;
+                // arg without sub.
                 auto scores = [&]() {
+                    float s[2 * R];
 #pragma unroll
-                    for (int c = 0; c < R; c += kStep) {
-                        float s[2 * kStep];
+                    for (int x = 0; x < 2 * R; x += 8) tmem_ld8_nowait(s_addr + x, s + x);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < kStep; x += 8) {
-                            tmem_ld8_nowait(s_addr + c + x, s + x);
-                            tmem_ld8_nowait(s_addr + R + c + x, s + kStep + x);
-                        }
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int x = 0; x < kStep; ++x) {
-                            arg[c + x] = fmaf(s[x] + s[kStep + x], q_scale[c + x] * ks, log_vs);
-                            if (!whole) arg[c + x] = c + x >= r0 && c + x < r1 ? arg[c + x] : -INFINITY;
-                        }
+                    for (int x = 0; x < R; ++x) {
+                        arg[x] = fmaf(s[x] + s[R + x], q_scale[x] * ks, log_vs);
+                        if (!whole) arg[x] = x >= r0 && x < r1 ? arg[x] : -INFINITY;
                     }
                 };
                 scores();

@@ -325,20 +325,18 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
         return -1;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Up to 16 rows an item, by the mean, the keys are the products' tall side, else the
+    // rows. 32 sequences over 2000 to 16000 keys, heads of 128, few | many: 7 rows
+    // 58 | 86 us, 14 rows 70 | 90; with 32 rows to an item, 28 rows took 167 | 97.
     const uint64_t rows = (uint64_t)((a->rows + a->batch - 1) / a->batch) * p.group;
-    if (rows > 32)
+    if (rows > 16)
         return a->head_dim == 64 ? launch_attention_many<64>(k_map, v_map, p, device, ctas, st)
                                  : launch_attention_many<128>(k_map, v_map, p, device, ctas, st);
-    const int least = p.group <= 8 ? 8 : (p.group <= 16 ? 16 : 32);
-    const int r = std::max(least, rows <= 8 ? 8 : (rows <= 16 ? 16 : 32));
-    if (a->head_dim == 64) {
-        return r == 8    ? launch_attention_few<64, 8>(k_map, v_map, p, device, ctas, st)
-               : r == 16 ? launch_attention_few<64, 16>(k_map, v_map, p, device, ctas, st)
-                         : launch_attention_few<64, 32>(k_map, v_map, p, device, ctas, st);
-    }
-    return r == 8    ? launch_attention_few<128, 8>(k_map, v_map, p, device, ctas, st)
-           : r == 16 ? launch_attention_few<128, 16>(k_map, v_map, p, device, ctas, st)
-                     : launch_attention_few<128, 32>(k_map, v_map, p, device, ctas, st);
+    if (a->head_dim == 64)
+        return rows <= 8 ? launch_attention_few<64, 8>(k_map, v_map, p, device, ctas, st)
+                         : launch_attention_few<64, 16>(k_map, v_map, p, device, ctas, st);
+    return rows <= 8 ? launch_attention_few<128, 8>(k_map, v_map, p, device, ctas, st)
+                     : launch_attention_few<128, 16>(k_map, v_map, p, device, ctas, st);
 }
 
 int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream) {
