@@ -147,19 +147,28 @@ struct Kv8Walk {
     TreeSplit split;
 
     __device__ __forceinline__ void init(const Kv8AttnParams &p) {
-        // A lane per sequence; the units of the first kKept * 32 stay in registers.
+        // A lane per sequence; the units of the first kKept * 32 stay in registers. (Loads
+        // side by side, the rest in loops that pass the registers on: this code runs once,
+        // and what it costs is above all to fetch it.)
         constexpr int kKept = 4;
         const int lane = threadIdx.x % kWarp;
         auto units_of = [&](int i) -> int { return i < p.batch ? Cost::head(p, kv8_seq(p, i)) * p.kv_heads : 0; };
-        int kept[kKept], total = 0;
+        int kept[kKept] = {}, total = 0;
         Kv8Seq first[kKept];
 #pragma unroll
-        for (int k = 0; k < kKept; ++k) first[k] = kv8_seq(p, min(lane + k * kWarp, p.batch - 1));  // loads side by side
-#pragma unroll
+        for (int k = 0; k < kKept; ++k) first[k] = kv8_seq(p, min(lane + k * kWarp, p.batch - 1));
+#pragma unroll 1
         for (int k = 0; k < kKept; ++k) {
-            kept[k] = lane + k * kWarp < p.batch ? Cost::head(p, first[k]) * p.kv_heads : 0;
-            total += kept[k];
+            const int units = lane + k * kWarp < p.batch ? Cost::head(p, first[0]) * p.kv_heads : 0;
+            total += units;
+#pragma unroll
+            for (int i = 0; i + 1 < kKept; ++i) {
+                first[i] = first[i + 1];
+                kept[i] = kept[i + 1];
+            }
+            kept[kKept - 1] = units;
         }
+#pragma unroll 1
         for (int i = lane + kKept * kWarp; i < p.batch; i += kWarp) total += units_of(i);
         total = __reduce_add_sync(0xFFFFFFFFu, total);
         share = max(Cost::MIN_SHARE, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
@@ -182,11 +191,12 @@ struct Kv8Walk {
             before = __shfl_sync(0xFFFFFFFFu, end, kWarp - 1);
         };
         if (u0 < total) {
+#pragma unroll 1
+            for (int b0 = 0; b0 < p.batch && start < 0; b0 += kWarp) {
+                look(b0, b0 < kKept * kWarp ? kept[0] : units_of(b0 + lane));
 #pragma unroll
-            for (int k = 0; k < kKept; ++k) {
-                if (start < 0) look(k * kWarp, kept[k]);
+                for (int i = 0; i + 1 < kKept; ++i) kept[i] = kept[i + 1];
             }
-            for (int b0 = kKept * kWarp; b0 < p.batch && start < 0; b0 += kWarp) look(b0, units_of(b0 + lane));
         }
         b = start;
         left = min(share, total - u0);

@@ -220,6 +220,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t s_addr = tmem + lane_off + grp * kKv8Keys;
         const uint32_t o_addr = tmem + lane_off + C::kOCol + grp * HD;
         uint32_t q_phase = 0, s_phase = 0, done_phase = 0, x_phase = 0;
+        // Row of a tile to its node: x / group, exact for x < 256 and group <= 32.
+        const uint32_t group_inv = 65536u / p.group + 1u;
+        auto node_of = [&](int x) -> int { return (int)(x * group_inv >> 16); };
         for (int seg = 0; next(seg); ++seg) {
             const Kv8Segment &g = sh.queue[seg % kKv8Queue];
             const int tiles = g.jobs;
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const int rows = min(g.nodes, p.tile_nodes) * p.group;
             const int part_rows = rows <= 32 ? 32 : (rows <= 64 ? 64 : kManyRows);
             const int item_row = r & (part_rows - 1), key_part = r / part_rows;
-            const int node_of_r = item_row / p.group, head_of_r = item_row % p.group;
+            const int node_of_r = node_of(item_row), head_of_r = item_row - node_of_r * p.group;
             const int node = tile_node + node_of_r;
             const bool live = node_of_r < p.tile_nodes && node < g.nodes;
             uint16_t *out_row = p.out + ((long long)(g.row0 + node) * p.q_heads + g.kvh * p.group + head_of_r) * HD;
@@ -252,11 +255,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const int c = lane % kCells, first = quad * (part_rows / 4), end = first + part_rows / 4;
                 const uint16_t *q = p.q + (long long)(g.row0 + tile_node) * p.q_stride + (long long)g.kvh * p.group * HD + c * 16;
 #pragma unroll 1
-                for (int y0 = first + lane / kCells; y0 - lane / kCells < end; y0 += kLoads * kRowsAt) {
+                for (int y0 = first; y0 < end; y0 += kLoads * kRowsAt) {
                     uint4 raw[kLoads][2];
 #pragma unroll
                     for (int i = 0; i < kLoads; ++i) {
-                        const int y = y0 + i * kRowsAt, n = y / p.group, h = y - n * p.group;
+                        const int y = y0 + i * kRowsAt + lane / kCells, n = node_of(y), h = y - n * p.group;
                         raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
                         if (y < end && n < p.tile_nodes && tile_node + n < g.nodes) {
                             const uint4 *src = reinterpret_cast<const uint4 *>(q + n * p.q_stride + h * HD);
@@ -264,12 +267,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             raw[i][1] = __ldg(src + 1);
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < kLoads; ++i) {
-                        const int y = y0 + i * kRowsAt;
-                        if (y - lane / kCells >= end) break;  // (the whole warp)
+#pragma unroll 1
+                    for (int y1 = y0; y1 < min(y0 + kLoads * kRowsAt, end); y1 += kRowsAt) {
+                        const int y = y1 + lane / kCells;
                         uint4 hi, lo;
-                        const float scale = kv8_split_q<HD>(raw[i], hi, lo);
+                        const float scale = kv8_split_q<HD>(raw[0], hi, lo);
+#pragma unroll
+                        for (int i = 0; i + 1 < kLoads; ++i) raw[i][0] = raw[i + 1][0], raw[i][1] = raw[i + 1][1];
+#pragma unroll 1
                         for (int x = y; x < kManyRows; x += part_rows) {
                             const uint32_t at = e4m3_tile_offset<HD>(x, c);
                             *reinterpret_cast<uint4 *>(tile + at) = hi;
