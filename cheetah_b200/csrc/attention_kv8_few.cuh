@@ -47,7 +47,8 @@ struct Kv8Few {
     static constexpr uint32_t kCols = kGroups * 6 * R <= 256 ? 256 : 512;
     static_assert(kGroups * 6 * R <= (int)kCols, "TMEM columns");
     static_assert(kRowsX % 8 == 0 && R % kRowsX == 0, "rows are joined 8 at a time");
-    using Cost = Kv8Cost<2, 1, 1, 6>;
+    // Shares of three tiles pay for their join: with six the shortest calls took a fifth more.
+    using Cost = Kv8Cost<4, 1, 1, 3>;
     static constexpr int kDims = HD == 128 ? 32 : 16;               // dimensions (lanes) of a warp's part of O^T
 };
 

@@ -40,7 +40,9 @@ struct Kv8Many {
     // TMEM: S_A | S_B | O_A | O_B; the weights' parts take the columns of the S
     // they came from, those of 64 keys in the columns of these.
     static constexpr uint32_t kHalfCol = 64, kLoCol = 16;
-    using Cost = Kv8Cost<6, 2, 3, 6>;
+    // Beginning and end of an item cost what 6 to 8 of its tiles do, and a tile of both
+    // row tiles twice one. Lower units (6, 2, 3) took 5% more for prompts.
+    using Cost = Kv8Cost<16, 2, 4, 4>;
 };
 
 template <int STAGES>

@@ -327,7 +327,7 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Up to 16 rows an item, by the mean, the keys are the products' tall side, else the
     // rows. 32 sequences over 2000 to 16000 keys, heads of 128, few | many: 7 rows
-    // 58 | 77 us, 14 rows 67 | 78; with 32 rows to an item, 28 rows took 167 | 78.
+    // 58 | 75 us, 14 rows 66 | 75; with 32 rows to an item, 28 rows took 167 | 73.
     const uint64_t rows = (uint64_t)((a->rows + a->batch - 1) / a->batch) * p.group;
     if (rows > 16)
         return a->head_dim == 64 ? launch_attention_many<64>(k_map, v_map, p, device, ctas, st)
