@@ -122,7 +122,7 @@ __device__ __forceinline__ Kv8Range kv8_range(const Kv8AttnParams &p, const Kv8S
 // key tile, by its row tiles. A share holds MIN_SHARE at least, which hold a tile.
 template <int ITEM_, int ONE, int TWO, int MIN_SHARE_>
 struct Kv8Cost {
-    static constexpr int ITEM = ITEM_, MIN_SHARE = MIN_SHARE_;
+    static constexpr int ITEM = ITEM_, TWO_TILES = TWO, MIN_SHARE = MIN_SHARE_;
     static_assert(MIN_SHARE >= TWO && TWO >= ONE, "every share holds a tile");
     static __device__ __forceinline__ int tile(const Kv8AttnParams &p, const Kv8Seq &s, int j) {
         return s.n - j * p.item_nodes > p.tile_nodes ? TWO : ONE;

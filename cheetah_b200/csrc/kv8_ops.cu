@@ -240,6 +240,15 @@ int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *a, void *stream) {
     return bf16 ? launch_read<uint16_t, 128>(p, st) : launch_read<float, 128>(p, st);
 }
 
+// Rows of an item at most, of the kernel that takes the call. Up to 16 rows by the
+// sequences' mean the keys are the products' tall side, else the rows. 32 sequences
+// over 2000 to 16000 keys, heads of 128, few | many: 7 rows 58 | 75 us, 14 rows 66 |
+// 75; with 32 rows to an item of the few, 28 rows took 167 | 73.
+static int attention_item_rows(const CheetahCudaAttentionKv8 *a) {
+    const uint64_t rows = (uint64_t)((a->rows + a->batch - 1) / a->batch) * (a->q_heads / a->kv_heads);
+    return rows <= 8 ? 8 : (rows <= 16 ? 16 : 2 * cheetah::kManyRows);
+}
+
 static int check_attention_kv8(const CheetahCudaAttentionKv8 *a) {
     CH_REQUIRE(a != nullptr, "cheetah_cuda_op_attention_kv8: null argument");
     CH_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "cheetah_cuda_op_attention_kv8: head_dim must be 64 or 128");
@@ -256,11 +265,16 @@ static int check_attention_kv8(const CheetahCudaAttentionKv8 *a) {
                "cheetah_cuda_op_attention_kv8: a table row holds at most 2^31 - 129 tokens");
     CH_REQUIRE(a->sliding_window <= 0x7FFFFFFFu && a->sinks <= 0x7FFFFFFFu,
                "cheetah_cuda_op_attention_kv8: sliding_window or sinks is too large");
-    // The kernel counts its cost units (a key tile each, and a few per item) in
-    // 31 bits.
-    const uint64_t items = ((uint64_t)a->rows / (8 / std::min(8u, a->q_heads / a->kv_heads)) + a->batch) * a->kv_heads;
+    // The kernel counts its cost units in 31 bits.
+    const uint32_t group = a->q_heads / a->kv_heads;
     const uint64_t tiles = (uint64_t)a->max_pages_per_seq * a->page_tokens / cheetah::kKv8Keys + 1;
-    CH_REQUIRE(items * (3 * tiles + 8) <= 0x7FFFFFFFull, "cheetah_cuda_op_attention_kv8: too many rows and cached positions");
+    const int rows = attention_item_rows(a);
+    using Many = cheetah::Kv8Many<128>::Cost;
+    using Few = cheetah::Kv8Few<128, 8>::Cost;
+    const uint64_t nodes = rows == 2 * cheetah::kManyRows ? 2 * (cheetah::kManyRows / group) : rows / group;
+    const uint64_t items = ((uint64_t)a->rows / nodes + a->batch) * a->kv_heads;
+    const uint64_t units = rows == 2 * cheetah::kManyRows ? Many::TWO_TILES * tiles + Many::ITEM : Few::TWO_TILES * tiles + Few::ITEM;
+    CH_REQUIRE(items * units <= 0x7FFFFFFFull, "cheetah_cuda_op_attention_kv8: too many rows and cached positions");
     return 0;
 }
 
@@ -325,18 +339,15 @@ int cheetah_cuda_op_attention_kv8(const CheetahCudaAttentionKv8 *a, void *stream
         return -1;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Up to 16 rows an item, by the mean, the keys are the products' tall side, else the
-    // rows. 32 sequences over 2000 to 16000 keys, heads of 128, few | many: 7 rows
-    // 58 | 75 us, 14 rows 66 | 75; with 32 rows to an item, 28 rows took 167 | 73.
-    const uint64_t rows = (uint64_t)((a->rows + a->batch - 1) / a->batch) * p.group;
-    if (rows > 16)
-        return a->head_dim == 64 ? launch_attention_many<64>(k_map, v_map, p, device, ctas, st)
-                                 : launch_attention_many<128>(k_map, v_map, p, device, ctas, st);
-    if (a->head_dim == 64)
-        return rows <= 8 ? launch_attention_few<64, 8>(k_map, v_map, p, device, ctas, st)
-                         : launch_attention_few<64, 16>(k_map, v_map, p, device, ctas, st);
-    return rows <= 8 ? launch_attention_few<128, 8>(k_map, v_map, p, device, ctas, st)
-                     : launch_attention_few<128, 16>(k_map, v_map, p, device, ctas, st);
+    const int rows = attention_item_rows(a);
+    if (a->head_dim == 64) {
+        return rows == 8    ? launch_attention_few<64, 8>(k_map, v_map, p, device, ctas, st)
+               : rows == 16 ? launch_attention_few<64, 16>(k_map, v_map, p, device, ctas, st)
+                            : launch_attention_many<64>(k_map, v_map, p, device, ctas, st);
+    }
+    return rows == 8    ? launch_attention_few<128, 8>(k_map, v_map, p, device, ctas, st)
+           : rows == 16 ? launch_attention_few<128, 16>(k_map, v_map, p, device, ctas, st)
+                        : launch_attention_many<128>(k_map, v_map, p, device, ctas, st);
 }
 
 int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream) {

@@ -512,6 +512,73 @@ def test_attention_is_the_same_every_time():
         assert torch.equal(c.run(), first)
 
 
+@pytest.mark.parametrize("q_heads,kvh,D", [(28, 4, 128), (14, 2, 64), (16, 1, 128), (32, 1, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 5)])
+def test_attention_of_a_batch_of_any_rows(q_heads, kvh, D, window, sinks):
+    """Items of one row up to two full tiles of rows side by side, whole and cut,
+    one without room and some without rows among them."""
+    rows = [1, 40, 0, 9, 130, 2, 5, 18, 4, 1, 64, 3]
+    ctx = [2000, 0, 70, 513, 1000, 3000, 126, 900, 5, 0, 1, 2500]
+    c = Attend(q_heads + window, ctx, rows, q_heads, kvh, D, 64, window, sinks)
+    c.lens[6] = 4
+    c.check(c.run())
+
+
+def test_attention_calls_that_overlap():
+    """Two captured calls on two streams, each with a workspace of its own."""
+    from cheetah_b200 import runtime as R
+    calls, keep = [], []
+    for rows, D in ((1, 64), (30, 128)):
+        c = Attend(rows, [3000, 7000], [rows, rows], 14, 2, D, 64)
+        (kc, ks), (vc, vs) = to_gpu(*c.k), to_gpu(*c.v)
+        args = (c.q.cuda(), kc, vc, ks, vs, i32(c.table), i32(c.lens), i32(c.starts))
+        want = R.attention_kv8(*args)
+        out = torch.empty_like(want)
+        work = torch.empty(R.attention_kv8_workspace(D), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(4):
+                R.attention_kv8(*args, out=out, workspace=work)
+        calls.append((graph, torch.cuda.Stream(), out, want))
+        keep.append((args, work))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, stream, _, _ in calls:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, want in calls:
+        assert torch.equal(out, want)
+
+
+def test_attention_join_after_a_wait_that_gave_up(tmp_path):
+    """The join alone, on a list of split items in which one CTA has given up:
+    every row is NaN, those behind the last sequence stay. Without one that has,
+    and without anything to join, it writes nothing."""
+    import ctypes as C
+    import subprocess
+    from pathlib import Path
+    from cheetah_b200 import build
+    here = Path(__file__).resolve().parent
+    lib = tmp_path / "kv8_join.so"
+    subprocess.run([build.nvcc(), *build.ARCH_FLAGS, "-O1", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-I", str(build.CSRC),
+                    "-I", str(build.INCLUDE), "--expt-relaxed-constexpr", "-o", str(lib), str(here / "kv8_join_entry.cu")],
+                   check=True, capture_output=True, timeout=300)
+    join = C.CDLL(str(lib)).kv8_join
+    rows, q_heads, ctas = 20, 3, 5
+    starts = i32([0, 4, 13])
+    splits = torch.zeros(32 * ctas, dtype=torch.uint8, device="cuda")
+    for parts, given_up in (([0, 0, -1, 0, 0], True), ([0, 1, 0, 1, 0], False), ([-1] * 5, True)):
+        out = torch.full((rows, q_heads, 64), 2.5, dtype=torch.bfloat16, device="cuda")
+        rc = join((C.c_int * ctas)(*parts), ctas, C.c_void_p(starts.data_ptr()), 2, rows, q_heads, C.c_void_p(splits.data_ptr()),
+                  C.c_void_p(out.data_ptr()), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert rc == 0
+        assert bool(torch.isnan(out[:13]).all()) if given_up else bool((out[:13] == 2.5).all())
+        assert bool((out[13:] == 2.5).all())
+
+
 # ---- verify_drafts --------------------------------------------------------------
 
 def verify_case(seed, drafts, vocab, given=True, extra=3, wide=0, agree=0.4):

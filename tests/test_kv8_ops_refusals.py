@@ -63,6 +63,7 @@ CASES = [
     (attend, dict(max_pages_per_seq=(1 << 27) - 1), "table row"), (attend, dict(sliding_window=1 << 31), "sliding_window"),
     (attend, dict(sinks=1 << 31), "sinks"), (attend, dict(q_stride=13 * 64), "overlap"), (attend, dict(q_stride=14 * 64 + 4), "aligned"),
     (attend, dict(out=P + 8), "aligned"), (attend, dict(v_codes=P + 8), "aligned"), (attend, dict(workspace=P + 16), "aligned"),
+    (attend, dict(rows=1 << 20, max_pages_per_seq=1 << 21), "too many"), (attend, dict(rows=4096, batch=4096, max_pages_per_seq=1 << 23), "too many"),
     (verify, dict(target_probs=None), "null"), (verify, dict(out_tokens=None), "null"), (verify, dict(rows=0), "rows"),
     (verify, dict(vocab=0), "vocab"), (verify, dict(vocab=(1 << 30) + 1, target_stride=1 << 31, draft_stride=1 << 31), "vocab"),
     (verify, dict(batch=0), "batch"), (verify, dict(batch=65536), "batch"), (verify, dict(target_stride=99), "overlap"),
