@@ -15,6 +15,12 @@
 // end. A group's next S is computed while it works on one, and its next weights are
 // written while the last are multiplied. One barrier says that a product is done to
 // those who wait for its result and to the loads that wait for its operand's place.
+//
+// Bound by the loads of K and V where keys are many: 64 sequences of 1000 to 16000
+// keys, one row each, 28 + 4 heads of 128, 597 MB: 121 us, 4.9 TB/s. One sequence of
+// 700 keys takes 10.8 us: two launches, and a chain of starts, page, tile, S, weights,
+// O, join. Two groups instead of three took 141 us, rows as the tall side (the
+// other kernel) 75 us instead of 58 at 32 sequences.
 #pragma once
 
 #include "attention_kv8.cuh"
