@@ -148,8 +148,8 @@ struct Kv8Walk {
 
     __device__ __forceinline__ void init(const Kv8AttnParams &p) {
         // A lane per sequence; the units of the first kKept * 32 stay in registers. (Loads
-        // side by side, the rest in loops that pass the registers on: this code runs once,
-        // and what it costs is above all to fetch it.)
+        // side by side, the rest in loops that pass the registers on: this code runs once
+        // and is the faster for being short.)
         constexpr int kKept = 4;
         const int lane = threadIdx.x % kWarp;
         auto units_of = [&](int i) -> int { return i < p.batch ? Cost::head(p, kv8_seq(p, i)) * p.kv_heads : 0; };

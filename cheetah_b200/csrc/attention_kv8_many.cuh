@@ -25,8 +25,8 @@
 // two groups) is issue-bound. One pass with a running maximum took 473 us (weights of a
 // tile done again where the reference moved) against 335 us of two at the time. 32
 // sequences of 1 to 9 rows in a window of 4096: 54 us, starts and ends of items
-// half of it. A piece of code that runs once costs what its fetch does, about 100
-// cycles for 8 instructions: what an item does once is written in loops.
+// half of it. What an item does once is written in loops: unrolled it took 60.6 us
+// instead of 56.0 at the time.
 #pragma once
 
 #include <type_traits>
