@@ -363,6 +363,9 @@ int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream
                "cheetah_cuda_op_verify_drafts: rows must not overlap");
     CH_REQUIRE(aligned(a->target_probs, 4) && aligned(a->draft_probs, 4),
                "cheetah_cuda_op_verify_drafts: probabilities must be aligned to their type");
+    // CTAs of a sequence read its tokens while one writes what it kept.
+    CH_REQUIRE(a->out_tokens + a->rows <= a->tokens || a->tokens + a->rows <= a->out_tokens,
+               "cheetah_cuda_op_verify_drafts: out_tokens must not overlap tokens");
     cheetah::VerifyDraftsParams p = {};
     p.target = a->target_probs;
     p.draft = a->draft_probs;

@@ -635,7 +635,7 @@ typedef struct CheetahCudaVerifyDrafts {
     const float *accept_u;     /* [rows] in [0, 1) */
     const float *sample_u;     /* [batch] in [0, 1) */
     int32_t *accepted;         /* [batch] */
-    int32_t *out_tokens;       /* [rows] */
+    int32_t *out_tokens;       /* [rows], apart from tokens */
 } CheetahCudaVerifyDrafts;
 CHEETAH_CUDA_API int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *args, void *stream);
 

@@ -68,6 +68,7 @@ CASES = [
     (verify, dict(vocab=0), "vocab"), (verify, dict(vocab=(1 << 30) + 1, target_stride=1 << 31, draft_stride=1 << 31), "vocab"),
     (verify, dict(batch=0), "batch"), (verify, dict(batch=65536), "batch"), (verify, dict(target_stride=99), "overlap"),
     (verify, dict(draft_stride=99), "overlap"), (verify, dict(target_probs=P + 2), "aligned"), (verify, dict(draft_probs=P + 1), "aligned"),
+    (verify, dict(out_tokens=P + 8), "overlap tokens"), (verify, dict(tokens=P + 4, out_tokens=P), "overlap tokens"),
 ]
 
 
