@@ -112,10 +112,11 @@ __device__ __forceinline__ Kv8Range kv8_range(const Kv8AttnParams &p, const Kv8S
     if (s.ctx < 0) return r;  // without room for its rows: one tile that writes zeros
     const int node0 = j * p.item_nodes, nodes = min(s.n - node0, p.item_nodes);
     r.low = p.window > 0 ? max(0, s.ctx + node0 - p.window + 1) : 0;
-    const int lo = r.low / kKv8Keys, hi = (min(s.ctx + node0 + nodes, s.len) + kKv8Keys - 1) / kKv8Keys;
+    // Up to the last row, within the table (a window may begin behind it).
+    const int hi = (min(s.ctx + node0 + nodes, s.len) + kKv8Keys - 1) / kKv8Keys, lo = min(r.low / kKv8Keys, hi);
     r.sink_tiles = min((p.sinks + (kKv8Keys - 1LL)) / kKv8Keys, (long long)lo);
     r.skip = lo - r.sink_tiles;
-    r.tiles = max(1, r.sink_tiles + max(hi - lo, 0));
+    r.tiles = max(1, r.sink_tiles + hi - lo);
     return r;
 }
 // Cost units of a kernel: ITEM for an item's beginning and end, ONE or TWO for a

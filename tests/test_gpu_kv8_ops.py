@@ -579,6 +579,24 @@ def test_attention_join_after_a_wait_that_gave_up(tmp_path):
         assert bool((out[13:] == 2.5).all())
 
 
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (16, 5), (16, 2 ** 31 - 1), (2 ** 31 - 1, 0)])
+def test_attention_of_the_largest_length(rows, window, sinks):
+    """A length of 2^31 - 1 over a table of 96 positions: the rows see what those of
+    length 5000 do: of a short window its sinks alone."""
+    outs = []
+    for length in (5000, 2 ** 31 - 1):
+        c = Attend(rows, [96 - rows], [rows], 14, 2, 64, 32, window, sinks)
+        c.lens = [length]
+        outs.append(c.run().float())
+    # Two roundings of the output and of two orders of f32 sums.
+    assert bool(((outs[0] - outs[1]).abs() <= 2.0 ** -7 * outs[0].abs() + 2.0 ** -20).all())
+    if window == 16:
+        c = Attend(rows, [96 - rows], [rows], 14, 2, 64, 32, window, 0)
+        c.lens = [2 ** 31 - 1]
+        assert bool((c.run() == 0).all())
+
+
 # ---- verify_drafts --------------------------------------------------------------
 
 def verify_case(seed, drafts, vocab, given=True, extra=3, wide=0, agree=0.4):
