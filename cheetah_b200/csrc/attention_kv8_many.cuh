@@ -22,11 +22,11 @@
 // Prompts of 2 x 2000 rows behind up to 6000 keys, 28 + 4 heads of 128: 300 us, 666
 // TFLOP/s of the formula's operations, of which the split doubles the products; bound
 // by the chain S, softmax, PV of a tile (the softmax of 128 keys 3300 cycles beside
-// the other group's; issue slots 44%, tensor pipe 32%, exponentials 33%). One pass with a running maximum took 473 us (weights of a
-// tile done again where the reference moved) against 335 us of two at the time. 32
-// sequences of 1 to 9 rows in a window of 4096: 54 us, starts and ends of items
-// half of it. What an item does once is written in loops: unrolled it took 60.6 us
-// instead of 56.0 at the time.
+// the other group's; issue slots 44%, tensor pipe 32%, exponentials 33%). One pass
+// with a running maximum took 473 us (weights of a tile done again where the
+// reference moved) against 335 us of two at the time. 32 sequences of 1 to 9 rows in
+// a window of 4096: 54 us, starts and ends of items half of it. What an item does
+// once is written in loops: unrolled it took 60.6 us instead of 56.0 at the time.
 #pragma once
 
 #include <type_traits>
