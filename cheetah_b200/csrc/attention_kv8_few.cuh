@@ -70,7 +70,10 @@ struct Kv8FewShared {
     alignas(16) float scales[STAGES_V][16];  // K's, then V's
     alignas(16) float q_scale[2][R];
     alignas(16) int far[GROUPS][2][4];               // by place: a warp may be a tile ahead of one that has yet to read
-    float top[GROUPS][4][R];               // maxima, at a segment's end sums
+    float top[GROUPS][4][R];               // maxima of a tile whose reference moves
+    // A segment's sums have a place of their own: no barrier of a group's warps lies
+    // between the last tile's maxima, which all four read, and the first one's sums.
+    float sum[GROUPS][4][R];
     float m[GROUPS][R];
 };
 
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                     v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], 16);
                     if (lane / 8 == c / 8) sum = v[0];  // row c + lane % 8
                 }
-                if (lane < R) sh.top[grp][quad][lane] = sum;
+                if (lane < R) sh.sum[grp][quad][lane] = sum;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (lane == r && quad == 0) sh.m[grp][r] = sub[r] == kNone ? -INFINITY : kKv8TopLog2 - sub[r];
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                 const float mz = sh.m[z][row_of_lane];
                 const float f = mz == -INFINITY ? 0.0f : fast_exp2(mz - largest);
                 if (z == grp) factor = f;
-                sum += f * ((sh.top[z][0][row_of_lane] + sh.top[z][1][row_of_lane]) + (sh.top[z][2][row_of_lane] + sh.top[z][3][row_of_lane]));
+                sum += f * ((sh.sum[z][0][row_of_lane] + sh.sum[z][1][row_of_lane]) + (sh.sum[z][2][row_of_lane] + sh.sum[z][3][row_of_lane]));
             }
             const int slot = g.slot;
             const bool patch = *reinterpret_cast<volatile int *>(&sh.non_finite) != 0;
