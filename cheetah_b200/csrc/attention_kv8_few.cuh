@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
 #pragma unroll
                     for (int c = 0; c < C::kRowsX; c += 8) {
                         float o[16];
+                        __syncwarp();  // lanes part at the stores; the loads from TMEM are the whole warp's
                         tmem_ld8_nowait(o_addr + c0 + c, o);
                         tmem_ld8_nowait(o_addr + R + c0 + c, o + 8);
                         tmem_wait_ld();

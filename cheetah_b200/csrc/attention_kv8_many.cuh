@@ -554,6 +554,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll 1
                 for (int c = part_rows < kManyRows ? d1 : d0; c < d1; c += 32) {
                     float ov[32];
+                    __syncwarp();  // lanes part below where not all are live; the loads from TMEM are the whole warp's
                     if (joined) {
                         float ox[32];
                         tmem_ld32_nowait(own + c, ov);
