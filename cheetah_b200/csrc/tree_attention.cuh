@@ -988,6 +988,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll 1
                 for (int c = d0; c < d1; c += 32) {
                     float ov[32];
+                    __syncwarp();  // lanes part at a part's stores; the loads from TMEM are the whole warp's
                     if (joined) {
                         float ox[32];
                         tmem_ld32_nowait(own + c, ov);
