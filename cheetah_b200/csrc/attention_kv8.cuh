@@ -8,12 +8,17 @@
 //   w_j = 2^(t_j + log2(vs) - m),   o' = sum_j w_j vc_j,   l = sum_j w_j / vs,   o = o' / l.
 //
 // The codes are multiplied as they are (tcgen05 kind::f8f6f4). What meets them
-// is split into e4m3 parts that are multiplied one after the other: q, over a
-// power of two of its row, into two (exact for elements within 2^-10 of the
-// row's largest, else off by 2^-18 of that), the weights times V's scale into
-// two as well (2^-8, as bf16 holds, or 2^-15 of the row's largest). K's scale
-// joins the factor of the scores. m follows t_j + log2(vs), so the weights fill
-// e4m3's range however V's scales differ.
+// is split into 8-bit parts that are multiplied one after the other: q, over a
+// power of two of its row that puts the largest element at 224 or above, into two of
+// e4m3 (exact for elements within 2^-10 of the row's largest, else off by half the
+// smallest step, 2^-10 / 224 = 2^-17.8 of that); the weights times V's scale, through
+// f16, into three of e5m2: off by 2^-9 + 2^-11 of themselves (bf16 holds 2^-8), or by
+// half the smallest step, 2^-29 of the row's largest. That floor is what a tail of many
+// small weights behind a heavy key needs: what is lost adds up over the keys,
+// while l counts every weight in full. Two e4m3 parts, whose floor is 2^-16 of the largest,
+// lost a third of such rows over 32768 keys; two of e5m2 hold 2^-6. K's scale joins
+// the factor of the scores. m follows t_j + log2(vs), so the weights fill e5m2's
+// range however V's scales differ.
 //
 // Work. An item is a run of rows of one (sequence, KV head): nodes (new tokens)
 // times the query heads of the group, so K and V are read once for all of them.
@@ -51,10 +56,12 @@ constexpr int kKv8Keys = 128;     // keys per tile
 constexpr int kKv8MaxCtas = kTreeMaxCtas;
 constexpr int kKv8Queue = 4;      // segments the scheduler may be ahead
 // Weights are scaled to at most 2^kKv8TopLog2 when a row's reference is set, and it
-// moves when one would pass 2^kKv8RoomLog2 times that (e4m3 ends at 448 = 2^8.8). A
-// move costs a pass over O, and in 32 rows one moves soon: with 7 and 1.75 nearly
-// every tile of a prompt had one.
-constexpr float kKv8TopLog2 = 6.0f, kKv8RoomLog2 = 2.75f;
+// moves when one would pass 2^kKv8RoomLog2 times that (e5m2 ends at 57344 = 2^15.8). A
+// move costs a pass over O, and in 32 rows one moves soon; but what the room takes the
+// floor loses. Prompts of 2 x 2000 rows took 318 us with 14 and 1.75, 317 with these,
+// 314.6 with 12 and 3.75.
+constexpr float kKv8TopLog2 = 13.0f, kKv8RoomLog2 = 2.75f;
+constexpr int kKv8Parts = 3;      // of a weight
 
 struct Kv8AttnParams {
     const uint16_t *q;

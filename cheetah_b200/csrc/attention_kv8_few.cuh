@@ -3,7 +3,7 @@
 //
 // The keys are the tall side of the products, so few rows cost little:
 //   S^T [128 keys x 2R] = K [128 x D] . [q1 | q2]^T         (q's two parts)
-//   O^T [D x 2R] += V^T [D x 128 keys] . [w1 | w2]^T         (the weights')
+//   O^T [D x 3R] += V^T [D x 128 keys] . [w1 | w2 | w3]^T    (the weights')
 // K and V are used as they lie in the cache, K with the head's dimensions along
 // the products' inner axis, V with the keys along it. A thread has one key of a
 // tile and all R rows: its scales are one number each, its exponentials R.
@@ -18,7 +18,7 @@
 //
 // Bound by the loads of K and V where keys are many: 64 sequences of 1000 to 16000
 // keys, one row each, 28 + 4 heads of 128, 597 MB: 121 us, 4.9 TB/s. One sequence of
-// 700 keys takes 10.8 us: two launches, and a chain of starts, page, tile, S, weights,
+// 700 keys takes 10.9 us: two launches, and a chain of starts, page, tile, S, weights,
 // O, join. Two groups instead of three took 141 us, rows as the tall side (the
 // other kernel) 75 us instead of 58 at 32 sequences.
 #pragma once
@@ -34,13 +34,17 @@ struct Kv8Few {
     static constexpr int kThreads = 128 + kGroups * 128;
     static constexpr int kTile = kKv8Keys * HD;                     // one K or V tile
     static constexpr int kAhead = 2;                                // tiles of weights that a group may be ahead of their product
-    static constexpr int kP = 2 * R * kKv8Keys;                     // the weights of a tile
+    // Columns of O^T and rows of the weights: three parts, and what fills them up to a
+    // multiple of 16 (nobody reads the columns of those rows, whatever they hold).
+    static constexpr int kN = (kKv8Parts * R + 15) / 16 * 16;
+    static constexpr int kP = kN * kKv8Keys;                        // the weights of a tile
+    static_assert(kP % 1024 == 0, "whole swizzle atoms");
     static constexpr int kPX = kGroups * kAhead * kP;               // at a segment's end the groups' O
     static constexpr int kRowsX = kPX / (kGroups * HD * 4) < R ? kPX / (kGroups * HD * 4) : R;  // rows of them at a time
     static constexpr int kQ = 2 * R * HD;                           // q's parts, one segment's
     // V tiles stay until their weights are there, K tiles only for S: the ring of V
     // is the deeper one.
-    static constexpr int kStagesK = (R == 8 ? 6 : 5) * (128 / HD), kStagesV = (R == 8 ? 7 : 6) * (128 / HD);
+    static constexpr int kStagesK = (R == 8 ? 6 : 5) * (128 / HD), kStagesV = 6 * (128 / HD);
     // S products ahead of the weights': within the places of S, and such that a
     // barrier's next phase can only end once its group has waited for the last: S of
     // tile x + kStagesK follows the weights of tile x, the products of tile x +
@@ -50,8 +54,8 @@ struct Kv8Few {
     static constexpr int kBytes = (kStagesK + kStagesV) * kTile + kPX + 2 * kQ;
     // TMEM: two S per group, so that the next is there when a group has read one, and O.
     static constexpr uint32_t kOCol = kGroups * 4 * R;
-    static constexpr uint32_t kCols = kGroups * 6 * R <= 256 ? 256 : 512;
-    static_assert(kGroups * 6 * R <= (int)kCols, "TMEM columns");
+    static constexpr uint32_t kCols = kGroups * (4 * R + kN) <= 256 ? 256 : 512;
+    static_assert(kGroups * (4 * R + kN) <= (int)kCols, "TMEM columns");
     static_assert(kRowsX % 8 == 0 && R % kRowsX == 0, "rows are joined 8 at a time");
     // Shares of three tiles pay for their join: with six the shortest calls took a fifth more.
     using Cost = Kv8Cost<4, 1, 1, 3>;
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
     using C = Kv8Few<HD, R>;
     constexpr int kGroups = C::kGroups, kStagesK = C::kStagesK, kStagesV = C::kStagesV;
     constexpr uint32_t kIdescS = umma_idesc_e4m3(kKv8Keys, 2 * R);
-    constexpr uint32_t kIdescO = umma_idesc_e4m3(HD, 2 * R) | (1u << 15);  // V MN-major
+    constexpr uint32_t kIdescO = umma_idesc_e4m3(HD, C::kN) | kIdescBE5m2 | (1u << 15);  // V MN-major
     extern __shared__ __align__(1024) uint8_t few_smem[];
     uint8_t *k_ring = few_smem, *v_ring = k_ring + kStagesK * C::kTile;
     uint8_t *px = v_ring + kStagesV * C::kTile;
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                         const uint64_t pd = p_desc + (uint32_t)((C::kAhead == 2 ? at : at >> 1) * C::kP >> 4);
 #pragma unroll
                         for (int k = 0; k < kKv8Keys / 32; ++k)
-                            umma_e4m3(tmem + C::kOCol + (at >> 1) * 2 * R, vd + (uint32_t)(k * 32 * HD >> 4), pd + 2 * k, kIdescO,
+                            umma_e4m3(tmem + C::kOCol + (at >> 1) * C::kN, vd + (uint32_t)(k * 32 * HD >> 4), pd + 2 * k, kIdescO,
                                       (i >= kGroups || k > 0) ? 1u : 0u);
                         umma_commit(smem_u32(&sh.o_done[v_buf]));
                     }
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
         const int key = quad * 32 + lane;
         const int tid = threadIdx.x - 128;
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-        const uint32_t o_addr = tmem + lane_off + C::kOCol + grp * 2 * R;
+        const uint32_t o_addr = tmem + lane_off + C::kOCol + grp * C::kN;
         // This key's byte in rows 0..7 of the weights (8 rows repeat the swizzle).
         uint32_t p_row[8];
 #pragma unroll
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                         }
                         if (!first) {
 #pragma unroll
-                            for (int part = 0; part < 2; ++part) {
+                            for (int part = 0; part < kKv8Parts; ++part) {
                                 float o[8];
                                 tmem_ld8_nowait(o_addr + part * R + c, o);
                                 tmem_wait_ld();
@@ -453,13 +457,14 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                     const float w0 = fast_exp2(arg[r]), w1 = fast_exp2(arg[r + 1]);
                     l[r] = fmaf(w0, inv_vs, l[r]);
                     l[r + 1] = fmaf(w1, inv_vs, l[r + 1]);
-                    uint32_t hi, lo;
-                    split_e4m3x2(w0, w1, hi, lo);
+                    uint32_t w = pack_f16x2(w0, w1);
                     const uint32_t at0 = p_row[r % 8] + p_at + r / 8 * 1024, at1 = p_row[(r + 1) % 8] + p_at + (r + 1) / 8 * 1024;
-                    st_shared_u8(at0, hi);
-                    st_shared_u8(at1, hi >> 8);
-                    st_shared_u8(at0 + R * 128, lo);
-                    st_shared_u8(at1 + R * 128, lo >> 8);
+#pragma unroll
+                    for (int part = 0; part < kKv8Parts; ++part) {
+                        const uint32_t code = part + 1 < kKv8Parts ? cut_e5m2x2(w) : last_e5m2x2(w);
+                        st_shared_u8(at0 + part * R * 128, code >> 8);
+                        st_shared_u8(at1 + part * R * 128, code >> 24);
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 tc_fence_before();
@@ -559,15 +564,15 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                 if (grp < active) {
 #pragma unroll
                     for (int c = 0; c < C::kRowsX; c += 8) {
-                        float o[16];
+                        float o[8 * kKv8Parts];
                         __syncwarp();  // lanes part at the stores; the loads from TMEM are the whole warp's
-                        tmem_ld8_nowait(o_addr + c0 + c, o);
-                        tmem_ld8_nowait(o_addr + R + c0 + c, o + 8);
+#pragma unroll
+                        for (int part = 0; part < kKv8Parts; ++part) tmem_ld8_nowait(o_addr + part * R + c0 + c, o + 8 * part);
                         tmem_wait_ld();
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
                             const float f = __shfl_sync(0xFFFFFFFFu, factor, c0 + c + x);
-                            if (lane < C::kDims) exch[(grp * C::kRowsX + c + x) * HD + d] = (o[x] + o[8 + x]) * f;
+                            if (lane < C::kDims) exch[(grp * C::kRowsX + c + x) * HD + d] = (o[x] + (o[8 + x] + o[16 + x])) * f;
                         }
                     }
                 }

@@ -3,7 +3,7 @@
 // of an MMA, in one or two tiles that share the key tiles.
 //
 //   S [128 rows x 128 keys] = (q1 + q2) K^T          (q's two parts, from shared memory)
-//   O [128 rows x D] += (w1 + w2) V                    (the weights' two parts, from TMEM)
+//   O [128 rows x D] += (w1 + w2 + w3) V              (the weights' parts, from TMEM)
 //
 // The roles of the warps and the order of the MMAs are tree_attention's: warps 0
 // and 1 load K and V tiles, warp 2 issues the MMAs, warp 3 cuts the share into
@@ -19,13 +19,14 @@
 // fused operation and one exponential; the sum l takes a block's weights divided by
 // its scale again.
 //
-// Prompts of 2 x 2000 rows behind up to 6000 keys, 28 + 4 heads of 128: 300 us, 666
-// TFLOP/s of the formula's operations, of which the split doubles the products; bound
-// by the chain S, softmax, PV of a tile (the softmax of 128 keys 3300 cycles beside
-// the other group's; issue slots 44%, tensor pipe 32%, exponentials 33%). One pass
-// with a running maximum took 473 us (weights of a tile done again where the
-// reference moved) against 335 us of two at the time. 32 sequences of 1 to 9 rows in
-// a window of 4096: 54 us, starts and ends of items half of it. What an item does
+// Prompts of 2 x 2000 rows behind up to 6000 keys, 28 + 4 heads of 128: 317 us, 630
+// TFLOP/s of the formula's operations, of which the splits do S twice and PV three
+// times; bound by the chain S, softmax, PV of a tile. (With weights in two e4m3 parts,
+// which lose long tails: 300 us; the softmax of 128 keys 3300 cycles beside the other
+// group's, issue slots 44%, tensor pipe 32%, exponentials 33%.) One pass with a running
+// maximum took 473 us (weights of a tile done again where the reference moved)
+// against 335 us of two at the time. 32 sequences of 1 to 9 rows in a window of
+// 4096: 57 us, starts and ends of items half of it. What an item does
 // once is written in loops: unrolled it took 60.6 us instead of 56.0 at the time.
 #pragma once
 
@@ -48,7 +49,8 @@ struct Kv8Many {
     static constexpr uint32_t kOCol = 2 * kKv8Keys;
     // TMEM: S_A | S_B | O_A | O_B; the weights' parts take the columns of the S
     // they came from, those of 64 keys in the columns of these.
-    static constexpr uint32_t kHalfCol = 64, kLoCol = 16;
+    static constexpr uint32_t kHalfCol = 64, kPartCol = 16;
+    static_assert(kKv8Parts * kPartCol <= kHalfCol, "the parts of 64 keys");
     // Beginning and end of an item cost what 6 to 8 of its tiles do, and a tile of both
     // row tiles twice one. Lower units (6, 2, 3) took 5% more for prompts.
     using Cost = Kv8Cost<16, 2, 4, 4>;
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     using C = Kv8Many<HD>;
     constexpr int kStages = C::kStages;
     constexpr uint32_t kIdescS = umma_idesc_e4m3(kManyRows, kKv8Keys);
-    constexpr uint32_t kIdescO = umma_idesc_e4m3(kManyRows, HD) | (1u << 16);  // V MN-major
+    constexpr uint32_t kIdescO = umma_idesc_e4m3(kManyRows, HD) | kIdescAE5m2 | (1u << 16);  // V MN-major
     extern __shared__ __align__(1024) uint8_t many_smem[];
     uint8_t *q_s = many_smem, *ring = many_smem + 4 * C::kTile;  // [tile][part], [stage][K, V]
     Kv8ManyShared<kStages> &sh = *reinterpret_cast<Kv8ManyShared<kStages> *>(many_smem + C::kBytes);
@@ -199,10 +201,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (leader) {
                     const uint64_t vd = ring_desc + (uint32_t)((2 * buf + 1) * C::kTile >> 4);
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) {
+                    for (int part = 0; part < kKv8Parts; ++part) {
 #pragma unroll
                         for (int k = 0; k < kKv8Keys / 32; ++k)
-                            umma_e4m3_ta(tmem + C::kOCol + grp * HD, tmem + grp * kKv8Keys + (k >> 1) * C::kHalfCol + part * C::kLoCol + (k & 1) * 8,
+                            umma_e4m3_ta(tmem + C::kOCol + grp * HD, tmem + grp * kKv8Keys + (k >> 1) * C::kHalfCol + part * C::kPartCol + (k & 1) * 8,
                                          vd + (uint32_t)(k * 32 * HD >> 4), kIdescO, (i > 1 || part + k > 0) ? 1u : 0u);
                     }
                     if (!two || grp == 1) umma_commit(smem_u32(&sh.v_empty[buf]));
@@ -399,8 +401,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         for (int c = 0; c < kKv8Keys; c += 32) {
                             if (c >= k0 && c < k0 + KEYS) continue;
                             const uint32_t at = s_addr + C::kHalfCol * (c / 64) + c % 64 / 4;
-                            tmem_st8_nowait(at, zero);
-                            tmem_st8_nowait(at + C::kLoCol, zero);
+#pragma unroll
+                            for (int part = 0; part < kKv8Parts; ++part) tmem_st8_nowait(at + part * C::kPartCol, zero);
                         }
                     }
                     const float base = kKv8TopLog2 - (m_run == -INFINITY ? 0.0f : m_run);
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         if (piece < kPieces - 1) load(piece);
 #pragma unroll
                         for (int c = 0; c < kPiece / 32; ++c) {
-                            uint32_t hi[8], lo[8];
+                            uint32_t code[kKv8Parts][8];
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const int at16 = 2 * c + h, b = piece * (kPiece / 16) + at16;
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                 unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll
                                 for (int x = 0; x < 4; ++x) {
-                                    uint32_t part[2][2];
+                                    uint32_t w[2];
 #pragma unroll
                                     for (int y = 0; y < 2; ++y) {
                                         const int k = 16 * at16 + 4 * x + 2 * y;
@@ -426,10 +428,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                         e0 = fast_exp2(e0);
                                         e1 = fast_exp2(e1);
                                         sums[y] = add_pair(sums[y], pair_f32(e0, e1));
-                                        split_e4m3x2(e0, e1, part[0][y], part[1][y]);
+                                        w[y] = pack_f16x2(e0, e1);
                                     }
-                                    hi[4 * h + x] = part[0][0] | part[0][1] << 16;
-                                    lo[4 * h + x] = part[1][0] | part[1][1] << 16;
+#pragma unroll
+                                    for (int part = 0; part + 1 < kKv8Parts; ++part) {
+                                        const uint32_t cut = cut_e5m2x2(w[0]);
+                                        code[part][4 * h + x] = codes_e5m2x4(cut, cut_e5m2x2(w[1]));
+                                    }
+                                    code[kKv8Parts - 1][4 * h + x] = codes_e5m2x4(last_e5m2x2(w[0]), last_e5m2x2(w[1]));
                                 }
                                 float s0, s1;
                                 unpair_f32(add_pair(sums[0], sums[1]), s0, s1);
@@ -439,8 +445,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             }
                             const int key = k0 + kPiece * piece + 32 * c;
                             const uint32_t at = s_addr + C::kHalfCol * (key / 64) + key % 64 / 4;
-                            tmem_st8_nowait(at, reinterpret_cast<const float *>(hi));
-                            tmem_st8_nowait(at + C::kLoCol, reinterpret_cast<const float *>(lo));
+#pragma unroll
+                            for (int part = 0; part < kKv8Parts; ++part) tmem_st8_nowait(at + part * C::kPartCol, reinterpret_cast<const float *>(code[part]));
                         }
                     }
                     tmem_wait_st();

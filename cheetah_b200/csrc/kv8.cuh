@@ -26,21 +26,24 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
     return r;
 }
-// Two values as two e4m3 parts each, hi + lo: through f16, in which what hi leaves
-// off is exact.
-__device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t &hi, uint32_t &lo) {
-    uint16_t h, l;
-    asm("{\n\t.reg .b32 w, r;\n\t"
-        "cvt.rn.f16x2.f32 w, %3, %2;\n\t"
-        "cvt.rn.satfinite.e4m3x2.f16x2 %0, w;\n\t"
-        "cvt.rn.f16x2.e4m3x2 r, %0;\n\t"
-        "sub.f16x2 w, w, r;\n\t"
-        "cvt.rn.satfinite.e4m3x2.f16x2 %1, w;\n\t}"
-        : "=h"(h), "=h"(l)
-        : "f"(a), "f"(b));
-    hi = h;
-    lo = l;
+// Two f32 as an f16 pair.
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+    uint32_t w;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
 }
+// An e5m2 is the upper byte of an f16, so a pair of f16 >= 0 comes apart into e5m2 parts
+// without conversions: three bits of each are cut off, and what remains is exact.
+// The parts' codes are the upper bytes of what is returned, and of what
+// last_e5m2x2 rounds (half upwards).
+__device__ __forceinline__ uint32_t cut_e5m2x2(uint32_t &w) {
+    const uint32_t part = w & 0xFF00FF00u;
+    asm("sub.f16x2 %0, %0, %1;" : "+r"(w) : "r"(part));
+    return part;
+}
+__device__ __forceinline__ uint32_t last_e5m2x2(uint32_t w) { return w + 0x00800080u; }
+// The codes of four values: the upper bytes of two pairs.
+__device__ __forceinline__ uint32_t codes_e5m2x4(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7531); }
 __device__ __forceinline__ void unpack_e4m3x2(uint32_t w, float &a, float &b) {
     asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}" : "=f"(a), "=f"(b) : "r"(e4m3x2_to_f16x2(w)));
 }

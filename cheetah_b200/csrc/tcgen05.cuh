@@ -57,7 +57,8 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, u
 }
 
 // kind::f8f6f4, A = B = e4m3, D = f32 (both K-major unless a transpose bit, 15
-// for A and 16 for B, is added): 32 k per instruction.
+// for A and 16 for B, is added; e5m2 with one of the type bits): 32 k per instruction.
+constexpr uint32_t kIdescAE5m2 = 1u << 7, kIdescBE5m2 = 1u << 10;
 __host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }

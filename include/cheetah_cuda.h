@@ -568,10 +568,13 @@ CHEETAH_CUDA_API int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *args, vo
  * see never reach it, NaN codes and scales of blocks that hold none of its
  * positions included. Rows from row_starts[batch] on stay as they were; a
  * sequence with seq_lens[b] < n gives zeros. Scales must be positive where a
- * row sees the block. Sums and statistics are f32; the softmax weights, times
- * V's scale, enter the products as two e4m3 parts (about 8 bits, as bf16
- * holds, or 2^-15 of a row's largest such product). If a wait inside the
- * kernel gives up, every row is NaN.
+ * row sees the block. Sums and statistics are f32. q enters the products as
+ * two e4m3 parts (off by 2^-17.8 of its row's largest element at most), the
+ * softmax weights times V's scale as three e5m2 parts: off by 2^-9 + 2^-11 of
+ * themselves (bf16 weights: 2^-8), or by 2^-29 of the row's largest such product,
+ * which over L keys adds at most L 2^-29 of it times V's largest code to what
+ * bf16 weights would be off by. If a wait inside the kernel gives up, every
+ * row is NaN.
  *
  * `workspace` holds partial results between the launches of a call:
  * cheetah_cuda_op_attention_kv8_workspace says how many bytes (256-byte

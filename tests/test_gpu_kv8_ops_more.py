@@ -4,10 +4,11 @@ whose softmax has one heavy key over a long tail."""
 
 import math
 
-import numpy as np
 import pytest
 
-from tests.test_gpu_kv8_ops import Attend, E4M3, _cuda, i32, to_gpu  # noqa: F401  (_cuda is the fixture)
+from tests import kv8_peaked_ref as VP
+from tests import kv8_ref as V8
+from tests.test_gpu_kv8_ops import Attend, E4M3, _cuda  # noqa: F401  (_cuda is the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -46,3 +47,94 @@ def test_attention_of_rows_beside_lanes_that_hold_none(q_heads, kvh, D, rows, ct
     hit[c.starts[2]:] = torch.isnan(got[c.starts[2]:])  # rows behind the last sequence are not written
     assert bool(torch.isnan(got[hit]).all())
     assert torch.equal(got[:c.starts[2]][~hit[:c.starts[2]]], base[:c.starts[2]][~hit[:c.starts[2]]])
+
+
+def peaked(seed, ctx, rows, q_heads, kvh, D, weight, heavy, common, window=0, sinks=0, sink_v=1.0, noise=0.0, extra=0):
+    """A call whose every row gives the key `heavy` about `weight` of its softmax and
+    spreads the rest over the others; V = common + a normal part, that of the heavy key
+    times sink_v."""
+    c = Attend(seed, [ctx], [rows], q_heads, kvh, D, 64, window, sinks, extra_rows=extra)
+    g = torch.Generator().manual_seed(seed)
+    length = c.lens[0]
+    # q and the heavy key along one direction, the other keys across it (and some noise).
+    u = torch.sign(torch.randn(D, generator=g))
+    n = min(length, window + sinks) if window else length
+    score = math.log(weight / (1.0 - weight) * n)  # of the heavy key above the others
+    c.q = (u * 2.0).expand_as(c.q).to(torch.bfloat16).contiguous()
+    c.q_wide = c.q.reshape(c.q.shape[0], -1)
+    k = noise * torch.randn(length, kvh, D, generator=g)
+    k -= (k @ u)[..., None] * u / D * (0.0 if noise else 1.0)
+    k[heavy] = u * (score / (2.0 * math.sqrt(D)))
+    v = common + torch.randn(length, kvh, D, generator=g)
+    v[heavy] *= sink_v
+    for (codes, scales), x in ((c.k, k), (c.v, v)):
+        for i in range(-(-length // 64)):
+            page = c.table[0, i]
+            part = torch.zeros(64, kvh, D)
+            part[:min(64, length - i * 64)] = x[i * 64:(i + 1) * 64]
+            part = part.transpose(0, 1).reshape(kvh, 4, 16, D)
+            e = torch.ceil(torch.log2(part.abs().amax((-1, -2)).clamp(min=2.0 ** -55) / 448.0))
+            codes[page] = (part / torch.exp2(e)[..., None, None]).to(E4M3).reshape(kvh, 64, D).view(torch.uint8)
+            scales[page] = torch.exp2(e)
+    return c
+
+
+def check_peaked(c, heads, sequences=(0,)):
+    """Against the reference, under its own tolerance: relative to each weight. (All
+    sequences share pages, length and number of rows.)"""
+    got = c.run().cpu().double()
+    length, n = c.lens[0], c.starts[1]
+    group = c.q.shape[1] // c.kvh
+    k, _ = V8.cached(*c.k, c.table[0], length)
+    v, _ = V8.cached(*c.v, c.table[0], length)
+    codes = V8.cached(c.v[0], torch.ones_like(c.v[1]), c.table[0], length)[0]
+    scales = V8.cached(torch.zeros_like(c.v[0]) + 56, c.v[1], c.table[0], length)[0][:, :, 0]
+    pos, j = torch.arange(length - n, length)[:, None], torch.arange(length)
+    seen = j <= pos
+    if c.window:
+        seen &= (j > pos - c.window) | (j < c.sinks)
+    some = torch.arange(n) if n <= 8 else torch.tensor([r for r in sorted({0, 1, 17, 18, 36, n // 2, n - 2, n - 1}) if r < n])
+    for h in heads:
+        kv = h // group
+        for b in sequences:
+            rows = c.starts[b] + some
+            o, tol = VP.attend(c.q[rows, h].double(), k[:, kv], v[:, kv], codes[:, kv], scales[:, kv], seen[some])
+            err = (got[rows, h] - o).abs()
+            assert bool((err <= tol).all()), (h, b, float((err / tol).max()), float((err.norm() / o.norm())))
+
+
+@pytest.mark.parametrize("rows,q_heads,kvh,D", [(1, 7, 1, 128), (1, 16, 1, 64), (4, 4, 1, 64), (4, 4, 1, 128), (9, 3, 1, 128),
+                                                 (12, 4, 1, 64), (40, 7, 1, 128), (300, 7, 1, 64)])
+@pytest.mark.parametrize("ctx", [4000, 16300, 32700])
+@pytest.mark.parametrize("weight", [0.5, 0.7, 0.9, 0.97])
+def test_attention_of_a_heavy_key_and_a_long_tail(rows, q_heads, kvh, D, ctx, weight):
+    """The first key holds most of the weight, the others spread the rest: an attention sink."""
+    check_peaked(peaked(ctx + rows, ctx, rows, q_heads, kvh, D, weight, 0, 0.5), [0, q_heads - 1])
+
+
+@pytest.mark.parametrize("rows,D", [(1, 64), (4, 128), (9, 128), (40, 64), (300, 128)])
+@pytest.mark.parametrize("weight", [0.8, 0.97])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (8192, 4)])
+def test_attention_of_a_sink_without_a_value(rows, D, weight, window, sinks):
+    """A sink whose V is near zero: the output is the tail's. With a window the sinks stay visible."""
+    check_peaked(peaked(rows, 20000, rows, 4, 1, D, weight, 0, 0.3, window, sinks, sink_v=2.0 ** -7, noise=0.4), [1])
+
+
+@pytest.mark.parametrize("rows,D", [(1, 128), (4, 64), (9, 64), (40, 128), (300, 64)])
+@pytest.mark.parametrize("heavy", [5000, 11999])
+def test_attention_of_a_heavy_key_behind_the_tail(rows, D, heavy):
+    """The heavy key comes after others, the last ahead of the rows: the tail is rescaled, not lost."""
+    check_peaked(peaked(rows + heavy, 12000, rows, 4, 1, D, 0.9, heavy, 0.5, noise=0.2), [0, 3])
+
+
+@pytest.mark.parametrize("rows,q_heads,D", [(1, 7, 128), (1, 16, 64), (4, 7, 128), (9, 7, 64), (18, 7, 128), (36, 7, 64)])
+@pytest.mark.parametrize("ctx,weight", [(8000, 0.9), (32700, 0.7), (32700, 0.95)])
+def test_attention_of_a_heavy_key_in_items_that_one_cta_walks_through(rows, q_heads, D, ctx, weight):
+    """So many sequences (over the same pages) that a CTA has whole items: one reference
+    from the heavy key to the end of the tail."""
+    c = peaked(rows + D, ctx, rows, q_heads, 1, D, weight, 0, 0.5, noise=0.1)
+    copies = 160
+    c.table, c.lens, c.starts = c.table.repeat(copies, 0), c.lens * copies, [rows * i for i in range(copies + 1)]
+    c.q = c.q.repeat(copies, 1, 1)
+    c.q_wide = c.q.reshape(c.q.shape[0], -1)
+    check_peaked(c, [0, q_heads - 1], (0, 80, 159))
