@@ -62,6 +62,9 @@ __device__ __forceinline__ float round_to_odd(double x) {
     return (double)f == x ? f : __uint_as_float(bits | 1u);
 }
 
+// Whether these are the bits of a power of two whose inverse is a normal number too.
+__device__ __forceinline__ bool kv8_power_of_two(uint32_t bits) { return (bits & 0x7FFFFFu) == 0 && bits >= 0x00800000u && bits <= 0x7E800000u; }
+
 // The smallest power of two, 2^kKv8LeastLog2 at least, whose 448-fold reaches the
 // magnitude whose f32 bits these are.
 __device__ __forceinline__ float kv8_scale_for(uint32_t top_bits) {

@@ -242,7 +242,7 @@ __device__ __noinline__ void kv8_exact(const Kv8AppendParams &p, bool is_k, uint
     widen_chunk<TIN>(r1, wide[1]);
     const bool normed = is_k && p.q.k_norm != nullptr;
     const uint32_t bits = __float_as_uint(scale);
-    const bool power = (bits & 0x7FFFFFu) == 0 && bits >= 0x00800000u;
+    const bool power = kv8_power_of_two(bits);
     const double by = (double)__uint_as_float((254u << 23) - bits);  // 1 / scale, where that is a power of two
     double inv = 1.0;
     if (normed) {
@@ -522,7 +522,7 @@ __device__ __forceinline__ void kv8_append_rows(const Kv8AppendParams &p, const 
         // Products by a power of two are exact; a scale that was not set here may be
         // none, and is divided by in 64 bits.
         const uint32_t scale_bits = __float_as_uint(scale);
-        const bool power = (scale_bits & 0x7FFFFFu) == 0 && scale_bits >= 0x00800000u;
+        const bool power = kv8_power_of_two(scale_bits);
         const float inv = __uint_as_float((254u << 23) - scale_bits);  // of a power of two: exponents add up to 254
         const Pair minus2 = pair_f32(-1.0f, -1.0f);
 #pragma unroll

@@ -8,7 +8,7 @@ import pytest
 
 from tests import kv8_peaked_ref as VP
 from tests import kv8_ref as V8
-from tests.test_gpu_kv8_ops import Attend, E4M3, _cuda  # noqa: F401  (_cuda is the fixture)
+from tests.test_gpu_kv8_ops import Attend, E4M3, _cuda, check_append, random_pool  # noqa: F401  (_cuda is the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -138,3 +138,18 @@ def test_attention_of_a_heavy_key_in_items_that_one_cta_walks_through(rows, q_he
     c.q = c.q.repeat(copies, 1, 1)
     c.q_wide = c.q.reshape(c.q.shape[0], -1)
     check_peaked(c, [0, q_heads - 1], (0, 80, 159))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("old", [2.0 ** 126, 2.0 ** 127])
+def test_append_behind_the_largest_scales(old, dtype):
+    """A scale that only a caller can have set, whose inverse is the least normal number or none."""
+    g = torch.Generator().manual_seed(8)
+    kvh, D, pt, pages = 2, 128, 16, 3
+    x = (torch.randn(3, 6, D, generator=g) * 1e38).clamp(-3e38, 3e38).to(dtype)
+    pools = [random_pool(g, pages, kvh, pt, D) for _ in range(2)]
+    for _, s in pools:
+        s.fill_(old)
+    slots = torch.tensor([16 + 5, 16 + 6, 16 + 7], dtype=torch.int32)
+    cos, sin = torch.ones(4, D // 2), torch.zeros(4, D // 2)
+    check_append(x, 2, kvh, torch.zeros(3, dtype=torch.int32), slots, cos, sin, [None, None], pools, 1e-6, 4)
