@@ -62,6 +62,12 @@ __device__ __forceinline__ float round_to_odd(double x) {
     return (double)f == x ? f : __uint_as_float(bits | 1u);
 }
 
+// a * b cut off, and the last bit set where that left something off.
+__device__ __forceinline__ float product_to_odd(float a, float b) {
+    const float f = __fmul_rz(a, b);
+    return fmaf(a, b, -f) != 0.0f ? __uint_as_float(__float_as_uint(f) | 1u) : f;
+}
+
 // Whether these are the bits of a power of two whose inverse is a normal number too.
 __device__ __forceinline__ bool kv8_power_of_two(uint32_t bits) { return (bits & 0x7FFFFFu) == 0 && bits >= 0x00800000u && bits <= 0x7E800000u; }
 

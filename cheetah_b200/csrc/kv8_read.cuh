@@ -29,10 +29,20 @@ __device__ __forceinline__ void kv8_store(TOUT *dst, uint2 codes, float scale) {
     float a[4], b[4];
     unpack_e4m3x4(codes.x, a);
     unpack_e4m3x4(codes.y, b);
+    // Products by a power of two are exact. Another scale's may not fit f32: rounded
+    // there to odd first, they are rounded once.
+    if (sizeof(TOUT) == 2 && (__float_as_uint(scale) & 0x7FFFFFu) != 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        a[i] *= scale;
-        b[i] *= scale;
+        for (int i = 0; i < 4; ++i) {
+            a[i] = product_to_odd(a[i], scale);
+            b[i] = product_to_odd(b[i], scale);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] *= scale;
+            b[i] *= scale;
+        }
     }
     if constexpr (sizeof(TOUT) == 2) {
         uint32_t w[4];

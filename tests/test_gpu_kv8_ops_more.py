@@ -153,3 +153,28 @@ def test_append_behind_the_largest_scales(old, dtype):
     slots = torch.tensor([16 + 5, 16 + 6, 16 + 7], dtype=torch.int32)
     cos, sin = torch.ones(4, D // 2), torch.zeros(4, D // 2)
     check_append(x, 2, kvh, torch.zeros(3, dtype=torch.int32), slots, cos, sin, [None, None], pools, 1e-6, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_kv8_read_rounds_a_product_once(dtype):
+    """Scales that are no powers of two: the product of a code's 4 bits and a scale's 24
+    does not fit f32, and bf16 of the rounded product is not always that of the product."""
+    from cheetah_b200 import runtime as R
+    kvh, D, pt = 1, 64, 16
+    # All codes, and scales for which code * scale lies just beside the middle of two bf16:
+    # (middle + 2^-20) / 1.125, so that the product rounded to f32 is the middle itself for some.
+    g = torch.Generator().manual_seed(4)
+    pages = 512
+    codes = torch.randint(0, 127, (pages, kvh, pt, D), generator=g).to(torch.uint8)
+    odd = 2 * torch.randint(0, 128, (pages,), generator=g) + 257
+    scales = (odd.double() / 256 / (1 + torch.randint(1, 8, (pages,), generator=g).double() / 8)).float().reshape(pages, 1, 1)
+    want = (codes.view(E4M3).double() * scales.double()[..., None])
+    slots = torch.arange(pages * pt, dtype=torch.int32, device="cuda")
+    k, v = R.kv8_read(*[codes.cuda().view(E4M3)] * 2, *[scales.cuda()] * 2, slots, dtype=dtype)
+    got = k.cpu().reshape(pages, pt, kvh, D).transpose(1, 2)
+    # The two neighbours in the output's type: the result is the nearer one.
+    step = want.abs() * torch.finfo(dtype).eps
+    err = (got.double() - want).abs()
+    for other in (torch.nextafter(got, torch.full_like(got, math.inf)), torch.nextafter(got, torch.full_like(got, -math.inf))):
+        assert bool((err <= (other.double() - want).abs()).all())
+    assert bool((err <= step).all()) and torch.equal(k, v)
