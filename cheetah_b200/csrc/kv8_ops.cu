@@ -354,8 +354,9 @@ int cheetah_cuda_op_verify_drafts(const CheetahCudaVerifyDrafts *a, void *stream
     CH_REQUIRE(a != nullptr && a->target_probs && a->tokens && a->row_starts && a->accept_u && a->sample_u && a->accepted &&
                    a->out_tokens,
                "cheetah_cuda_op_verify_drafts: null argument");
-    CH_REQUIRE(a->rows > 0 && a->rows <= 0x7FFFFFFFu && a->vocab > 0 && a->vocab <= (1u << 30),
-               "cheetah_cuda_op_verify_drafts: rows must be positive and vocab 1..2^30");
+    // (Rows are walked in steps of up to a block, in 31 bits.)
+    CH_REQUIRE(a->rows > 0 && a->rows <= (1u << 30) && a->vocab > 0 && a->vocab <= (1u << 30),
+               "cheetah_cuda_op_verify_drafts: rows and vocab must be 1..2^30");
     CH_REQUIRE(a->batch > 0 && a->batch <= 65535, "cheetah_cuda_op_verify_drafts: batch must be 1..65535");
     CH_REQUIRE((a->target_stride >= a->vocab || a->rows == 1) && a->target_stride < ((size_t)1 << 40) &&
                    (a->draft_probs == nullptr ||

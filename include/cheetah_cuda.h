@@ -630,7 +630,7 @@ typedef struct CheetahCudaVerifyDrafts {
     size_t target_stride;      /* elements between rows */
     const float *draft_probs;  /* [rows][vocab] or NULL; a sequence's last row is not read */
     size_t draft_stride;
-    uint32_t rows;
+    uint32_t rows;             /* 1..2^30 */
     uint32_t vocab;            /* 1..2^30 */
     const int32_t *tokens;     /* [rows] the step's input tokens */
     const int32_t *row_starts; /* [batch+1], ascending from 0 */
