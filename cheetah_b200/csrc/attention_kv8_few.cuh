@@ -33,14 +33,14 @@ struct Kv8Few {
     static constexpr int kGroups = 3;
     static constexpr int kThreads = 128 + kGroups * 128;
     static constexpr int kTile = kKv8Keys * HD;                     // one K or V tile
-    static constexpr int kAhead = 2;                                // tiles of weights that a group may be ahead of their product
+    static constexpr int kAhead = 2;                                // places for a group's weights: one ahead of their product
     // Columns of O^T and rows of the weights: three parts, and what fills them up to a
     // multiple of 16 (nobody reads the columns of those rows, whatever they hold).
     static constexpr int kN = (kKv8Parts * R + 15) / 16 * 16;
     static constexpr int kP = kN * kKv8Keys;                        // the weights of a tile
     static_assert(kP % 1024 == 0, "whole swizzle atoms");
     static constexpr int kPX = kGroups * kAhead * kP;               // at a segment's end the groups' O
-    static constexpr int kRowsX = kPX / (kGroups * HD * 4) < R ? kPX / (kGroups * HD * 4) : R;  // rows of them at a time
+    static_assert(kPX >= kGroups * R * HD * 4, "the groups' O");
     static constexpr int kQ = 2 * R * HD;                           // q's parts, one segment's
     // V tiles stay until their weights are there, K tiles only for S: the ring of V
     // is the deeper one.
@@ -56,7 +56,6 @@ struct Kv8Few {
     static constexpr uint32_t kOCol = kGroups * 4 * R;
     static constexpr uint32_t kCols = kGroups * (4 * R + kN) <= 256 ? 256 : 512;
     static_assert(kGroups * (4 * R + kN) <= (int)kCols, "TMEM columns");
-    static_assert(kRowsX % 8 == 0 && R % kRowsX == 0, "rows are joined 8 at a time");
     // Shares of three tiles pay for their join: with six the shortest calls took a fifth more.
     using Cost = Kv8Cost<4, 1, 1, 3>;
     static constexpr int kDims = HD == 128 ? 32 : 16;               // dimensions (lanes) of a warp's part of O^T
@@ -254,7 +253,7 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                     tc_fence_after();
                     if (leader) {
                         const uint64_t vd = v_desc + (uint32_t)(v_buf * C::kTile >> 4);
-                        const uint64_t pd = p_desc + (uint32_t)((C::kAhead == 2 ? at : at >> 1) * C::kP >> 4);
+                        const uint64_t pd = p_desc + (uint32_t)(at * C::kP >> 4);
 #pragma unroll
                         for (int k = 0; k < kKv8Keys / 32; ++k)
                             umma_e4m3(tmem + C::kOCol + (at >> 1) * C::kN, vd + (uint32_t)(k * 32 * HD >> 4), pd + 2 * k, kIdescO,
@@ -446,12 +445,12 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
                 const float inv_vs = fast_rcp(vs);
                 // The weights' place is free once its last product is done, and every
                 // warp has read what the segment before left there.
-                ok = C::kAhead == 2 ? wait_o(older) : wait_o(newer);
+                ok = wait_o(older);
                 if (!met) ok = ok && wait(sh.exchange, x_phase);
                 if (!ok) break;
                 if (!met) x_phase ^= 1;
                 met = true;
-                const uint32_t p_at = C::kAhead == 2 ? (uint32_t)place * C::kP : 0u;
+                const uint32_t p_at = (uint32_t)place * C::kP;
 #pragma unroll
                 for (int r = 0; r < R; r += 2) {
                     const float w0 = fast_exp2(arg[r]), w1 = fast_exp2(arg[r + 1]);
@@ -488,8 +487,8 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
             if (!ok) break;
             tile_at += jobs;
             turns += (jobs + kGroups - 1) / kGroups;
-            // The segment's end: the groups' sums and references, then their O,
-            // kRowsX rows at a time, through shared memory.
+            // The segment's end: the groups' sums and references, then their O, through
+            // shared memory.
             auto arrive = [&]() {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.exchange));
@@ -550,66 +549,57 @@ __global__ void __launch_bounds__(Kv8Few<HD, R>::kThreads, 1)
             }
             const int slot = g.slot;
             const bool patch = *reinterpret_cast<volatile int *>(&sh.non_finite) != 0;
-            float *exch = reinterpret_cast<float *>(px);  // [group][kRowsX][HD]
+            float *exch = reinterpret_cast<float *>(px);  // [group][R][HD]
             const int active = min(jobs, kGroups);
             const int d = quad * C::kDims + lane;
             const float inv_sum = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll 1
-            for (int c0 = 0; c0 < rows; c0 += C::kRowsX) {
-                if (c0 > 0) {
-                    arrive();  // every warp has read the rows before
-                    ok = meet();
-                    if (!ok) break;
-                }
-                if (grp < active) {
+            if (grp < active) {
 #pragma unroll
-                    for (int c = 0; c < C::kRowsX; c += 8) {
-                        float o[8 * kKv8Parts];
-                        __syncwarp();  // lanes part at the stores; the loads from TMEM are the whole warp's
+                for (int c = 0; c < R; c += 8) {
+                    float o[8 * kKv8Parts];
+                    __syncwarp();  // lanes part at the stores; the loads from TMEM are the whole warp's
 #pragma unroll
-                        for (int part = 0; part < kKv8Parts; ++part) tmem_ld8_nowait(o_addr + part * R + c0 + c, o + 8 * part);
-                        tmem_wait_ld();
+                    for (int part = 0; part < kKv8Parts; ++part) tmem_ld8_nowait(o_addr + part * R + c, o + 8 * part);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            const float f = __shfl_sync(0xFFFFFFFFu, factor, c0 + c + x);
-                            if (lane < C::kDims) exch[(grp * C::kRowsX + c + x) * HD + d] = (o[x] + (o[8 + x] + o[16 + x])) * f;
-                        }
-                    }
-                }
-                arrive();
-                ok = meet();
-                if (!ok) break;
-                for (int x = tid; x < C::kRowsX * HD / 2; x += kGroups * 128) {
-                    // (A row is one warp's or several.)
-                    const int y = x / (HD / 2), e = x % (HD / 2) * 2, r = c0 + y;
-                    const float inv = __shfl_sync(0xFFFFFFFFu, inv_sum, r), row_sum = __shfl_sync(0xFFFFFFFFu, sum, r),
-                                row_top = __shfl_sync(0xFFFFFFFFu, largest, r);
-                    if (r >= rows) continue;
-                    float a = 0.0f, b = 0.0f;
-#pragma unroll
-                    for (int z = 0; z < kGroups; ++z) {
-                        if (z >= active) break;
-                        const float2 v = *reinterpret_cast<const float2 *>(exch + (z * C::kRowsX + y) * HD + e);
-                        a += v.x;
-                        b += v.y;
-                    }
-                    const int node = r / p.group, h = r - node * p.group;
-                    if (patch) {
-                        if (kv8_patch(p, g, HD, pos0 + node, e)) a = NAN;
-                        if (kv8_patch(p, g, HD, pos0 + node, e + 1)) b = NAN;
-                    }
-                    if (slot >= 0) {
-                        const long long row = (2LL * blockIdx.x + slot) * R + r;
-                        *reinterpret_cast<float2 *>(p.part_o + row * HD + e) = make_float2(a, b);
-                        if (e == 0) p.part_ml[row] = make_float2(row_top, row_sum);
-                    } else {
-                        uint32_t w;
-                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b * inv), "f"(a * inv));
-                        *reinterpret_cast<uint32_t *>(out + ((long long)node * p.q_heads + h) * HD + e) = w;
+                    for (int x = 0; x < 8; ++x) {
+                        const float f = __shfl_sync(0xFFFFFFFFu, factor, c + x);
+                        if (lane < C::kDims) exch[(grp * R + c + x) * HD + d] = (o[x] + (o[8 + x] + o[16 + x])) * f;
                     }
                 }
             }
+            arrive();
+            ok = meet();
             if (!ok) break;
+            for (int x = tid; x < R * HD / 2; x += kGroups * 128) {
+                // (A row is one warp's or several.)
+                const int r = x / (HD / 2), e = x % (HD / 2) * 2;
+                const float inv = __shfl_sync(0xFFFFFFFFu, inv_sum, r), row_sum = __shfl_sync(0xFFFFFFFFu, sum, r),
+                            row_top = __shfl_sync(0xFFFFFFFFu, largest, r);
+                if (r >= rows) continue;
+                float a = 0.0f, b = 0.0f;
+#pragma unroll
+                for (int z = 0; z < kGroups; ++z) {
+                    if (z >= active) break;
+                    const float2 v = *reinterpret_cast<const float2 *>(exch + (z * R + r) * HD + e);
+                    a += v.x;
+                    b += v.y;
+                }
+                const int node = r / p.group, h = r - node * p.group;
+                if (patch) {
+                    if (kv8_patch(p, g, HD, pos0 + node, e)) a = NAN;
+                    if (kv8_patch(p, g, HD, pos0 + node, e + 1)) b = NAN;
+                }
+                if (slot >= 0) {
+                    const long long row = (2LL * blockIdx.x + slot) * R + r;
+                    *reinterpret_cast<float2 *>(p.part_o + row * HD + e) = make_float2(a, b);
+                    if (e == 0) p.part_ml[row] = make_float2(row_top, row_sum);
+                } else {
+                    uint32_t w;
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b * inv), "f"(a * inv));
+                    *reinterpret_cast<uint32_t *>(out + ((long long)node * p.q_heads + h) * HD + e) = w;
+                }
+            }
             arrive();
             met = false;  // waited for before the next weights
             tc_fence_before();
