@@ -59,7 +59,7 @@ constexpr int kKv8Queue = 4;      // segments the scheduler may be ahead
 // moves when one would pass 2^kKv8RoomLog2 times that (e5m2 ends at 57344 = 2^15.8). A
 // move costs a pass over O, and in 32 rows one moves soon; but what the room takes the
 // floor loses. Prompts of 2 x 2000 rows took 318 us with 14 and 1.75, 317 with these,
-// 314.6 with 12 and 3.75.
+// 315 with 12 and 3.75.
 constexpr float kKv8TopLog2 = 13.0f, kKv8RoomLog2 = 2.75f;
 constexpr int kKv8Parts = 3;      // of a weight
 

@@ -19,8 +19,9 @@
 // Bound by the loads of K and V where keys are many: 64 sequences of 1000 to 16000
 // keys, one row each, 28 + 4 heads of 128, 597 MB: 121 us, 4.9 TB/s. One sequence of
 // 700 keys takes 10.9 us: two launches, and a chain of starts, page, tile, S, weights,
-// O, join. Two groups instead of three took 141 us, rows as the tall side (the
-// other kernel) 75 us instead of 58 at 32 sequences.
+// O, join. Three groups instead of two, one barrier per product and faster ends took
+// the first case from 151 to 141 us together, loads without divisions to 120 from there;
+// rows as the tall side (the other kernel) took 75 us instead of 58 at 32 sequences.
 #pragma once
 
 #include "attention_kv8.cuh"

@@ -19,11 +19,11 @@
 // fused operation and one exponential; the sum l takes a block's weights divided by
 // its scale again.
 //
-// Prompts of 2 x 2000 rows behind up to 6000 keys, 28 + 4 heads of 128: 317 us, 630
+// Prompts of 2 x 2000 rows behind up to 6000 keys, 28 + 4 heads of 128: 318 us, 627
 // TFLOP/s of the formula's operations, of which the splits do S twice and PV three
-// times; bound by the chain S, softmax, PV of a tile. (With weights in two e4m3 parts,
-// which lose long tails: 300 us; the softmax of 128 keys 3300 cycles beside the other
-// group's, issue slots 44%, tensor pipe 32%, exponentials 33%.) One pass with a running
+// times; 333 us where it runs for long, at the power limit (1.86 GHz). Bound by the
+// chain S, softmax, PV of a tile (issue slots 42%, tensor pipe 37%, exponentials 33%).
+// With weights in two e4m3 parts, which lose long tails, 300 us. One pass with a running
 // maximum took 473 us (weights of a tile done again where the reference moved)
 // against 335 us of two at the time. 32 sequences of 1 to 9 rows in a window of
 // 4096: 57 us, starts and ends of items half of it. What an item does

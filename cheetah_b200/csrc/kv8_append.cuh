@@ -25,8 +25,9 @@
 // exact. All of k in 64 bits took 243 us for 32768 rows of 28 + 2 * 4 heads of 128.
 //
 // Measured: 583 MB for 32768 rows of 28 + 2 * 4 heads of 128, bf16, 145 us, 4.0
-// TB/s (the arithmetic of k and the codes, then memory); 256 sequences of 1 to 7 rows
-// 15.8 us and one row 3.4 us, chains of dependent reads.
+// TB/s: 16 warps an SM, which their registers allow, leave latencies uncovered (issue
+// slots 40%, DRAM 45%); 256 sequences of 1 to 7 rows 15.8 us and one row 3.3 us, chains
+// of dependent reads (issue slots 13%).
 #pragma once
 
 #include "common.cuh"

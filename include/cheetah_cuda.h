@@ -497,7 +497,8 @@ CHEETAH_CUDA_API int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogpro
  * of a cell is code * scale. Rows, sequences and slots are those of
  * cheetah_cuda_op_page_slots. All are asynchronous on `stream` (a stream of
  * the current device), allocate nothing, keep nothing between calls and may be
- * captured into a graph. No counterpart in the reference (its cache is f32). */
+ * captured into a graph. Outputs must not overlap inputs or each other. No
+ * counterpart in the reference (its cache is f32). */
 #define CHEETAH_CUDA_KV8_BLOCK 16
 
 /* cheetah_cuda_op_qk_norm_rope with an append in 8 bits. A block's cells are
@@ -506,10 +507,11 @@ CHEETAH_CUDA_API int cheetah_cuda_op_token_logprobs(const CheetahCudaTokenLogpro
  * new cells need, and the cells ahead of the first new one keep their values,
  * rounded again where the scale grew; other cells keep their codes. What cells
  * need is the smallest power of two, at least 2^-64, whose 448-fold reaches
- * their largest finite magnitude. Codes are the nearest e4m3 values (ties to
- * even) of exact quotients, k itself computed in 64 bits; a NaN or an infinity
- * becomes the NaN code. The slots of one call must be distinct and the rows of
- * one block within 32 rows of each other (as page_slots numbers them); cells of
+ * their largest finite magnitude (a k beyond f32 counts as f32's largest value).
+ * Codes are the nearest e4m3 values (ties to even) of exact quotients, k itself
+ * computed in 64 bits; a NaN or an infinity becomes the NaN code. The slots of
+ * one call must be distinct and the rows of one block lie within a run of 32
+ * rows (as page_slots numbers them); cells of
  * a block that breaks this have undefined values. Rows whose position or slot
  * is out of range are treated as there. */
 typedef struct CheetahCudaQkNormRopeKv8 {
@@ -567,14 +569,22 @@ CHEETAH_CUDA_API int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *args, vo
  * unseen, and a row that sees nothing gives zeros. Cells that a row does not
  * see never reach it, NaN codes and scales of blocks that hold none of its
  * positions included. Rows from row_starts[batch] on stay as they were; a
- * sequence with seq_lens[b] < n gives zeros. Scales must be positive where a
- * row sees the block. Sums and statistics are f32. q enters the products as
+ * sequence with seq_lens[b] < n gives zeros. Scales must be positive normal
+ * numbers where a row sees the block, V's within 2^100 of each other among a
+ * row's keys (farther apart, a weight may be lost). q is bf16: that of an f32
+ * append has to be cast. Sums and statistics are f32. q enters the products as
  * two e4m3 parts (off by 2^-17.8 of its row's largest element at most), the
  * softmax weights times V's scale as three e5m2 parts: off by 2^-9 + 2^-11 of
  * themselves (bf16 weights: 2^-8), or by 2^-29 of the row's largest such product,
  * which over L keys adds at most L 2^-29 of it times V's largest code to what
  * bf16 weights would be off by. If a wait inside the kernel gives up, every
  * row is NaN.
+ *
+ * Which of two kernels runs goes by rows / batch, rounded up, times the heads of
+ * a group: up to 16 the one for few rows. Results are right either way. A batch
+ * of single tokens takes up to 1.4 times as long where `rows` leaves room for
+ * more, and single tokens with a prompt chunk among them up to 1.5 times what a
+ * call for each takes.
  *
  * `workspace` holds partial results between the launches of a call:
  * cheetah_cuda_op_attention_kv8_workspace says how many bytes (256-byte
