@@ -581,10 +581,10 @@ CHEETAH_CUDA_API int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *args, vo
  * row is NaN.
  *
  * Which of two kernels runs goes by rows / batch, rounded up, times the heads of
- * a group: up to 16 the one for few rows. Results are right either way. A batch
- * of single tokens takes up to 1.4 times as long where `rows` leaves room for
- * more, and single tokens with a prompt chunk among them up to 1.5 times what a
- * call for each takes.
+ * a group: up to 16 the one for few rows. Results are right either way. 64 single
+ * tokens take 1.4 times as long where `rows` leaves room for three each, and 256
+ * with a prompt chunk of 256 among them 1.5 times what a call for each takes, the
+ * more the longer the chunk and what lies before it.
  *
  * `workspace` holds partial results between the launches of a call:
  * cheetah_cuda_op_attention_kv8_workspace says how many bytes (256-byte
