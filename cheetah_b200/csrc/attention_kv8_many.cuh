@@ -303,7 +303,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (!ok) break;
                 q_phase ^= 1;
             }
-            const float q_scale = sh.ml[grp][item_row].x;
+            // (A group without a job does not hold up the segment's end, after which the
+            // place is written again.)
+            const float q_scale = grp < jobs ? sh.ml[grp][item_row].x : 0.0f;
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             // Positions of this row, and of this group's first and last.
             const int pos = g.pos0 + node, first_pos = g.pos0 + tile_node, len = g.len;

@@ -178,3 +178,14 @@ def test_kv8_read_rounds_a_product_once(dtype):
     for other in (torch.nextafter(got, torch.full_like(got, math.inf)), torch.nextafter(got, torch.full_like(got, -math.inf))):
         assert bool((err <= (other.double() - want).abs()).all())
     assert bool((err <= step).all()) and torch.equal(k, v)
+
+
+@pytest.mark.parametrize("q_heads,kvh,D,rows", [(7, 1, 128, 3), (7, 1, 128, 9), (14, 2, 64, 17)])
+def test_attention_of_items_with_one_key_tile(q_heads, kvh, D, rows):
+    """One job to a segment, so the second group has none and waits for its end alone:
+    many such segments, each time the same rows and right."""
+    c = Attend(rows + D, [(5 * i) % (128 - rows) for i in range(200)], [rows] * 200, q_heads, kvh, D, 64, q_scale=4.0)
+    first = c.run()
+    c.check(first, sample=range(0, 200, 23))
+    for _ in range(20):
+        assert torch.equal(c.run(), first)
