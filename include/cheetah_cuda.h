@@ -569,10 +569,11 @@ CHEETAH_CUDA_API int cheetah_cuda_op_kv8_read(const CheetahCudaKv8Read *args, vo
  * unseen, and a row that sees nothing gives zeros. Cells that a row does not
  * see never reach it, NaN codes and scales of blocks that hold none of its
  * positions included. Rows from row_starts[batch] on stay as they were; a
- * sequence with seq_lens[b] < n gives zeros. Scales must be positive normal
- * numbers where a row sees the block, V's within 2^100 of each other among a
- * row's keys (farther apart, a weight may be lost). q is bf16: that of an f32
- * append has to be cast. Sums and statistics are f32. q enters the products as
+ * sequence with seq_lens[b] < n gives zeros. Scales must be positive where a
+ * row sees the block, V's from 2^-100 to 2^100 and within 2^100 of each other
+ * among a row's keys (beyond, weights may be lost: an append of V above 2^108
+ * sets such scales). q is bf16: that of an f32 append has to be cast. Sums and
+ * statistics are f32. q enters the products as
  * two e4m3 parts (off by 2^-17.8 of its row's largest element at most), the
  * softmax weights times V's scale as three e5m2 parts: off by 2^-9 + 2^-11 of
  * themselves (bf16 weights: 2^-8), or by 2^-29 of the row's largest such product,

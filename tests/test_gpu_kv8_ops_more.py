@@ -189,3 +189,15 @@ def test_attention_of_items_with_one_key_tile(q_heads, kvh, D, rows):
     c.check(first, sample=range(0, 200, 23))
     for _ in range(20):
         assert torch.equal(c.run(), first)
+
+
+@pytest.mark.parametrize("low,high", [(-100, -100), (100, 100), (-50, 50), (-100, 0), (0, 100)])
+@pytest.mark.parametrize("rows,q_heads,kvh,D", [(1, 7, 1, 128), (4, 4, 1, 64), (40, 7, 1, 128), (5, 7, 1, 64)])
+def test_attention_of_v_scales_at_the_ends_of_their_range(rows, q_heads, kvh, D, low, high):
+    """The sum of the weights counts keys whose V is 2^100 smaller than others', and
+    neither end of the range overflows or vanishes."""
+    c = Attend(rows + D, [900], [rows], q_heads, kvh, D, 64)
+    g = torch.Generator().manual_seed(rows)
+    pick = torch.rand(c.v[1].shape, generator=g) < 0.5
+    c.v[1][:] = torch.where(pick, torch.tensor(2.0 ** low), torch.tensor(2.0 ** high))
+    check_peaked(c, [0, q_heads - 1])
